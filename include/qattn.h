@@ -375,6 +375,107 @@ int qattn_ragged_tree_attn_fwd_noalloc(const void *q, const int64_t q_stride[4],
                                        int32_t num_splits, void *stream);
 
 /*
+ * Causal attention of packed prompts (no counterpart in the reference: its
+ * callers run the prompt through the model's own attention).  Token x of a
+ * sequence attends tokens 0 .. x of it:
+ *   o[t,h] = softmax_{j <= x}(scale q[t,h].k[cu[s]+j,kvh]) . v[cu[s]+j,kvh]
+ * q, o [total_tokens, num_q_heads, head_dim], k, v [total_tokens,
+ * num_kv_heads, head_dim]; the token strides of k and v are non-negative and
+ * below 2^25 elements (else QATTN_ERR_LAYOUT).  Keys a token does not attend
+ * never reach it, infinities and NaN in them included.  Rows of q that belong
+ * to no sequence are neither read nor written.  scale > 0.
+ */
+int qattn_prompt_fwd(const void *q, const int64_t q_stride[3],
+                     const void *k, const int64_t k_stride[3],
+                     const void *v, const int64_t v_stride[3],
+                     void *o, const int64_t o_stride[3],
+                     float *lse, const int64_t lse_stride[2],
+                     const int32_t *cu_seqlens, int32_t batch, int32_t max_seqlen,
+                     int64_t total_tokens, int32_t num_q_heads, int32_t num_kv_heads,
+                     int32_t head_dim, float scale, int32_t dtype, void *stream);
+
+/*
+ * Attention of query tokens over their sequence's context in a paged K/V
+ * cache, with LSE: qattn_prefix_fwd for a cache in pages, every sequence with
+ * a context length of its own (no counterpart in the reference, whose paged
+ * kernel reads tree nodes only).  Every query token of sequence s attends
+ * positions 0 .. context_lens[s] - 1; cache and page table are those of
+ * qattn_tree_paged_fwd.  cu_seqlens NULL: row s of q is sequence s's one
+ * query token (max_seqlen counts as 1).  context_lens is a DEVICE int32
+ * [batch] array; a length is taken into [0, pt_cols * page_size], which must
+ * not exceed 2^30.  A page index outside [0, num_pages) removes its keys; a
+ * query that attends nothing gets o = 0 and lse = -inf.  What lies in the
+ * slots behind a context never shows.  The cache strides are non-negative and
+ * a cache spans less than 64 GiB (else QATTN_ERR_LAYOUT).  scale > 0.
+ * workspace: device memory, 256-byte aligned, of at least
+ * qattn_prefix_paged_workspace_bytes() for the same sizes (max_seqlen 1 with
+ * cu_seqlens NULL); it is written and read by this call only, so calls that
+ * may overlap need one each.
+ */
+int64_t qattn_prefix_paged_workspace_bytes(int32_t batch, int32_t max_seqlen, int64_t total_tokens,
+                                           int32_t num_q_heads, int32_t num_kv_heads,
+                                           int32_t head_dim, int32_t pt_cols, int32_t page_size);
+
+int qattn_prefix_paged_fwd(const void *q, const int64_t q_stride[3],
+                           const void *k_cache, const int64_t k_stride[4],
+                           const void *v_cache, const int64_t v_stride[4],
+                           const int32_t *page_table, int32_t pt_cols, int32_t num_pages,
+                           int32_t page_size, const int32_t *context_lens,
+                           void *o, const int64_t o_stride[3],
+                           float *lse, const int64_t lse_stride[2],
+                           const int32_t *cu_seqlens, int32_t batch, int32_t max_seqlen,
+                           int64_t total_tokens, int32_t num_q_heads, int32_t num_kv_heads,
+                           int32_t head_dim, float scale, int32_t dtype, void *workspace,
+                           int64_t workspace_size, void *stream);
+
+/*
+ * New K/V rows into a paged cache: row i of sequence s (row cu_seqlens[s] + i
+ * of k and v, i < max_seqlen; cu_seqlens NULL: row s is sequence s's one row)
+ * goes to position context_lens[s] + i.  Positions at or beyond pt_cols *
+ * page_size (at most 2^30) and pages outside [0, num_pages) take no row;
+ * sequences with a negative context length or bad offsets are left alone.
+ * new_lens (DEVICE int32 [batch]) receives context_lens[s] plus the rows that
+ * the page table had positions for; it must not overlap context_lens.  Two
+ * sequences that share the page of a written position race.
+ */
+int qattn_kv_append(const void *k, const int64_t k_stride[3], const void *v, const int64_t v_stride[3],
+                    void *k_cache, const int64_t kc_stride[4], void *v_cache, const int64_t vc_stride[4],
+                    const int32_t *page_table, int32_t pt_cols, int32_t num_pages, int32_t page_size,
+                    const int32_t *context_lens, int32_t *new_lens, const int32_t *cu_seqlens,
+                    int32_t batch, int32_t max_seqlen, int64_t total_tokens, int32_t num_kv_heads,
+                    int32_t head_dim, int32_t dtype, void *stream);
+
+/*
+ * The rows of an accepted draft path moved together behind each context, in
+ * every layer of a cache [num_layers, num_pages, page_size, num_kv_heads,
+ * head_dim] (5 strides each): row context_lens[s] + accepted[s, j] goes to
+ * position context_lens[s] + j.  accepted is a DEVICE int32 [batch, path_cols]
+ * array; a path is strictly increasing (ancestors precede descendants) and
+ * ends before the first entry that is not above its predecessor, is negative
+ * or lies beyond the page table.  new_lens[s] = context_lens[s] + the path's
+ * length.  A row whose page or whose place's page does not exist is not
+ * moved.  A sequence with a negative context length is left alone.  Sequences
+ * that share a page among those positions race.
+ */
+int qattn_kv_compact(void *k_cache, const int64_t kc_stride[5], void *v_cache, const int64_t vc_stride[5],
+                     int32_t num_layers, const int32_t *page_table, int32_t pt_cols, int32_t num_pages,
+                     int32_t page_size, const int32_t *context_lens, const int32_t *accepted,
+                     int32_t path_cols, int32_t *new_lens, int32_t batch, int32_t num_kv_heads,
+                     int32_t head_dim, int32_t dtype, void *stream);
+
+/*
+ * Whole pages copied inside a cache, in every layer: page dst_pages[i] takes
+ * page src_pages[i] of K and of V, i < n (DEVICE int32 arrays).  Pairs with a
+ * page outside [0, num_pages) are passed over.  No page may be the
+ * destination of two pairs or the destination of one and the source of
+ * another: the copies run side by side.
+ */
+int qattn_kv_copy_pages(void *k_cache, const int64_t kc_stride[5], void *v_cache, const int64_t vc_stride[5],
+                        int32_t num_layers, int32_t num_pages, int32_t page_size,
+                        const int32_t *src_pages, const int32_t *dst_pages, int32_t n,
+                        int32_t num_kv_heads, int32_t head_dim, int32_t dtype, void *stream);
+
+/*
  * Two-state softmax merge.
  *
  * Replaces _fused_lse_merge_kernel (src/ragged_attn.py:1575-1616) launched by

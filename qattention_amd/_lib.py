@@ -70,6 +70,20 @@ SIGNATURES = {
     "qattn_ragged_tree_attn_fwd_noalloc": (C.c_int, [
         _p, _i64p, _p, _i64p, _p, _i64p, _p, _i64p, _p, _i64p, _p, _i64,
         _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _f32, _i32, _i32, _p]),
+    "qattn_prompt_fwd": (C.c_int, [
+        _p, _i64p, _p, _i64p, _p, _i64p, _p, _i64p, _p, _i64p,
+        _p, _i32, _i32, _i64, _i32, _i32, _i32, _f32, _i32, _p]),
+    "qattn_prefix_paged_workspace_bytes": (C.c_int64, [_i32, _i32, _i64, _i32, _i32, _i32, _i32, _i32]),
+    "qattn_prefix_paged_fwd": (C.c_int, [
+        _p, _i64p, _p, _i64p, _p, _i64p, _p, _i32, _i32, _i32, _p, _p, _i64p, _p, _i64p,
+        _p, _i32, _i32, _i64, _i32, _i32, _i32, _f32, _i32, _p, _i64, _p]),
+    "qattn_kv_append": (C.c_int, [
+        _p, _i64p, _p, _i64p, _p, _i64p, _p, _i64p, _p, _i32, _i32, _i32, _p, _p, _p,
+        _i32, _i32, _i64, _i32, _i32, _i32, _p]),
+    "qattn_kv_compact": (C.c_int, [
+        _p, _i64p, _p, _i64p, _i32, _p, _i32, _i32, _i32, _p, _p, _i32, _p, _i32, _i32, _i32, _i32, _p]),
+    "qattn_kv_copy_pages": (C.c_int, [
+        _p, _i64p, _p, _i64p, _i32, _i32, _i32, _p, _p, _i32, _i32, _i32, _i32, _p]),
     "qattn_lse_merge": (C.c_int, [
         _p, _i64p, _p, _i64p, _p, _i64p, _p, _i64p, _p, _i64p,
         _i32, _i32, _i32, _i32, _i32, _p]),
@@ -154,7 +168,7 @@ def check(rc: int, what: str) -> None:
         raise QAttnError(f"{what} failed: {ERRORS.get(rc, rc)}: {last_error()}")
 
 
-_I64 = {n: C.c_int64 * n for n in (2, 3, 4)}  # (forming the array type costs as much as filling it)
+_I64 = {n: C.c_int64 * n for n in (2, 3, 4, 5)}  # (forming the array type costs as much as filling it)
 
 
 def i64arr(vals):

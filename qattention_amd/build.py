@@ -18,8 +18,9 @@ PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(PKG_DIR, "csrc")
 LIB_PATH = os.path.join(PKG_DIR, "libqattn.so")
 OBJ_DIR = os.path.join(PKG_DIR, "_build")
-SOURCES = ["tree_attn.hip", "subtree_stream.hip", "prefix_attn.hip"]
-HEADERS = ["qattn_common.h", "qattn_device.h", "tree_walk.h"]
+SOURCES = ["tree_attn.hip", "subtree_stream.hip", "prefix_attn.hip", "paged_attn.hip", "prompt_attn.hip",
+           "kv_pages.hip"]
+HEADERS = ["qattn_common.h", "qattn_device.h", "kv_tiles.h", "tree_walk.h"]
 ARCH = os.environ.get("QATTN_ARCH", "gfx950")
 
 

@@ -46,6 +46,11 @@ __device__ __forceinline__ int32_t heap_parent(int32_t c, const Divider& dv) {
     return divide(m, dv);
 }
 
+// Positions of a paged sequence (pt_cols * page_size) that the kernels of
+// paged_attn.hip and kv_pages.hip take: 32-bit arithmetic a little past the
+// last one cannot wrap.
+constexpr int64_t kMaxPositions = int64_t(1) << 30;
+
 // ---------------------------------------------------------------------------
 // Parameter block of the tree kernels (passed by value as a kernel argument).
 // Strides are in elements; the d-stride of every tensor is 1.

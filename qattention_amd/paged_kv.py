@@ -1,0 +1,285 @@
+"""A paged K/V cache around tree verification: attending it, filling it, keeping
+the accepted path, copying pages.
+
+The cache layout is build_paged_kv's: K_cache / V_cache [pages, page_size, Hkv,
+D] and a page_table [B, max_pages] of int32 physical pages; position p of
+sequence s is slot p % page_size of page page_table[s, p // page_size], and
+context_lens[s] rows of it are filled.  compact_paged_kv and copy_kv_pages also
+take the caches of all layers in one tensor, [layers, pages, page_size, Hkv, D]
+(a layer's slice is the cache of the other calls).  Which pages a sequence owns
+is the business of whoever fills the page table; no call here allocates or frees
+pages.
+
+A serving step over these calls, every tensor on the GPU (such a step can be
+captured in a graph):
+
+    # prompt: causal attention within it, its rows into the pages
+    O = prompt_attention(Q, K, V, cu, max_seqlen)
+    lens = append_paged_kv(K, V, K_cache, V_cache, table, lens, cu, max_seqlen)
+    # decode: one token per sequence
+    lens = append_paged_kv(k, v, K_cache, V_cache, table, lens)
+    O, _ = prefix_attention_paged(q, K_cache, V_cache, table, lens)
+    # verify a draft tree: context and tree, merged; its rows behind the context
+    Oc, Lc = prefix_attention_paged(q, K_cache, V_cache, table, lens, cu, max_seqlen)
+    Ot, Lt = ragged_attention_with_lse(q, k, v, cu, b, depth, max_seqlen)
+    O = fused_lse_merge(...)
+    append_paged_kv(k, v, K_cache, V_cache, table, lens, cu, max_seqlen)
+    # keep the accepted path
+    lens = compact_paged_kv(K_caches, V_caches, table, lens, accepted)
+
+The calls run on torch's current stream, take contexts, offsets and page tables
+on the host too (a copy each call), and serve inference: tensors that ask for
+gradients are refused while autograd records.
+"""
+from __future__ import annotations
+
+import math
+from typing import Optional, Sequence, Tuple, Union
+
+import torch
+
+from . import _lib
+from .ragged_attn import (_SUPPORTED, _check_dtypes, _dtype_code, _no_grad, _on, _require_device, _seqlens, _stream,
+                          _vec, _vec_ok)
+
+
+def _int32(t: torch.Tensor, device) -> torch.Tensor:
+    return t.to(device=device, dtype=torch.int32, non_blocking=True).contiguous()
+
+
+def _check_caches(K_cache, V_cache, dims: Tuple[int, ...]) -> None:
+    """Caches that a call writes in place: no copy can stand in for them."""
+    if K_cache.dim() not in dims or K_cache.shape != V_cache.shape:
+        raise ValueError(f"caches must be {' or '.join(f'{d}-D' for d in dims)} and of one shape (got "
+                         f"{tuple(K_cache.shape)}, {tuple(V_cache.shape)})")
+    if K_cache.dtype not in _SUPPORTED or V_cache.dtype != K_cache.dtype:
+        raise AssertionError(f"Inputs must be fp16 or bf16 (got {K_cache.dtype}, {V_cache.dtype})")
+    if not K_cache.numel():
+        return
+    for c in (K_cache, V_cache):
+        if not _vec_ok(c):
+            raise ValueError(f"cache of shape {tuple(c.shape)} and strides {tuple(c.stride())} is not writable as "
+                             "16-byte rows (unit last stride, 8-element aligned strides, 16-byte aligned base)")
+        if any(st == 0 and n > 1 for st, n in zip(c.stride(), c.shape)):
+            raise ValueError("cache rows overlap (a stride of 0)")
+    if K_cache.data_ptr() == V_cache.data_ptr():
+        raise ValueError("K_cache and V_cache are the same memory")
+
+
+def _layered(cache) -> tuple:
+    """Layers, and the 5 strides {layer, page, slot, head, dim}."""
+    st = cache.stride()
+    return (cache.shape[0], _lib.i64arr(st)) if cache.dim() == 5 else (1, _lib.i64arr((0, *st)))
+
+
+def _table(page_table, B: int, device) -> torch.Tensor:
+    if page_table.dim() != 2 or page_table.shape[0] < B:
+        raise ValueError(f"page_table must be [B, max_pages] with B >= {B} (got {tuple(page_table.shape)})")
+    return _int32(page_table, device)
+
+
+def _lengths(context_lens, device) -> torch.Tensor:
+    if context_lens.dim() != 1:
+        raise ValueError(f"context_lens must be [B] (got {tuple(context_lens.shape)})")
+    return _int32(context_lens, device)
+
+
+def _rows(T: int, B: int, cu_seqlens, max_seqlen, device):
+    """max_seqlen and the device offsets of packed rows; without offsets row s is sequence s's."""
+    if cu_seqlens is None:
+        if T != B:
+            raise ValueError(f"without cu_seqlens there is one row per sequence (got {T} rows, {B} sequences)")
+        return 1, None
+    if cu_seqlens.dim() != 1 or cu_seqlens.shape[0] != B + 1:
+        raise ValueError(f"cu_seqlens must have {B + 1} entries (got {tuple(cu_seqlens.shape)})")
+    return _seqlens(cu_seqlens, B, device, max_seqlen)
+
+
+def prefix_attention_paged(
+    Q: torch.Tensor,
+    K_cache: torch.Tensor,
+    V_cache: torch.Tensor,
+    page_table: torch.Tensor,
+    context_lens: torch.Tensor,
+    cu_seqlens: Optional[torch.Tensor] = None,
+    max_seqlen: int = None,
+    return_lse: bool = True,
+):
+    """Attention of query tokens over their sequence's context in a paged cache:
+    prefix_attention for pages, with a context length per sequence.
+
+    Q: packed [T, Hq, D]; K_cache, V_cache: [pages, page_size, Hkv, D], Hkv
+    dividing Hq; page_table [B, max_pages]; context_lens [B].  Every query token
+    of sequence s attends positions 0 .. context_lens[s] - 1 (those that the
+    table has columns for), not itself: append its row first, or merge another
+    block by its LSE.  cu_seqlens None: one token per sequence (a decode step);
+    otherwise the packed offsets of the query tokens (draft trees, prompt
+    chunks), max_seqlen as everywhere.  A page outside the cache removes its
+    keys; a query without any gets 0 and an LSE of -inf.  Rows of Q that
+    belong to no sequence are not computed.  Returns O [T, Hq, D] (and LSE
+    [T, Hq] fp32, natural log, if return_lse)."""
+    assert K_cache.shape == V_cache.shape, "K and V cache shapes must match"
+    _check_dtypes(Q, K_cache, V_cache)
+    device = _require_device(Q, K_cache, V_cache)
+    _no_grad(Q, K_cache, V_cache)
+    if Q.dim() != 3 or K_cache.dim() != 4:
+        raise ValueError(f"expected Q [T, Hq, D] and caches [pages, page_size, Hkv, D] (got {tuple(Q.shape)}, "
+                         f"{tuple(K_cache.shape)})")
+    T, Hq, D = Q.shape
+    num_pages, page_size, Hkv, Dk = K_cache.shape
+    if Dk != D or Hkv < 1 or Hq % Hkv != 0 or page_size < 1:
+        raise ValueError(f"cache shape {tuple(K_cache.shape)} incompatible with Q {tuple(Q.shape)}")
+    ctx = _lengths(context_lens, device)
+    B = ctx.shape[0]
+    ms, cu = _rows(T, B, cu_seqlens, max_seqlen, device)
+    pt = _table(page_table, B, device)
+    Q, K_cache, V_cache = _vec(Q), _vec(K_cache), _vec(V_cache)
+    O = torch.empty_like(Q)
+    if not _vec_ok(O):
+        O = torch.empty(Q.shape, dtype=Q.dtype, device=device)
+    LSE = torch.empty(T, Hq, dtype=torch.float32, device=device) if return_lse else None
+    L = _lib.lib()
+    cols = pt.shape[1]
+    ws_bytes = L.qattn_prefix_paged_workspace_bytes(B, ms, T, Hq, Hkv, D, cols, page_size)
+    ws = torch.empty(max(ws_bytes, 1), dtype=torch.uint8, device=device)
+    with _on(device):
+        rc = L.qattn_prefix_paged_fwd(
+            Q.data_ptr(), _lib.i64arr(Q.stride()), K_cache.data_ptr(), _lib.i64arr(K_cache.stride()),
+            V_cache.data_ptr(), _lib.i64arr(V_cache.stride()), pt.data_ptr(), cols, num_pages, page_size,
+            ctx.data_ptr(), O.data_ptr(), _lib.i64arr(O.stride()), _lib.ptr(LSE),
+            _lib.i64arr(LSE.stride()) if LSE is not None else None, _lib.ptr(cu), B, ms, T, Hq, Hkv, D,
+            1.0 / math.sqrt(D), _dtype_code(Q), ws.data_ptr(), ws_bytes, _stream(device))
+    _lib.check(rc, "qattn_prefix_paged_fwd")
+    return (O, LSE) if return_lse else O
+
+
+def append_paged_kv(
+    K: torch.Tensor,
+    V: torch.Tensor,
+    K_cache: torch.Tensor,
+    V_cache: torch.Tensor,
+    page_table: torch.Tensor,
+    context_lens: torch.Tensor,
+    cu_seqlens: Optional[torch.Tensor] = None,
+    max_seqlen: int = None,
+) -> torch.Tensor:
+    """Store new K/V rows behind each context, in place: row i of sequence s goes
+    to position context_lens[s] + i.
+
+    K, V: packed [T, Hkv, D]; cu_seqlens as in prefix_attention_paged (None: one
+    row per sequence).  Returns the lengths afterwards, int32 [B] on the device;
+    context_lens itself stays (rows behind a context do not count, so storing a
+    draft tree and dropping the result leaves the context as it was).  A
+    position that the table has no column for takes no row and does not count; a
+    row whose page lies outside the cache is dropped.  A sequence with a negative
+    length is passed over.  The written pages must be the sequence's own."""
+    _check_caches(K_cache, V_cache, (4,))
+    _check_dtypes(K_cache, K, V)
+    device = _require_device(K_cache, V_cache, K, V)
+    _no_grad(K, V, K_cache, V_cache)
+    num_pages, page_size, Hkv, D = K_cache.shape
+    T = K.shape[0]
+    if K.dim() != 3 or K.shape != V.shape or K.shape[1:] != K_cache.shape[2:] or page_size < 1:
+        raise ValueError(f"rows {tuple(K.shape)}, {tuple(V.shape)} incompatible with cache {tuple(K_cache.shape)}")
+    ctx = _lengths(context_lens, device)
+    B = ctx.shape[0]
+    ms, cu = _rows(T, B, cu_seqlens, max_seqlen, device)
+    pt = _table(page_table, B, device)
+    K, V = _vec(K), _vec(V)
+    new = torch.empty_like(ctx)
+    with _on(device):
+        rc = _lib.lib().qattn_kv_append(
+            K.data_ptr(), _lib.i64arr(K.stride()), V.data_ptr(), _lib.i64arr(V.stride()),
+            K_cache.data_ptr(), _lib.i64arr(K_cache.stride()), V_cache.data_ptr(), _lib.i64arr(V_cache.stride()),
+            pt.data_ptr(), pt.shape[1], num_pages, page_size, ctx.data_ptr(), new.data_ptr(), _lib.ptr(cu), B, ms, T,
+            Hkv, D, _dtype_code(K_cache), _stream(device))
+    _lib.check(rc, "qattn_kv_append")
+    return new
+
+
+def compact_paged_kv(
+    K_cache: torch.Tensor,
+    V_cache: torch.Tensor,
+    page_table: torch.Tensor,
+    context_lens: torch.Tensor,
+    accepted: torch.Tensor,
+) -> torch.Tensor:
+    """Keep the accepted path of a draft tree whose rows were appended behind the
+    context, in place: the row of node accepted[s, j] (position context_lens[s] +
+    accepted[s, j]) moves to position context_lens[s] + j, in every layer.
+
+    K_cache, V_cache: [layers, pages, page_size, Hkv, D] or one layer's [pages,
+    page_size, Hkv, D]; accepted: int32 [B, P], strictly increasing along a path
+    (breadth-first order has ancestors before descendants), -1 behind its end; a
+    path ends before the first entry that is not above its predecessor or that
+    the table has no column for.  Returns the lengths afterwards, context plus
+    path, int32 [B] on the device.  Pages of the moved positions must be the
+    sequence's own."""
+    _check_caches(K_cache, V_cache, (4, 5))
+    device = _require_device(K_cache, V_cache)
+    _no_grad(K_cache, V_cache)
+    num_pages, page_size, Hkv, D = K_cache.shape[-4:]
+    ctx = _lengths(context_lens, device)
+    B = ctx.shape[0]
+    if accepted.dim() != 2 or accepted.shape[0] != B or page_size < 1:
+        raise ValueError(f"accepted must be [{B}, path length] (got {tuple(accepted.shape)})")
+    pt, path = _table(page_table, B, device), _int32(accepted, device)
+    new = torch.empty_like(ctx)
+    layers, ks = _layered(K_cache)
+    with _on(device):
+        rc = _lib.lib().qattn_kv_compact(
+            K_cache.data_ptr(), ks, V_cache.data_ptr(), _layered(V_cache)[1], layers, pt.data_ptr(), pt.shape[1],
+            num_pages, page_size, ctx.data_ptr(), path.data_ptr(), path.shape[1], new.data_ptr(), B, Hkv, D,
+            _dtype_code(K_cache), _stream(device))
+    _lib.check(rc, "qattn_kv_compact")
+    return new
+
+
+_Pages = Union[torch.Tensor, Sequence[int]]
+
+
+def _page_lists(src, dst, num_pages: int, device):
+    """Both lists on the device.  Lists on the host are checked: every page in
+    the cache, no destination twice, none that is also a source."""
+    src = src if isinstance(src, torch.Tensor) else torch.tensor(list(src), dtype=torch.int32)
+    dst = dst if isinstance(dst, torch.Tensor) else torch.tensor(list(dst), dtype=torch.int32)
+    if src.dim() != 1 or src.shape != dst.shape:
+        raise ValueError(f"src_pages and dst_pages must be lists of one length (got {tuple(src.shape)}, "
+                         f"{tuple(dst.shape)})")
+    s, d = (None if t.is_cuda else t.tolist() for t in (src, dst))
+    for pages in (s, d):
+        if pages is not None and any(not 0 <= p < num_pages for p in pages):
+            raise ValueError(f"page outside [0, {num_pages})")
+    if d is not None and len(set(d)) != len(d):
+        raise ValueError("a page is the destination of two copies")
+    if s is not None and d is not None:
+        to = dict(zip(d, s))  # (a page copied onto itself stays as it is)
+        if any(to.get(a, a) != a for a in s):
+            raise ValueError("a page is the destination of one copy and the source of another")
+    return _int32(src, device), _int32(dst, device)
+
+
+def copy_kv_pages(K_cache: torch.Tensor, V_cache: torch.Tensor, src_pages: _Pages, dst_pages: _Pages) -> None:
+    """Copy whole pages inside a cache, in place and in every layer: page
+    dst_pages[i] takes page src_pages[i] of K and of V (the shared last page of a
+    forked sequence, pages gathered to free others).
+
+    K_cache, V_cache: [layers, pages, page_size, Hkv, D] or one layer's [pages,
+    page_size, Hkv, D].  The copies run side by side, so no page may be the
+    destination of two or the destination of one and the source of another:
+    lists on the host are checked for that (ValueError); of lists on the GPU,
+    pairs with a page outside the cache are passed over, the rest is the
+    caller's to keep."""
+    _check_caches(K_cache, V_cache, (4, 5))
+    device = _require_device(K_cache, V_cache)
+    _no_grad(K_cache, V_cache)
+    num_pages, page_size, Hkv, D = K_cache.shape[-4:]
+    src, dst = _page_lists(src_pages, dst_pages, num_pages, device)
+    if not src.shape[0] or not K_cache.numel():
+        return
+    layers, ks = _layered(K_cache)
+    with _on(device):
+        rc = _lib.lib().qattn_kv_copy_pages(
+            K_cache.data_ptr(), ks, V_cache.data_ptr(), _layered(V_cache)[1], layers, num_pages, page_size,
+            src.data_ptr(), dst.data_ptr(), src.shape[0], Hkv, D, _dtype_code(K_cache), _stream(device))
+    _lib.check(rc, "qattn_kv_copy_pages")

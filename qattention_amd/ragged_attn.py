@@ -94,6 +94,12 @@ def _require_device(*ts):
     return dev
 
 
+def _no_grad(*ts) -> None:
+    """Refuse tensors that ask for gradients where there is no backward pass."""
+    if torch.is_grad_enabled() and any(t.requires_grad for t in ts):
+        raise RuntimeError("this call has no backward pass: use torch.no_grad() or detach its inputs")
+
+
 def _stream(device) -> int:
     _lib.ensure_init(device)
     # (the handle alone: torch.cuda.current_stream builds a Stream object, 1.5 us)
@@ -659,6 +665,52 @@ def ragged_tree_attn(
             _lib.ptr(par), par_stride, B, N, L, Hq, Hkv, D, int(branching_factor), int(max_depth),
             1.0 / math.sqrt(D), _dtype_code(Q), ws.data_ptr(), ws_bytes, int(num_splits), _stream(device))
     _lib.check(rc, "qattn_ragged_tree_attn_fwd")
+    return (O, LSE) if return_lse else O
+
+
+def prompt_attention(
+    Q: torch.Tensor,
+    K: torch.Tensor,
+    V: torch.Tensor,
+    cu_seqlens: torch.Tensor,
+    max_seqlen: int = None,
+    return_lse: bool = False,
+):
+    """Causal attention within packed prompts: token x of a sequence attends
+    tokens 0 .. x of it.
+
+    Q: packed [sum L_i, Hq, D] fp16/bf16; K, V: [sum L_i, Hkv, D], Hkv dividing
+    Hq; cu_seqlens and max_seqlen as in ragged_attention.  What later tokens'
+    rows hold, infinities and NaN included, never reaches a token.  Rows of no
+    sequence are not computed.  With return_lse its output merges with an earlier
+    chunk's context (prefix_attention, prefix_attention_paged) through
+    fused_lse_merge.  Serves inference: tensors that ask for gradients are
+    refused while autograd records.  Returns O [sum L_i, Hq, D] (and LSE
+    [sum L_i, Hq] fp32, natural log, if return_lse)."""
+    _check_dtypes(Q, K, V)
+    device = _require_device(Q, K, V)
+    _no_grad(Q, K, V)
+    if Q.dim() != 3 or K.dim() != 3 or V.dim() != 3:
+        raise ValueError(f"expected packed [T, H, D] tensors (got {tuple(Q.shape)}, {tuple(K.shape)}, "
+                         f"{tuple(V.shape)})")
+    T, Hq, Hkv, D = _heads(Q, K, V)
+    if K.shape[0] != T or V.shape[0] != T:
+        raise ValueError("packed Q, K, V must have the same number of tokens")
+    B = int(cu_seqlens.shape[0]) - 1
+    ms, cu_dev = _seqlens(cu_seqlens, B, device, max_seqlen)
+    Q, K, V = _vec(Q), _vec(K), _vec(V)
+    O = torch.empty_like(Q)
+    if not _vec_ok(O):
+        O = torch.empty(Q.shape, dtype=Q.dtype, device=device)
+    LSE = torch.empty(T, Hq, dtype=torch.float32, device=device) if return_lse else None
+    L = _lib.lib()
+    with _on(device):
+        rc = L.qattn_prompt_fwd(
+            Q.data_ptr(), _lib.i64arr(Q.stride()), K.data_ptr(), _lib.i64arr(K.stride()),
+            V.data_ptr(), _lib.i64arr(V.stride()), O.data_ptr(), _lib.i64arr(O.stride()), _lib.ptr(LSE),
+            _lib.i64arr(LSE.stride()) if LSE is not None else None, cu_dev.data_ptr(), B, ms, T, Hq, Hkv, D,
+            1.0 / math.sqrt(D), _dtype_code(Q), _stream(device))
+    _lib.check(rc, "qattn_prompt_fwd")
     return (O, LSE) if return_lse else O
 
 

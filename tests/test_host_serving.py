@@ -1,0 +1,182 @@
+"""Refusals of the serving calls, on the CPU: nothing is launched."""
+from __future__ import annotations
+
+import ctypes as C
+
+import pytest
+import torch
+
+import qattention_amd as qa
+from qattention_amd import _lib, paged_kv
+
+ARG, DTYPE, HEAD_DIM, LAYOUT, WORKSPACE = -1, -2, -3, -4, -5
+
+
+def i64(*v):
+    return (C.c_int64 * len(v))(*v)
+
+
+def test_exports():
+    import src.ragged_attn as sra
+    for name in ("prompt_attention", "prefix_attention_paged", "append_paged_kv", "compact_paged_kv", "copy_kv_pages"):
+        assert getattr(sra, name) is getattr(qa, name)
+
+
+def prompt(q=16, k=16, v=16, o=16, qs=(512, 128, 1), ks=(256, 128, 1), cu=16, B=1, ms=8, T=8, Hq=4, Hkv=2, D=128,
+           scale=0.1, dtype=0, lse=None):
+    return _lib.lib().qattn_prompt_fwd(q, i64(*qs), k, i64(*ks), v, i64(*ks), o, i64(*qs), lse, None, cu, B, ms, T, Hq,
+                                       Hkv, D, scale, dtype, None)
+
+
+@pytest.mark.parametrize("rc,kw", [
+    (DTYPE, dict(dtype=2)), (HEAD_DIM, dict(D=96)), (ARG, dict(Hq=5)), (ARG, dict(B=-1)), (ARG, dict(T=1 << 31)),
+    (ARG, dict(scale=0.0)), (ARG, dict(scale=float("nan"))), (ARG, dict(scale=float("inf"))), (ARG, dict(q=None)),
+    (ARG, dict(cu=None)), (ARG, dict(lse=16)), (LAYOUT, dict(q=18)), (LAYOUT, dict(qs=(512, 127, 1))),
+    (LAYOUT, dict(ks=(256, 128, 2))), (LAYOUT, dict(ks=(1 << 25, 128, 1))), (0, dict(B=0)), (0, dict(ms=0)),
+    (0, dict(T=0)),
+])
+def test_prompt_abi(rc, kw):
+    assert prompt(**kw) == rc
+    assert rc == 0 or _lib.last_error()
+
+
+def paged(q=16, kc=16, vc=16, o=16, qs=(512, 128, 1), cs=(4096, 256, 128, 1), table=16, cols=4, pages=8, ps=16,
+          ctx=16, cu=16, B=1, ms=8, T=8, Hq=4, Hkv=2, D=128, scale=0.1, dtype=0, ws=256, ws_bytes=1 << 40, lse=None):
+    return _lib.lib().qattn_prefix_paged_fwd(
+        q, i64(*qs), kc, i64(*cs), vc, i64(*cs), table, cols, pages, ps, ctx, o, i64(*qs), lse, None, cu, B, ms, T, Hq,
+        Hkv, D, scale, dtype, ws, ws_bytes, None)
+
+
+@pytest.mark.parametrize("rc,kw", [
+    (DTYPE, dict(dtype=3)), (HEAD_DIM, dict(D=256)), (ARG, dict(Hq=3)), (ARG, dict(ps=0)), (ARG, dict(cols=-1)),
+    (ARG, dict(pages=-1)), (ARG, dict(cols=1 << 27)), (ARG, dict(scale=-1.0)), (ARG, dict(ctx=None)),
+    (ARG, dict(table=None)), (ARG, dict(kc=None)), (ARG, dict(lse=16)), (LAYOUT, dict(o=8)),
+    (LAYOUT, dict(cs=(4096, 255, 128, 1))), (LAYOUT, dict(cs=(-4096, 256, 128, 1))),
+    (LAYOUT, dict(cs=(1 << 35, 256, 128, 1))), (WORKSPACE, dict(ws=None)), (WORKSPACE, dict(ws=264)),
+    (WORKSPACE, dict(ws_bytes=100)), (0, dict(B=0)), (0, dict(T=0)), (0, dict(ms=0)),
+])
+def test_paged_abi(rc, kw):
+    assert paged(**kw) == rc
+    assert rc == 0 or _lib.last_error()
+
+
+def test_paged_workspace():
+    ws = _lib.lib().qattn_prefix_paged_workspace_bytes
+    assert ws(0, 1, 0, 32, 8, 128, 10, 16) == 0 and ws(4, 1, 4, 32, 7, 128, 10, 16) == 0
+    small, large = ws(1, 1, 1, 32, 8, 128, 8, 16), ws(64, 1, 64, 32, 8, 128, 1000, 16)
+    assert 0 < small < large < 64 << 20
+    # it does not grow with the table past what the launch can share out
+    assert ws(64, 1, 64, 32, 8, 128, 8000, 16) == large
+
+
+def pages_call(which, kc=16, vc=16, cs=(32768, 4096, 256, 128, 1), layers=2, table=16, cols=4, pages=8, ps=16, ctx=16,
+               acc=16, pcols=4, new=16, B=2, Hkv=2, D=128, dtype=0, k=16, ks=(256, 128, 1), cu=16, ms=4, T=8, n=3):
+    L = _lib.lib()
+    if which == "append":
+        return L.qattn_kv_append(k, i64(*ks), k, i64(*ks), kc, i64(*cs[1:]), vc, i64(*cs[1:]), table, cols, pages, ps,
+                                 ctx, new, cu, B, ms, T, Hkv, D, dtype, None)
+    if which == "compact":
+        return L.qattn_kv_compact(kc, i64(*cs), vc, i64(*cs), layers, table, cols, pages, ps, ctx, acc, pcols, new, B,
+                                  Hkv, D, dtype, None)
+    return L.qattn_kv_copy_pages(kc, i64(*cs), vc, i64(*cs), layers, pages, ps, acc, acc, n, Hkv, D, dtype, None)
+
+
+@pytest.mark.parametrize("which", ["append", "compact", "copy"])
+@pytest.mark.parametrize("rc,kw", [
+    (DTYPE, dict(dtype=7)), (HEAD_DIM, dict(D=80)), (ARG, dict(Hkv=0)), (ARG, dict(ps=0)), (ARG, dict(pages=-1)),
+    (ARG, dict(kc=None)), (LAYOUT, dict(vc=24)), (LAYOUT, dict(cs=(32768, 4096, 250, 128, 1))),
+    (LAYOUT, dict(cs=(32768, 4096, 256, 128, 2))), (ARG, dict(ps=1 << 28)),
+])
+def test_pages_abi(which, rc, kw):
+    assert pages_call(which, **kw) == rc and _lib.last_error()
+
+
+@pytest.mark.parametrize("which,rc,kw", [
+    ("append", ARG, dict(B=-1)), ("append", ARG, dict(cols=1 << 27)), ("append", ARG, dict(ctx=None)),
+    ("append", ARG, dict(new=None)), ("append", ARG, dict(table=None)), ("append", ARG, dict(ms=-1)),
+    ("append", ARG, dict(T=1 << 31)), ("append", ARG, dict(k=None)), ("append", LAYOUT, dict(ks=(255, 128, 1))),
+    ("append", 0, dict(B=0)),
+    ("compact", ARG, dict(pcols=-1)), ("compact", ARG, dict(acc=None)), ("compact", ARG, dict(layers=0)),
+    ("compact", ARG, dict(new=None)), ("compact", 0, dict(B=0)),
+    ("copy", ARG, dict(n=-1)), ("copy", ARG, dict(acc=None)), ("copy", 0, dict(n=0)), ("copy", 0, dict(layers=0)),
+])
+def test_pages_abi_own(which, rc, kw):
+    assert pages_call(which, **kw) == rc
+
+
+def T(*shape, dtype=torch.float16):
+    return torch.zeros(*shape, dtype=dtype)
+
+
+def test_cpu_tensors_fail_loudly():
+    cu = torch.tensor([0, 4], dtype=torch.int32)
+    cache, table, lens = (T(3, 16, 2, 64), T(3, 16, 2, 64)), torch.zeros(1, 2, dtype=torch.int32), cu[1:]
+    with pytest.raises(RuntimeError, match="GPU only"):
+        qa.prompt_attention(T(4, 4, 64), T(4, 2, 64), T(4, 2, 64), cu)
+    with pytest.raises(RuntimeError, match="GPU only"):
+        qa.prefix_attention_paged(T(1, 4, 64), *cache, table, lens)
+    with pytest.raises(RuntimeError, match="GPU only"):
+        qa.append_paged_kv(T(1, 2, 64), T(1, 2, 64), *cache, table, lens)
+    with pytest.raises(RuntimeError, match="GPU only"):
+        qa.compact_paged_kv(*cache, table, lens, table)
+    with pytest.raises(RuntimeError, match="GPU only"):
+        qa.copy_kv_pages(*cache, [0], [1])
+
+
+def test_types_and_caches():
+    cu = torch.tensor([0, 4], dtype=torch.int32)
+    with pytest.raises(AssertionError, match="fp16 or bf16"):
+        qa.prompt_attention(T(4, 4, 64, dtype=torch.float32), T(4, 2, 64), T(4, 2, 64), cu)
+    chk = paged_kv._check_caches
+    good = T(3, 16, 2, 64)
+    with pytest.raises(ValueError, match="one shape"):
+        chk(good, T(3, 16, 2, 32), (4,))
+    with pytest.raises(ValueError, match="4-D"):
+        chk(T(1, 3, 16, 2, 64), T(1, 3, 16, 2, 64), (4,))
+    with pytest.raises(AssertionError, match="fp16 or bf16"):
+        chk(good, good.bfloat16(), (4,))
+    with pytest.raises(ValueError, match="16-byte rows"):
+        chk(good, T(3, 16, 2, 65)[..., 1:], (4,))
+    with pytest.raises(ValueError, match="overlap"):
+        chk(good, T(1, 16, 2, 64).expand(3, 16, 2, 64), (4,))
+    with pytest.raises(ValueError, match="same memory"):
+        chk(good, good, (4,))
+    chk(good, T(3, 16, 2, 64), (4,))
+
+
+def test_row_offsets():
+    rows, lens = paged_kv._rows, torch.tensor([0, 2, 3], dtype=torch.int32)
+    with pytest.raises(ValueError, match="one row per sequence"):
+        rows(3, 2, None, None, "cpu")
+    with pytest.raises(ValueError, match="must have 4 entries"):
+        rows(3, 3, lens, None, "cpu")
+    assert rows(2, 2, None, None, "cpu") == (1, None) and rows(3, 2, lens, None, "cpu")[0] == 2
+    with pytest.raises(ValueError, match="B >= 3"):
+        paged_kv._table(torch.zeros(2, 4), 3, "cpu")
+    with pytest.raises(ValueError, match=r"must be \[B\]"):
+        paged_kv._lengths(torch.zeros(2, 4), "cpu")
+
+
+@pytest.mark.parametrize("src,dst,what", [
+    ([0, 1], [2], "one length"), ([0, 9], [1, 2], "outside"), ([0, -1], [1, 2], "outside"), ([0, 1], [2, 9], "outside"),
+    ([0, 1], [2, 2], "two copies"), ([0, 2], [2, 3], "source of another"), ([1, 2], [2, 1], "source of another"),
+])
+def test_page_lists(src, dst, what):
+    with pytest.raises(ValueError, match=what):
+        paged_kv._page_lists(src, dst, 8, "cpu")
+
+
+def test_page_lists_taken():
+    for src, dst in (([0, 0, 3], [1, 2, 3]), ([], []), (torch.tensor([4]), [5])):
+        a, b = paged_kv._page_lists(src, dst, 8, "cpu")
+        assert a.tolist() == list(src) and b.tolist() == list(dst) and a.dtype == b.dtype == torch.int32
+
+
+def test_gradients_refused():
+    from qattention_amd.ragged_attn import _no_grad
+    x = torch.zeros(2, requires_grad=True)
+    with pytest.raises(RuntimeError, match="no backward pass"):
+        _no_grad(torch.zeros(2), x)
+    _no_grad(torch.zeros(2))
+    with torch.no_grad():
+        _no_grad(x)
