@@ -20,7 +20,7 @@ LIB_PATH = os.path.join(PKG_DIR, "libqattn.so")
 OBJ_DIR = os.path.join(PKG_DIR, "_build")
 SOURCES = ["tree_attn.hip", "subtree_stream.hip", "prefix_attn.hip", "paged_attn.hip", "prompt_attn.hip",
            "kv_pages.hip"]
-HEADERS = ["qattn_common.h", "qattn_device.h", "kv_tiles.h", "tree_walk.h"]
+HEADERS = ["qattn_common.h", "qattn_device.h", "kv_tiles.h", "dense_tiles.h", "tree_walk.h"]
 ARCH = os.environ.get("QATTN_ARCH", "gfx950")
 
 

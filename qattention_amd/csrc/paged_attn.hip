@@ -6,33 +6,40 @@
 //   o = sum_j softmax_j(scale q.k_j) v_j,  lse = m + ln sum_j exp(s_j - m)
 // in one pass with a running maximum m and sum l.
 //
-// Work: units of 128 keys of one (sequence, kv head, tile of 16 QB rows),
-// numbered sequence by sequence, heads, tiles and keys innermost.  The
-// workgroups of the launch take equal runs of all units, whatever the
-// contexts' lengths (no host knows them: the lengths stay on the device), so a
-// run may end inside an item.  A run's whole items are finished in the
-// workgroup; of a cut item every part leaves its state (m, l, numerator, fp32)
-// in the workspace and paged_merge_kernel joins them in key order, without
-// atomics: results do not depend on timing.
+// Work: units of 64 or 128 keys of one (sequence, kv head, row tile), numbered
+// sequence by sequence, heads, tiles and keys innermost.  The workgroups of the
+// launch take equal runs of all units, whatever the contexts' lengths (no host
+// knows them: the lengths stay on the device), so a run may end inside an item.
+// A run's whole items are finished in the workgroup; of a cut item every part
+// leaves its state (m, l, numerator, fp32) in the workspace and
+// paged_merge_kernel joins them in key order, without atomics: results do not
+// depend on timing.
 //
-// A unit's 128 keys are 32 per wave.  Per step a wave forms
-//   S^T = K Q^T      2 key tiles x D/32 products of v_mfma_f32_16x16x32
-//   O^T += V^T P^T   D/16 products
-// with K rows loaded from the cache straight into the A operand's layout and
-// V rows through a wave-private LDS block that the transposing reads
-// (ds_read_b64_tr_b16) take as V^T; S^T has one row (query) per lane column,
-// and its registers are the P^T operand.  The loads of the next step are
-// requested before the products of this one; page numbers one step earlier.
+// Two kernels by the longest sequence's rows:
+//   up to 32 (paged_attn_kernel): per step a wave forms, for 32 keys of its own,
+//     S^T = K Q^T      2 key tiles x D/32 products of v_mfma_f32_16x16x32
+//     O^T += V^T P^T   D/16 products
+//   with K rows loaded from the cache straight into the A operand's layout and
+//   V rows through a wave-private LDS block that the transposing reads
+//   (ds_read_b64_tr_b16) take as V^T; S^T has one row (query) per lane column,
+//   and its registers are the P^T operand.  The loads of the next step are
+//   requested before the products of this one; page numbers one step earlier.
+//   more (paged_wide_kernel): tiles of 128 rows share K/V blocks of 64 keys in
+//   LDS (dense_tiles.h).
 #include <algorithm>
 
-#include "kv_tiles.h"
+#include "dense_tiles.h"
 #include "qattn_common.h"
 #include "qattn_device.h"
 
 namespace qattn {
 
 constexpr int kPagedThreads = 256;
-constexpr int kUnit = 128;  // keys per unit: 4 waves x 32
+
+// Waves per SIMD of the narrow kernel: two, but one with 128-wide heads from 32
+// rows on, whose accumulators, K operand and loads in flight take the registers
+// of both.
+constexpr int narrow_waves(int d, int qb) { return d == 128 && qb > 1 ? 1 : 2; }
 
 struct PagedParams {
     const uint16_t* q;
@@ -49,25 +56,22 @@ struct PagedParams {
     int32_t B, Hq, Hkv, group, max_seqlen;
     int32_t pt_cols, num_pages, page_size, capacity;
     int32_t nwg;          // workgroups that share the units (a multiple of 8)
-    int32_t slots;        // rows of one workspace state: 16 QB
+    int32_t least;        // units that are worth a workgroup
     Divider pdiv, gdiv;   // page_size, group
     float scale_log2;
-    int64_t* base;        // [B + 1] first unit of each sequence (written by the main kernel)
-    float* part_m;        // [nwg][2][slots]
+    int32_t* base;        // [B + 1] first unit of each sequence (written by the main kernel)
+    float* part_m;        // [nwg][2][rows of a tile], in log2 units
     float* part_l;
-    float* part_acc;      // [nwg][2][slots][D]
+    float* part_acc;      // [nwg][2][rows of a tile][D]
 };
 
-// Waves per SIMD: two, but one with 128-wide heads from 32 rows on, whose
-// accumulators, K operand and loads in flight take the registers of both.
-constexpr int paged_waves(int d, int qb) { return d == 128 && qb > 1 ? 1 : 2; }
-
-// Rows, tiles and units of a sequence.
+// Rows and blocks of a sequence; unit (kv head, tile, block) of it is number
+// (kvh * tiles + tile) * blocks + block.
 struct SeqWork {
     int32_t s0, rows, tiles, ctx, blocks;
-    __device__ __forceinline__ int64_t units(int hkv) const { return (int64_t)hkv * tiles * blocks; }
+    __device__ __forceinline__ int32_t units(int hkv) const { return hkv * tiles * blocks; }
 };
-template <int QB>
+template <int ROWS, int KEYS>
 __device__ __forceinline__ SeqWork seq_work(const PagedParams& p, int s) {
     SeqWork w;
     w.s0 = p.cu ? p.cu[s] : s;
@@ -76,115 +80,161 @@ __device__ __forceinline__ SeqWork seq_work(const PagedParams& p, int s) {
     if (w.s0 < 0 || s1 < w.s0 || (int64_t)s1 > p.total_tokens) n = 0;
     n = min(n, p.max_seqlen);
     w.rows = n * p.group;
-    w.tiles = (w.rows + 16 * QB - 1) / (16 * QB);
+    w.tiles = (w.rows + ROWS - 1) / ROWS;
     w.ctx = max(0, min(p.ctx[s], p.capacity));
-    w.blocks = (w.ctx + kUnit - 1) / kUnit;
+    w.blocks = (w.ctx + KEYS - 1) / KEYS;
     return w;
 }
 
-// Workgroups that take units, and the first unit of workgroup w of them.
-__device__ __forceinline__ int64_t run_first(int64_t total, int nwg, int w) { return total * w / nwg; }
-__device__ __forceinline__ int runs_of(int64_t total, int nwg) { return (int)(total < nwg ? total : nwg); }
+// Equal runs of the units: run w starts at first(w).  (The host checks that
+// the units of the longest contexts stay below 2^31.)
+struct Runs {
+    int32_t n, q, rem;
+    __device__ __forceinline__ Runs(int32_t total, int nwg, int least) {
+        n = max(1, min(nwg, total / least));
+        q = (int32_t)((uint32_t)total / (uint32_t)n);
+        rem = total - q * n;
+    }
+    __device__ __forceinline__ int32_t first(int w) const { return w * q + min(w, rem); }
+    __device__ __forceinline__ int of(int32_t unit) const {
+        const int32_t big = rem * (q + 1);
+        return unit < big ? (int)((uint32_t)unit / (uint32_t)(q + 1)) : rem + (int)((uint32_t)(unit - big) / (uint32_t)q);
+    }
+};
+
+// This workgroup's run [u, end): the sequence that holds u and its first unit.
+// Workgroup 0 leaves the sequences' first units to the merge.  Every thread
+// calls it; false: no unit.
+struct Share {
+    int32_t u, end, start, seq, seq_base;
+};
+template <int ROWS, int KEYS>
+__device__ __forceinline__ bool find_share(const PagedParams& p, Share& sh) {
+    __shared__ int32_t sums[4];
+    __shared__ int32_t found[2];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    // consecutive runs on one XCD: tiles of one item share its L2
+    const int per = gridDim.x >> 3;
+    const int wg = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+    // exclusive prefix of `mine` over the workgroup, and the sum
+    auto scan = [&](int32_t mine, int32_t& sum) {
+        int32_t inc = mine;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const int32_t up = __shfl_up(inc, d);
+            if (lane >= d) inc += up;
+        }
+        __syncthreads();
+        if (lane == 63) sums[wave] = inc;
+        __syncthreads();
+        int32_t before = 0;
+        sum = 0;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            before += w < wave ? sums[w] : 0;
+            sum += sums[w];
+        }
+        return before + inc - mine;
+    };
+    int32_t total = 0, mine = 0, excl = 0;
+    for (int c = 0; c < p.B; c += kPagedThreads) {
+        int32_t sum;
+        mine = c + tid < p.B ? seq_work<ROWS, KEYS>(p, c + tid).units(p.Hkv) : 0;
+        excl = total + scan(mine, sum);
+        if (wg == 0 && c + tid < p.B) p.base[c + tid] = excl;
+        total += sum;
+    }
+    total = __builtin_amdgcn_readfirstlane(total);  // (what follows from it stays in scalar registers)
+    if (wg == 0 && tid == 0) p.base[p.B] = total;
+    const Runs runs(total, p.nwg, p.least);
+    if (wg >= runs.n || total == 0) return false;
+    sh.u = sh.start = runs.first(wg);
+    sh.end = runs.first(wg + 1);
+    if (p.B <= kPagedThreads) {
+        if (sh.u >= excl && sh.u < excl + mine) found[0] = tid, found[1] = excl;
+    } else {
+        int32_t before = 0;
+        for (int c = 0; c < p.B; c += kPagedThreads) {
+            int32_t sum;
+            mine = c + tid < p.B ? seq_work<ROWS, KEYS>(p, c + tid).units(p.Hkv) : 0;
+            excl = before + scan(mine, sum);
+            if (sh.u >= excl && sh.u < excl + mine) found[0] = c + tid, found[1] = excl;
+            before += sum;
+        }
+    }
+    __syncthreads();
+    sh.seq = __builtin_amdgcn_readfirstlane(found[0]);
+    sh.seq_base = __builtin_amdgcn_readfirstlane(found[1]);
+    return true;
+}
+
+// Workspace state of the part that starts at the run's unit u: 0 for the run's
+// first part, 1 for another (its last: parts in between are whole items).
+__device__ __forceinline__ int64_t part_slot(const Share& sh) {
+    const int per = gridDim.x >> 3;
+    return 2 * (int64_t)((blockIdx.x & 7) * per + (blockIdx.x >> 3)) + (sh.u == sh.start ? 0 : 1);
+}
+
+// The part of an item that starts at the run's unit u: blocks b0 .. b1 - 1 of
+// (seq, kvh, tile); moves the share on to it and returns the sequence's work.
+struct Part {
+    int32_t kvh, tile, b0, b1;
+    bool whole;
+};
+template <int ROWS, int KEYS>
+__device__ __forceinline__ SeqWork next_part(const PagedParams& p, Share& sh, Part& part) {
+    SeqWork sw = seq_work<ROWS, KEYS>(p, sh.seq);
+    while (sh.u >= sh.seq_base + sw.units(p.Hkv)) {  // (empty sequences are passed over)
+        sh.seq_base += sw.units(p.Hkv);
+        sw = seq_work<ROWS, KEYS>(p, ++sh.seq);
+    }
+    const uint32_t in = (uint32_t)(sh.u - sh.seq_base);
+    const uint32_t item = in / (uint32_t)sw.blocks;
+    part.b0 = (int32_t)(in - item * (uint32_t)sw.blocks);
+    part.kvh = (int32_t)(item / (uint32_t)sw.tiles);
+    part.tile = (int32_t)(item - (uint32_t)part.kvh * (uint32_t)sw.tiles);
+    part.b1 = min(sw.blocks, part.b0 + (sh.end - sh.u));
+    part.whole = part.b0 == 0 && part.b1 == sw.blocks;
+    return sw;
+}
+
+// ---------------------------------------------------------------------------
+// Few rows (16 QB per tile): bound by reading the cache.  A unit's 128 keys are
+// 32 per wave; nothing is shared between the waves but the last join.
+// ---------------------------------------------------------------------------
+constexpr int kUnit = 128;
 
 template <typename T, int D, int QB>
 __global__ __launch_bounds__(kPagedThreads)
-    __attribute__((amdgpu_waves_per_eu(paged_waves(D, QB)))) void paged_attn_kernel(PagedParams p) {
+    __attribute__((amdgpu_waves_per_eu(narrow_waves(D, QB)))) void paged_attn_kernel(PagedParams p) {
     constexpr int NC = D / 32;     // k-steps of S^T over the head dim
     constexpr int ND = D / 16;     // d-tiles of O^T
     constexpr int DV = D / 8;      // 16-byte chunks per row
     constexpr int RPI = 512 / D;   // V rows per load instruction of a wave
     constexpr int NV = 32 / RPI;   // V loads per lane and step
     constexpr int WBLK = 32 * D;   // elements of a wave's V block
+    constexpr int ROWS = 16 * QB;
     // The waves' V blocks; after the key loop, the waves' numerators of one
     // row block (4 x 16 rows x D floats, the same size).
     __shared__ __attribute__((aligned(1024))) uint16_t vlds[4 * WBLK];
-    __shared__ float ml[2][4][16 * QB];
-    __shared__ int64_t scan[4];
-    __shared__ int found_seq;
-    __shared__ int64_t found_base;
+    __shared__ float ml[2][4][ROWS];
 
+    Share sh;
+    if (!find_share<ROWS, kUnit>(p, sh)) return;
     const int tid = threadIdx.x;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int lane = tid & 63;
     const int l16 = lane & 15, lq = lane >> 4;
-    // consecutive runs on one XCD: tiles of one item share its L2
-    const int per = gridDim.x >> 3;
-    const int wg = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
-
-    // ---- units of every sequence: their sum, then the sequence that holds
-    // this run's first unit.  Workgroup 0 leaves the table to the merge. ----
-    auto chunk_scan = [&](int s, int64_t& sum) {  // exclusive prefix within the chunk, and its sum
-        const int64_t mine = s < p.B ? seq_work<QB>(p, s).units(p.Hkv) : 0;
-        int64_t inc = mine;
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const int64_t up = __shfl_up(inc, d);
-            if (lane >= d) inc += up;
-        }
-        __syncthreads();
-        if (lane == 63) scan[wave] = inc;
-        __syncthreads();
-        int64_t before = 0;
-        sum = 0;
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-            before += w < wave ? scan[w] : 0;
-            sum += scan[w];
-        }
-        return before + inc - mine;
-    };
-    int64_t total = 0, excl0 = 0;
-    for (int c = 0; c < p.B; c += kPagedThreads) {
-        int64_t sum;
-        const int64_t e = chunk_scan(c + tid, sum);
-        if (c == 0) excl0 = e;
-        if (wg == 0 && c + tid < p.B) p.base[c + tid] = total + e;
-        total += sum;
-    }
-    if (wg == 0 && tid == 0) p.base[p.B] = total;
-    const int nrun = runs_of(total, p.nwg);
-    if (wg >= nrun) return;
-    int64_t u = run_first(total, nrun, wg);
-    const int64_t u_end = run_first(total, nrun, wg + 1);
-    {
-        int64_t before = 0;
-        for (int c = 0; c < p.B; c += kPagedThreads) {
-            int64_t sum;
-            const bool one = p.B <= kPagedThreads;
-            const int64_t e = one ? excl0 : before + chunk_scan(c + tid, sum);
-            const int s = c + tid;
-            if (s < p.B) {
-                const int64_t mine = seq_work<QB>(p, s).units(p.Hkv);
-                if (u >= e && u < e + mine) {
-                    found_seq = s;
-                    found_base = e;
-                }
-            }
-            if (!one) before += sum;
-        }
-        __syncthreads();
-    }
-    int seq = __builtin_amdgcn_readfirstlane(found_seq);
-    int64_t seq_base = found_base;
 
     // wave-private V block: chunk c of row r at c ^ kv_swz(r)
     uint16_t* const vblk = vlds + wave * WBLK;
     const int vr = 4 * lq + (l16 >> 2);
     const int vaddr0 = vr * D + 8 * (((l16 & 3) >> 1) ^ kv_swz(vr, DV)) + 4 * (l16 & 1);
 
-    while (u < u_end) {
-        SeqWork sw = seq_work<QB>(p, seq);
-        while (u >= seq_base + sw.units(p.Hkv)) {  // (empty sequences are passed over)
-            seq_base += sw.units(p.Hkv);
-            sw = seq_work<QB>(p, ++seq);
-        }
-        const int64_t in = u - seq_base;
-        const int item = (int)(in / sw.blocks);  // kv head * tiles + tile
-        const int b0 = (int)(in - (int64_t)item * sw.blocks);
-        const int kvh = item / sw.tiles;
-        const int tile = item - kvh * sw.tiles;
-        const int b1 = (int)min((int64_t)sw.blocks, b0 + (u_end - u));
-        const int ctx = sw.ctx;
+    while (sh.u < sh.end) {
+        Part part;
+        const SeqWork sw = next_part<ROWS, kUnit>(p, sh, part);
+        const int seq = sh.seq, kvh = part.kvh, tile = part.tile, b0 = part.b0, b1 = part.b1, ctx = sw.ctx;
 
         auto query_of = [&](int r, int64_t& qrow, int& qh) {
             const int rr = tile * 16 * QB + r;
@@ -360,8 +410,7 @@ __global__ __launch_bounds__(kPagedThreads)
                 ml[1][wave][16 * q + l16] = l_run[q];
             }
         }
-        const bool whole = b0 == 0 && b1 == sw.blocks;
-        const int64_t slot = 2 * (int64_t)wg + (u == run_first(total, nrun, wg) ? 0 : 1);
+        const int64_t slot = part_slot(sh);
         float4* const os = reinterpret_cast<float4*>(vlds);  // [4 waves][16 rows][D / 4], float4 c of row r at c ^ (r & 7)
         constexpr int C4 = D / 4;
 #pragma unroll
@@ -390,14 +439,14 @@ __global__ __launch_bounds__(kPagedThreads)
                 int64_t qrow;
                 int qh;
                 if (query_of(16 * q + row, qrow, qh)) {
-                    if (whole) {
+                    if (part.whole) {
                         const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
 #pragma unroll
                         for (int j = 0; j < 8; ++j) acc[j] *= inv;
                         st16(p.o + qrow * p.so_t + qh * p.so_h + 8 * ch, pack8<T>(acc));
                         if (p.lse && ch == 0) p.lse[qrow * p.sl_t + qh * p.sl_h] = (mc + fast_log2(l)) * kLn2;
                     } else {
-                        const int64_t r = slot * p.slots + 16 * q + row;
+                        const int64_t r = slot * ROWS + 16 * q + row;
                         if (ch == 0) {
                             p.part_m[r] = m * p.scale_log2;
                             p.part_l[r] = l;
@@ -410,156 +459,379 @@ __global__ __launch_bounds__(kPagedThreads)
             }
         }
         __syncthreads();  // the LDS is free for the next item
-        u += b1 - b0;
+        sh.u += b1 - b0;
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Many rows (128 per tile): the key loop of dense_tiles.h, the rows of a K/V
+// block found through a table of row offsets in LDS that the workgroup fills
+// for kTable blocks at a time.
+// ---------------------------------------------------------------------------
+constexpr int kWideKeys = 64;
+constexpr int kTable = 24;
+
+struct PageTable {
+    // per block, row r at (r / 16, r % RPI, r % 16 / RPI): the NI rows that a
+    // lane loads lie next to each other
+    uint32_t k[kTable][kWideKeys], v[kTable][kWideKeys];  // in 16-byte units
+    uint64_t have[kTable];                                // bit r: key r exists
+};
+
+template <typename T, int D>
+struct PagedKeys {
+    using Tile = DenseTile<T, D>;
+    static constexpr bool kEveryBlock = true;
+    static constexpr int NI = Tile::NI, RPI = Tile::RPI, DV = Tile::DV, BLK = Tile::BLK;
+    const PageTable* tab;
+    const char *kbase, *vbase;
+    int nb;             // blocks in the table
+    uint32_t bad;       // blocks with a key that does not exist
+    uint32_t colb, lds0, at;
+    int wave;
+
+    // Fills the table with blocks b0 .. b0 + n - 1 of the sequence.
+    __device__ __forceinline__ PagedKeys(const PagedParams& p, PageTable& t, const int32_t* pages, int ctx, int kvh,
+                                         int b0, int n, const uint16_t* smem)
+        : tab(&t), nb(n) {
+        const int lane = threadIdx.x & 63;
+        wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        kbase = (const char*)(p.kc + (int64_t)kvh * p.sk_head);
+        vbase = (const char*)(p.vc + (int64_t)kvh * p.sv_head);
+        colb = 16 * ((lane % DV) ^ kv_swz32(wave * NI * RPI + lane / DV, DV));
+        at = (wave * RPI + lane / DV) * NI;
+        lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void*)smem + wave * (NI * 1024);
+        const int place = ((lane / 16) * RPI + lane % RPI) * NI + lane % 16 / RPI;
+        __syncthreads();  // the table's and the buffers' last readers are done
+        for (int i = wave; i < n; i += 4) {
+            const int pos = (b0 + i) * kWideKeys + lane;
+            int page = -1;
+            const int col = divide(pos, p.pdiv);
+            if (pos < ctx) page = pages[col];
+            const int slot = pos - col * p.page_size;
+            const bool ok = (uint32_t)page < (uint32_t)p.num_pages;
+            // (keys that do not exist read the cache's first row)
+            t.k[i][place] = ok ? (uint32_t)((page * p.sk_page + slot * p.sk_slot) >> 3) : 0u;
+            t.v[i][place] = ok ? (uint32_t)((page * p.sv_page + slot * p.sv_slot) >> 3) : 0u;
+            const uint64_t have = __ballot(ok);
+            if (lane == 0) t.have[i] = have;
+        }
+        __syncthreads();
+        bad = (uint32_t)__ballot(lane < n && t.have[lane < n ? lane : 0] != ~0ull);
+    }
+    struct Offsets {
+        uint32_t x[NI];
+    };
+    __device__ __forceinline__ Offsets rows(const uint32_t (&tab_)[kTable][kWideKeys], int j) const {
+        const uint32_t* r = &tab_[min(j, nb - 1)][at];
+        Offsets o;
+        if constexpr (NI == 4) {
+            const uint4 x = *reinterpret_cast<const uint4*>(r);
+            o.x[0] = x.x, o.x[1] = x.y, o.x[2] = x.z, o.x[3] = x.w;
+        } else if constexpr (NI == 2) {
+            const uint2 x = *reinterpret_cast<const uint2*>(r);
+            o.x[0] = x.x, o.x[1] = x.y;
+        } else {
+            o.x[0] = *r;
+        }
+        return o;
+    }
+    static __device__ __forceinline__ void load(const char* base, uint32_t off, uint32_t col, uint32_t lds) {
+        const uint64_t a = (uint64_t)(uintptr_t)base + ((uint64_t)off << 4) + col;
+        asm volatile("global_load_lds_dwordx4 %0, off" ::"v"(a), "{m0}"(lds) : "memory");
+    }
+    struct Dma {
+        Offsets ko, vo;
+        uint32_t col, ld;
+        const char *gk, *gv;
+        __device__ __forceinline__ void k(int buf, int n) {
+            load(gk, ko.x[n], col ^ (16 * kv_swz32(n * RPI, DV)), ld + 2 * buf * BLK + n * 1024);
+        }
+        __device__ __forceinline__ void v(int buf, int n) {
+            load(gv, vo.x[n], col ^ (16 * kv_swz32(n * RPI, DV)), ld + 2 * (2 + buf) * BLK + n * 1024);
+        }
+    };
+    __device__ __forceinline__ Dma dma(int j) const {
+        Dma d{rows(tab->k, j + 3), rows(tab->v, j + 1), colb, lds0, kbase, vbase};
+        asm volatile("" : "+v"(d.col), "+s"(d.ld));
+        return d;
+    }
+    __device__ __forceinline__ void load_k(int j, uint16_t* buf) const {
+        const Offsets o = rows(tab->k, j);
+#pragma unroll
+        for (int n = 0; n < NI; ++n)
+            load(kbase, o.x[n], colb ^ (16 * kv_swz32(n * RPI, DV)),
+                 (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)(buf + (wave * NI + n) * 512));
+    }
+    __device__ __forceinline__ void load_v(int j, uint16_t* buf) const {
+        const Offsets o = rows(tab->v, j);
+#pragma unroll
+        for (int n = 0; n < NI; ++n)
+            load(vbase, o.x[n], colb ^ (16 * kv_swz32(n * RPI, DV)),
+                 (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)(buf + (wave * NI + n) * 512));
+    }
+    __device__ __forceinline__ void mask(int j, f16v_t (&s)[2]) const {
+        if (__builtin_expect(bad >> j & 1, 0)) {
+            const uint64_t have = tab->have[j] >> (4 * ((threadIdx.x >> 5) & 1));
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    if (!((uint32_t)(have >> (32 * t)) >> (8 * (r >> 2) + (r & 3)) & 1)) s[t][r] = -INFINITY;
+        }
+    }
+    __device__ __forceinline__ void clean(int j, uint16_t* v) const {
+        if (__builtin_expect(bad >> j & 1, 0)) {
+            const uint64_t have = tab->have[j];
+            for (int i = threadIdx.x; i < kWideKeys * DV; i += Tile::kThreads)
+                if (!(have >> (i / DV) & 1)) st16(v + 8 * i, Vec16{{0u, 0u, 0u, 0u}});
+            Tile::template publish<0>();
+        }
+    }
+};
+
+template <typename T, int D>
+__global__ __launch_bounds__(kPagedThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) void paged_wide_kernel(
+    PagedParams p) {
+    using Tile = DenseTile<T, D>;
+    constexpr int KS = Tile::KS, DT = Tile::DT, ROWS = Tile::kBM;
+    __shared__ __attribute__((aligned(1024))) uint16_t smem[Tile::kSmem];
+    __shared__ __attribute__((aligned(16))) PageTable table;
+
+    Share sh;
+    if (!find_share<ROWS, kWideKeys>(p, sh)) return;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63;
+    const int q32 = lane & 31, hl = lane >> 5;
+
+    while (sh.u < sh.end) {
+        Part part;
+        const SeqWork sw = next_part<ROWS, kWideKeys>(p, sh, part);
+        auto query_of = [&](int64_t& qrow, int& qh) {
+            const int rr = part.tile * ROWS + wave * 32 + q32;
+            const int tok = divide(rr, p.gdiv);
+            qh = part.kvh * p.group + (rr - tok * p.group);
+            qrow = (int64_t)sw.s0 + tok;
+            return rr < sw.rows;
+        };
+        Vec16 qf[KS];
+        {
+            int64_t qrow;
+            int qh;
+            const bool valid = query_of(qrow, qh);
+            const uint16_t* qp = p.q + qrow * p.sq_t + qh * p.sq_h + 8 * hl;
+#pragma unroll
+            for (int s = 0; s < KS; ++s) {
+                qf[s] = Vec16{{0u, 0u, 0u, 0u}};
+                if (valid) qf[s] = ld16(qp + 16 * s);
+            }
+        }
+        float m_run = -INFINITY, l_run = 0.f;
+        f16v_t oacc[DT];
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) oacc[dt][r] = 0.f;
+        const bool live = part.tile * ROWS + wave * 32 < sw.rows;
+        for (int b = part.b0; b < part.b1; b += kTable) {
+            const PagedKeys<T, D> src(p, table, p.table + (int64_t)sh.seq * p.pt_cols, sw.ctx, part.kvh, b,
+                                      min(kTable, part.b1 - b), smem);
+            Tile::keys(src, smem, qf, live, src.nb, p.scale_log2, m_run, l_run, oacc);
+        }
+        const float l = xor32_sum(l_run);
+        int64_t qrow;
+        int qh;
+        const bool valid = query_of(qrow, qh);
+        if (part.whole) {
+            const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+            Tile::store_row(oacc, inv, p.o + qrow * p.so_t + qh * p.so_h, valid);
+            if (valid && p.lse && hl == 0)
+                p.lse[qrow * p.sl_t + qh * p.sl_h] = (m_run * p.scale_log2 + fast_log2(l)) * kLn2;
+        } else if (valid) {
+            const int64_t r = part_slot(sh) * ROWS + wave * 32 + q32;
+            if (hl == 0) {
+                p.part_m[r] = m_run * p.scale_log2;
+                p.part_l[r] = l;
+            }
+            float* const acc = p.part_acc + r * D + 4 * hl;
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    *reinterpret_cast<float4*>(acc + 32 * dt + 8 * j) = make_float4(
+                        oacc[dt][4 * j], oacc[dt][4 * j + 1], oacc[dt][4 * j + 2], oacc[dt][4 * j + 3]);
+        }
+        sh.u += part.b1 - part.b0;
     }
 }
 
 // ---------------------------------------------------------------------------
 // Joins the parts of cut items, and answers rows without a context (o = 0,
-// lse = -inf).  Workgroup (sequence, query token, q head); wave w takes every
-// fourth part.
+// lse = -inf).  WPR waves per row (sequence, query token, q head): a wave holds
+// 64 parts' maxima and sums, one per lane, and adds their numerators with
+// lanes across the head dim.
 // ---------------------------------------------------------------------------
-template <typename T, int D, int QB>
-__global__ __launch_bounds__(kPagedThreads) void paged_merge_kernel(PagedParams p, Divider hqdiv, Divider msdiv) {
-    constexpr int E = D / 32;  // floats of a lane (lanes past D / E = 32 idle in the sums)
-    __shared__ float wm[4], wl[4];
-    __shared__ float wacc[4][D];
-    const int r0 = divide(blockIdx.x, hqdiv);
-    const int qh = blockIdx.x - r0 * p.Hq;
+template <typename T, int D, int ROWS, int KEYS, int WPR>
+__global__ __launch_bounds__(kPagedThreads) void paged_merge_kernel(PagedParams p, int32_t n_rows, Divider hqdiv,
+                                                                    Divider msdiv) {
+    constexpr int E = D / 64 ? D / 64 : 1;  // floats of a lane (D = 32: lanes 0 .. 31)
+    __shared__ float wl[WPR], wacc[WPR > 1 ? WPR * D : 1];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int row = WPR == 1 ? blockIdx.x * 4 + wave : blockIdx.x;
+    const int sub = WPR == 1 ? 0 : wave;
+    if (row >= n_rows) return;
+    const int r0 = divide(row, hqdiv);
+    const int qh = row - r0 * p.Hq;
     const int seq = divide(r0, msdiv);
     const int tok = r0 - seq * p.max_seqlen;
-    const SeqWork sw = seq_work<QB>(p, seq);
+    const SeqWork sw = seq_work<ROWS, KEYS>(p, seq);
     const int kvh = divide(qh, p.gdiv);
     const int rr = tok * p.group + (qh - kvh * p.group);
     if (rr >= sw.rows) return;
     uint16_t* const o = p.o + (int64_t)(sw.s0 + tok) * p.so_t + qh * p.so_h;
-    const int tid = threadIdx.x;
+    float* const lse = p.lse ? p.lse + (int64_t)(sw.s0 + tok) * p.sl_t + qh * p.sl_h : nullptr;
     if (sw.blocks == 0) {
-        if (tid < D / 8) st16(o + 8 * tid, Vec16{{0u, 0u, 0u, 0u}});
-        if (p.lse && tid == 0) p.lse[(int64_t)(sw.s0 + tok) * p.sl_t + qh * p.sl_h] = -INFINITY;
+        if (sub == 0 && lane < D / 8) st16(o + 8 * lane, Vec16{{0u, 0u, 0u, 0u}});
+        if (lse && sub == 0 && lane == 0) *lse = -INFINITY;
         return;
     }
-    const int64_t total = p.base[p.B];
-    const int nrun = runs_of(total, p.nwg);
-    const int tile = rr / (16 * QB);
-    const int64_t a = p.base[seq] + (int64_t)(kvh * sw.tiles + tile) * sw.blocks, b = a + sw.blocks;
-    // runs that hold the first and the last unit of the item
-    auto run_of = [&](int64_t x) {
-        int w = (int)(((x + 1) * nrun - 1) / total);
-        while (run_first(total, nrun, w) > x) --w;
-        while (run_first(total, nrun, w + 1) <= x) ++w;
-        return w;
-    };
-    const int w0 = run_of(a), w1 = run_of(b - 1);
+    const Runs runs(p.base[p.B], p.nwg, p.least);
+    const int tile = rr / ROWS;
+    const int32_t a = p.base[seq] + (kvh * sw.tiles + tile) * sw.blocks;
+    const int w0 = runs.of(a), w1 = runs.of(a + sw.blocks - 1);
     if (w0 == w1) return;  // finished by its workgroup
-    const int wave = tid >> 6, lane = tid & 63;
-    const int r = rr - tile * 16 * QB;
-    auto at = [&](int w) {  // row of the workspace that holds run w's part
-        return (2 * (int64_t)w + (run_first(total, nrun, w) >= a ? 0 : 1)) * p.slots + r;
-    };
-    // (a run that starts inside the item, or with it, holds its part in slot 0)
+    // row of the workspace that holds run w's part: a run that starts inside the
+    // item, or with it, holds it in state 0
+    auto at = [&](int w) { return (2 * (int64_t)w + (runs.first(w) >= a ? 0 : 1)) * ROWS + (rr - tile * ROWS); };
     float m = -INFINITY;
     for (int w = w0 + lane; w <= w1; w += 64) m = fmaxf(m, p.part_m[at(w)]);
     for (int d = 32; d; d >>= 1) m = fmaxf(m, __shfl_xor(m, d));
     const float mc = m == -INFINITY ? 0.f : m;
     float l = 0.f, acc[E] = {};
-    for (int w = w0 + wave; w <= w1; w += 4) {
-        const int64_t row = at(w);
-        const float f = fast_exp2(p.part_m[row] - mc);
-        l += f * p.part_l[row];
-        if (lane < 32) {
+    const bool in = lane * E < D;
+    for (int c = w0 + 64 * sub; c <= w1; c += 64 * WPR) {
+        // (of up to 64 parts the waves take a quarter each)
+        const bool mine = c + lane <= w1;
+        const float f = mine ? fast_exp2(p.part_m[at(c + lane)] - mc) : 0.f;
+        l += mine ? f * p.part_l[at(c + lane)] : 0.f;
+        const int n = min(64, w1 + 1 - c);
+        constexpr int U = 8;  // parts requested together
+        for (int i = 0; i < n; i += U) {
+            float x[U][E];
 #pragma unroll
-            for (int j = 0; j < E; ++j) acc[j] += f * p.part_acc[row * D + lane * E + j];
+            for (int u = 0; u < U; ++u) {
+                const float* from = p.part_acc + at(min(c + i + u, w1)) * D + (in ? lane * E : 0);
+#pragma unroll
+                for (int e = 0; e < E; ++e) x[u][e] = from[e];
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const float fi = __builtin_bit_cast(
+                    float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, f), min(i + u, 63)));
+#pragma unroll
+                for (int e = 0; e < E; ++e) acc[e] = __builtin_fmaf(fi, i + u < n ? x[u][e] : 0.f, acc[e]);
+            }
         }
     }
-    if (lane == 0) wl[wave] = l;
-    if (lane < 32) {
+    for (int d = 32; d; d >>= 1) l += __shfl_xor(l, d);
+    if constexpr (WPR > 1) {
+        if (lane == 0) wl[sub] = l;
+        if (in) {
 #pragma unroll
-        for (int j = 0; j < E; ++j) wacc[wave][lane * E + j] = acc[j];
-    }
-    __syncthreads();
-    if (tid < D / 8) {
-        l = wl[0] + wl[1] + wl[2] + wl[3];
-        const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
-        float x[8];
+            for (int e = 0; e < E; ++e) wacc[sub * D + lane * E + e] = acc[e];
+        }
+        __syncthreads();
+        if (sub) return;
+        l = 0.f;
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-            x[j] = (wacc[0][8 * tid + j] + wacc[1][8 * tid + j] + wacc[2][8 * tid + j] + wacc[3][8 * tid + j]) * inv;
-        st16(o + 8 * tid, pack8<T>(x));
-        if (p.lse && tid == 0)
-            p.lse[(int64_t)(sw.s0 + tok) * p.sl_t + qh * p.sl_h] = (mc + fast_log2(l)) * kLn2;
+        for (int w = 0; w < WPR; ++w) l += wl[w];
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            acc[e] = 0.f;
+#pragma unroll
+            for (int w = 0; w < WPR; ++w) acc[e] += in ? wacc[w * D + lane * E + e] : 0.f;
+        }
     }
-    (void)wm;
+    const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+    if (in) {
+        if constexpr (E == 2)
+            *reinterpret_cast<uint32_t*>(o + 2 * lane) = MfmaOps<T>::pack2(acc[0] * inv, acc[1] * inv);
+        else
+            o[lane] = (uint16_t)MfmaOps<T>::pack2(acc[0] * inv, 0.f);
+    }
+    if (lse && lane == 0) *lse = (mc + fast_log2(l)) * kLn2;
 }
 
 // ---------------------------------------------------------------------------
 // Host side
 // ---------------------------------------------------------------------------
-// Row blocks of a workgroup's tile: as many as the longest sequence fills.
-static int row_blocks(int64_t max_rows) { return max_rows <= 16 ? 1 : max_rows <= 32 ? 2 : 4; }
-
-// Workgroups of the launch: as many as run at once, no more than the units that
-// the page table has room for.
-static int paged_workgroups(int32_t batch, int64_t max_rows, int32_t hkv, int32_t capacity, int qb, int head_dim) {
-    const int64_t tiles = (max_rows + 16 * qb - 1) / (16 * qb);
-    const int64_t blocks = ((int64_t)capacity + kUnit - 1) / kUnit;
-    const int64_t most = 256 * paged_waves(head_dim, qb);
-    // batch * hkv * tiles * blocks, without passing 2^63
-    int64_t units = std::min<int64_t>((int64_t)batch * hkv, most);
-    units = std::min<int64_t>(units * std::min<int64_t>(tiles, most), most);
-    units = std::min<int64_t>(units * std::min<int64_t>(blocks, most), most);
-    return (int)((std::max<int64_t>(units, 1) + 7) / 8 * 8);
+// Kernel of a call: rows of a tile (0 row blocks: the wide kernel) and keys of a
+// unit.
+struct PagedShape {
+    int qb, rows, keys, waves;
+};
+static PagedShape paged_shape(int64_t max_rows, int head_dim) {
+    if (max_rows <= 32) {
+        const int qb = max_rows <= 16 ? 1 : 2;
+        return {qb, 16 * qb, kUnit, narrow_waves(head_dim, qb)};
+    }
+    return {0, 128, kWideKeys, 2};
 }
 
 struct PagedSpace {
     int64_t base, m, l, acc, bytes;
 };
-static PagedSpace paged_space(int32_t batch, int nwg, int qb, int head_dim) {
+static PagedSpace paged_space(int32_t batch, int nwg, int rows_of_tile, int head_dim) {
     auto up = [](int64_t x) { return (x + 255) / 256 * 256; };
-    const int64_t rows = 2 * (int64_t)nwg * 16 * qb;
+    const int64_t rows = 2 * (int64_t)nwg * rows_of_tile;
     PagedSpace s;
     s.base = 0;
-    s.m = up(((int64_t)batch + 1) * 8);
+    s.m = up(((int64_t)batch + 1) * 4);
     s.l = s.m + up(rows * 4);
     s.acc = s.l + up(rows * 4);
     s.bytes = s.acc + rows * head_dim * 4;
     return s;
 }
 
-template <typename T, int D, int QB>
-static int launch_paged_qb(const PagedParams& p, hipStream_t st) {
-    hipLaunchKernelGGL((paged_attn_kernel<T, D, QB>), dim3(p.nwg), dim3(kPagedThreads), 0, st, p);
-    const int rc = launch_status("paged_attn_kernel");
-    if (rc) return rc;
-    const int64_t blocks = (int64_t)p.B * p.max_seqlen * p.Hq;
-    if (blocks > INT32_MAX) {
-        set_error("grid too large (%lld blocks)", (long long)blocks);
+template <typename T, int D, int ROWS, int KEYS>
+static int launch_merge(const PagedParams& p, hipStream_t st) {
+    const int64_t rows = (int64_t)p.B * p.max_seqlen * p.Hq;
+    if (rows > INT32_MAX) {
+        set_error("grid too large (%lld rows)", (long long)rows);
         return QATTN_ERR_ARG;
     }
-    hipLaunchKernelGGL((paged_merge_kernel<T, D, QB>), dim3((uint32_t)blocks), dim3(kPagedThreads), 0, st, p,
-                       make_divider(p.Hq), make_divider(p.max_seqlen));
+    const Divider hq = make_divider(p.Hq), ms = make_divider(p.max_seqlen);
+    if (rows <= 512)
+        hipLaunchKernelGGL((paged_merge_kernel<T, D, ROWS, KEYS, 4>), dim3((uint32_t)rows), dim3(kPagedThreads), 0, st, p,
+                           (int32_t)rows, hq, ms);
+    else
+        hipLaunchKernelGGL((paged_merge_kernel<T, D, ROWS, KEYS, 1>), dim3((uint32_t)((rows + 3) / 4)),
+                           dim3(kPagedThreads), 0, st, p, (int32_t)rows, hq, ms);
     return launch_status("paged_merge_kernel");
 }
 
-template <typename T>
-static int launch_paged(const PagedParams& p, int head_dim, int qb, hipStream_t st) {
-    switch (head_dim * 8 + qb) {
-        case 32 * 8 + 1: return launch_paged_qb<T, 32, 1>(p, st);
-        case 32 * 8 + 2: return launch_paged_qb<T, 32, 2>(p, st);
-        case 32 * 8 + 4: return launch_paged_qb<T, 32, 4>(p, st);
-        case 64 * 8 + 1: return launch_paged_qb<T, 64, 1>(p, st);
-        case 64 * 8 + 2: return launch_paged_qb<T, 64, 2>(p, st);
-        case 64 * 8 + 4: return launch_paged_qb<T, 64, 4>(p, st);
-        case 128 * 8 + 1: return launch_paged_qb<T, 128, 1>(p, st);
-        case 128 * 8 + 2: return launch_paged_qb<T, 128, 2>(p, st);
-        default: return launch_paged_qb<T, 128, 4>(p, st);
-    }
+template <typename T, int D>
+static int launch_paged(const PagedParams& p, int qb, hipStream_t st) {
+    const dim3 grid(p.nwg), block(kPagedThreads);
+    if (qb == 1)
+        hipLaunchKernelGGL((paged_attn_kernel<T, D, 1>), grid, block, 0, st, p);
+    else if (qb == 2)
+        hipLaunchKernelGGL((paged_attn_kernel<T, D, 2>), grid, block, 0, st, p);
+    else
+        hipLaunchKernelGGL((paged_wide_kernel<T, D>), grid, block, 0, st, p);
+    const int rc = launch_status(qb ? "paged_attn_kernel" : "paged_wide_kernel");
+    if (rc) return rc;
+    return qb == 1   ? launch_merge<T, D, 16, kUnit>(p, st)
+           : qb == 2 ? launch_merge<T, D, 32, kUnit>(p, st)
+                     : launch_merge<T, D, 128, kWideKeys>(p, st);
 }
 
 // What the workspace size and the launch agree on; false: nothing to launch.
 struct PagedPlan {
     int32_t max_seqlen;
-    int qb, nwg;
+    PagedShape shape;
+    int nwg, least;
+    bool too_many;  // units past 32 bits
 };
 static bool paged_plan(PagedPlan& plan, int32_t batch, int32_t max_seqlen, int64_t total_tokens, int32_t hq,
                        int32_t hkv, int32_t head_dim, int32_t pt_cols, int32_t page_size) {
@@ -569,8 +841,16 @@ static bool paged_plan(PagedPlan& plan, int32_t batch, int32_t max_seqlen, int64
     plan.max_seqlen = (int32_t)std::min<int64_t>(max_seqlen, total_tokens);
     if (plan.max_seqlen <= 0) return false;
     const int64_t rows = (int64_t)plan.max_seqlen * (hq / hkv);
-    plan.qb = row_blocks(rows);
-    plan.nwg = paged_workgroups(batch, rows, hkv, pt_cols * page_size, plan.qb, head_dim);
+    plan.shape = paged_shape(rows, head_dim);
+    // As many workgroups as run at once, no more than the units that the page
+    // table has room for.
+    const int64_t tiles = (rows + plan.shape.rows - 1) / plan.shape.rows;
+    const int64_t blocks = ((int64_t)pt_cols * page_size + plan.shape.keys - 1) / plan.shape.keys;
+    const double units = (double)batch * hkv * tiles * blocks;
+    plan.too_many = units >= 2147483648.0;
+    plan.nwg = (int)std::min<double>(256.0 * plan.shape.waves, std::max(1.0, units));
+    plan.nwg = (plan.nwg + 7) / 8 * 8;
+    plan.least = plan.shape.qb ? 1 : 2;
     return true;
 }
 
@@ -587,7 +867,7 @@ int64_t qattn_prefix_paged_workspace_bytes(int32_t batch, int32_t max_seqlen, in
     if (head_dim <= 0 || !paged_plan(plan, batch, max_seqlen, total_tokens, num_q_heads, num_kv_heads, head_dim,
                                      pt_cols, page_size))
         return 0;
-    return paged_space(batch, plan.nwg, plan.qb, head_dim).bytes;
+    return paged_space(batch, plan.nwg, plan.shape.rows, head_dim).bytes;
 }
 
 int qattn_prefix_paged_fwd(const void* q, const int64_t q_stride[3], const void* k_cache, const int64_t k_stride[4],
@@ -618,8 +898,9 @@ int qattn_prefix_paged_fwd(const void* q, const int64_t q_stride[3], const void*
         set_error("null pointer argument");
         return QATTN_ERR_ARG;
     }
-    if ((int64_t)plan.max_seqlen * (num_q_heads / num_kv_heads) > INT32_MAX / 2) {
-        set_error("max_seqlen %d with %d q heads per kv head is too large", plan.max_seqlen, num_q_heads / num_kv_heads);
+    if (plan.too_many || (int64_t)plan.max_seqlen * (num_q_heads / num_kv_heads) > INT32_MAX / 2) {
+        set_error("sizes too large: batch=%d num_kv_heads=%d max_seqlen=%d group=%d pt_cols=%d page_size=%d", batch,
+                  num_kv_heads, plan.max_seqlen, num_q_heads / num_kv_heads, pt_cols, page_size);
         return QATTN_ERR_ARG;
     }
     if (!row_aligned(q, q_stride, 2) || !row_aligned(o, o_stride, 2)) {
@@ -640,7 +921,7 @@ int qattn_prefix_paged_fwd(const void* q, const int64_t q_stride[3], const void*
             }
         }
     }
-    const PagedSpace sp = paged_space(batch, plan.nwg, plan.qb, head_dim);
+    const PagedSpace sp = paged_space(batch, plan.nwg, plan.shape.rows, head_dim);
     if (!workspace || workspace_size < sp.bytes) {
         set_error("workspace of %lld bytes needed, %lld given", (long long)sp.bytes, (long long)workspace_size);
         return QATTN_ERR_WORKSPACE;
@@ -669,17 +950,24 @@ int qattn_prefix_paged_fwd(const void* q, const int64_t q_stride[3], const void*
     p.pt_cols = pt_cols, p.num_pages = num_pages, p.page_size = page_size;
     p.capacity = keys ? pt_cols * page_size : 0;  // (without pages no key exists)
     p.nwg = plan.nwg;
-    p.slots = 16 * plan.qb;
+    p.least = plan.least;
     p.pdiv = make_divider(page_size);
     p.gdiv = make_divider(p.group);
     p.scale_log2 = scale * kLog2e;
     char* const ws = (char*)workspace;
-    p.base = (int64_t*)(ws + sp.base);
+    p.base = (int32_t*)(ws + sp.base);
     p.part_m = (float*)(ws + sp.m);
     p.part_l = (float*)(ws + sp.l);
     p.part_acc = (float*)(ws + sp.acc);
-    return dtype == QATTN_DTYPE_F16 ? launch_paged<F16>(p, head_dim, plan.qb, (hipStream_t)stream)
-                                    : launch_paged<BF16>(p, head_dim, plan.qb, (hipStream_t)stream);
+    hipStream_t st = (hipStream_t)stream;
+    const int qb = plan.shape.qb;
+    if (dtype == QATTN_DTYPE_F16)
+        return head_dim == 32   ? launch_paged<F16, 32>(p, qb, st)
+               : head_dim == 64 ? launch_paged<F16, 64>(p, qb, st)
+                                : launch_paged<F16, 128>(p, qb, st);
+    return head_dim == 32   ? launch_paged<BF16, 32>(p, qb, st)
+           : head_dim == 64 ? launch_paged<BF16, 64>(p, qb, st)
+                            : launch_paged<BF16, 128>(p, qb, st);
 }
 
 }  // extern "C"
