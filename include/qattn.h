@@ -429,7 +429,8 @@ int qattn_prefix_paged_fwd(const void *q, const int64_t q_stride[3],
                            int64_t workspace_size, void *stream);
 
 /*
- * New K/V rows into a paged cache: row i of sequence s (row cu_seqlens[s] + i
+ * New K/V rows into a paged cache (5 strides {layer, page, slot, head, dim}, of
+ * which the first is not used: one layer's cache): row i of sequence s (row cu_seqlens[s] + i
  * of k and v, i < max_seqlen; cu_seqlens NULL: row s is sequence s's one row)
  * goes to position context_lens[s] + i.  Positions at or beyond pt_cols *
  * page_size (at most 2^30) and pages outside [0, num_pages) take no row;
@@ -439,7 +440,7 @@ int qattn_prefix_paged_fwd(const void *q, const int64_t q_stride[3],
  * sequences that share the page of a written position race.
  */
 int qattn_kv_append(const void *k, const int64_t k_stride[3], const void *v, const int64_t v_stride[3],
-                    void *k_cache, const int64_t kc_stride[4], void *v_cache, const int64_t vc_stride[4],
+                    void *k_cache, const int64_t kc_stride[5], void *v_cache, const int64_t vc_stride[5],
                     const int32_t *page_table, int32_t pt_cols, int32_t num_pages, int32_t page_size,
                     const int32_t *context_lens, int32_t *new_lens, const int32_t *cu_seqlens,
                     int32_t batch, int32_t max_seqlen, int64_t total_tokens, int32_t num_kv_heads,

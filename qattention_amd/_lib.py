@@ -168,11 +168,29 @@ def check(rc: int, what: str) -> None:
         raise QAttnError(f"{what} failed: {ERRORS.get(rc, rc)}: {last_error()}")
 
 
-_I64 = {n: C.c_int64 * n for n in (2, 3, 4, 5)}  # (forming the array type costs as much as filling it)
+_I64 = {n: C.c_int64 * n for n in (2, 3, 4)}  # (forming the array type costs as much as filling it)
 
 
 def i64arr(vals):
     return _I64[len(vals)](*map(int, vals))
+
+
+_LAYOUTS: dict = {}
+
+
+def layout(stride: tuple) -> tuple:
+    """(ctypes array of the strides, whether rows are 16-byte vectors, whether a
+    stride is 0) for a tensor's stride tuple.  Kept per value of the tuple:
+    forming the array and looking at every stride costs three times the lookup."""
+    e = _LAYOUTS.get(stride)
+    if e is None:
+        outer = 0
+        for s in stride[:-1]:
+            outer |= s
+        if len(_LAYOUTS) >= 4096:
+            _LAYOUTS.clear()
+        e = _LAYOUTS[stride] = ((C.c_int64 * len(stride))(*stride), stride[-1] == 1 and not outer & 7, 0 in stride)
+    return e
 
 
 def ptr(t) -> int:

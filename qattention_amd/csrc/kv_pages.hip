@@ -295,7 +295,7 @@ using namespace qattn;
 extern "C" {
 
 int qattn_kv_append(const void* k, const int64_t k_stride[3], const void* v, const int64_t v_stride[3],
-                    void* k_cache, const int64_t kc_stride[4], void* v_cache, const int64_t vc_stride[4],
+                    void* k_cache, const int64_t kc_stride[5], void* v_cache, const int64_t vc_stride[5],
                     const int32_t* page_table, int32_t pt_cols, int32_t num_pages, int32_t page_size,
                     const int32_t* context_lens, int32_t* new_lens, const int32_t* cu_seqlens, int32_t batch,
                     int32_t max_seqlen, int64_t total_tokens, int32_t num_kv_heads, int32_t head_dim, int32_t dtype,
@@ -305,10 +305,8 @@ int qattn_kv_append(const void* k, const int64_t k_stride[3], const void* v, con
         set_error("null stride array");
         return QATTN_ERR_ARG;
     }
-    const int64_t ks5[5] = {0, kc_stride[0], kc_stride[1], kc_stride[2], kc_stride[3]};
-    const int64_t vs5[5] = {0, vc_stride[0], vc_stride[1], vc_stride[2], vc_stride[3]};
     AppendParams p{};
-    int rc = fill_pages(p.pg, k_cache, ks5, v_cache, vs5, 1, num_pages, page_size, num_kv_heads, head_dim, dtype);
+    int rc = fill_pages(p.pg, k_cache, kc_stride, v_cache, vc_stride, 1, num_pages, page_size, num_kv_heads, head_dim, dtype);
     if (rc) return rc;
     rc = fill_table(p.pg, page_table, pt_cols, context_lens, new_lens, batch);
     if (rc) return rc;

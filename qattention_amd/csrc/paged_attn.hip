@@ -667,15 +667,17 @@ __global__ __launch_bounds__(kPagedThreads) __attribute__((amdgpu_waves_per_eu(2
 
 // ---------------------------------------------------------------------------
 // Joins the parts of cut items, and answers rows without a context (o = 0,
-// lse = -inf).  WPR waves per row (sequence, query token, q head): a wave holds
-// 64 parts' maxima and sums, one per lane, and adds their numerators with
-// lanes across the head dim.
+// lse = -inf).  WPR waves per row (sequence, query token, q head), each with an
+// equal share of the parts: one part's maximum and sum per lane, the
+// numerators with lanes across the head dim.  What bounds it is its chain of
+// dependent loads (lengths and units, then the states): four waves per row where
+// few rows leave the chip empty.
 // ---------------------------------------------------------------------------
 template <typename T, int D, int ROWS, int KEYS, int WPR>
 __global__ __launch_bounds__(kPagedThreads) void paged_merge_kernel(PagedParams p, int32_t n_rows, Divider hqdiv,
                                                                     Divider msdiv) {
     constexpr int E = D / 64 ? D / 64 : 1;  // floats of a lane (D = 32: lanes 0 .. 31)
-    __shared__ float wl[WPR], wacc[WPR > 1 ? WPR * D : 1];
+    __shared__ float wm[WPR], wl[WPR], wacc[WPR > 1 ? WPR * D : 1];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int row = WPR == 1 ? blockIdx.x * 4 + wave : blockIdx.x;
     const int sub = WPR == 1 ? 0 : wave;
@@ -684,6 +686,7 @@ __global__ __launch_bounds__(kPagedThreads) void paged_merge_kernel(PagedParams 
     const int qh = row - r0 * p.Hq;
     const int seq = divide(r0, msdiv);
     const int tok = r0 - seq * p.max_seqlen;
+    const int32_t total = p.base[p.B], base = p.base[seq];  // (asked for with the sequence's lengths)
     const SeqWork sw = seq_work<ROWS, KEYS>(p, seq);
     const int kvh = divide(qh, p.gdiv);
     const int rr = tok * p.group + (qh - kvh * p.group);
@@ -695,35 +698,46 @@ __global__ __launch_bounds__(kPagedThreads) void paged_merge_kernel(PagedParams 
         if (lse && sub == 0 && lane == 0) *lse = -INFINITY;
         return;
     }
-    const Runs runs(p.base[p.B], p.nwg, p.least);
+    const Runs runs(total, p.nwg, p.least);
     const int tile = rr / ROWS;
-    const int32_t a = p.base[seq] + (kvh * sw.tiles + tile) * sw.blocks;
-    const int w0 = runs.of(a), w1 = runs.of(a + sw.blocks - 1);
-    if (w0 == w1) return;  // finished by its workgroup
+    const int32_t a = base + (kvh * sw.tiles + tile) * sw.blocks;
+    const int w0 = runs.of(a), w1 = runs.of(a + sw.blocks - 1) + 1;
+    if (w0 + 1 == w1) return;  // finished by its workgroup
     // row of the workspace that holds run w's part: a run that starts inside the
     // item, or with it, holds it in state 0
     auto at = [&](int w) { return (2 * (int64_t)w + (runs.first(w) >= a ? 0 : 1)) * ROWS + (rr - tile * ROWS); };
-    float m = -INFINITY;
-    for (int w = w0 + lane; w <= w1; w += 64) m = fmaxf(m, p.part_m[at(w)]);
-    for (int d = 32; d; d >>= 1) m = fmaxf(m, __shfl_xor(m, d));
-    const float mc = m == -INFINITY ? 0.f : m;
-    float l = 0.f, acc[E] = {};
+    const int share = WPR == 1 ? w1 - w0 : (w1 - w0 + WPR - 1) / WPR;
+    const int lo = w0 + sub * share, hi = min(w1, lo + share);
     const bool in = lane * E < D;
-    for (int c = w0 + 64 * sub; c <= w1; c += 64 * WPR) {
-        // (of up to 64 parts the waves take a quarter each)
-        const bool mine = c + lane <= w1;
-        const float f = mine ? fast_exp2(p.part_m[at(c + lane)] - mc) : 0.f;
-        l += mine ? f * p.part_l[at(c + lane)] : 0.f;
-        const int n = min(64, w1 + 1 - c);
-        constexpr int U = 8;  // parts requested together
-        for (int i = 0; i < n; i += U) {
-            float x[U][E];
+    float m = -INFINITY, l = 0.f, acc[E] = {};
+    for (int c = lo; c < hi; c += 64) {
+        const int n = min(64, hi - c);
+        const bool mine = lane < n;
+        const int64_t own = at(min(c + lane, hi - 1));
+        const float mi = mine ? p.part_m[own] : -INFINITY;
+        const float li = mine ? p.part_l[own] : 0.f;
+        constexpr int U = 8;  // numerators requested together, the first ones before any maximum is known
+        float x[U][E];
+        auto request = [&](int i) {
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                const float* from = p.part_acc + at(min(c + i + u, w1)) * D + (in ? lane * E : 0);
+                const float* from = p.part_acc + at(min(c + i + u, hi - 1)) * D + (in ? lane * E : 0);
 #pragma unroll
                 for (int e = 0; e < E; ++e) x[u][e] = from[e];
             }
+        };
+        request(0);
+        float mn = mi;
+        for (int d = 32; d; d >>= 1) mn = fmaxf(mn, __shfl_xor(mn, d));
+        mn = fmaxf(mn, m);
+        const float mc = mn == -INFINITY ? 0.f : mn;
+        const float old = fast_exp2(m - mc);
+        const float f = mine ? fast_exp2(mi - mc) : 0.f;
+        l = l * old + f * li;
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[e] *= old;
+        for (int i = 0; i < n; i += U) {
+            if (i) request(i);
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 const float fi = __builtin_bit_cast(
@@ -732,26 +746,31 @@ __global__ __launch_bounds__(kPagedThreads) void paged_merge_kernel(PagedParams 
                 for (int e = 0; e < E; ++e) acc[e] = __builtin_fmaf(fi, i + u < n ? x[u][e] : 0.f, acc[e]);
             }
         }
+        m = mn;
     }
     for (int d = 32; d; d >>= 1) l += __shfl_xor(l, d);
     if constexpr (WPR > 1) {
-        if (lane == 0) wl[sub] = l;
+        if (lane == 0) wm[sub] = m, wl[sub] = l;
         if (in) {
 #pragma unroll
             for (int e = 0; e < E; ++e) wacc[sub * D + lane * E + e] = acc[e];
         }
         __syncthreads();
         if (sub) return;
-        l = 0.f;
+        m = -INFINITY, l = 0.f;
 #pragma unroll
-        for (int w = 0; w < WPR; ++w) l += wl[w];
+        for (int w = 0; w < WPR; ++w) m = fmaxf(m, wm[w]);
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-            acc[e] = 0.f;
+        for (int e = 0; e < E; ++e) acc[e] = 0.f;
 #pragma unroll
-            for (int w = 0; w < WPR; ++w) acc[e] += in ? wacc[w * D + lane * E + e] : 0.f;
+        for (int w = 0; w < WPR; ++w) {
+            const float f = fast_exp2(wm[w] - (m == -INFINITY ? 0.f : m));
+            l += f * wl[w];
+#pragma unroll
+            for (int e = 0; e < E; ++e) acc[e] += f * (in ? wacc[w * D + lane * E + e] : 0.f);
         }
     }
+    const float mc = m == -INFINITY ? 0.f : m;
     const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
     if (in) {
         if constexpr (E == 2)

@@ -7,9 +7,10 @@
 // Work unit: (sequence, kv head, tile of 128 rows); a row is a (token, q head)
 // pair of the kv head's group, tokens outermost, so a tile spans 128 / group
 // tokens and a K/V block staged in LDS serves every q head that reads it.
-// Units with the most keys come first (last tiles of every sequence), sequences
-// and heads innermost: with a multiple of 8 of those, every tile of one
-// (sequence, kv head) runs on one XCD and shares its L2.
+// All tiles of a (sequence, kv head) run on one XCD, one after the other and
+// the longest first, so the ~64 workgroups that run there at a time share the
+// K/V of one or a few heads in its L2; with fewer pairs than XCDs, or a number
+// that 8 does not divide, a pair's tiles are dealt to several.
 //
 // The key loop (dense_tiles.h) ends at the tile's last token; the blocks that
 // reach past a wave's first token are masked by row.
@@ -28,6 +29,10 @@ namespace qattn {
 
 constexpr int kPromptThreads = 256;
 constexpr int kBM = 128;  // rows per workgroup
+// Waves per SIMD: 64-wide heads have half the products per exponential, and a
+// third wave covers what two leave (16 x 1300 tokens, 32 / 8 heads: 161 us with
+// two, 152 with three).
+constexpr int prompt_waves(int d) { return d == 64 ? 3 : 2; }
 
 struct PromptParams {
     const uint16_t* q;
@@ -38,8 +43,9 @@ struct PromptParams {
     const int32_t* cu;
     int64_t sq_t, sq_h, sk_t, sk_h, sv_t, sv_h, so_t, so_h, sl_t, sl_h;
     int64_t total_tokens;
-    int32_t B, Hq, Hkv, group, max_seqlen, qtiles, pairs;
-    Divider gdiv, pairdiv, hkvdiv;  // group, pairs (B * Hkv), Hkv
+    int32_t B, Hq, Hkv, group, max_seqlen;
+    int32_t qtiles, spread, list;  // tiles of the longest prompt, log2 of lists per pair, tiles of a list
+    Divider gdiv, listdiv, hkvdiv;
     float scale_log2;
 };
 
@@ -187,15 +193,21 @@ struct PromptKeys {
 };
 
 template <typename T, int D>
-__global__ __launch_bounds__(kPromptThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) void prompt_attn_kernel(
+__global__ __launch_bounds__(kPromptThreads) __attribute__((amdgpu_waves_per_eu(prompt_waves(D), prompt_waves(D)))) void prompt_attn_kernel(
     PromptParams p) {
     using Tile = DenseTile<T, D>;
     constexpr int KS = Tile::KS, DT = Tile::DT;
     __shared__ __attribute__((aligned(1024))) uint16_t smem[Tile::kSmem];
 
-    const int r0 = divide(blockIdx.x, p.pairdiv);
-    const int pair = blockIdx.x - r0 * p.pairs;
-    const int qt = p.qtiles - 1 - r0;
+    // XCD x (blockIdx % 8) takes lists x, x + 8, ...: list v is every
+    // (1 << spread)-th tile of pair v >> spread, the longest first
+    const int i = blockIdx.x >> 3;
+    const int li = divide(i, p.listdiv);
+    const int v = (blockIdx.x & 7) + 8 * li;
+    const int pair = v >> p.spread;
+    const int rank = ((i - li * p.list) << p.spread) + (v & ((1 << p.spread) - 1));
+    const int qt = p.qtiles - 1 - rank;
+    if (qt < 0) return;
     const int seq = divide(pair, p.hkvdiv);
     const int kvh = pair - seq * p.Hkv;
     const int32_t s0 = p.cu[seq], s1 = p.cu[seq + 1];
@@ -322,15 +334,17 @@ int qattn_prompt_fwd(const void* q, const int64_t q_stride[3], const void* k, co
                   num_kv_heads);
         return QATTN_ERR_ARG;
     }
-    p.pairs = batch * num_kv_heads;
     p.qtiles = (p.max_seqlen * p.group + kBM - 1) / kBM;
-    const int64_t blocks = (int64_t)p.qtiles * p.pairs;
+    const int64_t pairs = (int64_t)batch * num_kv_heads;
+    while (pairs << p.spread & 7) ++p.spread;  // lists: a multiple of the 8 XCDs
+    p.list = (p.qtiles + (1 << p.spread) - 1) >> p.spread;
+    const int64_t blocks = (pairs << p.spread) * p.list;
     if (blocks > INT32_MAX) {
         set_error("grid too large (%lld blocks)", (long long)blocks);
         return QATTN_ERR_ARG;
     }
     p.gdiv = make_divider(p.group);
-    p.pairdiv = make_divider(p.pairs);
+    p.listdiv = make_divider(p.list);
     p.hkvdiv = make_divider(num_kv_heads);
     p.scale_log2 = scale * kLog2e;
     hipStream_t st = (hipStream_t)stream;

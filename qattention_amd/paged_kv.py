@@ -39,37 +39,37 @@ from typing import Optional, Sequence, Tuple, Union
 import torch
 
 from . import _lib
-from .ragged_attn import (_SUPPORTED, _check_dtypes, _dtype_code, _no_grad, _on, _require_device, _seqlens, _stream,
-                          _vec, _vec_ok)
+from .ragged_attn import (_SUPPORTED, _check_dtypes, _device_index, _dtype_code, _no_grad, _on, _out_like, _rows16,
+                          _seqlens, _stream)
 
 
 def _int32(t: torch.Tensor, device) -> torch.Tensor:
+    if t.dtype is torch.int32 and t.is_contiguous() and t.device == device:
+        return t
     return t.to(device=device, dtype=torch.int32, non_blocking=True).contiguous()
 
 
-def _check_caches(K_cache, V_cache, dims: Tuple[int, ...]) -> None:
-    """Caches that a call writes in place: no copy can stand in for them."""
+def _check_caches(K_cache, V_cache, dims: Tuple[int, ...]) -> tuple:
+    """Caches that a call writes in place: no copy can stand in for them.
+    Returns their addresses and 5 strides {layer, page, slot, head, dim} each."""
     if K_cache.dim() not in dims or K_cache.shape != V_cache.shape:
         raise ValueError(f"caches must be {' or '.join(f'{d}-D' for d in dims)} and of one shape (got "
                          f"{tuple(K_cache.shape)}, {tuple(V_cache.shape)})")
     if K_cache.dtype not in _SUPPORTED or V_cache.dtype != K_cache.dtype:
         raise AssertionError(f"Inputs must be fp16 or bf16 (got {K_cache.dtype}, {V_cache.dtype})")
-    if not K_cache.numel():
-        return
+    out = []
     for c in (K_cache, V_cache):
-        if not _vec_ok(c):
+        strides, aligned, zero = _lib.layout(c.stride() if c.dim() == 5 else (0, *c.stride()))
+        p = c.data_ptr()
+        if (not aligned or p & 15) and c.numel():
             raise ValueError(f"cache of shape {tuple(c.shape)} and strides {tuple(c.stride())} is not writable as "
                              "16-byte rows (unit last stride, 8-element aligned strides, 16-byte aligned base)")
-        if any(st == 0 and n > 1 for st, n in zip(c.stride(), c.shape)):
+        if zero and any(st == 0 and n > 1 for st, n in zip(c.stride(), c.shape)):
             raise ValueError("cache rows overlap (a stride of 0)")
-    if K_cache.data_ptr() == V_cache.data_ptr():
+        out += (p, strides)
+    if out[0] == out[2] and K_cache.numel():
         raise ValueError("K_cache and V_cache are the same memory")
-
-
-def _layered(cache) -> tuple:
-    """Layers, and the 5 strides {layer, page, slot, head, dim}."""
-    st = cache.stride()
-    return (cache.shape[0], _lib.i64arr(st)) if cache.dim() == 5 else (1, _lib.i64arr((0, *st)))
+    return tuple(out)
 
 
 def _table(page_table, B: int, device) -> torch.Tensor:
@@ -120,8 +120,9 @@ def prefix_attention_paged(
     [T, Hq] fp32, natural log, if return_lse)."""
     assert K_cache.shape == V_cache.shape, "K and V cache shapes must match"
     _check_dtypes(Q, K_cache, V_cache)
-    device = _require_device(Q, K_cache, V_cache)
+    _device_index(Q, K_cache, V_cache)
     _no_grad(Q, K_cache, V_cache)
+    device = Q.device
     if Q.dim() != 3 or K_cache.dim() != 4:
         raise ValueError(f"expected Q [T, Hq, D] and caches [pages, page_size, Hkv, D] (got {tuple(Q.shape)}, "
                          f"{tuple(K_cache.shape)})")
@@ -133,10 +134,10 @@ def prefix_attention_paged(
     B = ctx.shape[0]
     ms, cu = _rows(T, B, cu_seqlens, max_seqlen, device)
     pt = _table(page_table, B, device)
-    Q, K_cache, V_cache = _vec(Q), _vec(K_cache), _vec(V_cache)
-    O = torch.empty_like(Q)
-    if not _vec_ok(O):
-        O = torch.empty(Q.shape, dtype=Q.dtype, device=device)
+    Q, q, qs = _rows16(Q)
+    K_cache, k, ks = _rows16(K_cache)
+    V_cache, v, vs = _rows16(V_cache)
+    O, o, os_ = _out_like(Q)
     LSE = torch.empty(T, Hq, dtype=torch.float32, device=device) if return_lse else None
     L = _lib.lib()
     cols = pt.shape[1]
@@ -144,10 +145,8 @@ def prefix_attention_paged(
     ws = torch.empty(max(ws_bytes, 1), dtype=torch.uint8, device=device)
     with _on(device):
         rc = L.qattn_prefix_paged_fwd(
-            Q.data_ptr(), _lib.i64arr(Q.stride()), K_cache.data_ptr(), _lib.i64arr(K_cache.stride()),
-            V_cache.data_ptr(), _lib.i64arr(V_cache.stride()), pt.data_ptr(), cols, num_pages, page_size,
-            ctx.data_ptr(), O.data_ptr(), _lib.i64arr(O.stride()), _lib.ptr(LSE),
-            _lib.i64arr(LSE.stride()) if LSE is not None else None, _lib.ptr(cu), B, ms, T, Hq, Hkv, D,
+            q, qs, k, ks, v, vs, pt.data_ptr(), cols, num_pages, page_size, ctx.data_ptr(), o, os_, _lib.ptr(LSE),
+            None if LSE is None else _lib.layout(LSE.stride())[0], _lib.ptr(cu), B, ms, T, Hq, Hkv, D,
             1.0 / math.sqrt(D), _dtype_code(Q), ws.data_ptr(), ws_bytes, _stream(device))
     _lib.check(rc, "qattn_prefix_paged_fwd")
     return (O, LSE) if return_lse else O
@@ -173,10 +172,11 @@ def append_paged_kv(
     position that the table has no column for takes no row and does not count; a
     row whose page lies outside the cache is dropped.  A sequence with a negative
     length is passed over.  The written pages must be the sequence's own."""
-    _check_caches(K_cache, V_cache, (4,))
+    kc, kcs, vc, vcs = _check_caches(K_cache, V_cache, (4,))
     _check_dtypes(K_cache, K, V)
-    device = _require_device(K_cache, V_cache, K, V)
+    _device_index(K_cache, V_cache, K, V)
     _no_grad(K, V, K_cache, V_cache)
+    device = K.device
     num_pages, page_size, Hkv, D = K_cache.shape
     T = K.shape[0]
     if K.dim() != 3 or K.shape != V.shape or K.shape[1:] != K_cache.shape[2:] or page_size < 1:
@@ -185,14 +185,13 @@ def append_paged_kv(
     B = ctx.shape[0]
     ms, cu = _rows(T, B, cu_seqlens, max_seqlen, device)
     pt = _table(page_table, B, device)
-    K, V = _vec(K), _vec(V)
+    K, k, ks = _rows16(K)
+    V, v, vs = _rows16(V)
     new = torch.empty_like(ctx)
     with _on(device):
         rc = _lib.lib().qattn_kv_append(
-            K.data_ptr(), _lib.i64arr(K.stride()), V.data_ptr(), _lib.i64arr(V.stride()),
-            K_cache.data_ptr(), _lib.i64arr(K_cache.stride()), V_cache.data_ptr(), _lib.i64arr(V_cache.stride()),
-            pt.data_ptr(), pt.shape[1], num_pages, page_size, ctx.data_ptr(), new.data_ptr(), _lib.ptr(cu), B, ms, T,
-            Hkv, D, _dtype_code(K_cache), _stream(device))
+            k, ks, v, vs, kc, kcs, vc, vcs, pt.data_ptr(), pt.shape[1], num_pages, page_size, ctx.data_ptr(),
+            new.data_ptr(), _lib.ptr(cu), B, ms, T, Hkv, D, _dtype_code(K), _stream(device))
     _lib.check(rc, "qattn_kv_append")
     return new
 
@@ -215,9 +214,10 @@ def compact_paged_kv(
     the table has no column for.  Returns the lengths afterwards, context plus
     path, int32 [B] on the device.  Pages of the moved positions must be the
     sequence's own."""
-    _check_caches(K_cache, V_cache, (4, 5))
-    device = _require_device(K_cache, V_cache)
+    kc, kcs, vc, vcs = _check_caches(K_cache, V_cache, (4, 5))
+    _device_index(K_cache, V_cache)
     _no_grad(K_cache, V_cache)
+    device = K_cache.device
     num_pages, page_size, Hkv, D = K_cache.shape[-4:]
     ctx = _lengths(context_lens, device)
     B = ctx.shape[0]
@@ -225,12 +225,11 @@ def compact_paged_kv(
         raise ValueError(f"accepted must be [{B}, path length] (got {tuple(accepted.shape)})")
     pt, path = _table(page_table, B, device), _int32(accepted, device)
     new = torch.empty_like(ctx)
-    layers, ks = _layered(K_cache)
+    layers = K_cache.shape[0] if K_cache.dim() == 5 else 1
     with _on(device):
         rc = _lib.lib().qattn_kv_compact(
-            K_cache.data_ptr(), ks, V_cache.data_ptr(), _layered(V_cache)[1], layers, pt.data_ptr(), pt.shape[1],
-            num_pages, page_size, ctx.data_ptr(), path.data_ptr(), path.shape[1], new.data_ptr(), B, Hkv, D,
-            _dtype_code(K_cache), _stream(device))
+            kc, kcs, vc, vcs, layers, pt.data_ptr(), pt.shape[1], num_pages, page_size, ctx.data_ptr(),
+            path.data_ptr(), path.shape[1], new.data_ptr(), B, Hkv, D, _dtype_code(K_cache), _stream(device))
     _lib.check(rc, "qattn_kv_compact")
     return new
 
@@ -270,16 +269,17 @@ def copy_kv_pages(K_cache: torch.Tensor, V_cache: torch.Tensor, src_pages: _Page
     lists on the host are checked for that (ValueError); of lists on the GPU,
     pairs with a page outside the cache are passed over, the rest is the
     caller's to keep."""
-    _check_caches(K_cache, V_cache, (4, 5))
-    device = _require_device(K_cache, V_cache)
+    kc, kcs, vc, vcs = _check_caches(K_cache, V_cache, (4, 5))
+    _device_index(K_cache, V_cache)
     _no_grad(K_cache, V_cache)
+    device = K_cache.device
     num_pages, page_size, Hkv, D = K_cache.shape[-4:]
     src, dst = _page_lists(src_pages, dst_pages, num_pages, device)
     if not src.shape[0] or not K_cache.numel():
         return
-    layers, ks = _layered(K_cache)
+    layers = K_cache.shape[0] if K_cache.dim() == 5 else 1
     with _on(device):
         rc = _lib.lib().qattn_kv_copy_pages(
-            K_cache.data_ptr(), ks, V_cache.data_ptr(), _layered(V_cache)[1], layers, num_pages, page_size,
-            src.data_ptr(), dst.data_ptr(), src.shape[0], Hkv, D, _dtype_code(K_cache), _stream(device))
+            kc, kcs, vc, vcs, layers, num_pages, page_size, src.data_ptr(), dst.data_ptr(), src.shape[0], Hkv, D,
+            _dtype_code(K_cache), _stream(device))
     _lib.check(rc, "qattn_kv_copy_pages")

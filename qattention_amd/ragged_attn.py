@@ -96,8 +96,41 @@ def _require_device(*ts):
 
 def _no_grad(*ts) -> None:
     """Refuse tensors that ask for gradients where there is no backward pass."""
-    if torch.is_grad_enabled() and any(t.requires_grad for t in ts):
-        raise RuntimeError("this call has no backward pass: use torch.no_grad() or detach its inputs")
+    for t in ts:
+        if t.requires_grad and torch.is_grad_enabled():
+            break
+    else:
+        return
+    raise RuntimeError("this call has no backward pass: use torch.no_grad() or detach its inputs")
+
+
+def _rows16(t: torch.Tensor):
+    """_vec, with the address and the stride array of the result."""
+    strides, aligned, _ = _lib.layout(t.stride())
+    p = t.data_ptr()
+    if aligned and not p & 15:
+        return t, p, strides
+    t = _vec(t)
+    return t, t.data_ptr(), _lib.layout(t.stride())[0]
+
+
+def _device_index(*ts) -> int:
+    """The device that all tensors are on (_require_device's answer for those that are not)."""
+    idx = ts[0].get_device()
+    for t in ts:
+        if idx < 0 or t.get_device() != idx:
+            _require_device(*ts)
+    return idx
+
+
+def _out_like(Q: torch.Tensor):
+    """An output of Q's shape, with its address and stride array."""
+    O = torch.empty_like(Q)
+    strides, aligned, _ = _lib.layout(O.stride())
+    if not aligned:
+        O = torch.empty(Q.shape, dtype=Q.dtype, device=Q.device)
+        strides = _lib.layout(O.stride())[0]
+    return O, O.data_ptr(), strides
 
 
 def _stream(device) -> int:
@@ -688,8 +721,9 @@ def prompt_attention(
     refused while autograd records.  Returns O [sum L_i, Hq, D] (and LSE
     [sum L_i, Hq] fp32, natural log, if return_lse)."""
     _check_dtypes(Q, K, V)
-    device = _require_device(Q, K, V)
+    _device_index(Q, K, V)
     _no_grad(Q, K, V)
+    device = Q.device
     if Q.dim() != 3 or K.dim() != 3 or V.dim() != 3:
         raise ValueError(f"expected packed [T, H, D] tensors (got {tuple(Q.shape)}, {tuple(K.shape)}, "
                          f"{tuple(V.shape)})")
@@ -698,18 +732,15 @@ def prompt_attention(
         raise ValueError("packed Q, K, V must have the same number of tokens")
     B = int(cu_seqlens.shape[0]) - 1
     ms, cu_dev = _seqlens(cu_seqlens, B, device, max_seqlen)
-    Q, K, V = _vec(Q), _vec(K), _vec(V)
-    O = torch.empty_like(Q)
-    if not _vec_ok(O):
-        O = torch.empty(Q.shape, dtype=Q.dtype, device=device)
+    Q, q, qs = _rows16(Q)
+    K, k, ks = _rows16(K)
+    V, v, vs = _rows16(V)
+    O, o, os_ = _out_like(Q)
     LSE = torch.empty(T, Hq, dtype=torch.float32, device=device) if return_lse else None
-    L = _lib.lib()
     with _on(device):
-        rc = L.qattn_prompt_fwd(
-            Q.data_ptr(), _lib.i64arr(Q.stride()), K.data_ptr(), _lib.i64arr(K.stride()),
-            V.data_ptr(), _lib.i64arr(V.stride()), O.data_ptr(), _lib.i64arr(O.stride()), _lib.ptr(LSE),
-            _lib.i64arr(LSE.stride()) if LSE is not None else None, cu_dev.data_ptr(), B, ms, T, Hq, Hkv, D,
-            1.0 / math.sqrt(D), _dtype_code(Q), _stream(device))
+        rc = _lib.lib().qattn_prompt_fwd(
+            q, qs, k, ks, v, vs, o, os_, _lib.ptr(LSE), None if LSE is None else _lib.layout(LSE.stride())[0],
+            cu_dev.data_ptr(), B, ms, T, Hq, Hkv, D, 1.0 / math.sqrt(D), _dtype_code(Q), _stream(device))
     _lib.check(rc, "qattn_prompt_fwd")
     return (O, LSE) if return_lse else O
 

@@ -73,7 +73,7 @@ def pages_call(which, kc=16, vc=16, cs=(32768, 4096, 256, 128, 1), layers=2, tab
                acc=16, pcols=4, new=16, B=2, Hkv=2, D=128, dtype=0, k=16, ks=(256, 128, 1), cu=16, ms=4, T=8, n=3):
     L = _lib.lib()
     if which == "append":
-        return L.qattn_kv_append(k, i64(*ks), k, i64(*ks), kc, i64(*cs[1:]), vc, i64(*cs[1:]), table, cols, pages, ps,
+        return L.qattn_kv_append(k, i64(*ks), k, i64(*ks), kc, i64(*cs), vc, i64(*cs), table, cols, pages, ps,
                                  ctx, new, cu, B, ms, T, Hkv, D, dtype, None)
     if which == "compact":
         return L.qattn_kv_compact(kc, i64(*cs), vc, i64(*cs), layers, table, cols, pages, ps, ctx, acc, pcols, new, B,
