@@ -179,17 +179,36 @@ _LAYOUTS: dict = {}
 
 
 def layout(stride: tuple) -> tuple:
-    """(ctypes array of the strides, whether rows are 16-byte vectors, whether a
-    stride is 0) for a tensor's stride tuple.  Kept per value of the tuple:
-    forming the array and looking at every stride costs three times the lookup."""
+    """(ctypes array of the strides, whether rows are 16-byte vectors) for a
+    tensor's stride tuple.  Kept per value of the tuple: forming the array and
+    looking at every stride costs three times the lookup."""
     e = _LAYOUTS.get(stride)
     if e is None:
-        outer = 0
-        for s in stride[:-1]:
-            outer |= s
         if len(_LAYOUTS) >= 4096:
             _LAYOUTS.clear()
-        e = _LAYOUTS[stride] = ((C.c_int64 * len(stride))(*stride), stride[-1] == 1 and not outer & 7, 0 in stride)
+        e = _LAYOUTS[stride] = ((C.c_int64 * len(stride))(*stride), _aligned(stride))
+    return e
+
+
+def _aligned(stride) -> bool:
+    outer = 0
+    for s in stride[:-1]:
+        outer |= s
+    return stride[-1] == 1 and not outer & 7
+
+
+_CACHE_LAYOUTS: dict = {}
+
+
+def cache_layout(stride: tuple) -> tuple:
+    """layout for a cache's 4 or 5 strides: (ctypes array of 5, the layer's 0 for
+    a cache of one layer, whether rows are 16-byte vectors without a stride of 0)."""
+    e = _CACHE_LAYOUTS.get(stride)
+    if e is None:
+        if len(_CACHE_LAYOUTS) >= 4096:
+            _CACHE_LAYOUTS.clear()
+        five = stride if len(stride) == 5 else (0, *stride)
+        e = _CACHE_LAYOUTS[stride] = ((C.c_int64 * 5)(*five), _aligned(stride) and 0 not in stride)
     return e
 
 

@@ -7,9 +7,9 @@
 // Work unit: (sequence, kv head, tile of 128 rows); a row is a (token, q head)
 // pair of the kv head's group, tokens outermost, so a tile spans 128 / group
 // tokens and a K/V block staged in LDS serves every q head that reads it.
-// All tiles of a (sequence, kv head) run on one XCD, one after the other and
-// the longest first, so the ~64 workgroups that run there at a time share the
-// K/V of one or a few heads in its L2; with fewer pairs than XCDs, or a number
+// All tiles of a (sequence, kv head) run on one XCD, the longest first and
+// next to those of as many others as fit its L2, so the ~64 workgroups that run
+// there at a time read their K/V from it; with fewer pairs than XCDs, or a number
 // that 8 does not divide, a pair's tiles are dealt to several.
 //
 // The key loop (dense_tiles.h) ends at the tile's last token; the blocks that
@@ -44,8 +44,9 @@ struct PromptParams {
     int64_t sq_t, sq_h, sk_t, sk_h, sv_t, sv_h, so_t, so_h, sl_t, sl_h;
     int64_t total_tokens;
     int32_t B, Hq, Hkv, group, max_seqlen;
-    int32_t qtiles, spread, list;  // tiles of the longest prompt, log2 of lists per pair, tiles of a list
-    Divider gdiv, listdiv, hkvdiv;
+    int32_t qtiles, spread, list;    // tiles of the longest prompt, log2 of lists per pair, tiles of a list
+    int32_t xcd_lists, group_lists;  // lists per XCD, lists of a group
+    Divider gdiv, groupdiv, hkvdiv;  // group, tiles of a group of lists, Hkv
     float scale_log2;
 };
 
@@ -200,12 +201,16 @@ __global__ __launch_bounds__(kPromptThreads) __attribute__((amdgpu_waves_per_eu(
     __shared__ __attribute__((aligned(1024))) uint16_t smem[Tile::kSmem];
 
     // XCD x (blockIdx % 8) takes lists x, x + 8, ...: list v is every
-    // (1 << spread)-th tile of pair v >> spread, the longest first
+    // (1 << spread)-th tile of pair v >> spread, the longest first.  Lists are
+    // taken in groups, the longest tiles of a group's lists first.
     const int i = blockIdx.x >> 3;
-    const int li = divide(i, p.listdiv);
-    const int v = (blockIdx.x & 7) + 8 * li;
+    const int grp = divide(i, p.groupdiv);
+    const int in = i - grp * p.group_lists * p.list;
+    const int here = min(p.group_lists, p.xcd_lists - grp * p.group_lists);  // lists of this group
+    const int k = (int)((uint32_t)in / (uint32_t)here);
+    const int v = (blockIdx.x & 7) + 8 * (grp * p.group_lists + in - k * here);
     const int pair = v >> p.spread;
-    const int rank = ((i - li * p.list) << p.spread) + (v & ((1 << p.spread) - 1));
+    const int rank = (k << p.spread) + (v & ((1 << p.spread) - 1));
     const int qt = p.qtiles - 1 - rank;
     if (qt < 0) return;
     const int seq = divide(pair, p.hkvdiv);
@@ -339,12 +344,17 @@ int qattn_prompt_fwd(const void* q, const int64_t q_stride[3], const void* k, co
     while (pairs << p.spread & 7) ++p.spread;  // lists: a multiple of the 8 XCDs
     p.list = (p.qtiles + (1 << p.spread) - 1) >> p.spread;
     const int64_t blocks = (pairs << p.spread) * p.list;
+    // As many lists side by side as have their K/V in one XCD's L2 (4 MB): the
+    // longest tiles of them all start first, and the last ones end together.
+    const int64_t kv_bytes = 4 * (int64_t)p.max_seqlen * head_dim;
+    p.xcd_lists = (int32_t)((pairs << p.spread) / 8);
+    p.group_lists = (int32_t)std::min<int64_t>(p.xcd_lists, std::max<int64_t>(1, (4 << 20) / kv_bytes));
     if (blocks > INT32_MAX) {
         set_error("grid too large (%lld blocks)", (long long)blocks);
         return QATTN_ERR_ARG;
     }
     p.gdiv = make_divider(p.group);
-    p.listdiv = make_divider(p.list);
+    p.groupdiv = make_divider((int32_t)std::min<int64_t>((int64_t)p.group_lists * p.list, INT32_MAX));
     p.hkvdiv = make_divider(num_kv_heads);
     p.scale_log2 = scale * kLog2e;
     hipStream_t st = (hipStream_t)stream;

@@ -39,12 +39,12 @@ from typing import Optional, Sequence, Tuple, Union
 import torch
 
 from . import _lib
-from .ragged_attn import (_SUPPORTED, _check_dtypes, _device_index, _dtype_code, _no_grad, _on, _out_like, _rows16,
-                          _seqlens, _stream)
+from .ragged_attn import (_SUPPORTED, _check_dtypes, _device_index, _dtype_code, _launch, _no_grad, _out_like,
+                          _rows16, _seqlens, _vec_ok)
 
 
 def _int32(t: torch.Tensor, device) -> torch.Tensor:
-    if t.dtype is torch.int32 and t.is_contiguous() and t.device == device:
+    if t.dtype is torch.int32 and t.device == device and t.is_contiguous():
         return t
     return t.to(device=device, dtype=torch.int32, non_blocking=True).contiguous()
 
@@ -57,19 +57,18 @@ def _check_caches(K_cache, V_cache, dims: Tuple[int, ...]) -> tuple:
                          f"{tuple(K_cache.shape)}, {tuple(V_cache.shape)})")
     if K_cache.dtype not in _SUPPORTED or V_cache.dtype != K_cache.dtype:
         raise AssertionError(f"Inputs must be fp16 or bf16 (got {K_cache.dtype}, {V_cache.dtype})")
-    out = []
-    for c in (K_cache, V_cache):
-        strides, aligned, zero = _lib.layout(c.stride() if c.dim() == 5 else (0, *c.stride()))
-        p = c.data_ptr()
-        if (not aligned or p & 15) and c.numel():
-            raise ValueError(f"cache of shape {tuple(c.shape)} and strides {tuple(c.stride())} is not writable as "
-                             "16-byte rows (unit last stride, 8-element aligned strides, 16-byte aligned base)")
-        if zero and any(st == 0 and n > 1 for st, n in zip(c.stride(), c.shape)):
-            raise ValueError("cache rows overlap (a stride of 0)")
-        out += (p, strides)
-    if out[0] == out[2] and K_cache.numel():
-        raise ValueError("K_cache and V_cache are the same memory")
-    return tuple(out)
+    (ks, k_ok), (vs, v_ok) = _lib.cache_layout(K_cache.stride()), _lib.cache_layout(V_cache.stride())
+    k, v = K_cache.data_ptr(), V_cache.data_ptr()
+    if (not k_ok or not v_ok or (k | v) & 15 or k == v) and K_cache.numel():
+        for c in (K_cache, V_cache):
+            if not _vec_ok(c):
+                raise ValueError(f"cache of shape {tuple(c.shape)} and strides {tuple(c.stride())} is not writable as "
+                                 "16-byte rows (unit last stride, 8-element aligned strides, 16-byte aligned base)")
+            if any(st == 0 and n > 1 for st, n in zip(c.stride(), c.shape)):
+                raise ValueError("cache rows overlap (a stride of 0)")
+        if k == v:
+            raise ValueError("K_cache and V_cache are the same memory")
+    return k, ks, v, vs
 
 
 def _table(page_table, B: int, device) -> torch.Tensor:
@@ -120,7 +119,7 @@ def prefix_attention_paged(
     [T, Hq] fp32, natural log, if return_lse)."""
     assert K_cache.shape == V_cache.shape, "K and V cache shapes must match"
     _check_dtypes(Q, K_cache, V_cache)
-    _device_index(Q, K_cache, V_cache)
+    idx = _device_index(Q, K_cache, V_cache)
     _no_grad(Q, K_cache, V_cache)
     device = Q.device
     if Q.dim() != 3 or K_cache.dim() != 4:
@@ -143,12 +142,10 @@ def prefix_attention_paged(
     cols = pt.shape[1]
     ws_bytes = L.qattn_prefix_paged_workspace_bytes(B, ms, T, Hq, Hkv, D, cols, page_size)
     ws = torch.empty(max(ws_bytes, 1), dtype=torch.uint8, device=device)
-    with _on(device):
-        rc = L.qattn_prefix_paged_fwd(
+    _launch(idx, "qattn_prefix_paged_fwd", L.qattn_prefix_paged_fwd,
             q, qs, k, ks, v, vs, pt.data_ptr(), cols, num_pages, page_size, ctx.data_ptr(), o, os_, _lib.ptr(LSE),
             None if LSE is None else _lib.layout(LSE.stride())[0], _lib.ptr(cu), B, ms, T, Hq, Hkv, D,
-            1.0 / math.sqrt(D), _dtype_code(Q), ws.data_ptr(), ws_bytes, _stream(device))
-    _lib.check(rc, "qattn_prefix_paged_fwd")
+            1.0 / math.sqrt(D), _dtype_code(Q), ws.data_ptr(), ws_bytes)
     return (O, LSE) if return_lse else O
 
 
@@ -174,7 +171,7 @@ def append_paged_kv(
     length is passed over.  The written pages must be the sequence's own."""
     kc, kcs, vc, vcs = _check_caches(K_cache, V_cache, (4,))
     _check_dtypes(K_cache, K, V)
-    _device_index(K_cache, V_cache, K, V)
+    idx = _device_index(K_cache, V_cache, K, V)
     _no_grad(K, V, K_cache, V_cache)
     device = K.device
     num_pages, page_size, Hkv, D = K_cache.shape
@@ -188,11 +185,9 @@ def append_paged_kv(
     K, k, ks = _rows16(K)
     V, v, vs = _rows16(V)
     new = torch.empty_like(ctx)
-    with _on(device):
-        rc = _lib.lib().qattn_kv_append(
+    _launch(idx, "qattn_kv_append", _lib.lib().qattn_kv_append,
             k, ks, v, vs, kc, kcs, vc, vcs, pt.data_ptr(), pt.shape[1], num_pages, page_size, ctx.data_ptr(),
-            new.data_ptr(), _lib.ptr(cu), B, ms, T, Hkv, D, _dtype_code(K), _stream(device))
-    _lib.check(rc, "qattn_kv_append")
+            new.data_ptr(), _lib.ptr(cu), B, ms, T, Hkv, D, _dtype_code(K))
     return new
 
 
@@ -215,7 +210,7 @@ def compact_paged_kv(
     path, int32 [B] on the device.  Pages of the moved positions must be the
     sequence's own."""
     kc, kcs, vc, vcs = _check_caches(K_cache, V_cache, (4, 5))
-    _device_index(K_cache, V_cache)
+    idx = _device_index(K_cache, V_cache)
     _no_grad(K_cache, V_cache)
     device = K_cache.device
     num_pages, page_size, Hkv, D = K_cache.shape[-4:]
@@ -226,11 +221,9 @@ def compact_paged_kv(
     pt, path = _table(page_table, B, device), _int32(accepted, device)
     new = torch.empty_like(ctx)
     layers = K_cache.shape[0] if K_cache.dim() == 5 else 1
-    with _on(device):
-        rc = _lib.lib().qattn_kv_compact(
+    _launch(idx, "qattn_kv_compact", _lib.lib().qattn_kv_compact,
             kc, kcs, vc, vcs, layers, pt.data_ptr(), pt.shape[1], num_pages, page_size, ctx.data_ptr(),
-            path.data_ptr(), path.shape[1], new.data_ptr(), B, Hkv, D, _dtype_code(K_cache), _stream(device))
-    _lib.check(rc, "qattn_kv_compact")
+            path.data_ptr(), path.shape[1], new.data_ptr(), B, Hkv, D, _dtype_code(K_cache))
     return new
 
 
@@ -242,9 +235,12 @@ def _page_lists(src, dst, num_pages: int, device):
     the cache, no destination twice, none that is also a source."""
     src = src if isinstance(src, torch.Tensor) else torch.tensor(list(src), dtype=torch.int32)
     dst = dst if isinstance(dst, torch.Tensor) else torch.tensor(list(dst), dtype=torch.int32)
+    on_gpu = src.is_cuda and dst.is_cuda
     if src.dim() != 1 or src.shape != dst.shape:
         raise ValueError(f"src_pages and dst_pages must be lists of one length (got {tuple(src.shape)}, "
                          f"{tuple(dst.shape)})")
+    if on_gpu:
+        return _int32(src, device), _int32(dst, device)
     s, d = (None if t.is_cuda else t.tolist() for t in (src, dst))
     for pages in (s, d):
         if pages is not None and any(not 0 <= p < num_pages for p in pages):
@@ -270,7 +266,7 @@ def copy_kv_pages(K_cache: torch.Tensor, V_cache: torch.Tensor, src_pages: _Page
     pairs with a page outside the cache are passed over, the rest is the
     caller's to keep."""
     kc, kcs, vc, vcs = _check_caches(K_cache, V_cache, (4, 5))
-    _device_index(K_cache, V_cache)
+    idx = _device_index(K_cache, V_cache)
     _no_grad(K_cache, V_cache)
     device = K_cache.device
     num_pages, page_size, Hkv, D = K_cache.shape[-4:]
@@ -278,8 +274,6 @@ def copy_kv_pages(K_cache: torch.Tensor, V_cache: torch.Tensor, src_pages: _Page
     if not src.shape[0] or not K_cache.numel():
         return
     layers = K_cache.shape[0] if K_cache.dim() == 5 else 1
-    with _on(device):
-        rc = _lib.lib().qattn_kv_copy_pages(
+    _launch(idx, "qattn_kv_copy_pages", _lib.lib().qattn_kv_copy_pages,
             kc, kcs, vc, vcs, layers, num_pages, page_size, src.data_ptr(), dst.data_ptr(), src.shape[0], Hkv, D,
-            _dtype_code(K_cache), _stream(device))
-    _lib.check(rc, "qattn_kv_copy_pages")
+            _dtype_code(K_cache))

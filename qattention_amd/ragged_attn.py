@@ -106,7 +106,7 @@ def _no_grad(*ts) -> None:
 
 def _rows16(t: torch.Tensor):
     """_vec, with the address and the stride array of the result."""
-    strides, aligned, _ = _lib.layout(t.stride())
+    strides, aligned = _lib.layout(t.stride())
     p = t.data_ptr()
     if aligned and not p & 15:
         return t, p, strides
@@ -123,10 +123,23 @@ def _device_index(*ts) -> int:
     return idx
 
 
+def _launch(idx: int, what: str, fn, *args) -> None:
+    """fn(*args, stream) on device idx's current stream, the device made current for it."""
+    if idx not in _lib._initialised:
+        _lib.ensure_init(torch.device("cuda", idx))
+    if torch._C._cuda_getDevice() == idx:
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(idx))
+    else:
+        with torch.cuda.device(idx):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(idx))
+    if rc:
+        _lib.check(rc, what)
+
+
 def _out_like(Q: torch.Tensor):
     """An output of Q's shape, with its address and stride array."""
     O = torch.empty_like(Q)
-    strides, aligned, _ = _lib.layout(O.stride())
+    strides, aligned = _lib.layout(O.stride())
     if not aligned:
         O = torch.empty(Q.shape, dtype=Q.dtype, device=Q.device)
         strides = _lib.layout(O.stride())[0]
@@ -721,7 +734,7 @@ def prompt_attention(
     refused while autograd records.  Returns O [sum L_i, Hq, D] (and LSE
     [sum L_i, Hq] fp32, natural log, if return_lse)."""
     _check_dtypes(Q, K, V)
-    _device_index(Q, K, V)
+    idx = _device_index(Q, K, V)
     _no_grad(Q, K, V)
     device = Q.device
     if Q.dim() != 3 or K.dim() != 3 or V.dim() != 3:
@@ -737,11 +750,9 @@ def prompt_attention(
     V, v, vs = _rows16(V)
     O, o, os_ = _out_like(Q)
     LSE = torch.empty(T, Hq, dtype=torch.float32, device=device) if return_lse else None
-    with _on(device):
-        rc = _lib.lib().qattn_prompt_fwd(
+    _launch(idx, "qattn_prompt_fwd", _lib.lib().qattn_prompt_fwd,
             q, qs, k, ks, v, vs, o, os_, _lib.ptr(LSE), None if LSE is None else _lib.layout(LSE.stride())[0],
-            cu_dev.data_ptr(), B, ms, T, Hq, Hkv, D, 1.0 / math.sqrt(D), _dtype_code(Q), _stream(device))
-    _lib.check(rc, "qattn_prompt_fwd")
+            cu_dev.data_ptr(), B, ms, T, Hq, Hkv, D, 1.0 / math.sqrt(D), _dtype_code(Q))
     return (O, LSE) if return_lse else O
 
 
