@@ -409,8 +409,8 @@ int qattn_prompt_fwd(const void *q, const int64_t q_stride[3],
  * a cache spans less than 64 GiB (else QATTN_ERR_LAYOUT).  scale > 0.
  * workspace: device memory, 256-byte aligned, of at least
  * qattn_prefix_paged_workspace_bytes() for the same sizes (max_seqlen 1 with
- * cu_seqlens NULL); it is written and read by this call only, so calls that
- * may overlap need one each.
+ * cu_seqlens NULL; 0: none, and it may be NULL); it is written and read by this
+ * call only, so calls that may overlap need one each.
  */
 int64_t qattn_prefix_paged_workspace_bytes(int32_t batch, int32_t max_seqlen, int64_t total_tokens,
                                            int32_t num_q_heads, int32_t num_kv_heads,

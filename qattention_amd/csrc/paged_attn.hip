@@ -57,7 +57,9 @@ struct PagedParams {
     int32_t pt_cols, num_pages, page_size, capacity;
     int32_t nwg;          // workgroups that share the units (a multiple of 8)
     int32_t least;        // units that are worth a workgroup
+    int32_t tiles;        // tiles of the longest sequence (a workgroup per item)
     Divider pdiv, gdiv;   // page_size, group
+    Divider hkvdiv, tilediv;
     float scale_log2;
     int32_t* base;        // [B + 1] first unit of each sequence (written by the main kernel)
     float* part_m;        // [nwg][2][rows of a tile], in log2 units
@@ -107,11 +109,13 @@ struct Runs {
 // calls it; false: no unit.
 struct Share {
     int32_t u, end, start, seq, seq_base;
+    SeqWork sw;  // of seq
 };
 template <int ROWS, int KEYS>
 __device__ __forceinline__ bool find_share(const PagedParams& p, Share& sh) {
     __shared__ int32_t sums[4];
     __shared__ int32_t found[2];
+    __shared__ SeqWork found_work;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     // consecutive runs on one XCD: tiles of one item share its L2
     const int per = gridDim.x >> 3;
@@ -137,9 +141,11 @@ __device__ __forceinline__ bool find_share(const PagedParams& p, Share& sh) {
         return before + inc - mine;
     };
     int32_t total = 0, mine = 0, excl = 0;
+    SeqWork work{};
     for (int c = 0; c < p.B; c += kPagedThreads) {
         int32_t sum;
-        mine = c + tid < p.B ? seq_work<ROWS, KEYS>(p, c + tid).units(p.Hkv) : 0;
+        if (c + tid < p.B) work = seq_work<ROWS, KEYS>(p, c + tid);
+        mine = c + tid < p.B ? work.units(p.Hkv) : 0;
         excl = total + scan(mine, sum);
         if (wg == 0 && c + tid < p.B) p.base[c + tid] = excl;
         total += sum;
@@ -151,20 +157,26 @@ __device__ __forceinline__ bool find_share(const PagedParams& p, Share& sh) {
     sh.u = sh.start = runs.first(wg);
     sh.end = runs.first(wg + 1);
     if (p.B <= kPagedThreads) {
-        if (sh.u >= excl && sh.u < excl + mine) found[0] = tid, found[1] = excl;
+        if (sh.u >= excl && sh.u < excl + mine) found[0] = tid, found[1] = excl, found_work = work;
     } else {
         int32_t before = 0;
         for (int c = 0; c < p.B; c += kPagedThreads) {
             int32_t sum;
-            mine = c + tid < p.B ? seq_work<ROWS, KEYS>(p, c + tid).units(p.Hkv) : 0;
+            if (c + tid < p.B) work = seq_work<ROWS, KEYS>(p, c + tid);
+            mine = c + tid < p.B ? work.units(p.Hkv) : 0;
             excl = before + scan(mine, sum);
-            if (sh.u >= excl && sh.u < excl + mine) found[0] = c + tid, found[1] = excl;
+            if (sh.u >= excl && sh.u < excl + mine) found[0] = c + tid, found[1] = excl, found_work = work;
             before += sum;
         }
     }
     __syncthreads();
     sh.seq = __builtin_amdgcn_readfirstlane(found[0]);
     sh.seq_base = __builtin_amdgcn_readfirstlane(found[1]);
+    sh.sw.s0 = __builtin_amdgcn_readfirstlane(found_work.s0);
+    sh.sw.rows = __builtin_amdgcn_readfirstlane(found_work.rows);
+    sh.sw.tiles = __builtin_amdgcn_readfirstlane(found_work.tiles);
+    sh.sw.ctx = __builtin_amdgcn_readfirstlane(found_work.ctx);
+    sh.sw.blocks = __builtin_amdgcn_readfirstlane(found_work.blocks);
     return true;
 }
 
@@ -183,7 +195,7 @@ struct Part {
 };
 template <int ROWS, int KEYS>
 __device__ __forceinline__ SeqWork next_part(const PagedParams& p, Share& sh, Part& part) {
-    SeqWork sw = seq_work<ROWS, KEYS>(p, sh.seq);
+    SeqWork& sw = sh.sw;
     while (sh.u >= sh.seq_base + sw.units(p.Hkv)) {  // (empty sequences are passed over)
         sh.seq_base += sw.units(p.Hkv);
         sw = seq_work<ROWS, KEYS>(p, ++sh.seq);
@@ -199,13 +211,21 @@ __device__ __forceinline__ SeqWork next_part(const PagedParams& p, Share& sh, Pa
 }
 
 // ---------------------------------------------------------------------------
-// Few rows (16 QB per tile): bound by reading the cache.  A unit's 128 keys are
-// 32 per wave; nothing is shared between the waves but the last join.
+// Few rows (16 QB per tile): bound by reading the cache.  A unit's 32 NW keys
+// are 32 per wave; nothing is shared between the waves but the last join.
+// STREAM: runs of units, as above.  Otherwise a workgroup per item, for short
+// contexts, where the launch is all latency: no scan ahead of the first load and
+// no second kernel (2 x 700 keys, 32 / 8 heads: 11.8 us per call against 15, 10.9
+// against 10.4 in a graph).  A CU draws about 26 GB/s from far away however
+// many loads it has in flight (two steps of them were 3-10% slower than one),
+// so long contexts want many CUs: 2000 keys take 22.7 us so, 11.4 in runs.
 // ---------------------------------------------------------------------------
-constexpr int kUnit = 128;
+constexpr int kNarrowWaves = 4;             // waves of a STREAM workgroup
+constexpr int kUnit = 32 * kNarrowWaves;    // its keys per unit
+constexpr int kItemWaves = 8;               // waves of a workgroup per item
 
-template <typename T, int D, int QB>
-__global__ __launch_bounds__(kPagedThreads)
+template <typename T, int D, int QB, int NW, bool STREAM>
+__global__ __launch_bounds__(64 * NW)
     __attribute__((amdgpu_waves_per_eu(narrow_waves(D, QB)))) void paged_attn_kernel(PagedParams p) {
     constexpr int NC = D / 32;     // k-steps of S^T over the head dim
     constexpr int ND = D / 16;     // d-tiles of O^T
@@ -214,13 +234,18 @@ __global__ __launch_bounds__(kPagedThreads)
     constexpr int NV = 32 / RPI;   // V loads per lane and step
     constexpr int WBLK = 32 * D;   // elements of a wave's V block
     constexpr int ROWS = 16 * QB;
+    constexpr int KEYS = 32 * NW;  // of a unit
     // The waves' V blocks; after the key loop, the waves' numerators of one
-    // row block (4 x 16 rows x D floats, the same size).
-    __shared__ __attribute__((aligned(1024))) uint16_t vlds[4 * WBLK];
-    __shared__ float ml[2][4][ROWS];
+    // row block (NW x 16 rows x D floats, the same size).
+    __shared__ __attribute__((aligned(1024))) uint16_t vlds[NW * WBLK];
+    __shared__ float ml[2][NW][ROWS];
 
-    Share sh;
-    if (!find_share<ROWS, kUnit>(p, sh)) return;
+    Share sh{};
+    if constexpr (STREAM) {
+        if (!find_share<ROWS, KEYS>(p, sh)) return;
+    } else {
+        sh.end = 1;  // one part: the item
+    }
     const int tid = threadIdx.x;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int lane = tid & 63;
@@ -233,7 +258,18 @@ __global__ __launch_bounds__(kPagedThreads)
 
     while (sh.u < sh.end) {
         Part part;
-        const SeqWork sw = next_part<ROWS, kUnit>(p, sh, part);
+        SeqWork sw;
+        if constexpr (STREAM) {
+            sw = next_part<ROWS, KEYS>(p, sh, part);
+        } else {
+            const int item = divide(blockIdx.x, p.hkvdiv);
+            part.kvh = blockIdx.x - item * p.Hkv;
+            sh.seq = divide(item, p.tilediv);
+            part.tile = item - sh.seq * p.tiles;
+            sw = seq_work<ROWS, KEYS>(p, sh.seq);
+            if (part.tile >= sw.tiles) return;
+            part.b0 = 0, part.b1 = sw.blocks, part.whole = true;
+        }
         const int seq = sh.seq, kvh = part.kvh, tile = part.tile, b0 = part.b0, b1 = part.b1, ctx = sw.ctx;
 
         auto query_of = [&](int r, int64_t& qrow, int& qh) {
@@ -270,11 +306,12 @@ __global__ __launch_bounds__(kPagedThreads)
         const char* const vb = (const char*)(p.vc + kvh * p.sv_head);
         const int32_t* const pt = p.table + (int64_t)seq * p.pt_cols;
 
-        // key lane % 32 of step b: its page, or -1 (past the context)
-        auto key_at = [&](int b) { return kUnit * b + 32 * wave + (lane & 31); };
+        // key lane % 32 of step b: its page (asked for without waiting for the
+        // context's length), or -1 past the table
+        auto key_at = [&](int b) { return KEYS * b + 32 * wave + (lane & 31); };
         auto page_of = [&](int b) {
             const int pos = key_at(b);
-            return pos < ctx && b < b1 ? pt[divide(pos, p.pdiv)] : -1;
+            return pos < p.capacity ? pt[divide(pos, p.pdiv)] : -1;
         };
         // the step's loads: K rows in the A operand's layout, V rows by row
         // (load n: row n RPI + lane / DV, chunk lane % DV).  Keys that do not
@@ -282,9 +319,9 @@ __global__ __launch_bounds__(kPagedThreads)
         Vec16 kx[2][NC], vx[NV];
         uint32_t have = 0;  // bit j: key j of the step exists
         auto issue = [&](int b, int page) {
-            const bool ok = (uint32_t)page < (uint32_t)p.num_pages;
-            have = (uint32_t)__ballot(ok);
             const int pos = key_at(b);
+            const bool ok = (uint32_t)page < (uint32_t)p.num_pages && pos < ctx;
+            have = (uint32_t)__ballot(ok);
             const int slot = pos - divide(pos, p.pdiv) * p.page_size;
             // row offsets in 16-byte units (below 2^32: checked on the host)
             const uint32_t ko = ok ? (uint32_t)((page * p.sk_page + slot * p.sk_slot) >> 3) : 0u;
@@ -303,7 +340,7 @@ __global__ __launch_bounds__(kPagedThreads)
         };
         int page = page_of(b0);
         int next = page_of(b0 + 1);
-        issue(b0, page);
+        if (STREAM || b1 > 0) issue(b0, page);  // (no context: nothing to read)
         for (int b = b0; b < b1; ++b) {
             // V to LDS; rows of keys that do not exist as zeros (weight 0
             // times what lies there could be NaN)
@@ -401,7 +438,7 @@ __global__ __launch_bounds__(kPagedThreads)
             __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
         }
 
-        // ---- the four waves' states joined, row block by row block ----
+        // ---- the waves' states joined, row block by row block ----
 #pragma unroll
         for (int q = 0; q < QB; ++q) {
             l_run[q] = col4_sum(l_run[q]);
@@ -411,7 +448,7 @@ __global__ __launch_bounds__(kPagedThreads)
             }
         }
         const int64_t slot = part_slot(sh);
-        float4* const os = reinterpret_cast<float4*>(vlds);  // [4 waves][16 rows][D / 4], float4 c of row r at c ^ (r & 7)
+        float4* const os = reinterpret_cast<float4*>(vlds);  // [waves][16 rows][D / 4], float4 c of row r at c ^ (r & 7)
         constexpr int C4 = D / 4;
 #pragma unroll
         for (int q = 0; q < QB; ++q) {
@@ -425,10 +462,10 @@ __global__ __launch_bounds__(kPagedThreads)
             if (row < 16) {
                 float m = -INFINITY, l = 0.f, acc[8] = {};
 #pragma unroll
-                for (int w = 0; w < 4; ++w) m = fmaxf(m, ml[0][w][16 * q + row]);
+                for (int w = 0; w < NW; ++w) m = fmaxf(m, ml[0][w][16 * q + row]);
                 const float mc = m == -INFINITY ? 0.f : m * p.scale_log2;
 #pragma unroll
-                for (int w = 0; w < 4; ++w) {
+                for (int w = 0; w < NW; ++w) {
                     const float f = fast_exp2(__builtin_fmaf(ml[0][w][16 * q + row], p.scale_log2, -mc));
                     l += f * ml[1][w][16 * q + row];
                     const float4 x = os[(w * 16 + row) * C4 + ((2 * ch) ^ (row & 7))];
@@ -459,7 +496,7 @@ __global__ __launch_bounds__(kPagedThreads)
             }
         }
         __syncthreads();  // the LDS is free for the next item
-        sh.u += b1 - b0;
+        sh.u += STREAM ? b1 - b0 : 1;
     }
 }
 
@@ -784,17 +821,21 @@ __global__ __launch_bounds__(kPagedThreads) void paged_merge_kernel(PagedParams 
 // ---------------------------------------------------------------------------
 // Host side
 // ---------------------------------------------------------------------------
-// Kernel of a call: rows of a tile (0 row blocks: the wide kernel) and keys of a
-// unit.
+// Kernel of a call: row blocks of a tile (0: the wide kernel), rows of a tile,
+// keys of a unit, workgroups per CU, and whether every item is one workgroup's.
 struct PagedShape {
-    int qb, rows, keys, waves;
+    int qb, rows, keys, per_cu;
+    bool items;
 };
-static PagedShape paged_shape(int64_t max_rows, int head_dim) {
+static PagedShape paged_shape(int64_t max_rows, int64_t pairs, int64_t capacity, int head_dim) {
+    // a workgroup per item: three steps at most (four are slower than runs:
+    // 13.3 us against 10.4 in a graph), and every workgroup runs at once
+    if (max_rows <= 16 && capacity <= 3 * 32 * kItemWaves && pairs <= 256) return {1, 16, 32 * kItemWaves, 1, true};
     if (max_rows <= 32) {
         const int qb = max_rows <= 16 ? 1 : 2;
-        return {qb, 16 * qb, kUnit, narrow_waves(head_dim, qb)};
+        return {qb, 16 * qb, kUnit, narrow_waves(head_dim, qb), false};
     }
-    return {0, 128, kWideKeys, 2};
+    return {0, 128, kWideKeys, 2, false};
 }
 
 struct PagedSpace {
@@ -830,12 +871,17 @@ static int launch_merge(const PagedParams& p, hipStream_t st) {
 }
 
 template <typename T, int D>
-static int launch_paged(const PagedParams& p, int qb, hipStream_t st) {
+static int launch_paged(const PagedParams& p, int qb, bool items, hipStream_t st) {
     const dim3 grid(p.nwg), block(kPagedThreads);
+    if (items) {
+        hipLaunchKernelGGL((paged_attn_kernel<T, D, 1, kItemWaves, false>), dim3((uint32_t)(p.B * p.tiles * p.Hkv)),
+                           dim3(64 * kItemWaves), 0, st, p);
+        return launch_status("paged_attn_kernel, a workgroup per item");
+    }
     if (qb == 1)
-        hipLaunchKernelGGL((paged_attn_kernel<T, D, 1>), grid, block, 0, st, p);
+        hipLaunchKernelGGL((paged_attn_kernel<T, D, 1, kNarrowWaves, true>), grid, block, 0, st, p);
     else if (qb == 2)
-        hipLaunchKernelGGL((paged_attn_kernel<T, D, 2>), grid, block, 0, st, p);
+        hipLaunchKernelGGL((paged_attn_kernel<T, D, 2, kNarrowWaves, true>), grid, block, 0, st, p);
     else
         hipLaunchKernelGGL((paged_wide_kernel<T, D>), grid, block, 0, st, p);
     const int rc = launch_status(qb ? "paged_attn_kernel" : "paged_wide_kernel");
@@ -849,7 +895,7 @@ static int launch_paged(const PagedParams& p, int qb, hipStream_t st) {
 struct PagedPlan {
     int32_t max_seqlen;
     PagedShape shape;
-    int nwg, least;
+    int nwg, least, tiles;
     bool too_many;  // units past 32 bits
 };
 static bool paged_plan(PagedPlan& plan, int32_t batch, int32_t max_seqlen, int64_t total_tokens, int32_t hq,
@@ -860,14 +906,15 @@ static bool paged_plan(PagedPlan& plan, int32_t batch, int32_t max_seqlen, int64
     plan.max_seqlen = (int32_t)std::min<int64_t>(max_seqlen, total_tokens);
     if (plan.max_seqlen <= 0) return false;
     const int64_t rows = (int64_t)plan.max_seqlen * (hq / hkv);
-    plan.shape = paged_shape(rows, head_dim);
+    plan.shape = paged_shape(rows, (int64_t)batch * hkv, (int64_t)pt_cols * page_size, head_dim);
     // As many workgroups as run at once, no more than the units that the page
     // table has room for.
     const int64_t tiles = (rows + plan.shape.rows - 1) / plan.shape.rows;
     const int64_t blocks = ((int64_t)pt_cols * page_size + plan.shape.keys - 1) / plan.shape.keys;
     const double units = (double)batch * hkv * tiles * blocks;
     plan.too_many = units >= 2147483648.0;
-    plan.nwg = (int)std::min<double>(256.0 * plan.shape.waves, std::max(1.0, units));
+    plan.tiles = (int)std::min<int64_t>(tiles, INT32_MAX);
+    plan.nwg = (int)std::min<double>(256.0 * plan.shape.per_cu, std::max(1.0, units));
     plan.nwg = (plan.nwg + 7) / 8 * 8;
     plan.least = plan.shape.qb ? 1 : 2;
     return true;
@@ -886,7 +933,7 @@ int64_t qattn_prefix_paged_workspace_bytes(int32_t batch, int32_t max_seqlen, in
     if (head_dim <= 0 || !paged_plan(plan, batch, max_seqlen, total_tokens, num_q_heads, num_kv_heads, head_dim,
                                      pt_cols, page_size))
         return 0;
-    return paged_space(batch, plan.nwg, plan.shape.rows, head_dim).bytes;
+    return plan.shape.items ? 0 : paged_space(batch, plan.nwg, plan.shape.rows, head_dim).bytes;
 }
 
 int qattn_prefix_paged_fwd(const void* q, const int64_t q_stride[3], const void* k_cache, const int64_t k_stride[4],
@@ -941,11 +988,11 @@ int qattn_prefix_paged_fwd(const void* q, const int64_t q_stride[3], const void*
         }
     }
     const PagedSpace sp = paged_space(batch, plan.nwg, plan.shape.rows, head_dim);
-    if (!workspace || workspace_size < sp.bytes) {
+    if (!plan.shape.items && (!workspace || workspace_size < sp.bytes)) {
         set_error("workspace of %lld bytes needed, %lld given", (long long)sp.bytes, (long long)workspace_size);
         return QATTN_ERR_WORKSPACE;
     }
-    if ((uintptr_t)workspace & 255u) {
+    if (!plan.shape.items && (uintptr_t)workspace & 255u) {
         set_error("workspace must be 256-byte aligned");
         return QATTN_ERR_WORKSPACE;
     }
@@ -970,6 +1017,9 @@ int qattn_prefix_paged_fwd(const void* q, const int64_t q_stride[3], const void*
     p.capacity = keys ? pt_cols * page_size : 0;  // (without pages no key exists)
     p.nwg = plan.nwg;
     p.least = plan.least;
+    p.tiles = plan.tiles;
+    p.hkvdiv = make_divider(num_kv_heads);
+    p.tilediv = make_divider(plan.tiles);
     p.pdiv = make_divider(page_size);
     p.gdiv = make_divider(p.group);
     p.scale_log2 = scale * kLog2e;
@@ -980,13 +1030,14 @@ int qattn_prefix_paged_fwd(const void* q, const int64_t q_stride[3], const void*
     p.part_acc = (float*)(ws + sp.acc);
     hipStream_t st = (hipStream_t)stream;
     const int qb = plan.shape.qb;
+    const bool items = plan.shape.items;
     if (dtype == QATTN_DTYPE_F16)
-        return head_dim == 32   ? launch_paged<F16, 32>(p, qb, st)
-               : head_dim == 64 ? launch_paged<F16, 64>(p, qb, st)
-                                : launch_paged<F16, 128>(p, qb, st);
-    return head_dim == 32   ? launch_paged<BF16, 32>(p, qb, st)
-           : head_dim == 64 ? launch_paged<BF16, 64>(p, qb, st)
-                            : launch_paged<BF16, 128>(p, qb, st);
+        return head_dim == 32   ? launch_paged<F16, 32>(p, qb, items, st)
+               : head_dim == 64 ? launch_paged<F16, 64>(p, qb, items, st)
+                                : launch_paged<F16, 128>(p, qb, items, st);
+    return head_dim == 32   ? launch_paged<BF16, 32>(p, qb, items, st)
+           : head_dim == 64 ? launch_paged<BF16, 64>(p, qb, items, st)
+                            : launch_paged<BF16, 128>(p, qb, items, st);
 }
 
 }  // extern "C"

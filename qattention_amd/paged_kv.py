@@ -141,11 +141,11 @@ def prefix_attention_paged(
     L = _lib.lib()
     cols = pt.shape[1]
     ws_bytes = L.qattn_prefix_paged_workspace_bytes(B, ms, T, Hq, Hkv, D, cols, page_size)
-    ws = torch.empty(max(ws_bytes, 1), dtype=torch.uint8, device=device)
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=device) if ws_bytes else None
     _launch(idx, "qattn_prefix_paged_fwd", L.qattn_prefix_paged_fwd,
             q, qs, k, ks, v, vs, pt.data_ptr(), cols, num_pages, page_size, ctx.data_ptr(), o, os_, _lib.ptr(LSE),
             None if LSE is None else _lib.layout(LSE.stride())[0], _lib.ptr(cu), B, ms, T, Hq, Hkv, D,
-            1.0 / math.sqrt(D), _dtype_code(Q), ws.data_ptr(), ws_bytes)
+            1.0 / math.sqrt(D), _dtype_code(Q), _lib.ptr(ws), ws_bytes)
     return (O, LSE) if return_lse else O
 
 

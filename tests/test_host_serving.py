@@ -52,8 +52,8 @@ def paged(q=16, kc=16, vc=16, o=16, qs=(512, 128, 1), cs=(4096, 256, 128, 1), ta
     (ARG, dict(pages=-1)), (ARG, dict(cols=1 << 27)), (ARG, dict(scale=-1.0)), (ARG, dict(ctx=None)),
     (ARG, dict(table=None)), (ARG, dict(kc=None)), (ARG, dict(lse=16)), (LAYOUT, dict(o=8)),
     (LAYOUT, dict(cs=(4096, 255, 128, 1))), (LAYOUT, dict(cs=(-4096, 256, 128, 1))),
-    (LAYOUT, dict(cs=(1 << 35, 256, 128, 1))), (WORKSPACE, dict(ws=None)), (WORKSPACE, dict(ws=264)),
-    (WORKSPACE, dict(ws_bytes=100)), (0, dict(B=0)), (0, dict(T=0)), (0, dict(ms=0)),
+    (LAYOUT, dict(cs=(1 << 35, 256, 128, 1))), (WORKSPACE, dict(ws=None, cols=500)),
+    (WORKSPACE, dict(ws=264, cols=500)), (WORKSPACE, dict(ws_bytes=100, cols=500)), (0, dict(B=0)), (0, dict(T=0)), (0, dict(ms=0)),
 ])
 def test_paged_abi(rc, kw):
     assert paged(**kw) == rc
@@ -63,7 +63,8 @@ def test_paged_abi(rc, kw):
 def test_paged_workspace():
     ws = _lib.lib().qattn_prefix_paged_workspace_bytes
     assert ws(0, 1, 0, 32, 8, 128, 10, 16) == 0 and ws(4, 1, 4, 32, 7, 128, 10, 16) == 0
-    small, large = ws(1, 1, 1, 32, 8, 128, 8, 16), ws(64, 1, 64, 32, 8, 128, 1000, 16)
+    assert ws(1, 1, 1, 32, 8, 128, 8, 16) == 0  # a workgroup per item: no state leaves it
+    small, large = ws(1, 1, 1, 32, 8, 128, 200, 16), ws(64, 1, 64, 32, 8, 128, 1000, 16)
     assert 0 < small < large < 64 << 20
     # it does not grow with the table past what the launch can share out
     assert ws(64, 1, 64, 32, 8, 128, 8000, 16) == large
