@@ -383,8 +383,15 @@ int qattn_ragged_tree_attn_fwd_noalloc(const void *q, const int64_t q_stride[4],
  * num_kv_heads, head_dim]; the token strides of k and v are non-negative and
  * below 2^25 elements (else QATTN_ERR_LAYOUT).  Keys a token does not attend
  * never reach it, infinities and NaN in them included.  Rows of q that belong
- * to no sequence are neither read nor written.  scale > 0.
+ * to no sequence are neither read nor written.  scale > 0.  workspace: device
+ * memory, 256-byte aligned, of at least qattn_prompt_workspace_bytes() for the
+ * same sizes (0 for most: then it may be NULL); few long prompts with few heads
+ * leave the states of cut key ranges there.  Calls that may overlap need one
+ * each.
  */
+int64_t qattn_prompt_workspace_bytes(int32_t batch, int32_t max_seqlen, int64_t total_tokens,
+                                     int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim);
+
 int qattn_prompt_fwd(const void *q, const int64_t q_stride[3],
                      const void *k, const int64_t k_stride[3],
                      const void *v, const int64_t v_stride[3],
@@ -392,7 +399,8 @@ int qattn_prompt_fwd(const void *q, const int64_t q_stride[3],
                      float *lse, const int64_t lse_stride[2],
                      const int32_t *cu_seqlens, int32_t batch, int32_t max_seqlen,
                      int64_t total_tokens, int32_t num_q_heads, int32_t num_kv_heads,
-                     int32_t head_dim, float scale, int32_t dtype, void *stream);
+                     int32_t head_dim, float scale, int32_t dtype, void *workspace,
+                     int64_t workspace_size, void *stream);
 
 /*
  * Attention of query tokens over their sequence's context in a paged K/V

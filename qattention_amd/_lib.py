@@ -72,7 +72,8 @@ SIGNATURES = {
         _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _f32, _i32, _i32, _p]),
     "qattn_prompt_fwd": (C.c_int, [
         _p, _i64p, _p, _i64p, _p, _i64p, _p, _i64p, _p, _i64p,
-        _p, _i32, _i32, _i64, _i32, _i32, _i32, _f32, _i32, _p]),
+        _p, _i32, _i32, _i64, _i32, _i32, _i32, _f32, _i32, _p, _i64, _p]),
+    "qattn_prompt_workspace_bytes": (C.c_int64, [_i32, _i32, _i64, _i32, _i32, _i32]),
     "qattn_prefix_paged_workspace_bytes": (C.c_int64, [_i32, _i32, _i64, _i32, _i32, _i32, _i32, _i32]),
     "qattn_prefix_paged_fwd": (C.c_int, [
         _p, _i64p, _p, _i64p, _p, _i64p, _p, _i32, _i32, _i32, _p, _p, _i64p, _p, _i64p,

@@ -328,6 +328,17 @@ struct DenseTile {
         }
     }
 
+    // Stores the numerator as the fp32 row at acc.
+    static __device__ __forceinline__ void store_state(const f16v_t (&oacc)[DT], float* acc) {
+        acc += 4 * ((threadIdx.x >> 5) & 1);
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                *reinterpret_cast<float4*>(acc + 32 * dt + 8 * j) = make_float4(
+                    oacc[dt][4 * j], oacc[dt][4 * j + 1], oacc[dt][4 * j + 2], oacc[dt][4 * j + 3]);
+    }
+
     // Stores x = oacc * inv as the row at orow: a lane pair (l, l + 32) holds
     // dims 8 j + 0 .. 3 and 8 j + 4 .. 7 of its query; a half-wave exchange of
     // neighbouring groups gives each lane 16 contiguous bytes.  Returns 0, or NaN
@@ -346,7 +357,7 @@ struct DenseTile {
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         x[i] = oacc[dt][4 * (j + e) + i] * inv;
-                        odd += x[i] - x[i];
+                        odd = __builtin_fmaf(x[i], 0.f, odd);
                     }
                     w[e][0] = MfmaOps<T>::pack2(x[0], x[1]);
                     w[e][1] = MfmaOps<T>::pack2(x[2], x[3]);

@@ -6,7 +6,7 @@
 //   o = sum_j softmax_j(scale q.k_j) v_j,  lse = m + ln sum_j exp(s_j - m)
 // in one pass with a running maximum m and sum l.
 //
-// Work: units of 64 or 128 keys of one (sequence, kv head, row tile), numbered
+// Work: units of 32 to 128 keys of one (sequence, kv heads, row tile), numbered
 // sequence by sequence, heads, tiles and keys innermost.  The workgroups of the
 // launch take equal runs of all units, whatever the contexts' lengths (no host
 // knows them: the lengths stay on the device), so a run may end inside an item.
@@ -59,21 +59,23 @@ struct PagedParams {
     int32_t least;        // units that are worth a workgroup
     int32_t tiles;        // tiles of the longest sequence (a workgroup per item)
     Divider pdiv, gdiv;   // page_size, group
-    Divider hkvdiv, tilediv;
+    // kv heads of a workgroup and groups of them; log2 of the rows of a tile and
+    // of the keys of a unit (of one kv head)
+    int32_t heads, groups, row_shift, key_shift;
+    Divider groupdiv, tilediv, headdiv;  // groups, tiles, heads
     float scale_log2;
     int32_t* base;        // [B + 1] first unit of each sequence (written by the main kernel)
-    float* part_m;        // [nwg][2][rows of a tile], in log2 units
+    float* part_m;        // [nwg][2][heads][rows of a tile], in log2 units
     float* part_l;
-    float* part_acc;      // [nwg][2][rows of a tile][D]
+    float* part_acc;      // [nwg][2][heads][rows of a tile][D]
 };
 
-// Rows and blocks of a sequence; unit (kv head, tile, block) of it is number
-// (kvh * tiles + tile) * blocks + block.
+// Rows and blocks of a sequence; unit (group of kv heads, tile, block) of it is
+// number (group * tiles + tile) * blocks + block.
 struct SeqWork {
     int32_t s0, rows, tiles, ctx, blocks;
-    __device__ __forceinline__ int32_t units(int hkv) const { return hkv * tiles * blocks; }
+    __device__ __forceinline__ int32_t units(int groups) const { return groups * tiles * blocks; }
 };
-template <int ROWS, int KEYS>
 __device__ __forceinline__ SeqWork seq_work(const PagedParams& p, int s) {
     SeqWork w;
     w.s0 = p.cu ? p.cu[s] : s;
@@ -82,9 +84,9 @@ __device__ __forceinline__ SeqWork seq_work(const PagedParams& p, int s) {
     if (w.s0 < 0 || s1 < w.s0 || (int64_t)s1 > p.total_tokens) n = 0;
     n = min(n, p.max_seqlen);
     w.rows = n * p.group;
-    w.tiles = (w.rows + ROWS - 1) / ROWS;
+    w.tiles = (w.rows + (1 << p.row_shift) - 1) >> p.row_shift;
     w.ctx = max(0, min(p.ctx[s], p.capacity));
-    w.blocks = (w.ctx + KEYS - 1) / KEYS;
+    w.blocks = (w.ctx + (1 << p.key_shift) - 1) >> p.key_shift;
     return w;
 }
 
@@ -111,7 +113,6 @@ struct Share {
     int32_t u, end, start, seq, seq_base;
     SeqWork sw;  // of seq
 };
-template <int ROWS, int KEYS>
 __device__ __forceinline__ bool find_share(const PagedParams& p, Share& sh) {
     __shared__ int32_t sums[4];
     __shared__ int32_t found[2];
@@ -144,8 +145,8 @@ __device__ __forceinline__ bool find_share(const PagedParams& p, Share& sh) {
     SeqWork work{};
     for (int c = 0; c < p.B; c += kPagedThreads) {
         int32_t sum;
-        if (c + tid < p.B) work = seq_work<ROWS, KEYS>(p, c + tid);
-        mine = c + tid < p.B ? work.units(p.Hkv) : 0;
+        if (c + tid < p.B) work = seq_work(p, c + tid);
+        mine = c + tid < p.B ? work.units(p.groups) : 0;
         excl = total + scan(mine, sum);
         if (wg == 0 && c + tid < p.B) p.base[c + tid] = excl;
         total += sum;
@@ -162,8 +163,8 @@ __device__ __forceinline__ bool find_share(const PagedParams& p, Share& sh) {
         int32_t before = 0;
         for (int c = 0; c < p.B; c += kPagedThreads) {
             int32_t sum;
-            if (c + tid < p.B) work = seq_work<ROWS, KEYS>(p, c + tid);
-            mine = c + tid < p.B ? work.units(p.Hkv) : 0;
+            if (c + tid < p.B) work = seq_work(p, c + tid);
+            mine = c + tid < p.B ? work.units(p.groups) : 0;
             excl = before + scan(mine, sum);
             if (sh.u >= excl && sh.u < excl + mine) found[0] = c + tid, found[1] = excl, found_work = work;
             before += sum;
@@ -188,31 +189,33 @@ __device__ __forceinline__ int64_t part_slot(const Share& sh) {
 }
 
 // The part of an item that starts at the run's unit u: blocks b0 .. b1 - 1 of
-// (seq, kvh, tile); moves the share on to it and returns the sequence's work.
+// (seq, group, tile); moves the share on to it and returns the sequence's work.
 struct Part {
-    int32_t kvh, tile, b0, b1;
+    int32_t group, tile, b0, b1;
     bool whole;
 };
-template <int ROWS, int KEYS>
 __device__ __forceinline__ SeqWork next_part(const PagedParams& p, Share& sh, Part& part) {
     SeqWork& sw = sh.sw;
-    while (sh.u >= sh.seq_base + sw.units(p.Hkv)) {  // (empty sequences are passed over)
-        sh.seq_base += sw.units(p.Hkv);
-        sw = seq_work<ROWS, KEYS>(p, ++sh.seq);
+    while (sh.u >= sh.seq_base + sw.units(p.groups)) {  // (empty sequences are passed over)
+        sh.seq_base += sw.units(p.groups);
+        sw = seq_work(p, ++sh.seq);
     }
     const uint32_t in = (uint32_t)(sh.u - sh.seq_base);
     const uint32_t item = in / (uint32_t)sw.blocks;
     part.b0 = (int32_t)(in - item * (uint32_t)sw.blocks);
-    part.kvh = (int32_t)(item / (uint32_t)sw.tiles);
-    part.tile = (int32_t)(item - (uint32_t)part.kvh * (uint32_t)sw.tiles);
+    part.group = (int32_t)(item / (uint32_t)sw.tiles);
+    part.tile = (int32_t)(item - (uint32_t)part.group * (uint32_t)sw.tiles);
     part.b1 = min(sw.blocks, part.b0 + (sh.end - sh.u));
     part.whole = part.b0 == 0 && part.b1 == sw.blocks;
     return sw;
 }
 
 // ---------------------------------------------------------------------------
-// Few rows (16 QB per tile): bound by reading the cache.  A unit's 32 NW keys
-// are 32 per wave; nothing is shared between the waves but the last join.
+// Few rows (16 QB per tile): bound by reading the cache.  A workgroup's NW waves
+// are NW / HW for each of HW kv heads, 32 keys per wave and step; nothing is
+// shared between the waves but a head's last join.  Four heads per workgroup
+// read 1 KB of each cached token at a time where one head reads 256 bytes: 6.2
+// TB/s against 5.6 for the bare loads of 64 x 10240 keys.
 // STREAM: runs of units, as above.  Otherwise a workgroup per item, for short
 // contexts, where the launch is all latency: no scan ahead of the first load and
 // no second kernel (2 x 700 keys, 32 / 8 heads: 11.8 us per call against 15, 10.9
@@ -221,10 +224,9 @@ __device__ __forceinline__ SeqWork next_part(const PagedParams& p, Share& sh, Pa
 // so long contexts want many CUs: 2000 keys take 22.7 us so, 11.4 in runs.
 // ---------------------------------------------------------------------------
 constexpr int kNarrowWaves = 4;             // waves of a STREAM workgroup
-constexpr int kUnit = 32 * kNarrowWaves;    // its keys per unit
 constexpr int kItemWaves = 8;               // waves of a workgroup per item
 
-template <typename T, int D, int QB, int NW, bool STREAM>
+template <typename T, int D, int QB, int NW, int HW, bool STREAM>
 __global__ __launch_bounds__(64 * NW)
     __attribute__((amdgpu_waves_per_eu(narrow_waves(D, QB)))) void paged_attn_kernel(PagedParams p) {
     constexpr int NC = D / 32;     // k-steps of S^T over the head dim
@@ -234,7 +236,8 @@ __global__ __launch_bounds__(64 * NW)
     constexpr int NV = 32 / RPI;   // V loads per lane and step
     constexpr int WBLK = 32 * D;   // elements of a wave's V block
     constexpr int ROWS = 16 * QB;
-    constexpr int KEYS = 32 * NW;  // of a unit
+    constexpr int WPH = NW / HW;   // waves of a kv head
+    constexpr int KEYS = 32 * WPH;  // of a unit
     // The waves' V blocks; after the key loop, the waves' numerators of one
     // row block (NW x 16 rows x D floats, the same size).
     __shared__ __attribute__((aligned(1024))) uint16_t vlds[NW * WBLK];
@@ -242,7 +245,7 @@ __global__ __launch_bounds__(64 * NW)
 
     Share sh{};
     if constexpr (STREAM) {
-        if (!find_share<ROWS, KEYS>(p, sh)) return;
+        if (!find_share(p, sh)) return;
     } else {
         sh.end = 1;  // one part: the item
     }
@@ -260,17 +263,18 @@ __global__ __launch_bounds__(64 * NW)
         Part part;
         SeqWork sw;
         if constexpr (STREAM) {
-            sw = next_part<ROWS, KEYS>(p, sh, part);
+            sw = next_part(p, sh, part);
         } else {
-            const int item = divide(blockIdx.x, p.hkvdiv);
-            part.kvh = blockIdx.x - item * p.Hkv;
+            const int item = divide(blockIdx.x, p.groupdiv);
+            part.group = blockIdx.x - item * p.groups;
             sh.seq = divide(item, p.tilediv);
             part.tile = item - sh.seq * p.tiles;
-            sw = seq_work<ROWS, KEYS>(p, sh.seq);
+            sw = seq_work(p, sh.seq);
             if (part.tile >= sw.tiles) return;
             part.b0 = 0, part.b1 = sw.blocks, part.whole = true;
         }
-        const int seq = sh.seq, kvh = part.kvh, tile = part.tile, b0 = part.b0, b1 = part.b1, ctx = sw.ctx;
+        const int seq = sh.seq, tile = part.tile, b0 = part.b0, b1 = part.b1, ctx = sw.ctx;
+        const int kvh = part.group * HW + wave / WPH;
 
         auto query_of = [&](int r, int64_t& qrow, int& qh) {
             const int rr = tile * 16 * QB + r;
@@ -308,7 +312,7 @@ __global__ __launch_bounds__(64 * NW)
 
         // key lane % 32 of step b: its page (asked for without waiting for the
         // context's length), or -1 past the table
-        auto key_at = [&](int b) { return KEYS * b + 32 * wave + (lane & 31); };
+        auto key_at = [&](int b) { return KEYS * b + 32 * (wave % WPH) + (lane & 31); };
         auto page_of = [&](int b) {
             const int pos = key_at(b);
             return pos < p.capacity ? pt[divide(pos, p.pdiv)] : -1;
@@ -447,51 +451,52 @@ __global__ __launch_bounds__(64 * NW)
                 ml[1][wave][16 * q + l16] = l_run[q];
             }
         }
-        const int64_t slot = part_slot(sh);
-        float4* const os = reinterpret_cast<float4*>(vlds);  // [waves][16 rows][D / 4], float4 c of row r at c ^ (r & 7)
+        // a head's waves: [waves][16 rows][D / 4], float4 c of row r at c ^ (r & 7)
+        float4* const os = reinterpret_cast<float4*>(vlds + wave / WPH * WPH * WBLK);
         constexpr int C4 = D / 4;
+        constexpr int PASS = 64 * WPH / DV;  // rows that a head's threads take at a time
+        const int ht = tid % (64 * WPH), hw = wave / WPH * WPH;
 #pragma unroll
         for (int q = 0; q < QB; ++q) {
             __syncthreads();  // (q = 0: the key loops are done; later: the block before has been read)
 #pragma unroll
             for (int dt = 0; dt < ND; ++dt)
-                os[(wave * 16 + l16) * C4 + ((4 * dt + lq) ^ (l16 & 7))] =
+                os[(wave % WPH * 16 + l16) * C4 + ((4 * dt + lq) ^ (l16 & 7))] =
                     make_float4(oacc[q][dt][0], oacc[q][dt][1], oacc[q][dt][2], oacc[q][dt][3]);
             __syncthreads();
-            const int row = tid / DV, ch = tid % DV;
-            if (row < 16) {
+            const int ch = ht % DV;
+            for (int row = ht / DV; row < 16; row += PASS) {
+                int64_t qrow;
+                int qh;
+                if (!query_of(16 * q + row, qrow, qh)) break;
                 float m = -INFINITY, l = 0.f, acc[8] = {};
 #pragma unroll
-                for (int w = 0; w < NW; ++w) m = fmaxf(m, ml[0][w][16 * q + row]);
+                for (int w = 0; w < WPH; ++w) m = fmaxf(m, ml[0][hw + w][16 * q + row]);
                 const float mc = m == -INFINITY ? 0.f : m * p.scale_log2;
 #pragma unroll
-                for (int w = 0; w < NW; ++w) {
-                    const float f = fast_exp2(__builtin_fmaf(ml[0][w][16 * q + row], p.scale_log2, -mc));
-                    l += f * ml[1][w][16 * q + row];
+                for (int w = 0; w < WPH; ++w) {
+                    const float f = fast_exp2(__builtin_fmaf(ml[0][hw + w][16 * q + row], p.scale_log2, -mc));
+                    l += f * ml[1][hw + w][16 * q + row];
                     const float4 x = os[(w * 16 + row) * C4 + ((2 * ch) ^ (row & 7))];
                     const float4 y = os[(w * 16 + row) * C4 + ((2 * ch + 1) ^ (row & 7))];
                     acc[0] += f * x.x, acc[1] += f * x.y, acc[2] += f * x.z, acc[3] += f * x.w;
                     acc[4] += f * y.x, acc[5] += f * y.y, acc[6] += f * y.z, acc[7] += f * y.w;
                 }
-                int64_t qrow;
-                int qh;
-                if (query_of(16 * q + row, qrow, qh)) {
-                    if (part.whole) {
-                        const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+                if (part.whole) {
+                    const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) acc[j] *= inv;
-                        st16(p.o + qrow * p.so_t + qh * p.so_h + 8 * ch, pack8<T>(acc));
-                        if (p.lse && ch == 0) p.lse[qrow * p.sl_t + qh * p.sl_h] = (mc + fast_log2(l)) * kLn2;
-                    } else {
-                        const int64_t r = slot * ROWS + 16 * q + row;
-                        if (ch == 0) {
-                            p.part_m[r] = m * p.scale_log2;
-                            p.part_l[r] = l;
-                        }
-                        float4* a = reinterpret_cast<float4*>(p.part_acc + r * D + 8 * ch);
-                        a[0] = make_float4(acc[0], acc[1], acc[2], acc[3]);
-                        a[1] = make_float4(acc[4], acc[5], acc[6], acc[7]);
+                    for (int j = 0; j < 8; ++j) acc[j] *= inv;
+                    st16(p.o + qrow * p.so_t + qh * p.so_h + 8 * ch, pack8<T>(acc));
+                    if (p.lse && ch == 0) p.lse[qrow * p.sl_t + qh * p.sl_h] = (mc + fast_log2(l)) * kLn2;
+                } else {
+                    const int64_t r = (part_slot(sh) * HW + wave / WPH) * ROWS + 16 * q + row;
+                    if (ch == 0) {
+                        p.part_m[r] = m * p.scale_log2;
+                        p.part_l[r] = l;
                     }
+                    float4* a = reinterpret_cast<float4*>(p.part_acc + r * D + 8 * ch);
+                    a[0] = make_float4(acc[0], acc[1], acc[2], acc[3]);
+                    a[1] = make_float4(acc[4], acc[5], acc[6], acc[7]);
                 }
             }
         }
@@ -636,18 +641,18 @@ __global__ __launch_bounds__(kPagedThreads) __attribute__((amdgpu_waves_per_eu(2
     __shared__ __attribute__((aligned(16))) PageTable table;
 
     Share sh;
-    if (!find_share<ROWS, kWideKeys>(p, sh)) return;
+    if (!find_share(p, sh)) return;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int lane = threadIdx.x & 63;
     const int q32 = lane & 31, hl = lane >> 5;
 
     while (sh.u < sh.end) {
         Part part;
-        const SeqWork sw = next_part<ROWS, kWideKeys>(p, sh, part);
+        const SeqWork sw = next_part(p, sh, part);
         auto query_of = [&](int64_t& qrow, int& qh) {
             const int rr = part.tile * ROWS + wave * 32 + q32;
             const int tok = divide(rr, p.gdiv);
-            qh = part.kvh * p.group + (rr - tok * p.group);
+            qh = part.group * p.group + (rr - tok * p.group);
             qrow = (int64_t)sw.s0 + tok;
             return rr < sw.rows;
         };
@@ -671,7 +676,7 @@ __global__ __launch_bounds__(kPagedThreads) __attribute__((amdgpu_waves_per_eu(2
             for (int r = 0; r < 16; ++r) oacc[dt][r] = 0.f;
         const bool live = part.tile * ROWS + wave * 32 < sw.rows;
         for (int b = part.b0; b < part.b1; b += kTable) {
-            const PagedKeys<T, D> src(p, table, p.table + (int64_t)sh.seq * p.pt_cols, sw.ctx, part.kvh, b,
+            const PagedKeys<T, D> src(p, table, p.table + (int64_t)sh.seq * p.pt_cols, sw.ctx, part.group, b,
                                       min(kTable, part.b1 - b), smem);
             Tile::keys(src, smem, qf, live, src.nb, p.scale_log2, m_run, l_run, oacc);
         }
@@ -690,13 +695,7 @@ __global__ __launch_bounds__(kPagedThreads) __attribute__((amdgpu_waves_per_eu(2
                 p.part_m[r] = m_run * p.scale_log2;
                 p.part_l[r] = l;
             }
-            float* const acc = p.part_acc + r * D + 4 * hl;
-#pragma unroll
-            for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    *reinterpret_cast<float4*>(acc + 32 * dt + 8 * j) = make_float4(
-                        oacc[dt][4 * j], oacc[dt][4 * j + 1], oacc[dt][4 * j + 2], oacc[dt][4 * j + 3]);
+            Tile::store_state(oacc, p.part_acc + r * D);
         }
         sh.u += part.b1 - part.b0;
     }
@@ -710,7 +709,7 @@ __global__ __launch_bounds__(kPagedThreads) __attribute__((amdgpu_waves_per_eu(2
 // dependent loads (lengths and units, then the states): four waves per row where
 // few rows leave the chip empty.
 // ---------------------------------------------------------------------------
-template <typename T, int D, int ROWS, int KEYS, int WPR>
+template <typename T, int D, int WPR>
 __global__ __launch_bounds__(kPagedThreads) void paged_merge_kernel(PagedParams p, int32_t n_rows, Divider hqdiv,
                                                                     Divider msdiv) {
     constexpr int E = D / 64 ? D / 64 : 1;  // floats of a lane (D = 32: lanes 0 .. 31)
@@ -724,7 +723,7 @@ __global__ __launch_bounds__(kPagedThreads) void paged_merge_kernel(PagedParams 
     const int seq = divide(r0, msdiv);
     const int tok = r0 - seq * p.max_seqlen;
     const int32_t total = p.base[p.B], base = p.base[seq];  // (asked for with the sequence's lengths)
-    const SeqWork sw = seq_work<ROWS, KEYS>(p, seq);
+    const SeqWork sw = seq_work(p, seq);
     const int kvh = divide(qh, p.gdiv);
     const int rr = tok * p.group + (qh - kvh * p.group);
     if (rr >= sw.rows) return;
@@ -736,13 +735,18 @@ __global__ __launch_bounds__(kPagedThreads) void paged_merge_kernel(PagedParams 
         return;
     }
     const Runs runs(total, p.nwg, p.least);
-    const int tile = rr / ROWS;
-    const int32_t a = base + (kvh * sw.tiles + tile) * sw.blocks;
+    const int tile = rr >> p.row_shift;
+    const int grp = divide(kvh, p.headdiv);
+    const int32_t a = base + (grp * sw.tiles + tile) * sw.blocks;
     const int w0 = runs.of(a), w1 = runs.of(a + sw.blocks - 1) + 1;
     if (w0 + 1 == w1) return;  // finished by its workgroup
     // row of the workspace that holds run w's part: a run that starts inside the
     // item, or with it, holds it in state 0
-    auto at = [&](int w) { return (2 * (int64_t)w + (runs.first(w) >= a ? 0 : 1)) * ROWS + (rr - tile * ROWS); };
+    const int hl = kvh - grp * p.heads;
+    auto at = [&](int w) {
+        const int64_t state = 2 * (int64_t)w + (runs.first(w) >= a ? 0 : 1);
+        return ((state * p.heads + hl) << p.row_shift) + (rr - (tile << p.row_shift));
+    };
     const int share = WPR == 1 ? w1 - w0 : (w1 - w0 + WPR - 1) / WPR;
     const int lo = w0 + sub * share, hi = min(w1, lo + share);
     const bool in = lane * E < D;
@@ -821,29 +825,38 @@ __global__ __launch_bounds__(kPagedThreads) void paged_merge_kernel(PagedParams 
 // ---------------------------------------------------------------------------
 // Host side
 // ---------------------------------------------------------------------------
-// Kernel of a call: row blocks of a tile (0: the wide kernel), rows of a tile,
-// keys of a unit, workgroups per CU, and whether every item is one workgroup's.
+// Kernel of a call: row blocks of a tile (0: the wide kernel), log2 of its rows
+// and of a unit's keys, kv heads of a workgroup, workgroups per CU, and whether
+// every item is one workgroup's.
 struct PagedShape {
-    int qb, rows, keys, per_cu;
+    int qb, row_shift, key_shift, heads, per_cu;
     bool items;
 };
-static PagedShape paged_shape(int64_t max_rows, int64_t pairs, int64_t capacity, int head_dim) {
+static PagedShape paged_shape(int64_t max_rows, int64_t pairs, int hkv, int64_t capacity, int head_dim) {
     // a workgroup per item: three steps at most (four are slower than runs:
     // 13.3 us against 10.4 in a graph), and every workgroup runs at once
-    if (max_rows <= 16 && capacity <= 3 * 32 * kItemWaves && pairs <= 256) return {1, 16, 32 * kItemWaves, 1, true};
+    if (max_rows <= 16 && capacity <= 3 * 32 * kItemWaves && pairs <= 256) return {1, 4, 8, 1, 1, true};
     if (max_rows <= 32) {
         const int qb = max_rows <= 16 ? 1 : 2;
-        return {qb, 16 * qb, kUnit, narrow_waves(head_dim, qb), false};
+        const int per_cu = narrow_waves(head_dim, qb);
+        // Several kv heads per workgroup where the reading is most of the time:
+        // few rows, at least 16 steps per workgroup and no more than 16 parts
+        // per row, since each part leaves a state per head (64 x 8000 keys: 380 us
+        // with one head, 363 with four; 8 x 3000 keys, 32 rows: 27.1 against 36.6).
+        int heads = hkv % 4 == 0 ? 4 : hkv % 2 == 0 ? 2 : 1;
+        const int64_t steps = pairs * (((int64_t)capacity + 127) / 128);
+        if (max_rows > 8 || pairs / heads * 16 < 256 * per_cu || steps < 16 * 256 * per_cu) heads = 1;
+        return {qb, qb == 1 ? 4 : 5, heads == 4 ? 5 : heads == 2 ? 6 : 7, heads, per_cu, false};
     }
-    return {0, 128, kWideKeys, 2, false};
+    return {0, 7, 6, 1, 2, false};
 }
 
 struct PagedSpace {
     int64_t base, m, l, acc, bytes;
 };
-static PagedSpace paged_space(int32_t batch, int nwg, int rows_of_tile, int head_dim) {
+static PagedSpace paged_space(int32_t batch, int nwg, const PagedShape& shape, int head_dim) {
     auto up = [](int64_t x) { return (x + 255) / 256 * 256; };
-    const int64_t rows = 2 * (int64_t)nwg * rows_of_tile;
+    const int64_t rows = (2 * (int64_t)nwg * shape.heads) << shape.row_shift;
     PagedSpace s;
     s.base = 0;
     s.m = up(((int64_t)batch + 1) * 4);
@@ -853,7 +866,7 @@ static PagedSpace paged_space(int32_t batch, int nwg, int rows_of_tile, int head
     return s;
 }
 
-template <typename T, int D, int ROWS, int KEYS>
+template <typename T, int D>
 static int launch_merge(const PagedParams& p, hipStream_t st) {
     const int64_t rows = (int64_t)p.B * p.max_seqlen * p.Hq;
     if (rows > INT32_MAX) {
@@ -862,33 +875,33 @@ static int launch_merge(const PagedParams& p, hipStream_t st) {
     }
     const Divider hq = make_divider(p.Hq), ms = make_divider(p.max_seqlen);
     if (rows <= 512)
-        hipLaunchKernelGGL((paged_merge_kernel<T, D, ROWS, KEYS, 4>), dim3((uint32_t)rows), dim3(kPagedThreads), 0, st, p,
+        hipLaunchKernelGGL((paged_merge_kernel<T, D, 4>), dim3((uint32_t)rows), dim3(kPagedThreads), 0, st, p,
                            (int32_t)rows, hq, ms);
     else
-        hipLaunchKernelGGL((paged_merge_kernel<T, D, ROWS, KEYS, 1>), dim3((uint32_t)((rows + 3) / 4)),
+        hipLaunchKernelGGL((paged_merge_kernel<T, D, 1>), dim3((uint32_t)((rows + 3) / 4)),
                            dim3(kPagedThreads), 0, st, p, (int32_t)rows, hq, ms);
     return launch_status("paged_merge_kernel");
 }
 
 template <typename T, int D>
-static int launch_paged(const PagedParams& p, int qb, bool items, hipStream_t st) {
+static int launch_paged(const PagedParams& p, const PagedShape& sh, hipStream_t st) {
     const dim3 grid(p.nwg), block(kPagedThreads);
-    if (items) {
-        hipLaunchKernelGGL((paged_attn_kernel<T, D, 1, kItemWaves, false>), dim3((uint32_t)(p.B * p.tiles * p.Hkv)),
+    if (sh.items) {
+        hipLaunchKernelGGL((paged_attn_kernel<T, D, 1, kItemWaves, 1, false>), dim3((uint32_t)(p.B * p.tiles * p.Hkv)),
                            dim3(64 * kItemWaves), 0, st, p);
         return launch_status("paged_attn_kernel, a workgroup per item");
     }
-    if (qb == 1)
-        hipLaunchKernelGGL((paged_attn_kernel<T, D, 1, kNarrowWaves, true>), grid, block, 0, st, p);
-    else if (qb == 2)
-        hipLaunchKernelGGL((paged_attn_kernel<T, D, 2, kNarrowWaves, true>), grid, block, 0, st, p);
-    else
-        hipLaunchKernelGGL((paged_wide_kernel<T, D>), grid, block, 0, st, p);
-    const int rc = launch_status(qb ? "paged_attn_kernel" : "paged_wide_kernel");
-    if (rc) return rc;
-    return qb == 1   ? launch_merge<T, D, 16, kUnit>(p, st)
-           : qb == 2 ? launch_merge<T, D, 32, kUnit>(p, st)
-                     : launch_merge<T, D, 128, kWideKeys>(p, st);
+#define QATTN_NARROW(QB, HW) hipLaunchKernelGGL((paged_attn_kernel<T, D, QB, kNarrowWaves, HW, true>), grid, block, 0, st, p)
+    switch (8 * sh.qb + sh.heads) {
+        case 8 + 1: QATTN_NARROW(1, 1); break;
+        case 8 + 2: QATTN_NARROW(1, 2); break;
+        case 8 + 4: QATTN_NARROW(1, 4); break;
+        case 16 + 1: QATTN_NARROW(2, 1); break;
+        default: hipLaunchKernelGGL((paged_wide_kernel<T, D>), grid, block, 0, st, p);
+    }
+#undef QATTN_NARROW
+    const int rc = launch_status(sh.qb ? "paged_attn_kernel" : "paged_wide_kernel");
+    return rc ? rc : launch_merge<T, D>(p, st);
 }
 
 // What the workspace size and the launch agree on; false: nothing to launch.
@@ -906,12 +919,12 @@ static bool paged_plan(PagedPlan& plan, int32_t batch, int32_t max_seqlen, int64
     plan.max_seqlen = (int32_t)std::min<int64_t>(max_seqlen, total_tokens);
     if (plan.max_seqlen <= 0) return false;
     const int64_t rows = (int64_t)plan.max_seqlen * (hq / hkv);
-    plan.shape = paged_shape(rows, (int64_t)batch * hkv, (int64_t)pt_cols * page_size, head_dim);
+    plan.shape = paged_shape(rows, (int64_t)batch * hkv, hkv, (int64_t)pt_cols * page_size, head_dim);
     // As many workgroups as run at once, no more than the units that the page
     // table has room for.
-    const int64_t tiles = (rows + plan.shape.rows - 1) / plan.shape.rows;
-    const int64_t blocks = ((int64_t)pt_cols * page_size + plan.shape.keys - 1) / plan.shape.keys;
-    const double units = (double)batch * hkv * tiles * blocks;
+    const int64_t tiles = ((rows - 1) >> plan.shape.row_shift) + 1;
+    const int64_t blocks = ((int64_t)pt_cols * page_size + (1 << plan.shape.key_shift) - 1) >> plan.shape.key_shift;
+    const double units = (double)batch * (hkv / plan.shape.heads) * tiles * blocks;
     plan.too_many = units >= 2147483648.0;
     plan.tiles = (int)std::min<int64_t>(tiles, INT32_MAX);
     plan.nwg = (int)std::min<double>(256.0 * plan.shape.per_cu, std::max(1.0, units));
@@ -933,7 +946,7 @@ int64_t qattn_prefix_paged_workspace_bytes(int32_t batch, int32_t max_seqlen, in
     if (head_dim <= 0 || !paged_plan(plan, batch, max_seqlen, total_tokens, num_q_heads, num_kv_heads, head_dim,
                                      pt_cols, page_size))
         return 0;
-    return plan.shape.items ? 0 : paged_space(batch, plan.nwg, plan.shape.rows, head_dim).bytes;
+    return plan.shape.items ? 0 : paged_space(batch, plan.nwg, plan.shape, head_dim).bytes;
 }
 
 int qattn_prefix_paged_fwd(const void* q, const int64_t q_stride[3], const void* k_cache, const int64_t k_stride[4],
@@ -987,7 +1000,7 @@ int qattn_prefix_paged_fwd(const void* q, const int64_t q_stride[3], const void*
             }
         }
     }
-    const PagedSpace sp = paged_space(batch, plan.nwg, plan.shape.rows, head_dim);
+    const PagedSpace sp = paged_space(batch, plan.nwg, plan.shape, head_dim);
     if (!plan.shape.items && (!workspace || workspace_size < sp.bytes)) {
         set_error("workspace of %lld bytes needed, %lld given", (long long)sp.bytes, (long long)workspace_size);
         return QATTN_ERR_WORKSPACE;
@@ -1018,8 +1031,13 @@ int qattn_prefix_paged_fwd(const void* q, const int64_t q_stride[3], const void*
     p.nwg = plan.nwg;
     p.least = plan.least;
     p.tiles = plan.tiles;
-    p.hkvdiv = make_divider(num_kv_heads);
+    p.heads = plan.shape.heads;
+    p.groups = num_kv_heads / p.heads;
+    p.row_shift = plan.shape.row_shift;
+    p.key_shift = plan.shape.key_shift;
+    p.groupdiv = make_divider(p.groups);
     p.tilediv = make_divider(plan.tiles);
+    p.headdiv = make_divider(p.heads);
     p.pdiv = make_divider(page_size);
     p.gdiv = make_divider(p.group);
     p.scale_log2 = scale * kLog2e;
@@ -1029,15 +1047,13 @@ int qattn_prefix_paged_fwd(const void* q, const int64_t q_stride[3], const void*
     p.part_l = (float*)(ws + sp.l);
     p.part_acc = (float*)(ws + sp.acc);
     hipStream_t st = (hipStream_t)stream;
-    const int qb = plan.shape.qb;
-    const bool items = plan.shape.items;
     if (dtype == QATTN_DTYPE_F16)
-        return head_dim == 32   ? launch_paged<F16, 32>(p, qb, items, st)
-               : head_dim == 64 ? launch_paged<F16, 64>(p, qb, items, st)
-                                : launch_paged<F16, 128>(p, qb, items, st);
-    return head_dim == 32   ? launch_paged<BF16, 32>(p, qb, items, st)
-           : head_dim == 64 ? launch_paged<BF16, 64>(p, qb, items, st)
-                            : launch_paged<BF16, 128>(p, qb, items, st);
+        return head_dim == 32   ? launch_paged<F16, 32>(p, plan.shape, st)
+               : head_dim == 64 ? launch_paged<F16, 64>(p, plan.shape, st)
+                                : launch_paged<F16, 128>(p, plan.shape, st);
+    return head_dim == 32   ? launch_paged<BF16, 32>(p, plan.shape, st)
+           : head_dim == 64 ? launch_paged<BF16, 64>(p, plan.shape, st)
+                            : launch_paged<BF16, 128>(p, plan.shape, st);
 }
 
 }  // extern "C"

@@ -47,6 +47,13 @@ struct PromptParams {
     int32_t qtiles, spread, list;    // tiles of the longest prompt, log2 of lists per pair, tiles of a list
     int32_t xcd_lists, group_lists;  // lists per XCD, lists of a group
     Divider gdiv, groupdiv, hkvdiv;  // group, tiles of a group of lists, Hkv
+    // Cut tiles: blocks of a part at most (0: no tile is cut), parts of the
+    // longest tile; states [pair][tile][part][row] of those that are cut
+    int32_t part, parts;
+    Divider partdiv, hqdiv, msdiv;  // parts, Hq, max_seqlen
+    float* part_m;                  // in log2 units
+    float* part_l;
+    float* part_acc;                // [...][D]
     float scale_log2;
 };
 
@@ -95,6 +102,20 @@ __device__ void redo_row(const PromptParams& p, const uint16_t* q, const uint16_
 
 // The keys of a prompt tile: rows 0 .. k_hi - 1 of the sequence (the tile's last
 // token is k_hi - 1), contiguous at a token stride.
+// Parts of a tile of nb blocks; part c starts at block first(c).  Equal but for
+// one block, so with p.part >= 8 a part of a cut tile has four blocks or more:
+// the keys ahead of a tile's last part end 193 keys before the tile's last
+// token, and every row (of 128 tokens at most) sees the first block of each part.
+struct TileParts {
+    int32_t n, q, rem;
+    __device__ __forceinline__ TileParts(const PromptParams& p, int nb) {
+        n = (int)((uint32_t)(nb + p.part - 1) / (uint32_t)p.part);
+        q = (int)((uint32_t)nb / (uint32_t)n);
+        rem = nb - q * n;
+    }
+    __device__ __forceinline__ int first(int c) const { return c * q + min(c, rem); }
+};
+
 template <typename T, int D>
 struct PromptKeys {
     using Tile = DenseTile<T, D>;
@@ -102,20 +123,20 @@ struct PromptKeys {
     static constexpr int kBN = Tile::kBN, NI = Tile::NI, RPI = Tile::RPI, DV = Tile::DV, BLK = Tile::BLK;
     const char *kbase, *vbase;
     int64_t kst, vst;  // bytes between keys
-    int k_hi, nb;
+    int k_lo, k_hi, nb;  // the part's keys and blocks
     int tok_w, tok_l;  // first token of the wave, token of the lane: keys past them are masked
     uint32_t colb, krow, vrow, lds0;
     int wave;
 
-    __device__ __forceinline__ PromptKeys(const PromptParams& p, int64_t s0, int kvh, int row0, int hi,
+    __device__ __forceinline__ PromptKeys(const PromptParams& p, int64_t s0, int kvh, int row0, int lo, int hi,
                                           const uint16_t* smem) {
         const int lane = threadIdx.x & 63;
         wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
         kbase = (const char*)(p.k + s0 * p.sk_t + (int64_t)kvh * p.sk_h);
         vbase = (const char*)(p.v + s0 * p.sv_t + (int64_t)kvh * p.sv_h);
         kst = 2 * p.sk_t, vst = 2 * p.sv_t;
-        k_hi = hi;
-        nb = (hi + kBN - 1) / kBN;
+        k_lo = lo, k_hi = hi;
+        nb = (hi - lo + kBN - 1) / kBN;
         tok_w = divide(row0 + wave * 32, p.gdiv);
         tok_l = divide(row0 + wave * 32 + (lane & 31), p.gdiv);
         // Load n of wave w covers key rows (w NI + n) RPI .. + RPI - 1 of a
@@ -132,10 +153,10 @@ struct PromptKeys {
     // keys starts early (its first keys, also in the block before, are masked
     // and their V rows cleared), and a block past the end repeats it: every load
     // of the key loop is of 64 whole rows, without a bound to clamp to.
-    __device__ __forceinline__ int first(int j) const { return min(j * kBN, k_hi - kBN); }
+    __device__ __forceinline__ int first(int j) const { return min(k_lo + j * kBN, k_hi - kBN); }
     // block 0 may be the only one and shorter than 64 rows: rows past the last repeat it
     __device__ __forceinline__ void load(const char* base, int64_t st, uint32_t row, int j, uint16_t* buf) const {
-        const int kb = j == 0 ? 0 : first(j);
+        const int kb = j == 0 ? k_lo : first(j);
         const uint32_t last = (uint32_t)min(k_hi - 1 - kb, kBN - 1) * (uint32_t)st;
         const char* gb = base + (int64_t)kb * st;
 #pragma unroll
@@ -170,7 +191,7 @@ struct PromptKeys {
     }
     // keys below lo (they belong to the block before) and past the lane's token
     __device__ __forceinline__ void mask(int j, f16v_t (&s)[2]) const {
-        const int lo = j * kBN, kb = j == 0 ? 0 : first(j);
+        const int lo = k_lo + j * kBN, kb = j == 0 ? k_lo : first(j);
         if (__builtin_expect(kb < lo || kb + kBN - 1 > tok_w, 0)) {
             uint32_t k0 = (uint32_t)(kb - lo + 4 * ((threadIdx.x >> 5) & 1));
             asm volatile("" : "+v"(k0));  // (32 key numbers held across the loop would spill)
@@ -185,7 +206,7 @@ struct PromptKeys {
     }
     // the rows that the last block shares with the one before
     __device__ __forceinline__ void clean(int j, uint16_t* v) const {
-        const int shared = j > 0 ? j * kBN - first(j) : 0;
+        const int shared = j > 0 ? k_lo + j * kBN - first(j) : 0;
         if (shared > 0) {
             for (int i = threadIdx.x; i < shared * DV; i += Tile::kThreads) st16(v + 8 * i, Vec16{{0u, 0u, 0u, 0u}});
             Tile::template publish<0>();
@@ -193,7 +214,7 @@ struct PromptKeys {
     }
 };
 
-template <typename T, int D>
+template <typename T, int D, bool CUT>
 __global__ __launch_bounds__(kPromptThreads) __attribute__((amdgpu_waves_per_eu(prompt_waves(D), prompt_waves(D)))) void prompt_attn_kernel(
     PromptParams p) {
     using Tile = DenseTile<T, D>;
@@ -203,7 +224,10 @@ __global__ __launch_bounds__(kPromptThreads) __attribute__((amdgpu_waves_per_eu(
     // XCD x (blockIdx % 8) takes lists x, x + 8, ...: list v is every
     // (1 << spread)-th tile of pair v >> spread, the longest first.  Lists are
     // taken in groups, the longest tiles of a group's lists first.
-    const int i = blockIdx.x >> 3;
+    // (with cut tiles, a tile's parts next to each other)
+    const int i0 = blockIdx.x >> 3;
+    const int i = CUT ? divide(i0, p.partdiv) : i0;
+    const int cut = i0 - i * p.parts;
     const int grp = divide(i, p.groupdiv);
     const int in = i - grp * p.group_lists * p.list;
     const int here = min(p.group_lists, p.xcd_lists - grp * p.group_lists);  // lists of this group
@@ -222,6 +246,16 @@ __global__ __launch_bounds__(kPromptThreads) __attribute__((amdgpu_waves_per_eu(
     const int g = p.group;
     const int rows = n * g;
     if (qt * kBM >= rows) return;
+
+    const int k_hi = divide(min(qt * kBM + kBM, rows) - 1, p.gdiv) + 1;  // past the tile's last token
+    int k_first = 0, k_last = k_hi;
+    if constexpr (CUT) {
+        const TileParts tp(p, (k_hi + Tile::kBN - 1) / Tile::kBN);
+        if (cut >= tp.n) return;
+        k_first = tp.first(cut) * Tile::kBN;
+        k_last = min(k_hi, tp.first(cut + 1) * Tile::kBN);
+    }
+    const bool whole = !CUT || (k_first == 0 && k_last == k_hi);
 
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int lane = threadIdx.x & 63;
@@ -252,17 +286,27 @@ __global__ __launch_bounds__(kPromptThreads) __attribute__((amdgpu_waves_per_eu(
     for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
         for (int r = 0; r < 16; ++r) oacc[dt][r] = 0.f;
-    const int k_hi = divide(min(qt * kBM + kBM, rows) - 1, p.gdiv) + 1;  // past the tile's last token
-    const PromptKeys<T, D> src(p, s0, kvh, qt * kBM, k_hi, smem);
+    const PromptKeys<T, D> src(p, s0, kvh, qt * kBM, k_first, k_last, smem);
     Tile::keys(src, smem, qf, qt * kBM + wave * 32 < rows, src.nb, p.scale_log2, m_run, l_run, oacc);
 
     const float l_tot = xor32_sum(l_run);  // both halves of the query's keys
     int tok, qh;
     const bool valid = query_of(tok, qh);
+    if (CUT && !whole) {
+        if (valid) {
+            const int64_t r = (((int64_t)pair * p.qtiles + qt) * p.parts + cut) * kBM + wave * 32 + q32;
+            if (hl == 0) {
+                p.part_m[r] = m_run * p.scale_log2;
+                p.part_l[r] = l_tot;
+            }
+            Tile::store_state(oacc, p.part_acc + r * D);
+        }
+        return;
+    }
     uint16_t* const orow = p.o + ((int64_t)s0 + tok) * p.so_t + (int64_t)qh * p.so_h;
     float* const lrow = p.lse ? p.lse + ((int64_t)s0 + tok) * p.sl_t + (int64_t)qh * p.sl_h : nullptr;
     const float lse = (m_run * p.scale_log2 + fast_log2(l_tot)) * kLn2;
-    const float odd = (lse - lse) + Tile::store_row(oacc, 1.f / l_tot, orow, valid);  // 0, or NaN
+    const float odd = lse * 0.f + Tile::store_row(oacc, 1.f / l_tot, orow, valid);  // 0, or NaN
     if (valid && lrow && hl == 0) *lrow = lse;
     uint64_t again = __ballot(valid && odd != 0.f);
     if (__builtin_expect(again != 0, 0)) {
@@ -280,10 +324,128 @@ __global__ __launch_bounds__(kPromptThreads) __attribute__((amdgpu_waves_per_eu(
     }
 }
 
+// Joins the parts of cut tiles: a wave per row (token, q head), lanes across the
+// head dim.
+template <typename T, int D>
+__global__ __launch_bounds__(kPromptThreads) void prompt_merge_kernel(PromptParams p, int32_t n_rows) {
+    constexpr int E = D / 64 ? D / 64 : 1;  // floats of a lane (D = 32: lanes 0 .. 31)
+    constexpr int kBN = DenseTile<T, D>::kBN;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int row = blockIdx.x * 4 + wave;
+    if (row >= n_rows) return;
+    const int r0 = divide(row, p.hqdiv);
+    const int qh = row - r0 * p.Hq;
+    const int seq = divide(r0, p.msdiv);
+    const int tok = r0 - seq * p.max_seqlen;
+    const int32_t s0 = p.cu[seq], s1 = p.cu[seq + 1];
+    if (s0 < 0 || s1 < s0 || (int64_t)s1 > p.total_tokens) return;
+    const int n = min(s1 - s0, p.max_seqlen);
+    if (tok >= n) return;
+    const int kvh = divide(qh, p.gdiv);
+    const int rr = tok * p.group + (qh - kvh * p.group);
+    const int qt = rr / kBM;
+    const int k_hi = divide(min(qt * kBM + kBM, n * p.group) - 1, p.gdiv) + 1;
+    const int parts = TileParts(p, (k_hi + kBN - 1) / kBN).n;
+    if (parts == 1) return;  // finished by its workgroup
+    const int64_t first = (((int64_t)seq * p.Hkv + kvh) * p.qtiles + qt) * p.parts * kBM + (rr - qt * kBM);
+    const bool in = lane * E < D;
+    float m = -INFINITY, l = 0.f, acc[E] = {};
+    constexpr int U = 4;
+    for (int c = 0; c < parts; c += U) {
+        float mi[U], li[U], x[U][E];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int64_t r = first + (int64_t)min(c + u, parts - 1) * kBM;
+            mi[u] = p.part_m[r];
+            li[u] = p.part_l[r];
+#pragma unroll
+            for (int e = 0; e < E; ++e) x[u][e] = p.part_acc[r * D + (in ? lane * E : 0) + e];
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (c + u >= parts) break;
+            const float mn = fmaxf(m, mi[u]);
+            const float old = fast_exp2(m - mn), f = fast_exp2(mi[u] - mn);
+            l = l * old + f * li[u];
+#pragma unroll
+            for (int e = 0; e < E; ++e) acc[e] = acc[e] * old + f * x[u][e];
+            m = mn;
+        }
+    }
+    const int64_t t = (int64_t)s0 + tok;
+    uint16_t* const o = p.o + t * p.so_t + qh * p.so_h;
+    float* const lse = p.lse ? p.lse + t * p.sl_t + qh * p.sl_h : nullptr;
+    const float inv = 1.f / l, sum = (m + fast_log2(l)) * kLn2;
+    float odd = sum * 0.f;  // 0, or NaN if any result is not finite
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        acc[e] *= inv;
+        odd = __builtin_fmaf(acc[e], 0.f, odd);
+    }
+    if (__any(in && odd != 0.f)) {
+        redo_row<T, D>(p, p.q + t * p.sq_t + qh * p.sq_h, p.k + (int64_t)s0 * p.sk_t + (int64_t)kvh * p.sk_h,
+                       p.v + (int64_t)s0 * p.sv_t + (int64_t)kvh * p.sv_h, tok, o, lse, lane);
+        return;
+    }
+    if (in) {
+        if constexpr (E == 2)
+            *reinterpret_cast<uint32_t*>(o + 2 * lane) = MfmaOps<T>::pack2(acc[0], acc[1]);
+        else
+            o[lane] = (uint16_t)MfmaOps<T>::pack2(acc[0], 0.f);
+    }
+    if (lse && lane == 0) *lse = sum;
+}
+
 template <typename T, int D>
 static int launch_prompt(const PromptParams& p, int64_t blocks, hipStream_t st) {
-    hipLaunchKernelGGL((prompt_attn_kernel<T, D>), dim3((uint32_t)blocks), dim3(kPromptThreads), 0, st, p);
-    return launch_status("prompt_attn_kernel");
+    if (!p.part) {
+        hipLaunchKernelGGL((prompt_attn_kernel<T, D, false>), dim3((uint32_t)blocks), dim3(kPromptThreads), 0, st, p);
+        return launch_status("prompt_attn_kernel");
+    }
+    hipLaunchKernelGGL((prompt_attn_kernel<T, D, true>), dim3((uint32_t)(blocks * p.parts)), dim3(kPromptThreads), 0, st,
+                       p);
+    const int rc = launch_status("prompt_attn_kernel, cut tiles");
+    if (rc) return rc;
+    const int64_t rows = (int64_t)p.B * p.max_seqlen * p.Hq;
+    hipLaunchKernelGGL((prompt_merge_kernel<T, D>), dim3((uint32_t)((rows + 3) / 4)), dim3(kPromptThreads), 0, st, p,
+                       (int32_t)rows);
+    return launch_status("prompt_merge_kernel");
+}
+
+// Tiles of a call, and how they are cut.
+struct PromptPlan {
+    int32_t max_seqlen, group, qtiles, part, parts;
+    int64_t pairs, m, l, bytes;  // workspace: states' maxima at 0, sums at m, numerators at l
+    bool fits;
+};
+static PromptPlan prompt_plan(int32_t batch, int32_t max_seqlen, int64_t total_tokens, int32_t hq, int32_t hkv,
+                              int32_t head_dim) {
+    PromptPlan q{};
+    q.max_seqlen = (int32_t)std::min<int64_t>(max_seqlen, total_tokens);
+    q.group = hq / hkv;
+    q.pairs = (int64_t)batch * hkv;
+    q.fits = (int64_t)q.max_seqlen * q.group <= INT32_MAX / 2 && q.pairs <= INT32_MAX;
+    if (!q.fits || q.max_seqlen <= 0 || q.pairs <= 0) return q;
+    q.qtiles = (q.max_seqlen * q.group + kBM - 1) / kBM;
+    q.parts = 1;
+    // Tiles are cut where the longest one alone holds the call up: a CU with one
+    // workgroup takes 4/5 of the time per block that it takes with two, and the
+    // second kernel and the states cost what about 16 blocks take.  With as many
+    // tiles as slots the short ones next to the long ones even the CUs out by
+    // themselves (504 tiles of 2000 tokens: 42 us whole, 68 cut in two); 64 tiles
+    // of 2000 tokens: 23.4 us whole, 16.7 in parts.
+    const int64_t longest = (q.max_seqlen + 63) / 64;
+    const int64_t blocks = q.pairs * q.qtiles * (longest + 1) / 2;
+    const int64_t share = std::max<int64_t>(8, (blocks + 255) / 256);  // of a CU
+    if (longest > share * 5 / 4 + 16) {
+        q.part = (int32_t)share;
+        q.parts = (int32_t)((longest + share - 1) / share);
+        const int64_t rows = q.pairs * q.qtiles * q.parts * kBM;
+        q.m = rows * 4;
+        q.l = 2 * rows * 4;
+        q.bytes = q.l + rows * head_dim * 4;
+    }
+    return q;
 }
 
 }  // namespace qattn
@@ -292,11 +454,19 @@ using namespace qattn;
 
 extern "C" {
 
+int64_t qattn_prompt_workspace_bytes(int32_t batch, int32_t max_seqlen, int64_t total_tokens, int32_t num_q_heads,
+                                     int32_t num_kv_heads, int32_t head_dim) {
+    if (batch <= 0 || max_seqlen <= 0 || total_tokens <= 0 || num_q_heads <= 0 || num_kv_heads <= 0 || head_dim <= 0 ||
+        num_q_heads % num_kv_heads)
+        return 0;
+    return prompt_plan(batch, max_seqlen, total_tokens, num_q_heads, num_kv_heads, head_dim).bytes;
+}
+
 int qattn_prompt_fwd(const void* q, const int64_t q_stride[3], const void* k, const int64_t k_stride[3],
                      const void* v, const int64_t v_stride[3], void* o, const int64_t o_stride[3], float* lse,
                      const int64_t lse_stride[2], const int32_t* cu_seqlens, int32_t batch, int32_t max_seqlen,
                      int64_t total_tokens, int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim, float scale,
-                     int32_t dtype, void* stream) {
+                     int32_t dtype, void* workspace, int64_t workspace_size, void* stream) {
     clear_error();
     const int rc = check_common(dtype, head_dim, batch, max_seqlen, total_tokens, num_q_heads, num_kv_heads, 0);
     if (rc) return rc;
@@ -333,14 +503,30 @@ int qattn_prompt_fwd(const void* q, const int64_t q_stride[3], const void* k, co
     if (lse) p.sl_t = lse_stride[0], p.sl_h = lse_stride[1];
     p.total_tokens = total_tokens;
     p.B = batch, p.Hq = num_q_heads, p.Hkv = num_kv_heads, p.group = num_q_heads / num_kv_heads;
-    p.max_seqlen = (int32_t)std::min<int64_t>(max_seqlen, total_tokens);
-    if ((int64_t)p.max_seqlen * p.group > INT32_MAX / 2 || (int64_t)batch * num_kv_heads > INT32_MAX) {
-        set_error("sizes too large: max_seqlen=%d group=%d batch=%d num_kv_heads=%d", p.max_seqlen, p.group, batch,
+    const PromptPlan plan = prompt_plan(batch, max_seqlen, total_tokens, num_q_heads, num_kv_heads, head_dim);
+    if (!plan.fits || (plan.part && (int64_t)batch * plan.max_seqlen * num_q_heads > INT32_MAX)) {
+        set_error("sizes too large: max_seqlen=%d group=%d batch=%d num_kv_heads=%d", plan.max_seqlen, plan.group, batch,
                   num_kv_heads);
         return QATTN_ERR_ARG;
     }
-    p.qtiles = (p.max_seqlen * p.group + kBM - 1) / kBM;
-    const int64_t pairs = (int64_t)batch * num_kv_heads;
+    if (plan.bytes && (!workspace || workspace_size < plan.bytes || (uintptr_t)workspace & 255u)) {
+        set_error("a 256-byte aligned workspace of %lld bytes needed, %lld given", (long long)plan.bytes,
+                  (long long)workspace_size);
+        return QATTN_ERR_WORKSPACE;
+    }
+    p.max_seqlen = plan.max_seqlen;
+    p.qtiles = plan.qtiles;
+    p.part = plan.part;
+    p.parts = plan.parts;
+    if (plan.part) {
+        p.part_m = (float*)workspace;
+        p.part_l = (float*)((char*)workspace + plan.m);
+        p.part_acc = (float*)((char*)workspace + plan.l);
+        p.partdiv = make_divider(plan.parts);
+        p.hqdiv = make_divider(num_q_heads);
+        p.msdiv = make_divider(plan.max_seqlen);
+    }
+    const int64_t pairs = plan.pairs;
     while (pairs << p.spread & 7) ++p.spread;  // lists: a multiple of the 8 XCDs
     p.list = (p.qtiles + (1 << p.spread) - 1) >> p.spread;
     const int64_t blocks = (pairs << p.spread) * p.list;
@@ -349,7 +535,7 @@ int qattn_prompt_fwd(const void* q, const int64_t q_stride[3], const void* k, co
     const int64_t kv_bytes = 4 * (int64_t)p.max_seqlen * head_dim;
     p.xcd_lists = (int32_t)((pairs << p.spread) / 8);
     p.group_lists = (int32_t)std::min<int64_t>(p.xcd_lists, std::max<int64_t>(1, (4 << 20) / kv_bytes));
-    if (blocks > INT32_MAX) {
+    if (blocks * p.parts > INT32_MAX) {
         set_error("grid too large (%lld blocks)", (long long)blocks);
         return QATTN_ERR_ARG;
     }

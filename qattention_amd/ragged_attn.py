@@ -750,9 +750,12 @@ def prompt_attention(
     V, v, vs = _rows16(V)
     O, o, os_ = _out_like(Q)
     LSE = torch.empty(T, Hq, dtype=torch.float32, device=device) if return_lse else None
-    _launch(idx, "qattn_prompt_fwd", _lib.lib().qattn_prompt_fwd,
+    L = _lib.lib()
+    ws_bytes = L.qattn_prompt_workspace_bytes(B, ms, T, Hq, Hkv, D)
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=device) if ws_bytes else None
+    _launch(idx, "qattn_prompt_fwd", L.qattn_prompt_fwd,
             q, qs, k, ks, v, vs, o, os_, _lib.ptr(LSE), None if LSE is None else _lib.layout(LSE.stride())[0],
-            cu_dev.data_ptr(), B, ms, T, Hq, Hkv, D, 1.0 / math.sqrt(D), _dtype_code(Q))
+            cu_dev.data_ptr(), B, ms, T, Hq, Hkv, D, 1.0 / math.sqrt(D), _dtype_code(Q), _lib.ptr(ws), ws_bytes)
     return (O, LSE) if return_lse else O
 
 

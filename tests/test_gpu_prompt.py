@@ -143,7 +143,7 @@ def test_rows_of_no_sequence_stay():
     rc = _lib.lib().qattn_prompt_fwd(
         Q.data_ptr(), _lib.i64arr(Q.stride()), K.data_ptr(), _lib.i64arr(K.stride()), V.data_ptr(),
         _lib.i64arr(V.stride()), O.data_ptr(), _lib.i64arr(O.stride()), L.data_ptr(), _lib.i64arr(L.stride()),
-        cu.data_ptr(), 4, 120, T, Hq, Hkv, D, 1 / math.sqrt(D), 0, torch.cuda.current_stream().cuda_stream)
+        cu.data_ptr(), 4, 120, T, Hq, Hkv, D, 1 / math.sqrt(D), 0, None, 0, torch.cuda.current_stream().cuda_stream)
     _lib.check(rc, "qattn_prompt_fwd")
     done = torch.zeros(T, dtype=torch.bool, device=DEV)
     for a, b in ((3, 100), (90, 210)):
@@ -165,6 +165,33 @@ def test_long_prompt_rows():
     rows = torch.tensor([0, 1, 64, 65535, 65536, n - 65, n - 1], device=DEV)
     mask = torch.arange(n, device=DEV)[None, :] <= rows[:, None]
     check(O[rows], L[rows], attend64(Q[rows], K, V, mask))
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("lens,Hq,Hkv,D", [
+    ([2100], 4, 1, 128),
+    ([1900, 1899, 60], 2, 2, 64),
+    ([3001], 8, 1, 32),
+    ([1801], 3, 1, 128),
+])
+def test_cut_tiles(lens, Hq, Hkv, D, dtype):
+    """Few heads of long prompts: tiles cut into parts that a second kernel joins."""
+    from qattention_amd import _lib, prompt_attention
+    Q, K, V = inputs(lens, Hq, Hkv, D, dtype, 31)
+    say("cut", lens, Hq, Hkv, D, dtype)
+    O, L = prompt_attention(Q, K, V, offsets(lens), return_lse=True)
+    assert _lib.last_kernel() == "prompt_merge_kernel"
+    check(O, L, reference(Q, K, V, lens))
+    # what a later token holds stays out of every part
+    t = lens[0] // 2
+    V2 = V.clone()
+    V2[t, 0, 3] = math.nan
+    O2, L2 = prompt_attention(Q, K, V2, offsets(lens), return_lse=True)
+    hit = torch.zeros_like(O, dtype=torch.bool)
+    hit[t:lens[0], :Hq // Hkv, 3] = True
+    assert torch.equal(torch.isnan(O2), hit)
+    ref = reference(Q, K, V, lens)
+    check(O2.masked_fill(hit, 0), L2, [ref[0].masked_fill(hit, 0)] + list(ref[1:]))
 
 
 def test_other_stream_and_graph():

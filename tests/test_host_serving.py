@@ -23,9 +23,9 @@ def test_exports():
 
 
 def prompt(q=16, k=16, v=16, o=16, qs=(512, 128, 1), ks=(256, 128, 1), cu=16, B=1, ms=8, T=8, Hq=4, Hkv=2, D=128,
-           scale=0.1, dtype=0, lse=None):
+           scale=0.1, dtype=0, lse=None, ws=None, ws_bytes=0):
     return _lib.lib().qattn_prompt_fwd(q, i64(*qs), k, i64(*ks), v, i64(*ks), o, i64(*qs), lse, None, cu, B, ms, T, Hq,
-                                       Hkv, D, scale, dtype, None)
+                                       Hkv, D, scale, dtype, ws, ws_bytes, None)
 
 
 @pytest.mark.parametrize("rc,kw", [
@@ -33,11 +33,20 @@ def prompt(q=16, k=16, v=16, o=16, qs=(512, 128, 1), ks=(256, 128, 1), cu=16, B=
     (ARG, dict(scale=0.0)), (ARG, dict(scale=float("nan"))), (ARG, dict(scale=float("inf"))), (ARG, dict(q=None)),
     (ARG, dict(cu=None)), (ARG, dict(lse=16)), (LAYOUT, dict(q=18)), (LAYOUT, dict(qs=(512, 127, 1))),
     (LAYOUT, dict(ks=(256, 128, 2))), (LAYOUT, dict(ks=(1 << 25, 128, 1))), (0, dict(B=0)), (0, dict(ms=0)),
-    (0, dict(T=0)),
+    (0, dict(T=0)), (WORKSPACE, dict(ms=4000, T=4000)), (WORKSPACE, dict(ms=4000, T=4000, ws=256, ws_bytes=100)),
+    (WORKSPACE, dict(ms=4000, T=4000, ws=264, ws_bytes=1 << 40)),
 ])
 def test_prompt_abi(rc, kw):
     assert prompt(**kw) == rc
     assert rc == 0 or _lib.last_error()
+
+
+def test_prompt_workspace():
+    ws = _lib.lib().qattn_prompt_workspace_bytes
+    assert ws(1, 8, 8, 4, 2, 128) == 0 and ws(0, 4000, 4000, 4, 2, 128) == 0 and ws(1, 4000, 4000, 5, 2, 128) == 0
+    assert ws(64, 4000, 256000, 32, 8, 128) == 0  # tiles enough for every slot
+    rows = -(-4000 * 2 // 128) * 2 * 128
+    assert ws(1, 4000, 4000, 4, 2, 128) % (rows * 4 * 130) == 0 < ws(1, 4000, 4000, 4, 2, 128)
 
 
 def paged(q=16, kc=16, vc=16, o=16, qs=(512, 128, 1), cs=(4096, 256, 128, 1), table=16, cols=4, pages=8, ps=16,
