@@ -232,7 +232,13 @@ __global__ __launch_bounds__(kPromptThreads) __attribute__((amdgpu_waves_per_eu(
     const int in = i - grp * p.group_lists * p.list;
     const int here = min(p.group_lists, p.xcd_lists - grp * p.group_lists);  // lists of this group
     const int k = (int)((uint32_t)in / (uint32_t)here);
-    const int v = (blockIdx.x & 7) + 8 * (grp * p.group_lists + in - k * here);
+    // An XCD deals its workgroups to its shader engines in turn, however busy
+    // they are: with a list in the same place of every round, one engine would
+    // have the longest prompts' tiles to itself (16 prompts of 603 .. 2011 tokens:
+    // 210 us; turned by one place per round: 181).
+    int at = in - k * here;
+    if (!(here & 1)) at = (int)((uint32_t)(at + k) % (uint32_t)here);
+    const int v = (blockIdx.x & 7) + 8 * (grp * p.group_lists + at);
     const int pair = v >> p.spread;
     const int rank = (k << p.spread) + (v & ((1 << p.spread) - 1));
     const int qt = p.qtiles - 1 - rank;
