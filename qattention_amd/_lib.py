@@ -7,11 +7,12 @@ from __future__ import annotations
 
 import contextlib
 import ctypes as C
+import importlib.util
 import os
 
 import torch  # must be loaded first so libqattn.so binds torch's HIP runtime
 
-from .build import LIB_PATH
+from .build import CALLS_PATH, LIB_PATH
 
 QATTN_OK = 0
 ERRORS = {
@@ -91,6 +92,11 @@ SIGNATURES = {
 }
 
 _lib = None
+_calls = None
+
+# What _calls.bind takes, in its order.
+_BOUND = ("qattn_prompt_workspace_bytes", "qattn_prompt_fwd", "qattn_prefix_paged_workspace_bytes",
+          "qattn_prefix_paged_fwd", "qattn_kv_append", "qattn_kv_compact", "qattn_kv_copy_pages")
 
 
 class QAttnError(RuntimeError):
@@ -114,6 +120,25 @@ def lib():
     return _lib
 
 
+def calls():
+    """The module that makes a serving call whose operands need no conversion
+    (csrc/calls.cpp), bound to the library; raise if it has not been built."""
+    global _calls
+    if _calls is None:
+        L = lib()
+        if not os.path.exists(CALLS_PATH):
+            raise QAttnError(f"{CALLS_PATH} is missing: build it with `python -m qattention_amd.build`")
+        spec = importlib.util.spec_from_file_location("qattention_amd._calls", CALLS_PATH)
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
+        module.bind(*(C.cast(getattr(L, name), _p).value for name in _BOUND),
+                    torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream)
+        for idx in _initialised:
+            module.set_ready(idx)
+        _calls = module
+    return _calls
+
+
 _initialised = set()
 
 
@@ -128,6 +153,8 @@ def ensure_init(device) -> None:
     with torch.cuda.device(idx):
         check(lib().qattn_init(), "qattn_init")
     _initialised.add(idx)
+    if _calls is not None:
+        _calls.set_ready(idx)
 
 
 @contextlib.contextmanager

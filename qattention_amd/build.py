@@ -6,6 +6,10 @@ The library is a plain C-ABI shared object: it links only the HIP runtime.
 When loaded into a process that has already imported torch, the dynamic
 linker resolves libamdhip64.so.7 to torch's copy, so torch's streams and
 allocations are valid handles for it.
+
+_calls.so, a CPython module of the host compiler, takes the serving calls from
+torch tensors to that C ABI; it links torch's libraries, which the process has
+loaded by then.
 """
 from __future__ import annotations
 
@@ -13,6 +17,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 
 PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(PKG_DIR, "csrc")
@@ -21,6 +26,8 @@ OBJ_DIR = os.path.join(PKG_DIR, "_build")
 SOURCES = ["tree_attn.hip", "subtree_stream.hip", "prefix_attn.hip", "paged_attn.hip", "prompt_attn.hip",
            "kv_pages.hip"]
 HEADERS = ["qattn_common.h", "qattn_device.h", "kv_tiles.h", "dense_tiles.h", "tree_walk.h"]
+CALLS_SOURCE = "calls.cpp"
+CALLS_PATH = os.path.join(PKG_DIR, "_calls.so")
 ARCH = os.environ.get("QATTN_ARCH", "gfx950")
 
 
@@ -58,13 +65,28 @@ def _finish(proc, verbose):
     noise = "is not a recognized feature for this target"
     err = "\n".join(l for l in stderr.splitlines() if noise not in l)
     if proc.returncode != 0:
-        raise RuntimeError(f"hipcc failed ({proc.returncode}):\n{err}")
+        raise RuntimeError(f"{os.path.basename(proc.args[0])} failed ({proc.returncode}):\n{err}")
     if verbose and err.strip():
         print(err, file=sys.stderr)
 
 
+def calls_command(out: str) -> list:
+    """The host compiler's command for _calls.so."""
+    import torch
+    from torch.utils import cpp_extension
+
+    include = [*cpp_extension.include_paths(), sysconfig.get_paths()["include"]]
+    return [
+        os.environ.get("CXX") or shutil.which("g++") or "c++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall",
+        "-fvisibility=hidden", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+        *(f"-I{d}" for d in include), "-o", out, os.path.join(CSRC, CALLS_SOURCE),
+        "-L" + os.path.join(os.path.dirname(torch.__file__), "lib"), "-lc10", "-ltorch_cpu", "-ltorch_python",
+    ]
+
+
 def build(verbose: bool = True) -> str:
-    """Compile every HIP source into qattention_amd/libqattn.so (always rebuilds).
+    """Compile every HIP source into qattention_amd/libqattn.so and the call
+    module into qattention_amd/_calls.so (always rebuilds).
 
     Each source is compiled to an object in its own hipcc process (they run
     in parallel), then the objects are linked into the shared library."""
@@ -74,19 +96,22 @@ def build(verbose: bool = True) -> str:
         obj = os.path.join(OBJ_DIR, os.path.splitext(s)[0] + ".o")
         objs.append(obj)
         procs.append(_run([_hipcc(), *compile_flags(), "-c", "-o", obj, os.path.join(CSRC, s)], verbose))
+    calls_tmp = CALLS_PATH + ".tmp"
+    procs.append(_run(calls_command(calls_tmp), verbose))
     for proc in procs:
         _finish(proc, verbose)
     tmp = LIB_PATH + ".tmp"
     _finish(_run([_hipcc(), f"--offload-arch={ARCH}", "-shared", "-o", tmp, *objs], verbose), verbose)
+    os.replace(calls_tmp, CALLS_PATH)
     os.replace(tmp, LIB_PATH)
     return LIB_PATH
 
 
 def is_stale() -> bool:
-    if not os.path.exists(LIB_PATH):
+    if not os.path.exists(LIB_PATH) or not os.path.exists(CALLS_PATH):
         return True
-    t = os.path.getmtime(LIB_PATH)
-    deps = [os.path.join(CSRC, f) for f in SOURCES + HEADERS]
+    t = min(os.path.getmtime(LIB_PATH), os.path.getmtime(CALLS_PATH))
+    deps = [os.path.join(CSRC, f) for f in SOURCES + HEADERS + [CALLS_SOURCE]]
     deps.append(os.path.join(PKG_DIR, "..", "include", "qattn.h"))
     return any(os.path.getmtime(d) > t for d in deps if os.path.exists(d))
 

@@ -117,6 +117,9 @@ def prefix_attention_paged(
     keys; a query without any gets 0 and an LSE of -inf.  Rows of Q that
     belong to no sequence are not computed.  Returns O [T, Hq, D] (and LSE
     [T, Hq] fp32, natural log, if return_lse)."""
+    out = _lib.calls().paged(Q, K_cache, V_cache, page_table, context_lens, cu_seqlens, max_seqlen, return_lse)
+    if out is not None:
+        return out
     assert K_cache.shape == V_cache.shape, "K and V cache shapes must match"
     _check_dtypes(Q, K_cache, V_cache)
     idx = _device_index(Q, K_cache, V_cache)
@@ -169,6 +172,9 @@ def append_paged_kv(
     position that the table has no column for takes no row and does not count; a
     row whose page lies outside the cache is dropped.  A sequence with a negative
     length is passed over.  The written pages must be the sequence's own."""
+    new = _lib.calls().append(K, V, K_cache, V_cache, page_table, context_lens, cu_seqlens, max_seqlen)
+    if new is not None:
+        return new
     kc, kcs, vc, vcs = _check_caches(K_cache, V_cache, (4,))
     _check_dtypes(K_cache, K, V)
     idx = _device_index(K_cache, V_cache, K, V)
@@ -209,6 +215,9 @@ def compact_paged_kv(
     the table has no column for.  Returns the lengths afterwards, context plus
     path, int32 [B] on the device.  Pages of the moved positions must be the
     sequence's own."""
+    new = _lib.calls().compact(K_cache, V_cache, page_table, context_lens, accepted)
+    if new is not None:
+        return new
     kc, kcs, vc, vcs = _check_caches(K_cache, V_cache, (4, 5))
     idx = _device_index(K_cache, V_cache)
     _no_grad(K_cache, V_cache)
@@ -265,6 +274,8 @@ def copy_kv_pages(K_cache: torch.Tensor, V_cache: torch.Tensor, src_pages: _Page
     lists on the host are checked for that (ValueError); of lists on the GPU,
     pairs with a page outside the cache are passed over, the rest is the
     caller's to keep."""
+    if _lib.calls().copy(K_cache, V_cache, src_pages, dst_pages):
+        return
     kc, kcs, vc, vcs = _check_caches(K_cache, V_cache, (4, 5))
     idx = _device_index(K_cache, V_cache)
     _no_grad(K_cache, V_cache)

@@ -733,6 +733,9 @@ def prompt_attention(
     fused_lse_merge.  Serves inference: tensors that ask for gradients are
     refused while autograd records.  Returns O [sum L_i, Hq, D] (and LSE
     [sum L_i, Hq] fp32, natural log, if return_lse)."""
+    out = _lib.calls().prompt(Q, K, V, cu_seqlens, max_seqlen, return_lse)
+    if out is not None:
+        return out
     _check_dtypes(Q, K, V)
     idx = _device_index(Q, K, V)
     _no_grad(Q, K, V)
