@@ -34,6 +34,17 @@
 
 namespace qattn {
 
+// A mean of values of T lies in T's range; its rounded weights may carry it just
+// past: fp16's largest, 65504, would become an infinity.
+template <typename T>
+__device__ __forceinline__ float in_range(float x) {
+    if constexpr (T::kCode == F16::kCode) {
+        const float y = __builtin_amdgcn_fmed3f(x, -65504.f, 65504.f);
+        return __builtin_fabsf(x) < 131072.f ? y : x;  // (an infinity or NaN stays)
+    }
+    return x;
+}
+
 template <typename T, int D>
 struct DenseTile {
     static constexpr int kThreads = 256;
@@ -148,18 +159,16 @@ struct DenseTile {
         };
         // bf16 with a key for every row in block 0: the maximum of later blocks
         // is not looked for.  A weight keeps its 8 bits whatever its size, so the
-        // reference starts 60 powers of two above block 0's maximum (what is then
-        // flushed is 2^-66 of it) and follows a block's sum of weights after the
-        // fact, once that passes 2^kLazy.  Scores that rise by more than 2^187 in
-        // weight within one block are not finite, and the caller computes such
-        // rows again.  (fp16 weights end at 2^16.)  16384 tokens, 32 / 8 heads:
-        // 1848 -> 1803 us; 64-wide heads: 1132 -> 1078.
+        // reference follows a block's sum of weights after the fact, once that
+        // passes 2^kLazy.  Weights past 2^127 (scores that rise by 88 from one
+        // reference to the next block) are not finite, and the caller computes
+        // such rows again; fp16 weights end at 2^16 and keep the maximum.  16384
+        // tokens, 32 / 8 heads: 1848 -> 1803 us; 64-wide heads: 1132 -> 1078.
         constexpr bool kBySum = T::kCode == BF16::kCode && !Src::kEveryBlock;
-        constexpr float kLift = 60.f;
         auto follow_sum = [&](float sum) {
             sum = xor32_sum(sum);
             if (__builtin_expect(__any(sum > 256.f), 0)) {
-                const float up = sum > 256.f ? fast_log2(sum) + kLift : 0.f;
+                const float up = sum > 256.f ? fast_log2(sum) : 0.f;
                 const float alpha = fast_exp2(-up);
 #pragma unroll
                 for (int dt = 0; dt < DT; ++dt) oacc[dt] *= alpha;
@@ -296,10 +305,6 @@ struct DenseTile {
             }
             src.mask(0, sA);
             move_ref(block_max(sA));
-            if constexpr (kBySum) {
-                m_run += kLift / csc;
-                mc = m_run * csc;
-            }
             publish<0>();  // K_0 has been read; V_0 and K_1 have landed
             if (nb > 2) src.load_k(2, Kb0);
 #pragma unroll
@@ -385,7 +390,7 @@ struct DenseTile {
                     float x[4];
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        x[i] = oacc[dt][4 * (j + e) + i] * inv;
+                        x[i] = in_range<T>(oacc[dt][4 * (j + e) + i] * inv);
                         odd = __builtin_fmaf(x[i], 0.f, odd);
                     }
                     w[e][0] = MfmaOps<T>::pack2(x[0], x[1]);

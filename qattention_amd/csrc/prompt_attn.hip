@@ -95,7 +95,7 @@ __device__ void redo_row(const PromptParams& p, const uint16_t* q, const uint16_
     for (int d = 32; d; d >>= 1) l += __shfl_xor(l, d);
     if (live) {
 #pragma unroll
-        for (int e = 0; e < E; ++e) o[lane * E + e] = (uint16_t)MfmaOps<T>::pack2(acc[e] / l, 0.f);
+        for (int e = 0; e < E; ++e) o[lane * E + e] = (uint16_t)MfmaOps<T>::pack2(in_range<T>(acc[e] / l), 0.f);
     }
     if (lse && lane == 0) *lse = (m + fast_log2(l)) * kLn2;
 }
@@ -385,7 +385,7 @@ __global__ __launch_bounds__(kPromptThreads) void prompt_merge_kernel(PromptPara
     float odd = sum * 0.f;  // 0, or NaN if any result is not finite
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-        acc[e] *= inv;
+        acc[e] = in_range<T>(acc[e] * inv);
         odd = __builtin_fmaf(acc[e], 0.f, odd);
     }
     if (__any(in && odd != 0.f)) {

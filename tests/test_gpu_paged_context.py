@@ -219,6 +219,35 @@ def test_long_context():
     check(O, L, reference(Q, rows, [1]))
 
 
+@pytest.mark.parametrize("ctx,n", [(300, 1), (3000, 1), (3000, 60)])
+def test_largest_values(ctx, n):
+    from qattention_amd import prefix_attention_paged
+    Kc, Vc, table, lens, rows = paged([ctx], 16, 2, 128, torch.float16, 73)
+    Vc.copy_(torch.where(torch.isnan(Vc), Vc, torch.full_like(Vc, 65504.0)))
+    Q = queries(n, 8, 128, torch.float16, 73)
+    say("largest", ctx, n)
+    O = prefix_attention_paged(Q, Kc, Vc, table, lens, None if n == 1 else offsets([n]), return_lse=False)
+    assert bool((O == 65504.0).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_steep_scores(dtype):
+    """Scores that rise by hundreds along the context, one token and many."""
+    from qattention_amd import prefix_attention_paged
+    n, D = 1200, 64
+    Kc, Vc, table, lens, rows = paged([n], 16, 1, D, dtype, 79)
+    steps = torch.tensor([0, 30, 120, 400, 500, 100, 0], dtype=dtype, device=DEV)
+    at = table[0].long()[torch.arange(n, device=DEV) // 16], torch.arange(n, device=DEV) % 16
+    rows[0][0][:, 0, 0] = steps[torch.arange(n, device=DEV) * 7 // n]
+    Kc[at] = rows[0][0]
+    for toks in (1, 50):
+        Q = queries(toks, 2, D, dtype, 79)
+        Q[:, :, 0] = 8.0
+        say("steep", dtype, toks)
+        O, L = prefix_attention_paged(Q, Kc, Vc, table, lens, None if toks == 1 else offsets([toks]))
+        check(O, L, reference(Q, rows, [toks]))
+
+
 def test_rows_of_no_sequence_stay():
     from qattention_amd import _lib, prefix_attention_paged
     ctx, T, Hq, Hkv, D = [50, 60, 70], 40, 4, 2, 64

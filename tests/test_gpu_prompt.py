@@ -130,6 +130,31 @@ def test_scores_of_minus_infinity():
         check(O[~alone], L[~alone], [x[~alone] for x in ref])
 
 
+def test_largest_values():
+    """Means of fp16's largest value stay finite, whole tiles and cut ones."""
+    from qattention_amd import prompt_attention
+    for n, Hq, Hkv, D in ((300, 4, 2, 64), (2100, 4, 1, 128)):
+        Q, K, V = inputs([n], Hq, Hkv, D, torch.float16, 37)
+        V.fill_(-65504.0)
+        V[:, :, ::2] = 65504.0
+        say("largest", n)
+        O = prompt_attention(Q, K, V, offsets([n]))
+        assert torch.equal(O, V[:, :1].expand(n, Hq, D))
+
+
+def test_steep_scores():
+    """Scores that rise by hundreds from block to block, and fall again."""
+    from qattention_amd import prompt_attention
+    n, D = 400, 64
+    for dtype in (torch.float16, torch.bfloat16):
+        Q, K, V = inputs([n], 2, 1, D, dtype, 41)
+        Q[:, :, 0], K[:, :, 0] = 8.0, 0.0
+        K[:, 0, 0] = torch.tensor([0, 30, 120, 400, 500, 100, 0], device=DEV)[torch.arange(n, device=DEV) // 64]
+        say("steep", dtype)
+        O, L = prompt_attention(Q, K, V, offsets([n]), return_lse=True)
+        check(O, L, reference(Q, K, V, [n]))
+
+
 def test_rows_of_no_sequence_stay():
     """Through the C entry: rows in front of, between and behind the sequences keep
     what they held; bad offsets and max_seqlen cut what is computed."""
