@@ -18,14 +18,20 @@
 // iterations at a higher priority.
 //
 // A source says where the keys are:
-//   kEveryBlock         any block may hold keys that do not count (else: the last)
+//   kEveryBlock         any block may be without a key that a row attends (else
+//                       every row attends a key of block 0)
 //   load_k / load_v     all loads of block j into a buffer, before the loop
 //   dma(j)              the loads of iteration j one by one: k(n), v(n) of
 //                       K_{j+3} and V_{j+1} into the buffers of a parity
 //   mask(j, s)          -inf for the keys of block j that a row does not attend
-//   clean(j, v)         V rows of block j that no row attends set to 0 (their
-//                       weight is 0, and 0 times an infinity or a NaN is NaN): by
-//                       all waves of the workgroup, with the barrier that it needs
+//   clean<SCAN>(j, v, o...)
+//                       V rows of block j that no row attends set to 0.  SCAN:
+//                       also, what is not finite in rows that only some attend
+//                       (their weight is 0 for the others, and 0 times an infinity
+//                       or a NaN is NaN) taken out of the block and added to the
+//                       rows that do (o: the wave's numerators, none for a wave
+//                       without rows).  By all waves of the workgroup, with the
+//                       barriers it needs.
 #pragma once
 
 #include <type_traits>
@@ -68,14 +74,30 @@ struct DenseTile {
         asm volatile("s_barrier" ::: "memory");
     }
 
+    // LDS writes and reads of this wave are done, then the workgroup's barrier
+    // (loads in flight stay so).
+    static __device__ __forceinline__ void sync_lds() {
+        __builtin_amdgcn_s_waitcnt((63 & 15) | ((63 >> 4) << 14) | (7 << 4));  // lgkmcnt(0)
+        asm volatile("s_barrier" ::: "memory");
+    }
+
     // The wave's 32 rows (Q^T in qf) over blocks 0 .. nb - 1 of src, onto the
     // state m_run (maximum of raw scores), l_run (this lane's half of the sum)
     // and oacc.  live: the wave has rows (else it only stages its part of the
     // blocks).  Ends with the workgroup past its last use of the LDS only after
     // the caller's barrier.
-    template <class Src>
+    //
+    // BYSUM (bf16): the maximum of later blocks is not looked for.  A weight keeps
+    // its 8 bits whatever its size, so the reference follows a block's sum of
+    // weights after the fact, once that passes 2^8.  Weights past 2^127 (scores
+    // that rise by 88 from the reference to the next block) become infinities:
+    // the caller runs a tile whose results are not finite again, with the
+    // maximum.  16384 tokens, 32 / 8 heads: 1848 -> 1803 us; 64-wide heads:
+    // 1132 -> 1078.  (fp16 weights end at 2^16.)
+    template <bool BYSUM, bool SCAN, class Src>
     static __device__ __forceinline__ void keys(const Src& src, uint16_t* smem, const Vec16 (&qf)[KS], bool live,
                                                 int nb, float csc, float& m_run, float& l_run, f16v_t (&oacc)[DT]) {
+        static_assert(!BYSUM || (T::kCode == BF16::kCode && !Src::kEveryBlock));
         const int lane = threadIdx.x & 63;
         const int q32 = lane & 31, hl = lane >> 5;
         uint16_t *const Kb0 = smem, *const Kb1 = smem + BLK, *const Vb0 = smem + 2 * BLK;
@@ -141,8 +163,8 @@ struct DenseTile {
         constexpr float kLazy = 8.f;
         float mc = 0.f, ps0 = 0.f, ps1 = 0.f;
         auto set_mc = [&] {
-            // (no key yet: weights of -inf scores are 0, not NaN)
-            mc = Src::kEveryBlock && m_run == -INFINITY ? 0.f : m_run * csc;
+            // (no key yet, or none but of -inf scores: weights of 0, not NaN)
+            mc = m_run == -INFINITY ? 0.f : m_run * csc;
         };
         auto move_ref = [&](float mb) {
             mb = xor32_max(mb);
@@ -157,14 +179,6 @@ struct DenseTile {
             }
             set_mc();
         };
-        // bf16 with a key for every row in block 0: the maximum of later blocks
-        // is not looked for.  A weight keeps its 8 bits whatever its size, so the
-        // reference follows a block's sum of weights after the fact, once that
-        // passes 2^kLazy.  Weights past 2^127 (scores that rise by 88 from one
-        // reference to the next block) are not finite, and the caller computes
-        // such rows again; fp16 weights end at 2^16 and keep the maximum.  16384
-        // tokens, 32 / 8 heads: 1848 -> 1803 us; 64-wide heads: 1132 -> 1078.
-        constexpr bool kBySum = T::kCode == BF16::kCode && !Src::kEveryBlock;
         auto follow_sum = [&](float sum) {
             sum = xor32_sum(sum);
             if (__builtin_expect(__any(sum > 256.f), 0)) {
@@ -256,7 +270,7 @@ struct DenseTile {
                 for (int i = 0; i < NS; ++i) {
                     if (i == AB) {
                         publish<2 * NI>();
-                        if constexpr (Src::kEveryBlock) src.clean(j, Vb0 + P * BLK);
+                        if constexpr (Src::kEveryBlock || SCAN) src.template clean<SCAN>(j, Vb0 + P * BLK, oacc);
                     }
                     sn[i & 1] = mma32<T>(ka[i % FK], qf[i >> 1], sn[i & 1]);
                     if (i + FK < NS) ka[i % FK] = fetch_k(Pn{}, i + FK);
@@ -283,12 +297,12 @@ struct DenseTile {
                     weights_at(sc, NS + i);
 #pragma unroll
                     for (int e = 0; e < 16; ++e)
-                        if (!kBySum && 2 * DT + e * 2 * DT / 16 == i)
+                        if (!BYSUM && 2 * DT + e * 2 * DT / 16 == i)
                             mb = fmaxf(fmaxf(mb, sn[e >> 3][2 * (e & 7)]), sn[e >> 3][2 * (e & 7) + 1]);
                     fence();
                 }
                 l_run += ps0 + ps1;
-                if constexpr (kBySum)
+                if constexpr (BYSUM)
                     follow_sum(ps0 + ps1);
                 else
                     move_ref(mb);
@@ -305,6 +319,7 @@ struct DenseTile {
             }
             src.mask(0, sA);
             move_ref(block_max(sA));
+            if constexpr (BYSUM) m_run = m_run == -INFINITY ? 0.f : m_run;  // (a reference that can be kept)
             publish<0>();  // K_0 has been read; V_0 and K_1 have landed
             if (nb > 2) src.load_k(2, Kb0);
 #pragma unroll
@@ -323,7 +338,7 @@ struct DenseTile {
             // took D = 128 past 256 VGPRs) ----
             const uint32_t vbuf = 2 * (2 + ((nb - 1) & 1)) * BLK;
             publish<0>();
-            src.clean(nb - 1, Vb0 + ((nb - 1) & 1) * BLK);
+            src.template clean<SCAN>(nb - 1, Vb0 + ((nb - 1) & 1) * BLK, oacc);
 #pragma unroll
             for (int i = 0; i < FV; ++i) va[i] = fetch_v_at(vbuf, i);
             // its weights, those of each 16-key step beside the products of the one before
@@ -352,13 +367,13 @@ struct DenseTile {
 #pragma unroll
                 for (int n = 0; n < NI; ++n) dma.v(buf, n);
                 publish<2 * NI>();
-                if constexpr (Src::kEveryBlock) src.clean(j, Vb0 + (j & 1) * BLK);
+                if constexpr (Src::kEveryBlock || SCAN) src.template clean<SCAN>(j, Vb0 + (j & 1) * BLK);
 #pragma unroll
                 for (int n = 0; n < NI; ++n) dma.k(buf, n);
                 publish<2 * NI>();
             }
             publish<0>();
-            src.clean(nb - 1, Vb0 + ((nb - 1) & 1) * BLK);
+            src.template clean<SCAN>(nb - 1, Vb0 + ((nb - 1) & 1) * BLK);
         }
     }
 
@@ -373,13 +388,11 @@ struct DenseTile {
                     oacc[dt][4 * j], oacc[dt][4 * j + 1], oacc[dt][4 * j + 2], oacc[dt][4 * j + 3]);
     }
 
-    // Stores x = oacc * inv as the row at orow: a lane pair (l, l + 32) holds
-    // dims 8 j + 0 .. 3 and 8 j + 4 .. 7 of its query; a half-wave exchange of
-    // neighbouring groups gives each lane 16 contiguous bytes.  Returns 0, or NaN
-    // if an x is not finite.
-    static __device__ __forceinline__ float store_row(const f16v_t (&oacc)[DT], float inv, uint16_t* orow, bool valid) {
+    // Stores oacc * inv as the row at orow: a lane pair (l, l + 32) holds dims
+    // 8 j + 0 .. 3 and 8 j + 4 .. 7 of its query; a half-wave exchange of
+    // neighbouring groups gives each lane 16 contiguous bytes.
+    static __device__ __forceinline__ void store_row(const f16v_t (&oacc)[DT], float inv, uint16_t* orow, bool valid) {
         const int hl = (threadIdx.x >> 5) & 1;
-        float odd = 0.f;
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) {
 #pragma unroll
@@ -389,10 +402,7 @@ struct DenseTile {
                 for (int e = 0; e < 2; ++e) {
                     float x[4];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        x[i] = in_range<T>(oacc[dt][4 * (j + e) + i] * inv);
-                        odd = __builtin_fmaf(x[i], 0.f, odd);
-                    }
+                    for (int i = 0; i < 4; ++i) x[i] = in_range<T>(oacc[dt][4 * (j + e) + i] * inv);
                     w[e][0] = MfmaOps<T>::pack2(x[0], x[1]);
                     w[e][1] = MfmaOps<T>::pack2(x[2], x[3]);
                 }
@@ -404,7 +414,6 @@ struct DenseTile {
                          Vec16{{(uint32_t)a[0], (uint32_t)b[0], (uint32_t)a[1], (uint32_t)b[1]}});
             }
         }
-        return odd;
     }
 };
 

@@ -653,7 +653,8 @@ struct PagedKeys {
                     if (!((uint32_t)(have >> (32 * t)) >> (8 * (r >> 2) + (r & 3)) & 1)) s[t][r] = -INFINITY;
         }
     }
-    __device__ __forceinline__ void clean(int j, uint16_t* v) const {
+    template <bool SCAN, class... O>
+    __device__ __forceinline__ void clean(int j, uint16_t* v, O&...) const {
         if (__builtin_expect(bad >> j & 1, 0)) {
             const uint64_t have = tab->have[j];
             for (int i = threadIdx.x; i < kWideKeys * DV; i += Tile::kThreads)
@@ -709,7 +710,7 @@ __global__ __launch_bounds__(kPagedThreads) __attribute__((amdgpu_waves_per_eu(2
         for (int b = part.b0; b < part.b1; b += kTable) {
             const PagedKeys<T, D> src(p, table, p.table + (int64_t)sh.seq * p.pt_cols, sw.ctx, part.group, b,
                                       min(kTable, part.b1 - b), smem);
-            Tile::keys(src, smem, qf, live, src.nb, p.scale_log2, m_run, l_run, oacc);
+            Tile::template keys<false, false>(src, smem, qf, live, src.nb, p.scale_log2, m_run, l_run, oacc);
         }
         const float l = xor32_sum(l_run);
         int64_t qrow;

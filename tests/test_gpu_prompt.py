@@ -155,6 +155,41 @@ def test_steep_scores():
         check(O, L, reference(Q, K, V, [n]))
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("D,Hkv,n", [(128, 2, 300), (64, 4, 300), (32, 1, 190), (64, 1, 2100)])
+def test_infinities_and_nan_of_v(D, Hkv, n, dtype):
+    """A row is the finite values' mean plus the infinities and NaN that it attends,
+    by their dims; their neighbours in the same block do not change."""
+    from qattention_amd import prompt_attention
+    Hq = 4
+    Q, K, V = inputs([n], Hq, Hkv, D, dtype, 43)
+    for t, d, x in ((n - 7, 3, math.inf), (n - 40, 9, -math.inf), (n - 31, 9, math.inf), (n - 31, 20, math.nan),
+                    (130, 30, -math.inf), (5, 31, math.inf)):
+        V[t, Hkv - 1, d] = x
+    say("odd values", D, Hkv, n, dtype)
+    O, L = prompt_attention(Q, K, V, offsets([n]), return_lse=True)
+    finite = torch.where(V.isfinite(), V, 0)
+    odd = torch.where(V.isfinite(), 0, V).float().cumsum(0).repeat_interleave(Hq // Hkv, 1)
+    hit = odd != 0
+    assert torch.equal(O[hit].float().nan_to_num(9.0, 2.0, -2.0), odd[hit].nan_to_num(9.0, 2.0, -2.0))
+    ref = reference(Q, K, finite, [n])
+    check(O.masked_fill(hit, 0), L, [ref[0].masked_fill(hit, 0)] + list(ref[1:]))
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_low_scores_behind_minus_infinity(dtype):
+    """A whole block of -inf scores, then scores of about -100: only rows within
+    the block have no mean."""
+    from qattention_amd import prompt_attention
+    n, D, m = 230, 64, 64
+    Q, K, V = inputs([n], 2, 1, D, dtype, 47)
+    Q[:, :, 0], K[:, 0, 0], K[:m, 0, 0] = 8.0, -100.0, -math.inf
+    say("low", dtype)
+    O, L = prompt_attention(Q, K, V, offsets([n]), return_lse=True)
+    assert O[:m].isnan().all() and (L[:m] == -math.inf).all()
+    check(O[m:], L[m:], reference(Q[m:], K[m:], V[m:], [n - m]))
+
+
 def test_rows_of_no_sequence_stay():
     """Through the C entry: rows in front of, between and behind the sequences keep
     what they held; bad offsets and max_seqlen cut what is computed."""
