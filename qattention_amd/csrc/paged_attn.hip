@@ -61,10 +61,14 @@ struct PagedParams {
     Divider pdiv, gdiv;   // page_size, group
     // kv heads of a workgroup and groups of them; log2 of the rows of a tile and
     // of the keys of a unit (of one kv head)
-    int32_t heads, groups, row_shift, key_shift;
-    Divider groupdiv, tilediv, headdiv;  // groups, tiles, heads
+    int32_t heads, head_shift, groups, row_shift, key_shift;
+    Divider groupdiv, tilediv;  // groups, tiles
     float scale_log2;
-    int32_t* base;        // [B + 1] first unit of each sequence (written by the main kernel)
+    // what the merge needs of the work's order, written by the main kernel:
+    // the first unit of each sequence [B + 1], or (cuts not null) the item that
+    // each run's first unit lies in
+    int32_t* base;
+    struct RunStart* cuts;  // [nwg]
     float* part_m;        // [nwg][2][heads][rows of a tile], in log2 units
     float* part_l;
     float* part_acc;      // [nwg][2][heads][rows of a tile][D]
@@ -86,9 +90,15 @@ __device__ __forceinline__ SeqWork seq_work(const PagedParams& p, int s) {
     w.rows = n * p.group;
     w.tiles = (w.rows + (1 << p.row_shift) - 1) >> p.row_shift;
     w.ctx = max(0, min(p.ctx[s], p.capacity));
-    w.blocks = (w.ctx + (1 << p.key_shift) - 1) >> p.key_shift;
+    // (rows without a context are a block without keys: 0 and -inf)
+    w.blocks = max(1, (w.ctx + (1 << p.key_shift) - 1) >> p.key_shift);
     return w;
 }
+
+// The item that a run starts in; b0: the blocks of it that runs before hold.
+struct RunStart {
+    int32_t s0, rows, tile, group, b0, blocks, first, total;  // first: the item's first unit
+};
 
 // Equal runs of the units: run w starts at first(w).  (The host checks that
 // the units of the longest contexts stay below 2^31.)
@@ -110,9 +120,13 @@ struct Runs {
 // Workgroup 0 leaves the sequences' first units to the merge.  Every thread
 // calls it; false: no unit.
 struct Share {
-    int32_t u, end, start, seq, seq_base;
+    int32_t u, end, start, seq, seq_base, total;
     SeqWork sw;  // of seq
 };
+__device__ __forceinline__ bool no_share(const PagedParams& p, int wg) {
+    if (p.cuts && threadIdx.x == 0) p.cuts[wg] = RunStart{};
+    return false;
+}
 __device__ __forceinline__ bool find_share(const PagedParams& p, Share& sh) {
     __shared__ int32_t sums[4];
     __shared__ int32_t found[2];
@@ -139,9 +153,10 @@ __device__ __forceinline__ bool find_share(const PagedParams& p, Share& sh) {
             if (lane == 0) p.base[p.B] = total;
         }
         const Runs runs(total, p.nwg, p.least);
-        if (wg >= runs.n || total == 0) return false;
+        if (wg >= runs.n || total == 0) return no_share(p, wg);
         sh.u = sh.start = runs.first(wg);
         sh.end = runs.first(wg + 1);
+        sh.total = total;
         const int at = __builtin_ctzll(__ballot(sh.u < inc));  // the first sequence that ends past u
         sh.seq = at;
         sh.seq_base = __builtin_amdgcn_readlane(inc - mine, at);
@@ -185,9 +200,10 @@ __device__ __forceinline__ bool find_share(const PagedParams& p, Share& sh) {
     total = __builtin_amdgcn_readfirstlane(total);  // (what follows from it stays in scalar registers)
     if (wg == 0 && tid == 0) p.base[p.B] = total;
     const Runs runs(total, p.nwg, p.least);
-    if (wg >= runs.n || total == 0) return false;
+    if (wg >= runs.n || total == 0) return no_share(p, wg);
     sh.u = sh.start = runs.first(wg);
     sh.end = runs.first(wg + 1);
+    sh.total = total;
     if (p.B <= kPagedThreads) {
         if (sh.u >= excl && sh.u < excl + mine) found[0] = tid, found[1] = excl, found_work = work;
     } else {
@@ -238,6 +254,11 @@ __device__ __forceinline__ SeqWork next_part(const PagedParams& p, Share& sh, Pa
     part.tile = (int32_t)(item - (uint32_t)part.group * (uint32_t)sw.tiles);
     part.b1 = min(sw.blocks, part.b0 + (sh.end - sh.u));
     part.whole = part.b0 == 0 && part.b1 == sw.blocks;
+    if (p.cuts && sh.u == sh.start && threadIdx.x == 0) {
+        const int per = gridDim.x >> 3;
+        p.cuts[(blockIdx.x & 7) * per + (blockIdx.x >> 3)] =
+            RunStart{sw.s0, sw.rows, part.tile, part.group, part.b0, sw.blocks, sh.u - part.b0, sh.total};
+    }
     return sw;
 }
 
@@ -375,7 +396,7 @@ __global__ __launch_bounds__(64 * NW)
         };
         int page = page_of(b0);
         int next = page_of(b0 + 1);
-        if (STREAM || b1 > 0) issue(b0, page);  // (no context: nothing to read)
+        if (ctx > 0) issue(b0, page);  // (no context: nothing to read, maybe no cache)
         for (int b = b0; b < b1; ++b) {
             // V to LDS; rows of keys that do not exist as zeros (weight 0
             // times what lies there could be NaN)
@@ -707,7 +728,7 @@ __global__ __launch_bounds__(kPagedThreads) __attribute__((amdgpu_waves_per_eu(2
 #pragma unroll
             for (int r = 0; r < 16; ++r) oacc[dt][r] = 0.f;
         const bool live = part.tile * ROWS + wave * 32 < sw.rows;
-        for (int b = part.b0; b < part.b1; b += kTable) {
+        for (int b = part.b0; b < part.b1 && sw.ctx > 0; b += kTable) {
             const PagedKeys<T, D> src(p, table, p.table + (int64_t)sh.seq * p.pt_cols, sw.ctx, part.group, b,
                                       min(kTable, part.b1 - b), smem);
             Tile::template keys<false, false>(src, smem, qf, live, src.nb, p.scale_log2, m_run, l_run, oacc);
@@ -734,12 +755,15 @@ __global__ __launch_bounds__(kPagedThreads) __attribute__((amdgpu_waves_per_eu(2
 }
 
 // ---------------------------------------------------------------------------
-// Joins the parts of cut items, and answers rows without a context (o = 0,
-// lse = -inf).  WPR waves per row (sequence, query token, q head), each with an
-// equal share of the parts: one part's maximum and sum per lane, the
-// numerators with lanes across the head dim.  What bounds it is its chain of
-// dependent loads (lengths and units, then the states): four waves per row where
-// few rows leave the chip empty.
+// Joins the parts of cut items.  WPR waves per row, each with an equal share of
+// the parts: one part's maximum and sum per lane, the numerators with lanes
+// across the head dim.  What bounds it is its chain of dependent loads (lengths
+// and units, then the states): four waves per row where few rows leave the chip
+// empty.  Waves are dealt to every row that the call may have (sequence, query
+// token, q head) or, where most sequences are far shorter than the longest, to
+// the rows of the item that each run starts in: the first run that starts inside
+// an item joins it.  (64 sequences, one of 2048 tokens and the others of one,
+// contexts of 500, 32 / 8 heads: 500 us for rows that are not there, 67 so.)
 // ---------------------------------------------------------------------------
 template <typename T, int D, int WPR>
 __global__ __launch_bounds__(kPagedThreads) void paged_merge_kernel(PagedParams p, int32_t n_rows, Divider hqdiv,
@@ -750,34 +774,47 @@ __global__ __launch_bounds__(kPagedThreads) void paged_merge_kernel(PagedParams 
     const int row = WPR == 1 ? blockIdx.x * 4 + wave : blockIdx.x;
     const int sub = WPR == 1 ? 0 : wave;
     if (row >= n_rows) return;
-    const int r0 = divide(row, hqdiv);
-    const int qh = row - r0 * p.Hq;
-    const int seq = divide(r0, msdiv);
-    const int tok = r0 - seq * p.max_seqlen;
-    const int32_t total = p.base[p.B], base = p.base[seq];  // (asked for with the sequence's lengths)
-    const SeqWork sw = seq_work(p, seq);
-    const int kvh = divide(qh, p.gdiv);
-    const int rr = tok * p.group + (qh - kvh * p.group);
-    if (rr >= sw.rows) return;
-    uint16_t* const o = p.o + (int64_t)(sw.s0 + tok) * p.so_t + qh * p.so_h;
-    float* const lse = p.lse ? p.lse + (int64_t)(sw.s0 + tok) * p.sl_t + qh * p.sl_h : nullptr;
-    if (sw.blocks == 0) {
-        if (sub == 0 && lane < D / 8) st16(o + 8 * lane, Vec16{{0u, 0u, 0u, 0u}});
-        if (lse && sub == 0 && lane == 0) *lse = -INFINITY;
-        return;
+    int32_t s0, rows, tile, grp, hl, rr, a, blocks, total;  // hl, rr: kv head of the group, row of the tile
+    if (p.cuts) {
+        const int w = row >> (p.row_shift + p.head_shift);
+        const int in = row - (w << (p.row_shift + p.head_shift));
+        hl = in >> p.row_shift;
+        rr = in - (hl << p.row_shift);
+        const RunStart c = p.cuts[w];
+        if (c.b0 == 0) return;
+        s0 = c.s0, rows = c.rows, tile = c.tile, grp = c.group, a = c.first, blocks = c.blocks, total = c.total;
+        if (w > 0 && Runs(total, p.nwg, p.least).first(w - 1) > a) return;
+    } else {
+        const int r0 = divide(row, hqdiv);
+        const int qh = row - r0 * p.Hq;
+        const int seq = divide(r0, msdiv);
+        const int tok = r0 - seq * p.max_seqlen;
+        total = p.base[p.B];
+        const int32_t base = p.base[seq];  // (asked for with the sequence's lengths)
+        const SeqWork sw = seq_work(p, seq);
+        const int kvh = divide(qh, p.gdiv);
+        rr = tok * p.group + (qh - kvh * p.group);
+        s0 = sw.s0, rows = sw.rows, blocks = sw.blocks;
+        tile = rr >> p.row_shift;
+        rr -= tile << p.row_shift;
+        grp = kvh >> p.head_shift;
+        hl = kvh - (grp << p.head_shift);
+        a = base + (grp * sw.tiles + tile) * blocks;
     }
+    const int in_seq = (tile << p.row_shift) + rr;
+    if (in_seq >= rows) return;
     const Runs runs(total, p.nwg, p.least);
-    const int tile = rr >> p.row_shift;
-    const int grp = divide(kvh, p.headdiv);
-    const int32_t a = base + (grp * sw.tiles + tile) * sw.blocks;
-    const int w0 = runs.of(a), w1 = runs.of(a + sw.blocks - 1) + 1;
+    const int w0 = runs.of(a), w1 = runs.of(a + blocks - 1) + 1;
     if (w0 + 1 == w1) return;  // finished by its workgroup
+    const int tok = divide(in_seq, p.gdiv);
+    const int qh = ((grp << p.head_shift) + hl) * p.group + (in_seq - tok * p.group);
+    uint16_t* const o = p.o + (int64_t)(s0 + tok) * p.so_t + qh * p.so_h;
+    float* const lse = p.lse ? p.lse + (int64_t)(s0 + tok) * p.sl_t + qh * p.sl_h : nullptr;
     // row of the workspace that holds run w's part: a run that starts inside the
     // item, or with it, holds it in state 0
-    const int hl = kvh - grp * p.heads;
     auto at = [&](int w) {
         const int64_t state = 2 * (int64_t)w + (runs.first(w) >= a ? 0 : 1);
-        return ((state * p.heads + hl) << p.row_shift) + (rr - (tile << p.row_shift));
+        return ((((state << p.head_shift) + hl) << p.row_shift)) + rr;
     };
     const int share = WPR == 1 ? w1 - w0 : (w1 - w0 + WPR - 1) / WPR;
     const int lo = w0 + sub * share, hi = min(w1, lo + share);
@@ -884,14 +921,15 @@ static PagedShape paged_shape(int64_t max_rows, int64_t pairs, int hkv, int64_t 
 }
 
 struct PagedSpace {
-    int64_t base, m, l, acc, bytes;
+    int64_t base, cuts, m, l, acc, bytes;
 };
 static PagedSpace paged_space(int32_t batch, int nwg, const PagedShape& shape, int head_dim) {
     auto up = [](int64_t x) { return (x + 255) / 256 * 256; };
     const int64_t rows = (2 * (int64_t)nwg * shape.heads) << shape.row_shift;
     PagedSpace s;
     s.base = 0;
-    s.m = up(((int64_t)batch + 1) * 4);
+    s.cuts = up(((int64_t)batch + 1) * 4);
+    s.m = s.cuts + up(nwg * (int64_t)sizeof(RunStart));
     s.l = s.m + up(rows * 4);
     s.acc = s.l + up(rows * 4);
     s.bytes = s.acc + rows * head_dim * 4;
@@ -900,11 +938,7 @@ static PagedSpace paged_space(int32_t batch, int nwg, const PagedShape& shape, i
 
 template <typename T, int D>
 static int launch_merge(const PagedParams& p, hipStream_t st) {
-    const int64_t rows = (int64_t)p.B * p.max_seqlen * p.Hq;
-    if (rows > INT32_MAX) {
-        set_error("grid too large (%lld rows)", (long long)rows);
-        return QATTN_ERR_ARG;
-    }
+    const int64_t rows = p.cuts ? (int64_t)p.nwg * p.heads << p.row_shift : (int64_t)p.B * p.max_seqlen * p.Hq;
     const Divider hq = make_divider(p.Hq), ms = make_divider(p.max_seqlen);
     if (rows <= 512)
         hipLaunchKernelGGL((paged_merge_kernel<T, D, 4>), dim3((uint32_t)rows), dim3(kPagedThreads), 0, st, p,
@@ -955,7 +989,8 @@ static bool paged_plan(PagedPlan& plan, int32_t batch, int32_t max_seqlen, int64
     // As many workgroups as run at once, no more than the units that the page
     // table has room for.
     const int64_t tiles = ((rows - 1) >> plan.shape.row_shift) + 1;
-    const int64_t blocks = ((int64_t)pt_cols * page_size + (1 << plan.shape.key_shift) - 1) >> plan.shape.key_shift;
+    const int64_t blocks =
+        std::max<int64_t>(1, ((int64_t)pt_cols * page_size + (1 << plan.shape.key_shift) - 1) >> plan.shape.key_shift);
     const double units = (double)batch * (hkv / plan.shape.heads) * tiles * blocks;
     plan.too_many = units >= 2147483648.0;
     plan.tiles = (int)std::min<int64_t>(tiles, INT32_MAX);
@@ -1069,12 +1104,16 @@ int qattn_prefix_paged_fwd(const void* q, const int64_t q_stride[3], const void*
     p.key_shift = plan.shape.key_shift;
     p.groupdiv = make_divider(p.groups);
     p.tilediv = make_divider(plan.tiles);
-    p.headdiv = make_divider(p.heads);
+    p.head_shift = p.heads == 4 ? 2 : p.heads == 2 ? 1 : 0;
     p.pdiv = make_divider(page_size);
     p.gdiv = make_divider(p.group);
     p.scale_log2 = scale * kLog2e;
     char* const ws = (char*)workspace;
     p.base = (int32_t*)(ws + sp.base);
+    // (a wave of the merge that finds no row costs a fraction of one that joins
+    // parts, and a run's rows may be none of a cut item)
+    if ((double)batch * plan.max_seqlen * num_q_heads > 2.0 * ((int64_t)plan.nwg * p.heads << p.row_shift))
+        p.cuts = (RunStart*)(ws + sp.cuts);
     p.part_m = (float*)(ws + sp.m);
     p.part_l = (float*)(ws + sp.l);
     p.part_acc = (float*)(ws + sp.acc);

@@ -19,8 +19,8 @@
 // and 0 times an infinity or a NaN is NaN: a tile whose results are not all
 // finite is computed once more, and then infinities and NaN in V are taken out of
 // the blocks that hold masked keys and added to the rows that attend them by
-// themselves.  (Looking through those blocks always: 8 sequences of 1000 tokens
-// on average 166 -> 181 us.)
+// themselves.  (Looking through those blocks always: 16 prompts of 1300 tokens on
+// average, 32 / 8 heads of 64: 166 -> 181 us.)
 #include <algorithm>
 
 #include "dense_tiles.h"
@@ -49,8 +49,11 @@ struct PromptParams {
     int32_t qtiles, spread, list;    // tiles of the longest prompt, log2 of lists per pair, tiles of a list
     int32_t xcd_lists, group_lists;  // lists per XCD, lists of a group
     Divider gdiv, groupdiv, hkvdiv;  // group, tiles of a group of lists, Hkv
+    // Tiles that sequences of these lengths can have (a multiple of 8), if the
+    // launch numbers the tiles that there are; 0: every prompt has qtiles
+    int32_t tiles;
     // Cut tiles: blocks of a part at most (0: no tile is cut), parts of the
-    // longest tile; states [pair][tile][part][row] of those that are cut
+    // longest tile; states [tile][part][row] of those that are cut
     int32_t part, parts;
     Divider partdiv, hqdiv, msdiv;  // parts, Hq, max_seqlen
     float* part_m;                  // in log2 units
@@ -74,6 +77,42 @@ struct TileParts {
     }
     __device__ __forceinline__ int first(int c) const { return c * q + min(c, rem); }
 };
+
+// The sequence's tokens, 0 where its offsets are not ascending rows of Q.
+__device__ __forceinline__ int prompt_tokens(const PromptParams& p, int seq, int& s0) {
+    s0 = p.cu[seq];
+    const int32_t s1 = p.cu[seq + 1];
+    if (s0 < 0 || s1 < s0 || (int64_t)s1 > p.total_tokens) return 0;
+    return min(s1 - s0, p.max_seqlen);
+}
+
+// Tile i of a launch that numbers the tiles that there are: kv heads innermost
+// (8 of them lie on 8 XCDs), then a sequence's tiles, the longest first, then
+// sequences.  Every wave looks for it in the offsets by itself.
+__device__ __forceinline__ bool numbered_tile(const PromptParams& p, int i, int& seq, int& kvh, int& qt) {
+    const int lane = threadIdx.x & 63;
+    int t = divide(i, p.hkvdiv);
+    kvh = i - t * p.Hkv;
+    for (int c = 0; c < p.B; c += 64) {
+        int s0, tiles = 0;
+        if (c + lane < p.B) tiles = (prompt_tokens(p, c + lane, s0) * p.group + kBM - 1) / kBM;
+        int inc = tiles;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const int up = __shfl_up(inc, d);
+            if (lane >= d) inc += up;
+        }
+        const uint64_t past = __ballot(t < inc);
+        if (past) {
+            const int at = __builtin_ctzll(past);
+            seq = c + at;
+            qt = __builtin_amdgcn_readlane(inc, at) - 1 - t;
+            return true;
+        }
+        t -= __builtin_amdgcn_readlane(inc, 63);
+    }
+    return false;
+}
 
 template <typename T, int D>
 struct PromptKeys {
@@ -240,34 +279,38 @@ __global__ __launch_bounds__(kPromptThreads) __attribute__((amdgpu_waves_per_eu(
     __shared__ __attribute__((aligned(1024))) uint16_t smem[Tile::kSmem];
     __shared__ int flags[2];  // PromptKeys::found; a wave's results are not finite
 
-    // XCD x (blockIdx % 8) takes lists x, x + 8, ...: list v is every
-    // (1 << spread)-th tile of pair v >> spread, the longest first.  Lists are
-    // taken in groups, the longest tiles of a group's lists first.
-    // (with cut tiles, a tile's parts next to each other)
     const int i0 = blockIdx.x >> 3;
-    const int i = CUT ? divide(i0, p.partdiv) : i0;
+    const int i = CUT ? divide(i0, p.partdiv) : i0;  // (a tile's parts next to each other)
     const int cut = i0 - i * p.parts;
-    const int grp = divide(i, p.groupdiv);
-    const int in = i - grp * p.group_lists * p.list;
-    const int here = min(p.group_lists, p.xcd_lists - grp * p.group_lists);  // lists of this group
-    const int k = (int)((uint32_t)in / (uint32_t)here);
-    // An XCD deals its workgroups to its shader engines in turn, however busy
-    // they are: with a list in the same place of every round, one engine would
-    // have the longest prompts' tiles to itself (16 prompts of 603 .. 2011 tokens:
-    // 210 us; turned by one place per round: 181).
-    int at = in - k * here;
-    if (!(here & 1)) at = (int)((uint32_t)(at + k) % (uint32_t)here);
-    const int v = (blockIdx.x & 7) + 8 * (grp * p.group_lists + at);
-    const int pair = v >> p.spread;
-    const int rank = (k << p.spread) + (v & ((1 << p.spread) - 1));
-    const int qt = p.qtiles - 1 - rank;
-    if (qt < 0) return;
-    const int seq = divide(pair, p.hkvdiv);
-    const int kvh = pair - seq * p.Hkv;
-    const int32_t s0 = p.cu[seq], s1 = p.cu[seq + 1];
-    if (s0 < 0 || s1 < s0 || (int64_t)s1 > p.total_tokens) return;
-    int32_t n = s1 - s0;
-    if (n > p.max_seqlen) n = p.max_seqlen;
+    int seq, kvh, qt, slot;
+    if (p.tiles) {
+        slot = 8 * i + (blockIdx.x & 7);
+        if (!numbered_tile(p, slot, seq, kvh, qt)) return;
+    } else {
+        // XCD x (blockIdx % 8) takes lists x, x + 8, ...: list v is every
+        // (1 << spread)-th tile of pair v >> spread, the longest first.  Lists are
+        // taken in groups, the longest tiles of a group's lists first.
+        const int grp = divide(i, p.groupdiv);
+        const int in = i - grp * p.group_lists * p.list;
+        const int here = min(p.group_lists, p.xcd_lists - grp * p.group_lists);  // lists of this group
+        const int k = (int)((uint32_t)in / (uint32_t)here);
+        // An XCD deals its workgroups to its shader engines in turn, however busy
+        // they are: with a list in the same place of every round, one engine would
+        // have the longest prompts' tiles to itself (16 prompts of 603 .. 2011 tokens:
+        // 210 us; turned by one place per round: 181).
+        int at = in - k * here;
+        if (!(here & 1)) at = (int)((uint32_t)(at + k) % (uint32_t)here);
+        const int v = (blockIdx.x & 7) + 8 * (grp * p.group_lists + at);
+        const int pair = v >> p.spread;
+        const int rank = (k << p.spread) + (v & ((1 << p.spread) - 1));
+        qt = p.qtiles - 1 - rank;
+        if (qt < 0) return;
+        seq = divide(pair, p.hkvdiv);
+        kvh = pair - seq * p.Hkv;
+        slot = pair * p.qtiles + qt;
+    }
+    int32_t s0;
+    const int n = prompt_tokens(p, seq, s0);
     const int g = p.group;
     const int rows = n * g;
     if (qt * kBM >= rows) return;
@@ -347,7 +390,7 @@ __global__ __launch_bounds__(kPromptThreads) __attribute__((amdgpu_waves_per_eu(
     const bool valid = query_of(tok, qh);
     if (CUT && !whole) {
         if (valid) {
-            const int64_t r = (((int64_t)pair * p.qtiles + qt) * p.parts + cut) * kBM + wave * 32 + q32;
+            const int64_t r = ((int64_t)slot * p.parts + cut) * kBM + wave * 32 + q32;
             if (hl == 0) {
                 p.part_m[r] = m_run * p.scale_log2;
                 p.part_l[r] = l_tot;
@@ -371,21 +414,28 @@ __global__ __launch_bounds__(kPromptThreads) void prompt_merge_kernel(PromptPara
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int row = blockIdx.x * 4 + wave;
     if (row >= n_rows) return;
-    const int r0 = divide(row, p.hqdiv);
-    const int qh = row - r0 * p.Hq;
-    const int seq = divide(r0, p.msdiv);
-    const int tok = r0 - seq * p.max_seqlen;
-    const int32_t s0 = p.cu[seq], s1 = p.cu[seq + 1];
-    if (s0 < 0 || s1 < s0 || (int64_t)s1 > p.total_tokens) return;
-    const int n = min(s1 - s0, p.max_seqlen);
-    if (tok >= n) return;
-    const int kvh = divide(qh, p.gdiv);
-    const int rr = tok * p.group + (qh - kvh * p.group);
-    const int qt = rr / kBM;
-    const int k_hi = divide(min(qt * kBM + kBM, n * p.group) - 1, p.gdiv) + 1;
+    int seq, kvh, qt, slot, rr;  // rr: the row in its (sequence, kv head)
+    if (p.tiles) {
+        slot = row / kBM;
+        if (!numbered_tile(p, slot, seq, kvh, qt)) return;
+        rr = qt * kBM + row % kBM;
+    } else {
+        const int r0 = divide(row, p.hqdiv);
+        const int qh = row - r0 * p.Hq;
+        seq = divide(r0, p.msdiv);
+        kvh = divide(qh, p.gdiv);
+        rr = (r0 - seq * p.max_seqlen) * p.group + (qh - kvh * p.group);
+        qt = rr / kBM;
+        slot = (seq * p.Hkv + kvh) * p.qtiles + qt;
+    }
+    int32_t s0;
+    const int rows = prompt_tokens(p, seq, s0) * p.group;
+    if (rr >= rows) return;
+    const int tok = divide(rr, p.gdiv), qh = kvh * p.group + (rr - tok * p.group);
+    const int k_hi = divide(min(qt * kBM + kBM, rows) - 1, p.gdiv) + 1;
     const int parts = TileParts(p, (k_hi + kBN - 1) / kBN).n;
     if (parts == 1) return;  // finished by its workgroup
-    const int64_t first = (((int64_t)seq * p.Hkv + kvh) * p.qtiles + qt) * p.parts * kBM + (rr - qt * kBM);
+    const int64_t first = (int64_t)slot * p.parts * kBM + (rr - qt * kBM);
     const bool in = lane * E < D;
     float m = -INFINITY, l = 0.f, acc[E] = {};
     constexpr int U = 4;
@@ -436,7 +486,7 @@ static int launch_prompt(const PromptParams& p, int64_t blocks, hipStream_t st) 
                        p);
     const int rc = launch_status("prompt_attn_kernel, cut tiles");
     if (rc) return rc;
-    const int64_t rows = (int64_t)p.B * p.max_seqlen * p.Hq;
+    const int64_t rows = p.tiles ? (int64_t)p.tiles * kBM : (int64_t)p.B * p.max_seqlen * p.Hq;
     hipLaunchKernelGGL((prompt_merge_kernel<T, D>), dim3((uint32_t)((rows + 3) / 4)), dim3(kPromptThreads), 0, st, p,
                        (int32_t)rows);
     return launch_status("prompt_merge_kernel");
@@ -445,7 +495,9 @@ static int launch_prompt(const PromptParams& p, int64_t blocks, hipStream_t st) 
 // Tiles of a call, and how they are cut.
 struct PromptPlan {
     int32_t max_seqlen, group, qtiles, part, parts;
-    int64_t pairs, m, l, bytes;  // workspace: states' maxima at 0, sums at m, numerators at l
+    int32_t tiles;  // of launches that number them, else 0
+    int64_t pairs, slots, m, l, bytes;  // slots: tiles that the launch has a place for;
+                                        // workspace: states' maxima at 0, sums at m, numerators at l
     bool fits;
 };
 static PromptPlan prompt_plan(int32_t batch, int32_t max_seqlen, int64_t total_tokens, int32_t hq, int32_t hkv,
@@ -458,6 +510,18 @@ static PromptPlan prompt_plan(int32_t batch, int32_t max_seqlen, int64_t total_t
     if (!q.fits || q.max_seqlen <= 0 || q.pairs <= 0) return q;
     q.qtiles = (q.max_seqlen * q.group + kBM - 1) / kBM;
     q.parts = 1;
+    q.slots = q.pairs * q.qtiles;
+    int64_t full = batch;  // sequences, if all were of the longest one's length
+    // Numbering the tiles that there are costs a look through the offsets ahead
+    // of everything else; a workgroup without a tile costs 1/3 us of a slot (one
+    // prompt of 2048 tokens, 32 / 8 heads, with 63 of one token: 46 us
+    // numbered, 63 with a place for 64 prompts of 2048; with 255: 58 and 140).
+    const int64_t numbered = ((total_tokens * q.group + kBM - 1) / kBM + batch) * hkv;
+    if (q.slots > 4 * numbered && numbered < INT32_MAX / kBM - 8) {
+        q.tiles = (int32_t)((numbered + 7) / 8 * 8);
+        q.slots = q.tiles;
+        full = std::min<int64_t>(batch, (total_tokens + q.max_seqlen - 1) / q.max_seqlen);
+    }
     // Tiles are cut where the longest one alone holds the call up: a CU with one
     // workgroup takes 4/5 of the time per block that it takes with two, and the
     // second kernel and the states cost what about 16 blocks take.  With as many
@@ -465,12 +529,12 @@ static PromptPlan prompt_plan(int32_t batch, int32_t max_seqlen, int64_t total_t
     // themselves (504 tiles of 2000 tokens: 42 us whole, 68 cut in two); 64 tiles
     // of 2000 tokens: 23.4 us whole, 16.7 in parts.
     const int64_t longest = (q.max_seqlen + 63) / 64;
-    const int64_t blocks = q.pairs * q.qtiles * (longest + 1) / 2;
+    const int64_t blocks = full * hkv * q.qtiles * (longest + 1) / 2;
     const int64_t share = std::max<int64_t>(8, (blocks + 255) / 256);  // of a CU
     if (longest > share * 5 / 4 + 16) {
         q.part = (int32_t)share;
         q.parts = (int32_t)((longest + share - 1) / share);
-        const int64_t rows = q.pairs * q.qtiles * q.parts * kBM;
+        const int64_t rows = q.slots * q.parts * kBM;
         q.m = rows * 4;
         q.l = 2 * rows * 4;
         q.bytes = q.l + rows * head_dim * 4;
@@ -534,7 +598,8 @@ int qattn_prompt_fwd(const void* q, const int64_t q_stride[3], const void* k, co
     p.total_tokens = total_tokens;
     p.B = batch, p.Hq = num_q_heads, p.Hkv = num_kv_heads, p.group = num_q_heads / num_kv_heads;
     const PromptPlan plan = prompt_plan(batch, max_seqlen, total_tokens, num_q_heads, num_kv_heads, head_dim);
-    if (!plan.fits || (plan.part && (int64_t)batch * plan.max_seqlen * num_q_heads > INT32_MAX)) {
+    if (!plan.fits || plan.slots > INT32_MAX ||
+        (plan.part && !plan.tiles && (int64_t)batch * plan.max_seqlen * num_q_heads > INT32_MAX)) {
         set_error("sizes too large: max_seqlen=%d group=%d batch=%d num_kv_heads=%d", plan.max_seqlen, plan.group, batch,
                   num_kv_heads);
         return QATTN_ERR_ARG;
@@ -546,6 +611,7 @@ int qattn_prompt_fwd(const void* q, const int64_t q_stride[3], const void* k, co
     }
     p.max_seqlen = plan.max_seqlen;
     p.qtiles = plan.qtiles;
+    p.tiles = plan.tiles;
     p.part = plan.part;
     p.parts = plan.parts;
     if (plan.part) {
@@ -559,7 +625,7 @@ int qattn_prompt_fwd(const void* q, const int64_t q_stride[3], const void* k, co
     const int64_t pairs = plan.pairs;
     while (pairs << p.spread & 7) ++p.spread;  // lists: a multiple of the 8 XCDs
     p.list = (p.qtiles + (1 << p.spread) - 1) >> p.spread;
-    const int64_t blocks = (pairs << p.spread) * p.list;
+    const int64_t blocks = p.tiles ? p.tiles : (pairs << p.spread) * p.list;
     // As many lists side by side as have their K/V in one XCD's L2 (4 MB): the
     // longest tiles of them all start first, and the last ones end together.
     const int64_t kv_bytes = 4 * (int64_t)p.max_seqlen * head_dim;

@@ -34,6 +34,8 @@ def tables(B, cols, pages, seed):
     ([100, 0], [300, 5], 7, 32, 128),
     ([13], [2000], 64, 8, 64),
     ([3, 1], [5, 64], 16, 3, 32),
+    ([4, 0, 9, 17] * 20, [1] * 41 + [230] + [0, 2, 1] * 12 + [1, 1], 16, 8, 128),  # one long among many
+    ([4, 0, 9, 17] * 50, [1] * 101 + [900] + [3, 0] * 49, 5, 1, 32),
 ])
 def test_append(ctx, new, ps, Hkv, D, dtype):
     from qattention_amd import append_paged_kv
@@ -76,6 +78,41 @@ def test_append_what_has_no_place():
     got = append_paged_kv(K, V, Kc, Vc, table, ctx, cu, max_seqlen=4)
     assert got.tolist() == [8, 7, 6, -1, 0, 9]
     assert torch.equal(Kc, want[0]) and torch.equal(Vc, want[1])
+
+
+def test_append_what_has_no_place_among_many():
+    """The same for many sequences, most far shorter than the longest."""
+    from qattention_amd import append_paged_kv
+    ps, Hkv, D, B = 4, 2, 64, 150
+    Kc, Vc = cache(2 * B, ps, Hkv, D, torch.float16, 7)
+    new = [1] * 70 + [600] + [1] * 79
+    table = torch.arange(2 * B, dtype=torch.int32).view(B, 2)
+    ctx = torch.tensor([i % 9 for i in range(B)], dtype=torch.int32)
+    ctx[5], table[6, 1], table[7, 0], ctx[70] = -3, 2 * B, -1, 2
+    cu = offsets(new).cpu()
+    cu[101], cu[-1] = cu[100] - 1, sum(new) + 1  # sequence 100 and the last one are none; 101 has three rows
+    K, V = (x[0] for x in cache(1, sum(new), Hkv, D, torch.float16, 8))
+    want, after = [Kc.clone(), Vc.clone()], ctx.clone()
+    for s in range(B):
+        a, b = int(cu[s]), int(cu[s + 1])
+        if b < a or b > sum(new) or ctx[s] < 0:
+            continue
+        for i in range(min(b - a, 500)):
+            pos = int(ctx[s]) + i
+            if pos < 2 * ps:
+                after[s] += 1
+                page = int(table[s, pos // ps])
+                if 0 <= page < 2 * B:
+                    for w, x in zip(want, (K, V)):
+                        w[page, pos % ps] = x[a + i]
+    # (row 99 of the single ones belongs to two sequences now: either may have it)
+    say("no place among many")
+    got = append_paged_kv(K, V, Kc, Vc, table, ctx, cu, max_seqlen=500)
+    assert torch.equal(got.cpu(), after)
+    skip = [int(table[s, j]) for s in (99, 101) for j in (0, 1)]
+    for w, x in zip(want, (Kc, Vc)):
+        w[skip], x[skip] = 0, 0
+        assert torch.equal(x, w)
 
 
 def test_append_strided():

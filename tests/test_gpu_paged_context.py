@@ -95,6 +95,39 @@ def test_many_tokens(ctx, toks, ps, Hq, Hkv, D, dtype):
     check(*again, reference(Q, rows, toks))
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("many,long,ctx,Hq,Hkv,D", [
+    (79, 600, 200, 8, 2, 128),
+    (300, 90, 700, 16, 2, 64),
+    (1100, 8, 300, 8, 8, 64),   # few rows
+    (900, 7, 0, 16, 8, 32),     # a long one without a context
+])
+def test_one_long_chunk_among_single_tokens(many, long, ctx, Hq, Hkv, D, dtype):
+    from qattention_amd import prefix_attention_paged
+    toks = [(1, 1, 0, 2)[i % 4] for i in range(many)]
+    ctxs = [(0, 3, 64, 150, 20)[i % 5] for i in range(many)]
+    toks[many // 2], ctxs[many // 2] = long, ctx
+    Kc, Vc, table, lens, rows = paged(ctxs, 16, Hkv, D, dtype, 71)
+    Q = queries(sum(toks), Hq, D, dtype, 71)
+    say("mixed", many, long, ctx, Hq, Hkv, D, dtype)
+    O, L = prefix_attention_paged(Q, Kc, Vc, table, lens, offsets(toks))
+    check(O, L, reference(Q, rows, toks))
+
+
+@pytest.mark.parametrize("pages", [0, 3])
+def test_rows_without_contexts(pages):
+    """Chunks and single tokens without a context, with and without a cache."""
+    from qattention_amd import prefix_attention_paged
+    for toks in ([1] * 5, [100, 1, 0, 3], [40] * 3, [1] * 300 + [500], [6] * 70):
+        Q = queries(sum(toks), 8, 64, torch.float16, 73)
+        cache = torch.full((pages, 16, 2, 64), math.nan, dtype=torch.float16, device=DEV)
+        table = torch.zeros(len(toks), 60, dtype=torch.int32, device=DEV)
+        lens = torch.zeros(len(toks), dtype=torch.int32, device=DEV)
+        say("no contexts", pages, len(toks))
+        O, L = prefix_attention_paged(Q, cache, torch.full_like(cache, math.nan), table, lens, offsets(toks))
+        assert not O.any() and (L == -math.inf).all()
+
+
 def test_large_batch():
     """More sequences than a workgroup has threads, lengths from zero on."""
     from qattention_amd import prefix_attention_paged

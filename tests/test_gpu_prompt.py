@@ -190,6 +190,33 @@ def test_low_scores_behind_minus_infinity(dtype):
     check(O[m:], L[m:], reference(Q[m:], K[m:], V[m:], [n - m]))
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("lens,Hq,Hkv,D", [
+    ([1] * 30 + [700] + [0, 1, 2, 3] * 10, 4, 2, 128),
+    ([1] * 30 + [2000] + [1] * 39, 4, 2, 64),      # its tiles are cut
+    ([1300] + [1] * 200 + [900, 0], 3, 1, 32),
+    ([1] * 127 + [900] + [5] * 3, 9, 3, 64),
+])
+def test_one_long_prompt_among_short_ones(lens, Hq, Hkv, D, dtype):
+    from qattention_amd import prompt_attention
+    Q, K, V = inputs(lens, Hq, Hkv, D, dtype, 61)
+    cu = offsets(lens)
+    say("mixed", len(lens), max(lens), Hq, Hkv, D, dtype)
+    O, L = prompt_attention(Q, K, V, cu, return_lse=True)
+    check(O, L, reference(Q, K, V, lens))
+    # a sequence that is none (its end lies ahead of its start) and one that
+    # leaves Q: the others stay what they were
+    at = lens.index(max(lens))
+    bad = cu.clone()
+    bad[-1] = sum(lens) + 5
+    bad[at + 1] = cu[at] - 1  # (the next one now starts there)
+    keep = torch.ones(sum(lens), dtype=torch.bool, device=DEV)
+    keep[cu[at] - 1 if at else 0:cu[at + 2]] = False
+    keep[cu[-2]:] = False
+    O2, L2 = prompt_attention(Q, K, V, bad, max_seqlen=max(lens), return_lse=True)
+    assert torch.equal(O2[keep], O[keep]) and torch.equal(L2[keep], L[keep])
+
+
 def test_rows_of_no_sequence_stay():
     """Through the C entry: rows in front of, between and behind the sequences keep
     what they held; bad offsets and max_seqlen cut what is computed."""
