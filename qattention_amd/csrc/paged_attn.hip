@@ -270,10 +270,11 @@ __device__ __forceinline__ SeqWork next_part(const PagedParams& p, Share& sh, Pa
 // TB/s against 5.6 for the bare loads of 64 x 10240 keys.
 // STREAM: runs of units, as above.  Otherwise a workgroup per item, for short
 // contexts, where the launch is all latency: no scan ahead of the first load and
-// no second kernel (2 x 700 keys, 32 / 8 heads: 11.8 us per call against 15, 10.9
-// against 10.4 in a graph).  A CU draws about 26 GB/s from far away however
-// many loads it has in flight (two steps of them were 3-10% slower than one),
-// so long contexts want many CUs: 2000 keys take 22.7 us so, 11.4 in runs.
+// no second kernel (2 x 300 keys, 32 / 8 heads: 7.7 us against 10.5 in runs, 2 x
+// 700: 11.3 against 10.5 in a graph, 11.3 against 11 to 12 per eager call).  A CU
+// draws about 26 GB/s from far away however many loads it has in flight (two
+// steps of them were 3-10% slower than one), so a few long contexts want many
+// CUs: 2 x 2000 keys take 23.9 us so, 11 in runs.
 // ---------------------------------------------------------------------------
 constexpr int kNarrowWaves = 4;             // waves of a STREAM workgroup
 constexpr int kItemWaves = 8;               // waves of a workgroup per item
@@ -902,9 +903,13 @@ struct PagedShape {
     bool items;
 };
 static PagedShape paged_shape(int64_t max_rows, int64_t pairs, int hkv, int64_t capacity, int head_dim) {
-    // a workgroup per item: three steps at most (four are slower than runs:
-    // 13.3 us against 10.4 in a graph), and every workgroup runs at once
-    if (max_rows <= 16 && capacity <= 3 * 32 * kItemWaves && pairs <= 256) return {1, 4, 8, 1, 1, true};
+    // A workgroup per item, where every one runs at once: three steps at most, or
+    // four where the items fill half the chip by themselves (8 x 1024 keys, 8 kv
+    // heads: 15.3 us against 14.0 in runs, 16 x 1024: 16.0 against 20.5, 32 x 1024:
+    // 23.8 against 29.6; longer ones gain 5 us of 40 with equal contexts, and lose
+    // as much where they differ by a factor of three, which runs even out).
+    const int steps = pairs >= 128 ? 4 : 3;
+    if (max_rows <= 16 && capacity <= steps * 32 * kItemWaves && pairs <= 256) return {1, 4, 8, 1, 1, true};
     if (max_rows <= 32) {
         const int qb = max_rows <= 16 ? 1 : 2;
         const int per_cu = narrow_waves(head_dim, qb);
@@ -913,8 +918,8 @@ static PagedShape paged_shape(int64_t max_rows, int64_t pairs, int hkv, int64_t 
         // per row, since each part leaves a state per head (64 x 8000 keys: 380 us
         // with one head, 363 with four; 8 x 3000 keys, 32 rows: 27.1 against 36.6).
         int heads = hkv % 4 == 0 ? 4 : hkv % 2 == 0 ? 2 : 1;
-        const int64_t steps = pairs * (((int64_t)capacity + 127) / 128);
-        if (max_rows > 8 || pairs / heads * 16 < 256 * per_cu || steps < 16 * 256 * per_cu) heads = 1;
+        const int64_t work = pairs * (((int64_t)capacity + 127) / 128);
+        if (max_rows > 8 || pairs / heads * 16 < 256 * per_cu || work < 16 * 256 * per_cu) heads = 1;
         return {qb, qb == 1 ? 4 : 5, heads == 4 ? 5 : heads == 2 ? 6 : 7, heads, per_cu, false};
     }
     return {0, 7, 6, 1, 2, false};
