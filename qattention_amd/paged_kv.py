@@ -46,6 +46,8 @@ from .ragged_attn import (_SUPPORTED, _check_dtypes, _device_index, _dtype_code,
 def _int32(t: torch.Tensor, device) -> torch.Tensor:
     if t.dtype is torch.int32 and t.device == device and t.is_contiguous():
         return t
+    if t.is_floating_point() or t.is_complex():
+        raise ValueError(f"lengths, offsets and pages must be integers (got {t.dtype})")
     return t.to(device=device, dtype=torch.int32, non_blocking=True).contiguous()
 
 

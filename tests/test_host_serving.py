@@ -165,6 +165,10 @@ def test_row_offsets():
         paged_kv._table(torch.zeros(2, 4), 3, "cpu")
     with pytest.raises(ValueError, match=r"must be \[B\]"):
         paged_kv._lengths(torch.zeros(2, 4), "cpu")
+    with pytest.raises(ValueError, match="must be integers"):
+        paged_kv._lengths(torch.zeros(2), "cpu")
+    with pytest.raises(ValueError, match="must be integers"):
+        paged_kv._page_lists([1.5], torch.tensor([2.0]), 8, "cpu")
 
 
 @pytest.mark.parametrize("src,dst,what", [
