@@ -538,6 +538,9 @@ static PromptPlan prompt_plan(int32_t batch, int32_t max_seqlen, int64_t total_t
         q.m = rows * 4;
         q.l = 2 * rows * 4;
         q.bytes = q.l + rows * head_dim * 4;
+        // (a place for every short prompt's tile, too: thousands of them are not
+        // worth gigabytes that no one writes)
+        if (q.bytes > int64_t(1) << 29) q.part = 0, q.parts = 1, q.bytes = 0;
     }
     return q;
 }

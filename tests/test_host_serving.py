@@ -47,6 +47,8 @@ def test_prompt_workspace():
     assert ws(64, 4000, 256000, 32, 8, 128) == 0  # tiles enough for every slot
     rows = -(-4000 * 2 // 128) * 2 * 128
     assert ws(1, 4000, 4000, 4, 2, 128) % (rows * 4 * 130) == 0 < ws(1, 4000, 4000, 4, 2, 128)
+    # one long prompt among short ones: its tiles are cut, unless the short ones are thousands
+    assert 0 < ws(70, 2000, 2069, 4, 2, 64) < 1 << 29 and ws(10001, 2000, 12000, 1, 1, 64) == 0
 
 
 def paged(q=16, kc=16, vc=16, o=16, qs=(512, 128, 1), cs=(4096, 256, 128, 1), table=16, cols=4, pages=8, ps=16,
