@@ -86,18 +86,9 @@ struct DenseTile {
     // and oacc.  live: the wave has rows (else it only stages its part of the
     // blocks).  Ends with the workgroup past its last use of the LDS only after
     // the caller's barrier.
-    //
-    // BYSUM (bf16): the maximum of later blocks is not looked for.  A weight keeps
-    // its 8 bits whatever its size, so the reference follows a block's sum of
-    // weights after the fact, once that passes 2^8.  Weights past 2^127 (scores
-    // that rise by 88 from the reference to the next block) become infinities:
-    // the caller runs a tile whose results are not finite again, with the
-    // maximum.  16384 tokens, 32 / 8 heads: 1848 -> 1803 us; 64-wide heads:
-    // 1132 -> 1078.  (fp16 weights end at 2^16.)
-    template <bool BYSUM, bool SCAN, class Src>
+    template <bool SCAN, class Src>
     static __device__ __forceinline__ void keys(const Src& src, uint16_t* smem, const Vec16 (&qf)[KS], bool live,
                                                 int nb, float csc, float& m_run, float& l_run, f16v_t (&oacc)[DT]) {
-        static_assert(!BYSUM || (T::kCode == BF16::kCode && !Src::kEveryBlock));
         const int lane = threadIdx.x & 63;
         const int q32 = lane & 31, hl = lane >> 5;
         uint16_t *const Kb0 = smem, *const Kb1 = smem + BLK, *const Vb0 = smem + 2 * BLK;
@@ -178,18 +169,6 @@ struct DenseTile {
                 m_run = m_new;
             }
             set_mc();
-        };
-        auto follow_sum = [&](float sum) {
-            sum = xor32_sum(sum);
-            if (__builtin_expect(__any(sum > 256.f), 0)) {
-                const float up = sum > 256.f ? fast_log2(sum) : 0.f;
-                const float alpha = fast_exp2(-up);
-#pragma unroll
-                for (int dt = 0; dt < DT; ++dt) oacc[dt] *= alpha;
-                l_run *= alpha;
-                m_run += up / csc;
-                mc = m_run * csc;
-            }
         };
         // One block's 32 weights per lane, element n = 8 th + e of 16-key step
         // th, in three stages: exponent (0), exponential (1), sum and packing
@@ -297,15 +276,12 @@ struct DenseTile {
                     weights_at(sc, NS + i);
 #pragma unroll
                     for (int e = 0; e < 16; ++e)
-                        if (!BYSUM && 2 * DT + e * 2 * DT / 16 == i)
+                        if (2 * DT + e * 2 * DT / 16 == i)
                             mb = fmaxf(fmaxf(mb, sn[e >> 3][2 * (e & 7)]), sn[e >> 3][2 * (e & 7) + 1]);
                     fence();
                 }
                 l_run += ps0 + ps1;
-                if constexpr (BYSUM)
-                    follow_sum(ps0 + ps1);
-                else
-                    move_ref(mb);
+                move_ref(mb);
                 fence();
             };
             f16v_t sA[2], sB[2];
@@ -319,7 +295,6 @@ struct DenseTile {
             }
             src.mask(0, sA);
             move_ref(block_max(sA));
-            if constexpr (BYSUM) m_run = m_run == -INFINITY ? 0.f : m_run;  // (a reference that can be kept)
             publish<0>();  // K_0 has been read; V_0 and K_1 have landed
             if (nb > 2) src.load_k(2, Kb0);
 #pragma unroll

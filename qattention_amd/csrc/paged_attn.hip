@@ -732,7 +732,7 @@ __global__ __launch_bounds__(kPagedThreads) __attribute__((amdgpu_waves_per_eu(2
         for (int b = part.b0; b < part.b1 && sw.ctx > 0; b += kTable) {
             const PagedKeys<T, D> src(p, table, p.table + (int64_t)sh.seq * p.pt_cols, sw.ctx, part.group, b,
                                       min(kTable, part.b1 - b), smem);
-            Tile::template keys<false, false>(src, smem, qf, live, src.nb, p.scale_log2, m_run, l_run, oacc);
+            Tile::template keys<false>(src, smem, qf, live, src.nb, p.scale_log2, m_run, l_run, oacc);
         }
         const float l = xor32_sum(l_run);
         int64_t qrow;

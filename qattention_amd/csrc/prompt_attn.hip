@@ -275,7 +275,6 @@ __global__ __launch_bounds__(kPromptThreads) __attribute__((amdgpu_waves_per_eu(
     PromptParams p) {
     using Tile = DenseTile<T, D>;
     constexpr int KS = Tile::KS, DT = Tile::DT;
-    constexpr bool BYSUM = T::kCode == BF16::kCode;
     __shared__ __attribute__((aligned(1024))) uint16_t smem[Tile::kSmem];
     __shared__ int flags[2];  // PromptKeys::found; a wave's results are not finite
 
@@ -362,27 +361,23 @@ __global__ __launch_bounds__(kPromptThreads) __attribute__((amdgpu_waves_per_eu(
     if (threadIdx.x < 2) flags[threadIdx.x] = 0;  // (ahead of the key loop's first barrier)
     const PromptKeys<T, D> src(p, s0, kvh, qt * kBM, k_first, k_last, smem, flags);
     const bool live = qt * kBM + wave * 32 < rows;
-    Tile::template keys<BYSUM, false>(src, smem, qf, live, src.nb, p.scale_log2, m_run, l_run, oacc);
+    Tile::template keys<false>(src, smem, qf, live, src.nb, p.scale_log2, m_run, l_run, oacc);
 
-    // Results that are not finite, or lost to a reference that is too high (bf16,
-    // scores of -inf in a row's whole block 0 and low ones later): once more,
-    // with the maximum of every block and a look at V.
+    // Results that are not finite: once more, with a look at V.
     float odd = l_run * 0.f;  // 0, or NaN if anything is not finite
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
         for (int r = 0; r < 16; ++r) odd = __builtin_fmaf(oacc[dt][r], 0.f, odd);
     {
-        const float sum = xor32_sum(l_run);
         int tok, qh;
-        const bool lost = odd != 0.f || sum < 0x1p-100f;
-        if (__any(query_of(tok, qh) && lost) && lane == 0) flags[1] = 1;
+        if (__any(query_of(tok, qh) && odd != 0.f) && lane == 0) flags[1] = 1;
     }
     Tile::sync_lds();
     if (__builtin_expect(__builtin_amdgcn_readfirstlane(flags[1]), 0)) {
         load_q();
         clear();
-        Tile::template keys<false, true>(src, smem, qf, live, src.nb, p.scale_log2, m_run, l_run, oacc);
+        Tile::template keys<true>(src, smem, qf, live, src.nb, p.scale_log2, m_run, l_run, oacc);
     }
 
     const float l_tot = xor32_sum(l_run);  // both halves of the query's keys
