@@ -43,11 +43,16 @@ from .ragged_attn import (_SUPPORTED, _check_dtypes, _device_index, _dtype_code,
                           _rows16, _seqlens, _vec_ok)
 
 
+def _integers(t: torch.Tensor) -> torch.Tensor:
+    if t.is_floating_point() or t.is_complex():
+        raise ValueError(f"lengths, offsets and pages must be integers (got {t.dtype})")
+    return t
+
+
 def _int32(t: torch.Tensor, device) -> torch.Tensor:
     if t.dtype is torch.int32 and t.device == device and t.is_contiguous():
         return t
-    if t.is_floating_point() or t.is_complex():
-        raise ValueError(f"lengths, offsets and pages must be integers (got {t.dtype})")
+    _integers(t)
     return t.to(device=device, dtype=torch.int32, non_blocking=True).contiguous()
 
 
@@ -241,11 +246,18 @@ def compact_paged_kv(
 _Pages = Union[torch.Tensor, Sequence[int]]
 
 
+def _page_list(pages: _Pages) -> torch.Tensor:
+    if not isinstance(pages, torch.Tensor):
+        pages = list(pages)
+        # (without a dtype: given one, torch would cut fractions off)
+        pages = torch.tensor(pages) if pages else torch.empty(0, dtype=torch.int64)
+    return _integers(pages)
+
+
 def _page_lists(src, dst, num_pages: int, device):
     """Both lists on the device.  Lists on the host are checked: every page in
     the cache, no destination twice, none that is also a source."""
-    src = src if isinstance(src, torch.Tensor) else torch.tensor(list(src), dtype=torch.int32)
-    dst = dst if isinstance(dst, torch.Tensor) else torch.tensor(list(dst), dtype=torch.int32)
+    src, dst = _page_list(src), _page_list(dst)
     on_gpu = src.is_cuda and dst.is_cuda
     if src.dim() != 1 or src.shape != dst.shape:
         raise ValueError(f"src_pages and dst_pages must be lists of one length (got {tuple(src.shape)}, "

@@ -196,3 +196,10 @@ def test_gradients_refused():
     _no_grad(torch.zeros(2))
     with torch.no_grad():
         _no_grad(x)
+
+
+@pytest.mark.parametrize("src,dst", [([1.7], [2]), ([1], [2.0]), ([1], torch.tensor([2.5])), ([0, 1.0], [2, 3]),
+                                     (torch.tensor([1.0]), [2])])
+def test_page_lists_of_fractions(src, dst):
+    with pytest.raises(ValueError, match="must be integers"):
+        paged_kv._page_lists(src, dst, 8, "cpu")
