@@ -39,14 +39,8 @@ from typing import Optional, Sequence, Tuple, Union
 import torch
 
 from . import _lib
-from .ragged_attn import (_SUPPORTED, _check_dtypes, _device_index, _dtype_code, _launch, _no_grad, _out_like,
-                          _rows16, _seqlens, _vec_ok)
-
-
-def _integers(t: torch.Tensor) -> torch.Tensor:
-    if t.is_floating_point() or t.is_complex():
-        raise ValueError(f"lengths, offsets and pages must be integers (got {t.dtype})")
-    return t
+from .ragged_attn import (_SUPPORTED, _check_dtypes, _device_index, _dtype_code, _integers, _launch, _no_grad,
+                          _offsets, _out_like, _rows16, _vec_ok)
 
 
 def _int32(t: torch.Tensor, device) -> torch.Tensor:
@@ -98,7 +92,7 @@ def _rows(T: int, B: int, cu_seqlens, max_seqlen, device):
         return 1, None
     if cu_seqlens.dim() != 1 or cu_seqlens.shape[0] != B + 1:
         raise ValueError(f"cu_seqlens must have {B + 1} entries (got {tuple(cu_seqlens.shape)})")
-    return _seqlens(cu_seqlens, B, device, max_seqlen)
+    return _offsets(cu_seqlens, device, max_seqlen)
 
 
 def prefix_attention_paged(

@@ -186,6 +186,19 @@ def _seqlens(cu_seqlens: torch.Tensor, B: int, device, max_seqlen: Optional[int]
     return max(int(max_seqlen), 0), cu_dev.contiguous()
 
 
+def _integers(t: torch.Tensor) -> torch.Tensor:
+    if t.is_floating_point() or t.is_complex():
+        raise ValueError(f"lengths, offsets and pages must be integers (got {t.dtype})")
+    return t
+
+
+def _offsets(cu_seqlens: torch.Tensor, device, max_seqlen: Optional[int]):
+    """_seqlens for the serving calls: [B + 1] integers."""
+    if cu_seqlens.dim() != 1 or cu_seqlens.shape[0] < 1:
+        raise ValueError(f"cu_seqlens must be [B + 1] (got {tuple(cu_seqlens.shape)})")
+    return _seqlens(_integers(cu_seqlens), cu_seqlens.shape[0] - 1, device, max_seqlen)
+
+
 _ONE_SEQ_CU: dict = {}
 
 
@@ -746,8 +759,8 @@ def prompt_attention(
     T, Hq, Hkv, D = _heads(Q, K, V)
     if K.shape[0] != T or V.shape[0] != T:
         raise ValueError("packed Q, K, V must have the same number of tokens")
-    B = int(cu_seqlens.shape[0]) - 1
-    ms, cu_dev = _seqlens(cu_seqlens, B, device, max_seqlen)
+    ms, cu_dev = _offsets(cu_seqlens, device, max_seqlen)
+    B = cu_dev.shape[0] - 1
     Q, q, qs = _rows16(Q)
     K, k, ks = _rows16(K)
     V, v, vs = _rows16(V)

@@ -203,3 +203,17 @@ def test_gradients_refused():
 def test_page_lists_of_fractions(src, dst):
     with pytest.raises(ValueError, match="must be integers"):
         paged_kv._page_lists(src, dst, 8, "cpu")
+
+
+def test_offsets_are_a_list_of_integers():
+    from qattention_amd.ragged_attn import _offsets
+    for cu in (torch.tensor([0.0, 2.5, 4.0]), torch.tensor([0, 4]).half()):
+        with pytest.raises(ValueError, match="must be integers"):
+            _offsets(cu, "cpu", 4)
+        with pytest.raises(ValueError, match="must be integers"):
+            paged_kv._rows(4, cu.shape[0] - 1, cu, 4, "cpu")
+    for cu in (torch.tensor([[0, 4], [0, 4]]), torch.tensor(4), torch.empty(0, dtype=torch.int32)):
+        with pytest.raises(ValueError, match=r"\[B \+ 1\]"):
+            _offsets(cu, "cpu", 4)
+    ms, cu = _offsets(torch.tensor([0, 3, 4], dtype=torch.int16), "cpu", None)
+    assert ms == 3 and cu.dtype == torch.int32 and cu.tolist() == [0, 3, 4]
