@@ -46,8 +46,7 @@ from .ragged_attn import (_SUPPORTED, _check_dtypes, _device_index, _dtype_code,
 def _int32(t: torch.Tensor, device) -> torch.Tensor:
     if t.dtype is torch.int32 and t.device == device and t.is_contiguous():
         return t
-    _integers(t)
-    return t.to(device=device, dtype=torch.int32, non_blocking=True).contiguous()
+    return _integers(t).to(device=device, dtype=torch.int32, non_blocking=True).contiguous()
 
 
 def _check_caches(K_cache, V_cache, dims: Tuple[int, ...]) -> tuple:

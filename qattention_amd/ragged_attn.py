@@ -186,9 +186,19 @@ def _seqlens(cu_seqlens: torch.Tensor, B: int, device, max_seqlen: Optional[int]
     return max(int(max_seqlen), 0), cu_dev.contiguous()
 
 
+_INT32 = torch.iinfo(torch.int32)
+
+
 def _integers(t: torch.Tensor) -> torch.Tensor:
+    """t, its values within 32 bits: what lies past them goes to their end, which
+    is past every table, cache and row as well (2^32 + 3 is not page 3)."""
     if t.is_floating_point() or t.is_complex():
         raise ValueError(f"lengths, offsets and pages must be integers (got {t.dtype})")
+    if t.dtype is torch.uint64:
+        t = t.view(torch.int64)
+        t = t.masked_fill(t < 0, _INT32.max)
+    if t.dtype in (torch.int64, torch.uint32):
+        t = t.to(torch.int64).clamp(_INT32.min, _INT32.max)
     return t
 
 
@@ -196,7 +206,8 @@ def _offsets(cu_seqlens: torch.Tensor, device, max_seqlen: Optional[int]):
     """_seqlens for the serving calls: [B + 1] integers."""
     if cu_seqlens.dim() != 1 or cu_seqlens.shape[0] < 1:
         raise ValueError(f"cu_seqlens must be [B + 1] (got {tuple(cu_seqlens.shape)})")
-    return _seqlens(_integers(cu_seqlens), cu_seqlens.shape[0] - 1, device, max_seqlen)
+    max_seqlen, cu = _seqlens(_integers(cu_seqlens), cu_seqlens.shape[0] - 1, device, max_seqlen)
+    return min(max_seqlen, _INT32.max), cu
 
 
 _ONE_SEQ_CU: dict = {}

@@ -224,3 +224,25 @@ def test_rows_past_32_bits():
     copy_kv_pages(Kc, Vc, [pages - 1], [1])
     copy_kv_pages(Kc, Vc, [pages - 3], [pages - 2])
     assert torch.equal(Kc[1], Kc[pages - 1]) and torch.equal(Vc[pages - 2], Vc[pages - 3])
+
+
+def test_64_bit_values_do_not_wrap():
+    """Pages, lengths and steps past 32 bits on the GPU: outside of everything."""
+    from qattention_amd import append_paged_kv, compact_paged_kv, copy_kv_pages, prefix_attention_paged
+    ps, Hkv, D = 4, 2, 64
+    Kc, Vc = cache(8, ps, Hkv, D, torch.float16, 23)
+    K, V = (x[0] for x in cache(1, 2, Hkv, D, torch.float16, 24))
+    before, w = (Kc.clone(), Vc.clone()), 2 ** 32
+    table, lens = torch.tensor([[0, 1], [2, 3]], device=DEV), torch.tensor([w + 1, 2], device=DEV)
+    say("64 bits")
+    copy_kv_pages(Kc, Vc, torch.tensor([w + 1, 2], device=DEV), torch.tensor([5, w + 6], device=DEV))
+    got = append_paged_kv(K[:1], V[:1], Kc, Vc, table + w, lens[1:])  # no such pages: the row is dropped
+    assert got.tolist() == [3] and torch.equal(Kc, before[0]) and torch.equal(Vc, before[1])
+    got = append_paged_kv(K, V, Kc, Vc, table, lens)
+    assert got.tolist() == [2 ** 31 - 1, 3] and torch.equal(Kc[2, 2], K[1]) and torch.equal(Kc[:2], before[0][:2])
+    k = Kc.clone()
+    got = compact_paged_kv(Kc, Vc, table, torch.tensor([0, 0], device=DEV), torch.tensor([[1, w + 2], [w, 1]], device=DEV))
+    assert got.tolist() == [1, 0] and torch.equal(Kc[0, 0], k[0, 1]) and torch.equal(Kc[2:], k[2:])
+    Q = torch.empty(2, 4, D, dtype=torch.float16, device=DEV).normal_()
+    O = prefix_attention_paged(Q, Kc, Vc, table, lens, max_seqlen=w)[0]
+    assert torch.equal(O, prefix_attention_paged(Q, Kc, Vc, table, torch.tensor([2 * ps, 2], device=DEV))[0])

@@ -305,3 +305,18 @@ def test_other_stream_and_graph():
         want = prompt_attention(Q, K, V, cu, max_seqlen=140, return_lse=True)
         n = int(cu[-1])
         assert torch.equal(got[0][:n], want[0][:n]) and torch.equal(got[1][:n], want[1][:n])
+
+
+def test_lengths_past_32_bits():
+    """max_seqlen counts in full, and an offset of 2^32 and more is not one of Q's rows."""
+    from qattention_amd import prompt_attention
+    Q, K, V = inputs([50], 4, 2, 64, torch.float16, 53)
+    want = prompt_attention(Q, K, V, offsets([20, 30]), return_lse=True)
+    say("past 32 bits")
+    for ms in (30, 2 ** 31 + 7, 2 ** 40):
+        O, L = prompt_attention(Q, K, V, offsets([20, 30]), ms, return_lse=True)
+        assert torch.equal(O, want[0]) and torch.equal(L, want[1])
+    for device in ("cpu", DEV):
+        cu = torch.tensor([0, 20, 2 ** 32 + 50], device=device)
+        O, L = prompt_attention(Q, K, V, cu, return_lse=True)
+        assert torch.equal(O[:20], want[0][:20]) and torch.equal(L[:20], want[1][:20])

@@ -217,3 +217,22 @@ def test_offsets_are_a_list_of_integers():
             _offsets(cu, "cpu", 4)
     ms, cu = _offsets(torch.tensor([0, 3, 4], dtype=torch.int16), "cpu", None)
     assert ms == 3 and cu.dtype == torch.int32 and cu.tolist() == [0, 3, 4]
+
+
+def test_values_past_32_bits_do_not_wrap():
+    from qattention_amd.ragged_attn import _offsets
+    top, low = 2 ** 31 - 1, -2 ** 31
+    wide = torch.tensor([3, 2 ** 31 - 1, 2 ** 31, 2 ** 32 + 3, 2 ** 33 + 5, -1, -2 ** 32 + 1, -2 ** 63])
+    assert paged_kv._int32(wide, wide.device).tolist() == [3, top, top, top, top, -1, low, low]
+    assert paged_kv._lengths(wide[3:5], wide.device).tolist() == [top, top]
+    assert paged_kv._table(wide[None], 1, wide.device).tolist()[0][4] == top
+    assert paged_kv._int32(torch.tensor([7, 2 ** 32 - 1]).to(torch.uint32), wide.device).tolist() == [7, top]
+    assert paged_kv._int32(torch.tensor([7, -1]).view(torch.uint64), wide.device).tolist() == [7, top]
+    assert paged_kv._int32(torch.tensor([-3, 200], dtype=torch.int16), wide.device).tolist() == [-3, 200]
+    for pages in ([2 ** 32 + 3], torch.tensor([2 ** 32 + 3])):
+        with pytest.raises(ValueError, match="outside"):
+            paged_kv._page_lists(pages, [1], 8, "cpu")
+    ms, cu = _offsets(torch.tensor([0, 4, 2 ** 32 + 5]), "cpu", None)
+    assert ms == top - 4 and cu.tolist() == [0, 4, top]
+    # (the C entries take 32 bits: 2^40 would arrive as 0)
+    assert _offsets(torch.tensor([0, 4]), "cpu", 2 ** 40)[0] == top and paged_kv._rows(4, 1, cu[:2], 2 ** 33, "cpu")[0] == top
