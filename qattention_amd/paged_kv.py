@@ -28,8 +28,9 @@ captured in a graph):
     lens = compact_paged_kv(K_caches, V_caches, table, lens, accepted)
 
 The calls run on torch's current stream, take contexts, offsets and page tables
-on the host too (a copy each call), and serve inference: tensors that ask for
-gradients are refused while autograd records.
+on the host too (a copy each call, of what they hold at the call; not while a
+graph is captured), and serve inference: tensors that ask for gradients are
+refused while autograd records.
 """
 from __future__ import annotations
 
@@ -39,14 +40,14 @@ from typing import Optional, Sequence, Tuple, Union
 import torch
 
 from . import _lib
-from .ragged_attn import (_SUPPORTED, _check_dtypes, _device_index, _dtype_code, _integers, _launch, _no_grad,
-                          _offsets, _out_like, _rows16, _vec_ok)
+from .ragged_attn import (_SUPPORTED, _check_dtypes, _device_index, _dtype_code, _host, _integers, _launch,
+                          _no_grad, _offsets, _out_like, _rows16, _vec_ok)
 
 
 def _int32(t: torch.Tensor, device) -> torch.Tensor:
     if t.dtype is torch.int32 and t.device == device and t.is_contiguous():
         return t
-    return _integers(t).to(device=device, dtype=torch.int32, non_blocking=True).contiguous()
+    return _integers(_host(t, device)).to(device=device, dtype=torch.int32, non_blocking=True).contiguous()
 
 
 def _check_caches(K_cache, V_cache, dims: Tuple[int, ...]) -> tuple:

@@ -202,11 +202,25 @@ def _integers(t: torch.Tensor) -> torch.Tensor:
     return t
 
 
+def _host(t: torch.Tensor, device) -> torch.Tensor:
+    """An operand that may lie on the host, as it is now: a copy from pinned memory
+    waits for its turn in the stream, and the caller may write there meanwhile
+    (one from pageable memory has read it when it returns)."""
+    if t.is_cpu and torch.device(device).type == "cuda":
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("lengths, offsets and pages must be on the GPU while a graph is captured: it would read "
+                               "host memory at every replay")
+        if t.is_pinned():
+            t = t.clone()
+    return t
+
+
 def _offsets(cu_seqlens: torch.Tensor, device, max_seqlen: Optional[int]):
     """_seqlens for the serving calls: [B + 1] integers."""
     if cu_seqlens.dim() != 1 or cu_seqlens.shape[0] < 1:
         raise ValueError(f"cu_seqlens must be [B + 1] (got {tuple(cu_seqlens.shape)})")
-    max_seqlen, cu = _seqlens(_integers(cu_seqlens), cu_seqlens.shape[0] - 1, device, max_seqlen)
+    cu_seqlens = _integers(_host(cu_seqlens, device))
+    max_seqlen, cu = _seqlens(cu_seqlens, cu_seqlens.shape[0] - 1, device, max_seqlen)
     return min(max_seqlen, _INT32.max), cu
 
 

@@ -169,3 +169,70 @@ def test_serving_loop():
             mask = torch.ones(1, kept[layer][s][0].shape[0], dtype=torch.bool, device=DEV)
             check(O[s:s + 1], L[s:s + 1], attend64(q[s:s + 1], *kept[layer][s], mask))
     assert np.all(new.tolist() == lens.cpu().numpy() + 1)
+
+
+def test_host_operands_are_taken_at_the_call():
+    """Tables, lengths, offsets and paths on the host, pinned and not, that change while
+    the stream is still busy ahead of the call."""
+    import qattention_amd as qa
+    g = torch.Generator(device=DEV).manual_seed(9)
+    B, cols, toks = 3, 8, [4, 2, 3]
+    Kc, Vc = (rand(g, B * cols, PS, HKV, D, dtype=torch.float16) for _ in range(2))
+    Q, K, V = (rand(g, sum(toks), h, D, dtype=torch.float16) for h in (HQ, HKV, HKV))
+    wide = torch.zeros(B, 300000, dtype=torch.int32)  # (some MB: not what a copy holds by the way)
+    wide[:, :cols] = torch.arange(B * cols).view(B, cols)
+    host = dict(table=wide, lens=torch.tensor([100, 3, 57], dtype=torch.int32),
+                cu=offsets(toks).cpu(), path=torch.tensor([[0, 2], [1, 3], [2, -1]], dtype=torch.int32),
+                src=torch.tensor([0, 9], dtype=torch.int32), dst=torch.tensor([7, 15], dtype=torch.int32))
+    big = torch.ones(8192, 8192, dtype=torch.bfloat16, device=DEV)
+
+    def step(o):
+        kc, vc = Kc.clone(), Vc.clone()
+        out = [*qa.prefix_attention_paged(Q, kc, vc, o["table"], o["lens"], o["cu"], 4),
+               qa.prompt_attention(Q, K, V, o["cu"], 4),
+               qa.append_paged_kv(K, V, kc, vc, o["table"], o["lens"], o["cu"], 4),
+               qa.compact_paged_kv(kc, vc, o["table"], o["lens"], o["path"])]
+        qa.copy_kv_pages(kc, vc, o["src"], o["dst"])
+        return out + [kc, vc]
+
+    want = step({n: t.to(DEV) for n, t in host.items()})
+    for kind in ("pinned", "pageable"):
+        o = {n: t.clone().pin_memory() if kind == "pinned" else t.clone() for n, t in host.items()}
+        torch.cuda.synchronize()
+        say("host operands", kind)
+        for _ in range(30):
+            big @ big
+        got = step(o)
+        for t in o.values():  # (other rows of the same tensors: nothing out of range either way)
+            t.zero_()
+        torch.cuda.synchronize()
+        for i, (a, b) in enumerate(zip(got, want)):
+            same = torch.equal(a, b)
+            assert same, (kind, i)
+
+
+def test_host_operands_stay_out_of_graphs():
+    """A graph would read host memory at each replay, whatever it holds by then."""
+    import qattention_amd as qa
+    g = torch.Generator(device=DEV).manual_seed(10)
+    Kc, Vc = (rand(g, 4, PS, HKV, D, dtype=torch.float16) for _ in range(2))
+    Q, K, V = (rand(g, 2, h, D, dtype=torch.float16) for h in (HQ, HKV, HKV))
+    table, lens, cu = torch.tensor([[0, 1], [2, 3]], dtype=torch.int32), torch.tensor([5, 20]), offsets([1, 1]).cpu()
+    dev = [t.to(DEV, torch.int32) for t in (table, lens, cu)]
+    want = qa.prefix_attention_paged(Q, Kc, Vc, *dev, 1)
+    calls = [lambda t=t, l=l, c=c: qa.prefix_attention_paged(Q, Kc, Vc, t, l, c, 1)
+             for t, l, c in ((table, *dev[1:]), (dev[0], lens.pin_memory(), dev[2]), (*dev[:2], cu))]
+    calls += [lambda: qa.prompt_attention(Q, K, V, cu, 1), lambda: qa.copy_kv_pages(Kc, Vc, [0], [1]),
+              lambda: qa.append_paged_kv(K, V, Kc, Vc, dev[0], lens),
+              lambda: qa.compact_paged_kv(Kc, Vc, dev[0], dev[1], torch.tensor([[0], [1]]))]
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        for i, f in enumerate(calls):
+            say("in a graph", i)
+            with pytest.raises(RuntimeError, match="on the GPU while a graph is captured"):
+                f()
+        got = qa.prefix_attention_paged(Q, Kc, Vc, *dev, 1)
+    for _ in range(3):
+        graph.replay()
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
