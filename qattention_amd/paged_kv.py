@@ -40,14 +40,14 @@ from typing import Optional, Sequence, Tuple, Union
 import torch
 
 from . import _lib
-from .ragged_attn import (_SUPPORTED, _check_dtypes, _device_index, _dtype_code, _host, _integers, _launch,
-                          _no_grad, _offsets, _out_like, _rows16, _vec_ok)
+from .ragged_attn import (_SUPPORTED, _check_dtypes, _device_index, _dtype_code, _integers, _launch,
+                          _no_grad, _no_host_in_graph, _offsets, _out_like, _rows16, _to_device, _vec_ok)
 
 
 def _int32(t: torch.Tensor, device) -> torch.Tensor:
     if t.dtype is torch.int32 and t.device == device and t.is_contiguous():
         return t
-    return _integers(_host(t, device)).to(device=device, dtype=torch.int32, non_blocking=True).contiguous()
+    return _to_device(_integers(_no_host_in_graph(t, device)), device)
 
 
 def _check_caches(K_cache, V_cache, dims: Tuple[int, ...]) -> tuple:

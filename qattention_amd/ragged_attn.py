@@ -170,6 +170,16 @@ def _on(device):
     return _HERE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
 
 
+def _to_device(t: torch.Tensor, device) -> torch.Tensor:
+    """int32 on the device, of what t holds now: a copy from pinned memory waits for
+    its turn in the stream, and the caller may write there meanwhile (one from
+    pageable memory has read it when it returns)."""
+    if t.is_cpu and torch.device(device).type == "cuda" and t.is_pinned():
+        if not torch.cuda.is_current_stream_capturing():  # (a graph reads the caller's memory at every replay)
+            t = t.clone()
+    return t.to(device=device, dtype=torch.int32, non_blocking=True).contiguous()
+
+
 def _seqlens(cu_seqlens: torch.Tensor, B: int, device, max_seqlen: Optional[int]):
     """max_seqlen and a device int32 copy of cu_seqlens (src/ragged_attn.py:1136-1142).
 
@@ -180,10 +190,10 @@ def _seqlens(cu_seqlens: torch.Tensor, B: int, device, max_seqlen: Optional[int]
         cu_cpu = cu_seqlens.cpu()
         sl = cu_cpu.tolist()
         max_seqlen = int(max([e - b for b, e in zip(sl, sl[1:])])) if B else 1
-        cu_dev = cu_cpu.to(device=device, dtype=torch.int32, non_blocking=True)
+        cu_dev = _to_device(cu_cpu, device)
     else:
-        cu_dev = cu_seqlens.to(device=device, dtype=torch.int32, non_blocking=True)
-    return max(int(max_seqlen), 0), cu_dev.contiguous()
+        cu_dev = _to_device(cu_seqlens, device)
+    return max(int(max_seqlen), 0), cu_dev
 
 
 _INT32 = torch.iinfo(torch.int32)
@@ -202,16 +212,10 @@ def _integers(t: torch.Tensor) -> torch.Tensor:
     return t
 
 
-def _host(t: torch.Tensor, device) -> torch.Tensor:
-    """An operand that may lie on the host, as it is now: a copy from pinned memory
-    waits for its turn in the stream, and the caller may write there meanwhile
-    (one from pageable memory has read it when it returns)."""
-    if t.is_cpu and torch.device(device).type == "cuda":
-        if torch.cuda.is_current_stream_capturing():
-            raise RuntimeError("lengths, offsets and pages must be on the GPU while a graph is captured: it would read "
-                               "host memory at every replay")
-        if t.is_pinned():
-            t = t.clone()
+def _no_host_in_graph(t: torch.Tensor, device) -> torch.Tensor:
+    if t.is_cpu and torch.device(device).type == "cuda" and torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("lengths, offsets and pages must be on the GPU while a graph is captured: it would read "
+                           "host memory at every replay")
     return t
 
 
@@ -219,7 +223,7 @@ def _offsets(cu_seqlens: torch.Tensor, device, max_seqlen: Optional[int]):
     """_seqlens for the serving calls: [B + 1] integers."""
     if cu_seqlens.dim() != 1 or cu_seqlens.shape[0] < 1:
         raise ValueError(f"cu_seqlens must be [B + 1] (got {tuple(cu_seqlens.shape)})")
-    cu_seqlens = _integers(_host(cu_seqlens, device))
+    cu_seqlens = _integers(_no_host_in_graph(cu_seqlens, device))
     max_seqlen, cu = _seqlens(cu_seqlens, cu_seqlens.shape[0] - 1, device, max_seqlen)
     return min(max_seqlen, _INT32.max), cu
 
@@ -388,7 +392,7 @@ def ragged_attention_with_parents(
         raise ValueError(f"parents has {parents.numel()} entries for {T} tokens")
     B = int(cu_seqlens.shape[0]) - 1
     ms, cu_dev = _seqlens(cu_seqlens, B, device, max_seqlen)
-    par = parents.to(device=device, dtype=torch.int32, non_blocking=True).contiguous()
+    par = _to_device(parents, device)
     Q, K, V = _vec(Q), _vec(K), _vec(V)
     O = torch.empty_like(Q)
     if not _vec_ok(O):
@@ -442,7 +446,7 @@ def _paged_forward(Q, K_cache, V_cache, page_table, cu_seqlens, branching_factor
         raise ValueError(f"cache shape {tuple(K_cache.shape)} incompatible with Q {tuple(Q.shape)}")
     B = int(cu_seqlens.shape[0]) - 1
     ms, cu_dev = _seqlens(cu_seqlens, B, device, max_seqlen)
-    pt = page_table.to(device=device, dtype=torch.int32, non_blocking=True).contiguous()
+    pt = _to_device(page_table, device)
     if pt.dim() != 2 or pt.shape[0] < B:
         raise ValueError(f"page_table must be [B, max_pages] (got {tuple(page_table.shape)})")
     Q, K_cache, V_cache = _vec(Q), _vec(K_cache), _vec(V_cache)
@@ -615,7 +619,7 @@ def ragged_attention_prefix(
     if parents is not None:
         if parents.numel() < T:
             raise ValueError(f"parents has {parents.numel()} entries for {T} tokens")
-        par = parents.to(device=device, dtype=torch.int32, non_blocking=True).contiguous()
+        par = _to_device(parents, device)
     O, LSE = _prefix_tree_forward(Q, K, V, cu_dev, B, ms, K_prefix if L else None, kp_stride,
                                   V_prefix if L else None, vp_stride, L, branching_factor, max_depth, 0, 0,
                                   return_lse, num_splits, par)
@@ -737,7 +741,7 @@ def ragged_tree_attn(
         else:
             tree_parents = None  # the reference falls back to the heap walk (:1470, :1475)
         if tree_parents is not None:
-            par = tree_parents.to(device=device, dtype=torch.int32, non_blocking=True).contiguous()
+            par = _to_device(tree_parents, device)
     lib = _lib.lib()
     ws_bytes = int(lib.qattn_prefix_workspace_bytes(B, N, B * N, Hq, Hkv, D, L, int(num_splits))) if B * N else 0
     ws = torch.empty(max(ws_bytes, 1), dtype=torch.uint8, device=device)

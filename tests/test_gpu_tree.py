@@ -691,3 +691,40 @@ def test_graph_capture_replay(B, b, d, H):
         torch.cuda.synchronize()
         assert torch.equal(out, eager), f"replay {i}"
         del junk
+
+
+def test_host_operands_are_read_at_the_call():
+    """Offsets, parents and page tables in pinned memory that change while the stream is
+    still busy ahead of the call."""
+    from qattention_amd import ragged_attn as ra
+    g = torch.Generator(device=DEV).manual_seed(3)
+    lens, H, D, ps = [15, 31, 7], 4, 64, 16
+    T, L = sum(lens), 40
+    Q, K, V = (torch.empty(T, H, D, dtype=torch.float16, device=DEV).normal_(generator=g) for _ in range(3))
+    Kp, Vp = (torch.empty(3, L, H, D, dtype=torch.float16, device=DEV).normal_(generator=g) for _ in range(2))
+    Kc, Vc, table = ra.build_paged_kv(list(K.split(lens)), list(V.split(lens)), ps)
+    Qb, Kb, Vb = (torch.empty(2, H, n, D, dtype=torch.float16, device=DEV).normal_(generator=g) for n in (7, 47, 47))
+    up = lambda n: torch.tensor([max(i - 1, 0) // 2 for i in range(n)], dtype=torch.int32)  # noqa: E731
+    host = dict(cu=torch.tensor([0] + lens).cumsum(0).to(torch.int32), par=torch.cat([up(n) for n in lens]),
+                table=table, tree=up(7))
+    big = torch.ones(8192, 8192, dtype=torch.bfloat16, device=DEV)
+
+    def calls(o):
+        return [*ra.ragged_attention_with_lse(Q, K, V, o["cu"], 2, 4, 31),
+                *ra.ragged_attention_with_parents(Q, K, V, o["cu"], o["par"], 4, 31),
+                ra.ragged_attention_paged(Q, Kc, Vc, o["table"], o["cu"], 2, 4, 31),
+                ra.ragged_attention_prefix(Q, K, V, o["cu"], Kp, Vp, 2, 4, 31, parents=o["par"]),
+                ra.ragged_tree_attn(Qb, Kb, Vb, 2, 2, tree_parents=o["tree"])]
+
+    want = calls({n: t.to(DEV) for n, t in host.items()})
+    pinned = {n: t.clone().pin_memory() for n, t in host.items()}
+    torch.cuda.synchronize()
+    for _ in range(30):
+        big @ big
+    got = calls(pinned)
+    for t in pinned.values():
+        t.zero_()
+    torch.cuda.synchronize()
+    for i, (a, b) in enumerate(zip(got, want)):
+        same = torch.equal(a, b)
+        assert same, i
