@@ -64,6 +64,7 @@ struct Call {
         if (!THPVariable_CheckExact(o)) return false;
         t = &THPVariable_Unpack(o);
         if (!t->is_cuda() || t->layout() != at::kStrided || t->requires_grad()) return false;
+        if (t->_fw_grad(0).defined()) return false;  // (a tangent; there is one level only)
         const int d = t->get_device();
         if (device < 0) device = d;
         return d == device;

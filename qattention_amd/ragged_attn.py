@@ -28,6 +28,7 @@ import math
 from typing import List, Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -95,13 +96,12 @@ def _require_device(*ts):
 
 
 def _no_grad(*ts) -> None:
-    """Refuse tensors that ask for gradients where there is no backward pass."""
+    """Refuse tensors that ask for gradients or carry tangents: there is no derivative."""
     for t in ts:
         if t.requires_grad and torch.is_grad_enabled():
-            break
-    else:
-        return
-    raise RuntimeError("this call has no backward pass: use torch.no_grad() or detach its inputs")
+            raise RuntimeError("this call has no backward pass: use torch.no_grad() or detach its inputs")
+        if forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None:
+            raise RuntimeError("this call has no forward derivative: it takes tensors without tangents")
 
 
 def _rows16(t: torch.Tensor):

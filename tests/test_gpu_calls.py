@@ -131,3 +131,27 @@ def test_host_operands():
         c.bind(1, 2)
     with pytest.raises(ValueError):
         c.bind(*[0] * 7, len, len)
+
+
+@pytest.mark.gpu
+def test_tangents_are_refused():
+    """A dual tensor in every place of every call; the caches stay as they are."""
+    import torch.autograd.forward_ad as fwd
+    import qattention_amd as qa
+    all_calls(operands())
+    o = operands()
+    kc, vc = o["Kc"], o["Vc"]
+    calls = [(qa.prompt_attention, [o["Q"], o["K"], o["V"]], [o["cu"], 30]),
+             (qa.prefix_attention_paged, [o["Q"][:2], kc[0], vc[0]], [o["table"], o["ctx"]]),
+             (qa.append_paged_kv, [o["K"][:2], o["V"][:2], kc[0], vc[0]], [o["table"], o["ctx"]]),
+             (qa.compact_paged_kv, [kc, vc], [o["table"], o["ctx"], o["path"]]),
+             (qa.copy_kv_pages, [kc, vc], [o["src"], o["dst"]])]
+    before = kc.clone(), vc.clone()
+    for f, ts, rest in calls:
+        for i in range(len(ts)):
+            with fwd.dual_level():
+                dual = [fwd.make_dual(t, torch.ones_like(t)) if j == i else t for j, t in enumerate(ts)]
+                say("tangent", f.__name__, i)
+                with pytest.raises(RuntimeError, match="no forward derivative"):
+                    f(*dual, *rest)
+    assert torch.equal(kc, before[0]) and torch.equal(vc, before[1])

@@ -236,3 +236,17 @@ def test_values_past_32_bits_do_not_wrap():
     assert ms == top - 4 and cu.tolist() == [0, 4, top]
     # (the C entries take 32 bits: 2^40 would arrive as 0)
     assert _offsets(torch.tensor([0, 4]), "cpu", 2 ** 40)[0] == top and paged_kv._rows(4, 1, cu[:2], 2 ** 33, "cpu")[0] == top
+
+
+def test_tangents_refused():
+    import torch.autograd.forward_ad as fwd
+    from qattention_amd.ragged_attn import _no_grad
+    x = torch.zeros(2)
+    with fwd.dual_level():
+        _no_grad(x)
+        dual = fwd.make_dual(x, torch.ones(2))
+        with pytest.raises(RuntimeError, match="no forward derivative"):
+            _no_grad(x, dual)
+        with torch.no_grad(), pytest.raises(RuntimeError, match="no forward derivative"):
+            _no_grad(dual)
+    _no_grad(x)
