@@ -80,7 +80,9 @@ def _vec(t: torch.Tensor) -> torch.Tensor:
         raise ValueError(f"tensor of shape {tuple(t.shape)} and strides {tuple(t.stride())} is not readable as "
                          "16-byte rows (unit last stride, 8-element aligned strides, 16-byte aligned base) and "
                          "layout copies are off (set_layout_copies)")
-    return t.contiguous()
+    # (contiguous() would return t where it starts off a 16-byte boundary, or where
+    # the stride of a dim of one is what is odd)
+    return t.clone(memory_format=torch.contiguous_format)
 
 
 def _require_device(*ts):

@@ -320,3 +320,21 @@ def test_lengths_past_32_bits():
         cu = torch.tensor([0, 20, 2 ** 32 + 50], device=device)
         O, L = prompt_attention(Q, K, V, cu, return_lse=True)
         assert torch.equal(O[:20], want[0][:20]) and torch.equal(L[:20], want[1][:20])
+
+
+def test_contiguous_inputs_off_a_boundary():
+    """Rows that start off a 16-byte boundary, and one token whose unused stride is odd."""
+    from qattention_amd import prefix_attention_paged, prompt_attention, ragged_attention
+    lens, Hq, Hkv, D = [40, 9], 4, 2, 64
+    Q, K, V = inputs(lens, Hq, Hkv, D, torch.float16, 59)
+    cu = offsets(lens)
+    shifted = [torch.cat([x.new_zeros(3), x.flatten()])[3:].view(x.shape) for x in (Q, K, V)]
+    say("off a boundary")
+    assert torch.equal(prompt_attention(*shifted, cu), prompt_attention(Q, K, V, cu))
+    assert torch.equal(ragged_attention(*shifted, cu, 2, 5), ragged_attention(Q, K, V, cu, 2, 5))
+    table, ctx = torch.tensor([[0, 1]], dtype=torch.int32, device=DEV), torch.tensor([20], dtype=torch.int32, device=DEV)
+    cache = [x[:32].view(2, 16, Hkv, D) for x in (K, V)]
+    wide = Hq * D + 3
+    one = torch.cat([Q.view(49, -1), Q.new_zeros(49, 3)], 1).as_strided((1, Hq, D), (wide, D, 1), 8 * wide)
+    got, want = (prefix_attention_paged(q, *cache, table, ctx) for q in (one, Q[8:9]))
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])

@@ -319,3 +319,22 @@ def test_layout_copies_switch():
     finally:
         ra.set_layout_copies(prev)
     assert ra._vec(ok).is_contiguous()
+
+
+def test_layout_copies_of_contiguous_tensors():
+    """What torch calls contiguous may still start off a 16-byte boundary, or have an
+    odd stride in a dim of one."""
+    from qattention_amd import ragged_attn as ra
+
+    base = torch.arange(2 * 3 * 64 + 8).half()
+    for t in (base[1:1 + 2 * 3 * 64].view(2, 3, 64), base[4:4 + 3 * 64].view(1, 3, 64),
+              base[:65 * 3].view(3, 65)[:1, :64].unsqueeze(1), base.as_strided((1, 2, 64), (7, 64, 1))):
+        assert t.is_contiguous() and not ra._vec_ok(t)
+        c, p, strides = ra._rows16(t)
+        assert ra._vec_ok(c) and torch.equal(c, t) and p == c.data_ptr() and tuple(strides) == c.stride()
+        prev = ra.set_layout_copies(False)
+        try:
+            with pytest.raises(ValueError, match="set_layout_copies"):
+                ra._vec(t)
+        finally:
+            ra.set_layout_copies(prev)
