@@ -9,6 +9,8 @@ import contextlib
 import ctypes as C
 import importlib.util
 import os
+import types
+import warnings
 
 import torch  # must be loaded first so libqattn.so binds torch's HIP runtime
 
@@ -120,17 +122,28 @@ def lib():
     return _lib
 
 
+def _not_here(*args):
+    """A call of the module that is not there: none of its answers."""
+
+
 def calls():
     """The module that makes a serving call whose operands need no conversion
-    (csrc/calls.cpp), bound to the library; raise if it has not been built."""
+    (csrc/calls.cpp), bound to the library.  Where it has not been built, or not for
+    this torch, a stand-in that answers no call: each goes on in Python, to the
+    same kernels."""
     global _calls
     if _calls is None:
         L = lib()
-        if not os.path.exists(CALLS_PATH):
-            raise QAttnError(f"{CALLS_PATH} is missing: build it with `python -m qattention_amd.build`")
         spec = importlib.util.spec_from_file_location("qattention_amd._calls", CALLS_PATH)
-        module = importlib.util.module_from_spec(spec)
-        spec.loader.exec_module(module)
+        try:
+            module = importlib.util.module_from_spec(spec)
+            spec.loader.exec_module(module)
+        except ImportError as e:
+            warnings.warn(f"serving calls go through Python (4 to 8 us more each): {e}; build the call module with "
+                          "`python -m qattention_amd.build`", RuntimeWarning)
+            _calls = types.SimpleNamespace(**dict.fromkeys(
+                ("prompt", "paged", "append", "compact", "copy", "set_ready"), _not_here))
+            return _calls
         module.bind(*(C.cast(getattr(L, name), _p).value for name in _BOUND),
                     torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream)
         for idx in _initialised:

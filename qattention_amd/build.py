@@ -9,7 +9,8 @@ allocations are valid handles for it.
 
 _calls.so, a CPython module of the host compiler, takes the serving calls from
 torch tensors to that C ABI; it links torch's libraries, which the process has
-loaded by then.
+loaded by then.  It shortens the way to the library and is no part of it: without
+a host compiler or the headers it is left out, and the calls go through Python.
 """
 from __future__ import annotations
 
@@ -84,6 +85,29 @@ def calls_command(out: str) -> list:
     ]
 
 
+def _start_calls(out: str, verbose: bool):
+    """The compiler of the call module at work, or what kept it from starting."""
+    try:
+        return _run(calls_command(out), verbose)
+    except (ImportError, OSError) as e:
+        return e
+
+
+def _finish_calls(proc, out: str, verbose: bool) -> None:
+    """Puts the call module in its place; one that cannot be built is left out, and
+    so is an older one, which may not fit the library."""
+    try:
+        if isinstance(proc, Exception):
+            raise proc
+        _finish(proc, verbose)
+        os.replace(out, CALLS_PATH)
+    except (ImportError, OSError, RuntimeError) as e:
+        if os.path.exists(CALLS_PATH):
+            os.remove(CALLS_PATH)
+        print(f"[qattention_amd.build] no {os.path.basename(CALLS_PATH)}, serving calls go through Python: {e}",
+              file=sys.stderr, flush=True)
+
+
 def build(verbose: bool = True) -> str:
     """Compile every HIP source into qattention_amd/libqattn.so and the call
     module into qattention_amd/_calls.so (always rebuilds).
@@ -97,13 +121,13 @@ def build(verbose: bool = True) -> str:
         objs.append(obj)
         procs.append(_run([_hipcc(), *compile_flags(), "-c", "-o", obj, os.path.join(CSRC, s)], verbose))
     calls_tmp = CALLS_PATH + ".tmp"
-    procs.append(_run(calls_command(calls_tmp), verbose))
+    calls = _start_calls(calls_tmp, verbose)
     for proc in procs:
         _finish(proc, verbose)
     tmp = LIB_PATH + ".tmp"
     _finish(_run([_hipcc(), f"--offload-arch={ARCH}", "-shared", "-o", tmp, *objs], verbose), verbose)
-    os.replace(calls_tmp, CALLS_PATH)
     os.replace(tmp, LIB_PATH)
+    _finish_calls(calls, calls_tmp, verbose)
     return LIB_PATH
 
 

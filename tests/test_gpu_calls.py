@@ -155,3 +155,19 @@ def test_tangents_are_refused():
                 with pytest.raises(RuntimeError, match="no forward derivative"):
                     f(*dual, *rest)
     assert torch.equal(kc, before[0]) and torch.equal(vc, before[1])
+
+
+@pytest.mark.gpu
+def test_same_without_the_call_module(tmp_path, monkeypatch):
+    """All calls where the module is missing: the same bits, by the same kernels."""
+    from qattention_amd import _lib
+    o = operands()
+    direct = all_calls(o)
+    monkeypatch.setattr(_lib, "CALLS_PATH", str(tmp_path / "_calls.so"))
+    monkeypatch.setattr(_lib, "_calls", None)
+    say("no module")
+    with pytest.warns(RuntimeWarning, match="go through Python"):
+        python = all_calls(o)
+    assert _lib.calls().prompt(o["Q"], o["K"], o["V"], o["cu"], 30, False) is None
+    for a, b in zip(direct, python):
+        assert torch.equal(a, b)

@@ -250,3 +250,41 @@ def test_tangents_refused():
         with torch.no_grad(), pytest.raises(RuntimeError, match="no forward derivative"):
             _no_grad(dual)
     _no_grad(x)
+
+
+@pytest.mark.parametrize("broken", ["compiler fails", "no compiler", "no headers"])
+def test_library_is_built_without_the_call_module(broken, tmp_path, monkeypatch, capsys):
+    """hipcc is a stand-in that writes what it is asked for."""
+    from qattention_amd import build
+    hipcc = tmp_path / "hipcc"
+    hipcc.write_text('#!/bin/sh\nwhile [ "$1" != -o ]; do shift; done\necho built > "$2"\n')
+    hipcc.chmod(0o755)
+    for name, to in (("LIB_PATH", "lib.so"), ("CALLS_PATH", "calls.so"), ("OBJ_DIR", "obj")):
+        monkeypatch.setattr(build, name, str(tmp_path / to))
+    monkeypatch.setattr(build, "_hipcc", lambda: str(hipcc))
+    (tmp_path / "calls.so").write_text("of another build")
+    if broken == "no headers":
+        def gone(out):
+            raise ImportError("no torch headers")
+        monkeypatch.setattr(build, "calls_command", gone)
+    else:
+        monkeypatch.setenv("CXX", "/bin/false" if broken == "compiler fails" else str(tmp_path / "not there"))
+    assert build.build(verbose=False) == str(tmp_path / "lib.so")
+    assert (tmp_path / "lib.so").read_text() == "built\n" and not (tmp_path / "calls.so").exists()
+    assert "serving calls go through Python" in capsys.readouterr().err
+
+
+@pytest.mark.parametrize("there", [False, True])
+def test_calls_go_on_without_the_call_module(there, tmp_path, monkeypatch):
+    """Not built, and built for something else."""
+    path = tmp_path / "_calls.so"
+    if there:
+        path.write_text("no module")
+    monkeypatch.setattr(_lib, "CALLS_PATH", str(path))
+    monkeypatch.setattr(_lib, "_calls", None)
+    x, cu = T(4, 2, 64), torch.tensor([0, 4], dtype=torch.int32)
+    with pytest.warns(RuntimeWarning, match="go through Python"), pytest.raises(RuntimeError, match="GPU only"):
+        qa.prompt_attention(x, x, x, cu)
+    assert _lib.calls().append() is None and _lib.calls().set_ready(0) is None
+    with pytest.raises(RuntimeError, match="GPU only"):  # (told once)
+        qa.copy_kv_pages(T(3, 16, 2, 64), T(3, 16, 2, 64), [0], [1])
