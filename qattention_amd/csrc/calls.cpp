@@ -167,6 +167,19 @@ PyObject* wrap(const Tensor& O, const Tensor& LSE, bool want_lse) {
     return both;
 }
 
+// While it lives other Python threads run: a launch waits where the stream's queue is
+// full, an allocation where memory has to be freed first.  (Operands are held by the
+// caller's frame.)
+class Unlocked {
+    PyThreadState* state_ = PyEval_SaveThread();
+
+public:
+    Unlocked() = default;
+    Unlocked(const Unlocked&) = delete;
+    Unlocked& operator=(const Unlocked&) = delete;
+    ~Unlocked() { PyEval_RestoreThread(state_); }
+};
+
 PyObject* none() { Py_RETURN_NONE; }
 
 // C++ exceptions (an allocation that fails) end here: the Python function
@@ -196,15 +209,20 @@ PyObject* prompt(PyObject*, PyObject* const* a, Py_ssize_t n) {
             return none();
         const bool want = a[5] == Py_True;
         const int32_t B = (int32_t)cu->size(0) - 1;
-        const int64_t bytes = prompt_ws(B, ms, T, (int32_t)Hq, (int32_t)Hkv, (int32_t)D);
-        Tensor O, LSE, ws;
-        if (!outputs(c, *Q, want, O, LSE)) return none();
-        if (bytes) ws = at::empty({bytes}, c.options(at::kByte));
-        const int rc = prompt_fwd(
-            Q->data_ptr(), Q->strides().data(), K->data_ptr(), K->strides().data(), V->data_ptr(), V->strides().data(),
-            O.data_ptr(), O.strides().data(), want ? LSE.data_ptr<float>() : nullptr,
-            want ? LSE.strides().data() : nullptr, cu->data_ptr<int32_t>(), B, ms, T, (int32_t)Hq, (int32_t)Hkv,
-            (int32_t)D, (float)(1.0 / std::sqrt((double)D)), c.code(), bytes ? ws.data_ptr() : nullptr, bytes, c.stream);
+        Tensor O, LSE;
+        const int rc = [&] {
+            Unlocked others;
+            const int64_t bytes = prompt_ws(B, ms, T, (int32_t)Hq, (int32_t)Hkv, (int32_t)D);
+            if (!outputs(c, *Q, want, O, LSE)) return -1;
+            Tensor ws;
+            if (bytes) ws = at::empty({bytes}, c.options(at::kByte));
+            return prompt_fwd(Q->data_ptr(), Q->strides().data(), K->data_ptr(), K->strides().data(), V->data_ptr(),
+                              V->strides().data(), O.data_ptr(), O.strides().data(),
+                              want ? LSE.data_ptr<float>() : nullptr, want ? LSE.strides().data() : nullptr,
+                              cu->data_ptr<int32_t>(), B, ms, T, (int32_t)Hq, (int32_t)Hkv, (int32_t)D,
+                              (float)(1.0 / std::sqrt((double)D)), c.code(), bytes ? ws.data_ptr() : nullptr, bytes,
+                              c.stream);
+        }();
         return rc ? none() : wrap(O, LSE, want);
     });
 }
@@ -226,16 +244,21 @@ PyObject* paged(PyObject*, PyObject* const* a, Py_ssize_t n) {
             return none();
         const bool want = a[7] == Py_True;
         const int32_t cols = (int32_t)table->size(1), ps = (int32_t)K->size(1);
-        const int64_t bytes = paged_ws((int32_t)B, ms, T, (int32_t)Hq, (int32_t)Hkv, (int32_t)D, cols, ps);
-        Tensor O, LSE, ws;
-        if (!outputs(c, *Q, want, O, LSE)) return none();
-        if (bytes) ws = at::empty({bytes}, c.options(at::kByte));
-        const int rc = paged_fwd(
-            Q->data_ptr(), Q->strides().data(), K->data_ptr(), K->strides().data(), V->data_ptr(), V->strides().data(),
-            table->data_ptr<int32_t>(), cols, (int32_t)K->size(0), ps, ctx->data_ptr<int32_t>(), O.data_ptr(),
-            O.strides().data(), want ? LSE.data_ptr<float>() : nullptr, want ? LSE.strides().data() : nullptr, cu,
-            (int32_t)B, ms, T, (int32_t)Hq, (int32_t)Hkv, (int32_t)D, (float)(1.0 / std::sqrt((double)D)), c.code(),
-            bytes ? ws.data_ptr() : nullptr, bytes, c.stream);
+        Tensor O, LSE;
+        const int rc = [&] {
+            Unlocked others;
+            const int64_t bytes = paged_ws((int32_t)B, ms, T, (int32_t)Hq, (int32_t)Hkv, (int32_t)D, cols, ps);
+            if (!outputs(c, *Q, want, O, LSE)) return -1;
+            Tensor ws;
+            if (bytes) ws = at::empty({bytes}, c.options(at::kByte));
+            return paged_fwd(Q->data_ptr(), Q->strides().data(), K->data_ptr(), K->strides().data(), V->data_ptr(),
+                             V->strides().data(), table->data_ptr<int32_t>(), cols, (int32_t)K->size(0), ps,
+                             ctx->data_ptr<int32_t>(), O.data_ptr(), O.strides().data(),
+                             want ? LSE.data_ptr<float>() : nullptr, want ? LSE.strides().data() : nullptr, cu,
+                             (int32_t)B, ms, T, (int32_t)Hq, (int32_t)Hkv, (int32_t)D,
+                             (float)(1.0 / std::sqrt((double)D)), c.code(), bytes ? ws.data_ptr() : nullptr, bytes,
+                             c.stream);
+        }();
         return rc ? none() : wrap(O, LSE, want);
     });
 }
@@ -255,12 +278,16 @@ PyObject* append(PyObject*, PyObject* const* a, Py_ssize_t n) {
             T > kInt || B > kInt || table->size(1) > kInt || !offsets(c, a[6], a[7], T, B, cu, ms) || !c.here())
             return none();
         int64_t ks[5], vs[5];
-        Tensor after = at::empty_like(*ctx);
-        const int rc = kv_append(
-            K->data_ptr(), K->strides().data(), V->data_ptr(), V->strides().data(), Kc->data_ptr(), strides5(*Kc, ks),
-            Vc->data_ptr(), strides5(*Vc, vs), table->data_ptr<int32_t>(), (int32_t)table->size(1), (int32_t)Kc->size(0),
-            (int32_t)Kc->size(1), ctx->data_ptr<int32_t>(), after.data_ptr<int32_t>(), cu, (int32_t)B, ms, T,
-            (int32_t)Kc->size(2), (int32_t)Kc->size(3), c.code(), c.stream);
+        Tensor after;
+        const int rc = [&] {
+            Unlocked others;
+            after = at::empty_like(*ctx);
+            return kv_append(K->data_ptr(), K->strides().data(), V->data_ptr(), V->strides().data(), Kc->data_ptr(),
+                             strides5(*Kc, ks), Vc->data_ptr(), strides5(*Vc, vs), table->data_ptr<int32_t>(),
+                             (int32_t)table->size(1), (int32_t)Kc->size(0), (int32_t)Kc->size(1),
+                             ctx->data_ptr<int32_t>(), after.data_ptr<int32_t>(), cu, (int32_t)B, ms, T,
+                             (int32_t)Kc->size(2), (int32_t)Kc->size(3), c.code(), c.stream);
+        }();
         return rc ? none() : THPVariable_Wrap(after);
     });
 }
@@ -281,12 +308,16 @@ PyObject* compact(PyObject*, PyObject* const* a, Py_ssize_t n) {
             return none();
         int64_t ks[5], vs[5];
         const int64_t layers = dim == 5 ? Kc->size(0) : 1, o = dim - 4;
-        Tensor after = at::empty_like(*ctx);
-        const int rc = kv_compact(Kc->data_ptr(), strides5(*Kc, ks), Vc->data_ptr(), strides5(*Vc, vs), (int32_t)layers,
-                                  table->data_ptr<int32_t>(), (int32_t)table->size(1), (int32_t)Kc->size(o),
-                                  (int32_t)Kc->size(o + 1), ctx->data_ptr<int32_t>(), path->data_ptr<int32_t>(),
-                                  (int32_t)path->size(1), after.data_ptr<int32_t>(), (int32_t)B,
-                                  (int32_t)Kc->size(o + 2), (int32_t)Kc->size(o + 3), c.code(), c.stream);
+        Tensor after;
+        const int rc = [&] {
+            Unlocked others;
+            after = at::empty_like(*ctx);
+            return kv_compact(Kc->data_ptr(), strides5(*Kc, ks), Vc->data_ptr(), strides5(*Vc, vs), (int32_t)layers,
+                              table->data_ptr<int32_t>(), (int32_t)table->size(1), (int32_t)Kc->size(o),
+                              (int32_t)Kc->size(o + 1), ctx->data_ptr<int32_t>(), path->data_ptr<int32_t>(),
+                              (int32_t)path->size(1), after.data_ptr<int32_t>(), (int32_t)B, (int32_t)Kc->size(o + 2),
+                              (int32_t)Kc->size(o + 3), c.code(), c.stream);
+        }();
         return rc ? none() : THPVariable_Wrap(after);
     });
 }
@@ -303,10 +334,13 @@ PyObject* copy(PyObject*, PyObject* const* a, Py_ssize_t n) {
             return none();
         int64_t ks[5], vs[5];
         const int64_t layers = dim == 5 ? Kc->size(0) : 1, o = dim - 4;
-        const int rc = kv_copy(Kc->data_ptr(), strides5(*Kc, ks), Vc->data_ptr(), strides5(*Vc, vs), (int32_t)layers,
-                               (int32_t)Kc->size(o), (int32_t)Kc->size(o + 1), src->data_ptr<int32_t>(),
-                               dst->data_ptr<int32_t>(), (int32_t)src->size(0), (int32_t)Kc->size(o + 2),
-                               (int32_t)Kc->size(o + 3), c.code(), c.stream);
+        const int rc = [&] {
+            Unlocked others;
+            return kv_copy(Kc->data_ptr(), strides5(*Kc, ks), Vc->data_ptr(), strides5(*Vc, vs), (int32_t)layers,
+                           (int32_t)Kc->size(o), (int32_t)Kc->size(o + 1), src->data_ptr<int32_t>(),
+                           dst->data_ptr<int32_t>(), (int32_t)src->size(0), (int32_t)Kc->size(o + 2),
+                           (int32_t)Kc->size(o + 3), c.code(), c.stream);
+        }();
         if (rc) return none();
         Py_RETURN_TRUE;
     });

@@ -171,3 +171,52 @@ def test_same_without_the_call_module(tmp_path, monkeypatch):
     assert _lib.calls().prompt(o["Q"], o["K"], o["V"], o["cu"], 30, False) is None
     for a, b in zip(direct, python):
         assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", ["prompt", "paged", "append", "compact", "copy"])
+def test_other_threads_run_meanwhile(name):
+    """A library entry that waits (pause() in its place, until a timer's signal): Python's
+    other threads go on.  Nothing is launched."""
+    import ctypes
+    import signal
+    import threading
+    import time
+
+    from qattention_amd import _lib
+    all_calls(operands())
+    c, o = _lib.calls(), operands()
+    args = {"prompt": (o["Q"], o["K"], o["V"], o["cu"], 30, True),
+            "paged": (o["Q"], o["Kc"][0], o["Vc"][0], o["table"], o["ctx"], o["cu"], 30, True),
+            "append": (o["K"], o["V"], o["Kc"][0], o["Vc"][0], o["table"], o["ctx"], o["cu"], 30),
+            "compact": (o["Kc"], o["Vc"], o["table"], o["ctx"], o["path"]),
+            "copy": (o["Kc"], o["Vc"], o["src"], o["dst"])}[name]
+    address = lambda f: ctypes.cast(f, ctypes.c_void_p).value  # noqa: E731
+    real = [address(getattr(_lib.lib(), n)) for n in _lib._BOUND]
+    fake = list(real)
+    fake[("", "prompt", "", "paged", "append", "compact", "copy").index(name)] = address(ctypes.CDLL(None).pause)
+    torch_fns = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+    ticks, stop = [], threading.Event()
+
+    def tick():
+        while not stop.wait(0.002):
+            ticks.append(time.perf_counter())
+
+    thread = threading.Thread(target=tick)
+    handler = signal.signal(signal.SIGALRM, lambda *a: None)
+    c.bind(*fake, *torch_fns)
+    thread.start()
+    say("waiting entry", name)
+    try:
+        timer = signal.setitimer(signal.ITIMER_REAL, 0.3, 0.1)
+        a = time.perf_counter()
+        out = getattr(c, name)(*args)
+        b = time.perf_counter()
+    finally:
+        signal.setitimer(signal.ITIMER_REAL, *timer)
+        signal.signal(signal.SIGALRM, handler)
+        c.bind(*real, *torch_fns)
+        stop.set()
+        thread.join()
+    assert out is None and b - a > 0.2  # (pause() ends in an error: the call is left to Python)
+    assert sum(a + 0.05 < t < b - 0.05 for t in ticks) >= 10
