@@ -270,11 +270,11 @@ __device__ __forceinline__ SeqWork next_part(const PagedParams& p, Share& sh, Pa
 // TB/s against 5.6 for the bare loads of 64 x 10240 keys.
 // STREAM: runs of units, as above.  Otherwise a workgroup per item, for short
 // contexts, where the launch is all latency: no scan ahead of the first load and
-// no second kernel (2 x 300 keys, 32 / 8 heads: 7.7 us against 10.5 in runs, 2 x
-// 700: 11.3 against 10.5 in a graph, 11.3 against 11 to 12 per eager call).  A CU
-// draws about 26 GB/s from far away however many loads it has in flight (two
-// steps of them were 3-10% slower than one), so a few long contexts want many
-// CUs: 2 x 2000 keys take 23.9 us so, 11 in runs.
+// no second kernel (2 x 300 keys, 32 / 8 heads, in a graph: 8.1 us against 11.2 in
+// runs, 2 x 500: 9.4 against 11.3).  A workgroup draws about 53 GB/s from far away
+// however many loads it has in flight (two steps of them were 3-10% slower than
+// one), so a few longer contexts want many CUs: 2 x 700 keys take 12.0 us so and
+// 11.3 in runs, 2 x 2000 23.9 and 11.
 // ---------------------------------------------------------------------------
 constexpr int kNarrowWaves = 4;             // waves of a STREAM workgroup
 constexpr int kItemWaves = 8;               // waves of a workgroup per item
@@ -903,12 +903,18 @@ struct PagedShape {
     bool items;
 };
 static PagedShape paged_shape(int64_t max_rows, int64_t pairs, int hkv, int64_t capacity, int head_dim) {
-    // A workgroup per item, where every one runs at once: three steps at most, or
-    // four where the items fill half the chip by themselves (8 x 1024 keys, 8 kv
-    // heads: 15.3 us against 14.0 in runs, 16 x 1024: 16.0 against 20.5, 32 x 1024:
-    // 23.8 against 29.6; longer ones gain 5 us of 40 with equal contexts, and lose
-    // as much where they differ by a factor of three, which runs even out).
-    const int steps = pairs >= 128 ? 4 : 3;
+    // A workgroup per item, where every one runs at once: two steps at most, or
+    // four where the items fill half the chip by themselves (replays of a graph,
+    // 128-wide heads, 8 kv heads, against runs: 2 x 500 keys 9.4 us and 11.3, 2 x 700
+    // 12.0 and 11.3, 4 x 700 12.2 and 11.8, 8 x 700 15.6 and 15.5, 16 x 700 17.8 and
+    // 20.9, 32 x 700 21.8 and 28.0, 8 x 1000 20.3 and 16.9, 16 x 1024 23.2 and 23.4,
+    // 32 x 1024 29.5 and 35.6; eager calls give runs half a us more.  Longer ones
+    // gain 5 us of 40 with equal contexts, and lose as much where they differ by a
+    // factor of three, which runs even out).  The lengths stay on the device, so
+    // capacity, what the table has columns for, stands for them: 2 x 300 keys take
+    // 10.8 us with a table four times as wide, 12.5 with one of 32 times, 32 x 1024
+    // 34.6 with either, 64 x 500 34.2 against 32.6.
+    const int steps = pairs >= 128 ? 4 : 2;
     if (max_rows <= 16 && capacity <= steps * 32 * kItemWaves && pairs <= 256) return {1, 4, 8, 1, 1, true};
     if (max_rows <= 32) {
         const int qb = max_rows <= 16 ? 1 : 2;

@@ -288,3 +288,11 @@ def test_calls_go_on_without_the_call_module(there, tmp_path, monkeypatch):
     assert _lib.calls().append() is None and _lib.calls().set_ready(0) is None
     with pytest.raises(RuntimeError, match="GPU only"):  # (told once)
         qa.copy_kv_pages(T(3, 16, 2, 64), T(3, 16, 2, 64), [0], [1])
+
+
+def test_workgroup_per_item_limits():
+    """Two steps of 256 keys, four where the items fill half the chip: no workspace."""
+    ws = _lib.lib().qattn_prefix_paged_workspace_bytes
+    items = lambda B, cols: ws(B, 1, B, 32, 8, 128, cols, 16) == 0  # noqa: E731
+    assert items(2, 32) and not items(2, 33) and items(15, 32) and not items(15, 33)
+    assert items(16, 64) and not items(16, 65) and items(32, 64) and not items(33, 64)
