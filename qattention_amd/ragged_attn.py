@@ -178,7 +178,9 @@ def _to_device(t: torch.Tensor, device) -> torch.Tensor:
     pageable memory has read it when it returns)."""
     if t.is_cpu and torch.device(device).type == "cuda" and t.is_pinned():
         if not torch.cuda.is_current_stream_capturing():  # (a graph reads the caller's memory at every replay)
-            t = t.clone()
+            # (into pinned memory again, which torch keeps until it has been read: a copy
+            # of 4 MB from pageable memory waits for the stream, small ones do not)
+            t = torch.empty(t.shape, dtype=torch.int32, pin_memory=True).copy_(t)
     return t.to(device=device, dtype=torch.int32, non_blocking=True).contiguous()
 
 
