@@ -19,8 +19,9 @@
 // and 0 times an infinity or a NaN is NaN: a tile whose results are not all
 // finite is computed once more, and then infinities and NaN in V are taken out of
 // the blocks that hold masked keys and added to the rows that attend them by
-// themselves.  (Looking through those blocks always: 16 prompts of 1300 tokens on
-// average, 32 / 8 heads of 64: 166 -> 181 us.)
+// themselves.  (Looking through those blocks always: 16 prompts of 603 .. 2011
+// tokens, 32 / 8 heads of 64, bf16: 192 us, so 183.  8192 tokens, 32 / 8 heads of
+// 128: 519 us, with NaN in one V row 889.)
 #include <algorithm>
 
 #include "dense_tiles.h"
@@ -32,8 +33,8 @@ namespace qattn {
 constexpr int kPromptThreads = 256;
 constexpr int kBM = 128;  // rows per workgroup
 // Waves per SIMD: 64-wide heads have half the products per exponential, and a
-// third wave covers what two leave (16 x 1300 tokens, 32 / 8 heads: 161 us with
-// two, 152 with three).
+// third wave covers what two leave (16 x 1300 tokens, 32 / 8 heads, bf16: 159 us
+// with two, 150 with three).
 constexpr int prompt_waves(int d) { return d == 64 ? 3 : 2; }
 
 struct PromptParams {
@@ -62,8 +63,6 @@ struct PromptParams {
     float scale_log2;
 };
 
-// The keys of a prompt tile: rows 0 .. k_hi - 1 of the sequence (the tile's last
-// token is k_hi - 1), contiguous at a token stride.
 // Parts of a tile of nb blocks; part c starts at block first(c).  Equal but for
 // one block, so with p.part >= 8 a part of a cut tile has four blocks or more:
 // the keys ahead of a tile's last part end 193 keys before the tile's last
@@ -114,6 +113,9 @@ __device__ __forceinline__ bool numbered_tile(const PromptParams& p, int i, int&
     return false;
 }
 
+// The keys of a prompt tile, or of one part of it: rows k_lo .. k_hi - 1 of the
+// sequence, contiguous at a token stride (of a tile's last part k_hi - 1 is the
+// tile's last token).
 template <typename T, int D>
 struct PromptKeys {
     using Tile = DenseTile<T, D>;
@@ -295,8 +297,8 @@ __global__ __launch_bounds__(kPromptThreads) __attribute__((amdgpu_waves_per_eu(
         const int k = (int)((uint32_t)in / (uint32_t)here);
         // An XCD deals its workgroups to its shader engines in turn, however busy
         // they are: with a list in the same place of every round, one engine would
-        // have the longest prompts' tiles to itself (16 prompts of 603 .. 2011 tokens:
-        // 210 us; turned by one place per round: 181).
+        // have the longest prompts' tiles to itself (16 prompts of 603 .. 2011 tokens,
+        // 32 / 8 heads of 64, bf16: 215 us; turned by one place per round: 183).
         int at = in - k * here;
         if (!(here & 1)) at = (int)((uint32_t)(at + k) % (uint32_t)here);
         const int v = (blockIdx.x & 7) + 8 * (grp * p.group_lists + at);
@@ -509,8 +511,8 @@ static PromptPlan prompt_plan(int32_t batch, int32_t max_seqlen, int64_t total_t
     int64_t full = batch;  // sequences, if all were of the longest one's length
     // Numbering the tiles that there are costs a look through the offsets ahead
     // of everything else; a workgroup without a tile costs 1/3 us of a slot (one
-    // prompt of 2048 tokens, 32 / 8 heads, with 63 of one token: 46 us
-    // numbered, 63 with a place for 64 prompts of 2048; with 255: 58 and 140).
+    // prompt of 2048 tokens, 32 / 8 heads, bf16, with 63 of one token: 50 us
+    // numbered, 68 with a place for 64 prompts of 2048; with 255: 58 and 145).
     const int64_t numbered = ((total_tokens * q.group + kBM - 1) / kBM + batch) * hkv;
     if (q.slots > 4 * numbered && numbered < INT32_MAX / kBM - 8) {
         q.tiles = (int32_t)((numbered + 7) / 8 * 8);
@@ -521,8 +523,9 @@ static PromptPlan prompt_plan(int32_t batch, int32_t max_seqlen, int64_t total_t
     // workgroup takes 4/5 of the time per block that it takes with two, and the
     // second kernel and the states cost what about 16 blocks take.  With as many
     // tiles as slots the short ones next to the long ones even the CUs out by
-    // themselves (504 tiles of 2000 tokens: 42 us whole, 68 cut in two); 64 tiles
-    // of 2000 tokens: 23.4 us whole, 16.7 in parts.
+    // themselves (504 tiles of 2000 tokens, 32 / 8 heads, bf16: 46 us whole, 74 cut
+    // in two); 63 tiles of 2000 tokens, 4 heads over one: 36.0 us whole, 23.2 in
+    // parts; 4000 tokens of those: 66 and 45.
     const int64_t longest = (q.max_seqlen + 63) / 64;
     const int64_t blocks = full * hkv * q.qtiles * (longest + 1) / 2;
     const int64_t share = std::max<int64_t>(8, (blocks + 255) / 256);  // of a CU

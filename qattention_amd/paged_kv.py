@@ -30,7 +30,7 @@ captured in a graph):
 The calls run on torch's current stream, take contexts, offsets and page tables
 on the host too (a copy each call, of what they hold at the call; not while a
 graph is captured), and serve inference: tensors that ask for gradients are
-refused while autograd records.
+refused while autograd records, those with tangents always.
 """
 from __future__ import annotations
 
@@ -112,12 +112,18 @@ def prefix_attention_paged(
     dividing Hq; page_table [B, max_pages]; context_lens [B].  Every query token
     of sequence s attends positions 0 .. context_lens[s] - 1 (those that the
     table has columns for), not itself: append its row first, or merge another
-    block by its LSE.  cu_seqlens None: one token per sequence (a decode step);
-    otherwise the packed offsets of the query tokens (draft trees, prompt
-    chunks), max_seqlen as everywhere.  A page outside the cache removes its
-    keys; a query without any gets 0 and an LSE of -inf.  Rows of Q that
-    belong to no sequence are not computed.  Returns O [T, Hq, D] (and LSE
-    [T, Hq] fp32, natural log, if return_lse)."""
+    block by its LSE.  The lengths stay on the device, so the kernel is chosen by
+    the table's width: columns past the longest context cost up to 5 us of a
+    decode step's 8 to 30.  A cache spans less than 64 GiB, a layer's slice of one
+    with the layers side by side in each page as much as all of them (QAttnError
+    otherwise; the calls that move rows take any).
+
+    cu_seqlens None: one token per sequence (a decode step); otherwise the packed
+    offsets of the query tokens (draft trees, prompt chunks), max_seqlen as
+    everywhere.  A page outside the cache removes its keys; a query without any
+    gets 0 and an LSE of -inf.  Rows of Q that belong to no sequence are not
+    computed.  Returns O [T, Hq, D] (and LSE [T, Hq] fp32, natural log, if
+    return_lse)."""
     out = _lib.calls().paged(Q, K_cache, V_cache, page_table, context_lens, cu_seqlens, max_seqlen, return_lse)
     if out is not None:
         return out

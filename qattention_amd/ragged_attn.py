@@ -776,8 +776,9 @@ def prompt_attention(
     rows hold, infinities and NaN included, never reaches a token.  Rows of no
     sequence are not computed.  With return_lse its output merges with an earlier
     chunk's context (prefix_attention, prefix_attention_paged) through
-    fused_lse_merge.  Serves inference: tensors that ask for gradients are
-    refused while autograd records.  Returns O [sum L_i, Hq, D] (and LSE
+    fused_lse_merge.  Token strides of K and V are below 2^25 elements (QAttnError
+    otherwise).  Serves inference: tensors that ask for gradients are refused while
+    autograd records, those with tangents always.  Returns O [sum L_i, Hq, D] (and LSE
     [sum L_i, Hq] fp32, natural log, if return_lse)."""
     out = _lib.calls().prompt(Q, K, V, cu_seqlens, max_seqlen, return_lse)
     if out is not None:
