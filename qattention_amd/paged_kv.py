@@ -35,19 +35,20 @@ refused while autograd records, those with tangents always.
 from __future__ import annotations
 
 import math
+import operator
 from typing import Optional, Sequence, Tuple, Union
 
 import torch
 
 from . import _lib
-from .ragged_attn import (_SUPPORTED, _check_dtypes, _device_index, _dtype_code, _integers, _launch,
-                          _no_grad, _no_host_in_graph, _offsets, _out_like, _rows16, _to_device, _vec_ok)
+from .ragged_attn import (_SUPPORTED, _check_dtypes, _device_index, _dtype_code, _integers, _launch, _no_grad,
+                          _offsets, _out_like, _rows16, _to_device, _vec_ok)
 
 
 def _int32(t: torch.Tensor, device) -> torch.Tensor:
     if t.dtype is torch.int32 and t.device == device and t.is_contiguous():
         return t
-    return _to_device(_integers(_no_host_in_graph(t, device)), device)
+    return _to_device(_integers(t), device, in_graph=False)
 
 
 def _check_caches(K_cache, V_cache, dims: Tuple[int, ...]) -> tuple:
@@ -246,25 +247,21 @@ def compact_paged_kv(
 _Pages = Union[torch.Tensor, Sequence[int]]
 
 
-def _page_list(pages: _Pages) -> torch.Tensor:
-    if not isinstance(pages, torch.Tensor):
-        pages = list(pages)
-        # (without a dtype: given one, torch would cut fractions off)
-        pages = torch.tensor(pages) if pages else torch.empty(0, dtype=torch.int64)
-    return _integers(pages)
+def _whole(pages: Sequence[int]) -> list:
+    try:
+        return [operator.index(p) for p in pages]
+    except TypeError as e:
+        raise ValueError(f"pages must be integers ({e})") from None
 
 
 def _page_lists(src, dst, num_pages: int, device):
     """Both lists on the device.  Lists on the host are checked: every page in
     the cache, no destination twice, none that is also a source."""
-    src, dst = _page_list(src), _page_list(dst)
-    on_gpu = src.is_cuda and dst.is_cuda
-    if src.dim() != 1 or src.shape != dst.shape:
-        raise ValueError(f"src_pages and dst_pages must be lists of one length (got {tuple(src.shape)}, "
-                         f"{tuple(dst.shape)})")
-    if on_gpu:
-        return _int32(src, device), _int32(dst, device)
-    s, d = (None if t.is_cuda else t.tolist() for t in (src, dst))
+    src, dst = (_integers(t) if isinstance(t, torch.Tensor) else _whole(t) for t in (src, dst))
+    shapes = [tuple(t.shape) if isinstance(t, torch.Tensor) else (len(t),) for t in (src, dst)]
+    if len(shapes[0]) != 1 or shapes[0] != shapes[1]:
+        raise ValueError(f"src_pages and dst_pages must be lists of one length (got {shapes[0]}, {shapes[1]})")
+    s, d = (t if isinstance(t, list) else None if t.is_cuda else t.tolist() for t in (src, dst))
     for pages in (s, d):
         if pages is not None and any(not 0 <= p < num_pages for p in pages):
             raise ValueError(f"page outside [0, {num_pages})")
@@ -274,6 +271,7 @@ def _page_lists(src, dst, num_pages: int, device):
         to = dict(zip(d, s))  # (a page copied onto itself stays as it is)
         if any(to.get(a, a) != a for a in s):
             raise ValueError("a page is the destination of one copy and the source of another")
+    src, dst = (torch.tensor(t, dtype=torch.int32) if isinstance(t, list) else t for t in (src, dst))
     return _int32(src, device), _int32(dst, device)
 
 

@@ -99,10 +99,11 @@ def _require_device(*ts):
 
 def _no_grad(*ts) -> None:
     """Refuse tensors that ask for gradients or carry tangents: there is no derivative."""
+    duals = forward_ad._current_level >= 0
     for t in ts:
         if t.requires_grad and torch.is_grad_enabled():
             raise RuntimeError("this call has no backward pass: use torch.no_grad() or detach its inputs")
-        if forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None:
+        if duals and forward_ad.unpack_dual(t).tangent is not None:
             raise RuntimeError("this call has no forward derivative: it takes tensors without tangents")
 
 
@@ -172,19 +173,24 @@ def _on(device):
     return _HERE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
 
 
-def _to_device(t: torch.Tensor, device) -> torch.Tensor:
+def _to_device(t: torch.Tensor, device, in_graph: bool = True) -> torch.Tensor:
     """int32 on the device, of what t holds now: a copy from pinned memory waits for
     its turn in the stream, and the caller may write there meanwhile (one from
-    pageable memory has read it when it returns)."""
-    if t.is_cpu and torch.device(device).type == "cuda" and t.is_pinned():
-        if not torch.cuda.is_current_stream_capturing():  # (a graph reads the caller's memory at every replay)
+    pageable memory has read it when it returns).  A captured copy reads host memory
+    at every replay; in_graph False refuses it."""
+    if t.is_cpu and getattr(device, "type", device) == "cuda":
+        if torch._C._cuda_isCurrentStreamCapturing():
+            if not in_graph:
+                raise RuntimeError("lengths, offsets and pages must be on the GPU while a graph is captured: it would "
+                                   "read host memory at every replay")
+        elif t.is_pinned():
             # (into pinned memory again, which torch keeps until it has been read: a copy
             # of 4 MB from pageable memory waits for the stream, small ones do not)
             t = torch.empty(t.shape, dtype=torch.int32, pin_memory=True).copy_(t)
     return t.to(device=device, dtype=torch.int32, non_blocking=True).contiguous()
 
 
-def _seqlens(cu_seqlens: torch.Tensor, B: int, device, max_seqlen: Optional[int]):
+def _seqlens(cu_seqlens: torch.Tensor, B: int, device, max_seqlen: Optional[int], in_graph: bool = True):
     """max_seqlen and a device int32 copy of cu_seqlens (src/ragged_attn.py:1136-1142).
 
     When max_seqlen is None it is computed from a host copy of cu_seqlens
@@ -194,9 +200,9 @@ def _seqlens(cu_seqlens: torch.Tensor, B: int, device, max_seqlen: Optional[int]
         cu_cpu = cu_seqlens.cpu()
         sl = cu_cpu.tolist()
         max_seqlen = int(max([e - b for b, e in zip(sl, sl[1:])])) if B else 1
-        cu_dev = _to_device(cu_cpu, device)
+        cu_dev = _to_device(cu_cpu, device, in_graph)
     else:
-        cu_dev = _to_device(cu_seqlens, device)
+        cu_dev = _to_device(cu_seqlens, device, in_graph)
     return max(int(max_seqlen), 0), cu_dev
 
 
@@ -206,6 +212,8 @@ _INT32 = torch.iinfo(torch.int32)
 def _integers(t: torch.Tensor) -> torch.Tensor:
     """t, its values within 32 bits: what lies past them goes to their end, which
     is past every table, cache and row as well (2^32 + 3 is not page 3)."""
+    if t.dtype is torch.int32:
+        return t
     if t.is_floating_point() or t.is_complex():
         raise ValueError(f"lengths, offsets and pages must be integers (got {t.dtype})")
     if t.dtype is torch.uint64:
@@ -216,19 +224,11 @@ def _integers(t: torch.Tensor) -> torch.Tensor:
     return t
 
 
-def _no_host_in_graph(t: torch.Tensor, device) -> torch.Tensor:
-    if t.is_cpu and torch.device(device).type == "cuda" and torch.cuda.is_current_stream_capturing():
-        raise RuntimeError("lengths, offsets and pages must be on the GPU while a graph is captured: it would read "
-                           "host memory at every replay")
-    return t
-
-
 def _offsets(cu_seqlens: torch.Tensor, device, max_seqlen: Optional[int]):
     """_seqlens for the serving calls: [B + 1] integers."""
     if cu_seqlens.dim() != 1 or cu_seqlens.shape[0] < 1:
         raise ValueError(f"cu_seqlens must be [B + 1] (got {tuple(cu_seqlens.shape)})")
-    cu_seqlens = _integers(_no_host_in_graph(cu_seqlens, device))
-    max_seqlen, cu = _seqlens(cu_seqlens, cu_seqlens.shape[0] - 1, device, max_seqlen)
+    max_seqlen, cu = _seqlens(_integers(cu_seqlens), cu_seqlens.shape[0] - 1, device, max_seqlen, in_graph=False)
     return min(max_seqlen, _INT32.max), cu
 
 
