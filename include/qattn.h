@@ -68,6 +68,7 @@ extern "C" {
 
 #define QATTN_DTYPE_F16 0
 #define QATTN_DTYPE_BF16 1
+#define QATTN_DTYPE_U8 2 /* rows of bytes: qattn_kv_compact and qattn_kv_copy_pages only */
 
 /* Kernel selection for qattn_tree_fwd (QATTN_ALGO_AUTO picks per shape). */
 #define QATTN_ALGO_AUTO 0
@@ -464,7 +465,9 @@ int qattn_kv_append(const void *k, const int64_t k_stride[3], const void *v, con
  * or lies beyond the page table.  new_lens[s] = context_lens[s] + the path's
  * length.  A row whose page or whose place's page does not exist is not
  * moved.  A sequence with a negative context length is left alone.  Sequences
- * that share a page among those positions race.
+ * that share a page among those positions race.  dtype QATTN_DTYPE_U8: rows of
+ * head_dim (1 to 1024) bytes per head, strides in bytes, any alignment; the heads
+ * of a token lie together, or head_dim is a power of two.
  */
 int qattn_kv_compact(void *k_cache, const int64_t kc_stride[5], void *v_cache, const int64_t vc_stride[5],
                      int32_t num_layers, const int32_t *page_table, int32_t pt_cols, int32_t num_pages,
@@ -477,12 +480,76 @@ int qattn_kv_compact(void *k_cache, const int64_t kc_stride[5], void *v_cache, c
  * page src_pages[i] of K and of V, i < n (DEVICE int32 arrays).  Pairs with a
  * page outside [0, num_pages) are passed over.  No page may be the
  * destination of two pairs or the destination of one and the source of
- * another: the copies run side by side.
+ * another: the copies run side by side.  dtype as in qattn_kv_compact.
  */
 int qattn_kv_copy_pages(void *k_cache, const int64_t kc_stride[5], void *v_cache, const int64_t vc_stride[5],
                         int32_t num_layers, int32_t num_pages, int32_t page_size,
                         const int32_t *src_pages, const int32_t *dst_pages, int32_t n,
                         int32_t num_kv_heads, int32_t head_dim, int32_t dtype, void *stream);
+
+/*
+ * A paged cache held in 4 or 8 bits (`bits`): blocks of 32 elements along the
+ * head dim share a scale.  Elements are bytes [num_pages, page_size,
+ * num_kv_heads, head_dim * bits / 8]: e2m1 (the block's even elements in the
+ * low halves) or e4m3; scales are bytes [num_pages, page_size, num_kv_heads,
+ * head_dim / 32]: c for 2^(c - 127), 255 for a block that is no number.  K and V
+ * share the 4 byte strides {page, slot, head, byte}, the last of them 1, of
+ * their elements (multiples of 16, 16-byte aligned bases) and those of their
+ * scales (multiples of head_dim / 32, bases aligned to that).
+ *
+ * qattn_quant_append: qattn_kv_append with the rows (k, v of dtype) quantised.
+ * The scale is the smallest power of two s, at least 2^-126, with the block's
+ * largest magnitude no more than 1.75 * 2^T * s (T = 2 for 4 bits, 8 for 8), at
+ * most 2^(15 - T) for fp16 rows and 2^(127 - T) for bf16 rows; elements are
+ * x / s rounded to nearest, ties to the even code, and end at the format's
+ * largest, 6 or 448.  A block with an infinity or a NaN gets scale 255.
+ */
+int qattn_quant_append(const void *k, const int64_t k_stride[3], const void *v, const int64_t v_stride[3],
+                       void *k_cache, void *v_cache, const int64_t cache_stride[4],
+                       void *k_scale, void *v_scale, const int64_t scale_stride[4],
+                       const int32_t *page_table, int32_t pt_cols, int32_t num_pages, int32_t page_size,
+                       const int32_t *context_lens, int32_t *new_lens, const int32_t *cu_seqlens,
+                       int32_t batch, int32_t max_seqlen, int64_t total_tokens, int32_t num_kv_heads,
+                       int32_t head_dim, int32_t dtype, int32_t bits, void *stream);
+
+/*
+ * Rows of such a cache as fp16 or bf16 (k, v: 3 strides {token, head, dim}): row
+ * cu_seqlens[s] + i takes position starts[s] + i of sequence s, i < max_seqlen
+ * (cu_seqlens NULL: row s takes position starts[s]).  A position that is
+ * negative, has no column or whose page lies outside the cache reads as zeros;
+ * rows of no sequence are left as they were.  An element past fp16's range
+ * becomes an infinity there.
+ */
+int qattn_quant_read(const void *k_cache, const void *v_cache, const int64_t cache_stride[4],
+                     const void *k_scale, const void *v_scale, const int64_t scale_stride[4],
+                     const int32_t *page_table, int32_t pt_cols, int32_t num_pages, int32_t page_size,
+                     const int32_t *starts, void *k, const int64_t k_stride[3], void *v,
+                     const int64_t v_stride[3], const int32_t *cu_seqlens, int32_t batch,
+                     int32_t max_seqlen, int64_t total_tokens, int32_t num_kv_heads, int32_t head_dim,
+                     int32_t dtype, int32_t bits, void *stream);
+
+/*
+ * qattn_prefix_paged_fwd over such a cache: every row attends the values that the
+ * elements and scales stand for (with fp16 queries they have to lie in fp16's
+ * range, as those written from fp16 rows do).  The elements of a cache span less
+ * than 64 GiB, its scales less than 2^32 rows.  Workspace as there, of
+ * qattn_prefix_quant_workspace_bytes() bytes.
+ */
+int64_t qattn_prefix_quant_workspace_bytes(int32_t batch, int32_t max_seqlen, int64_t total_tokens,
+                                           int32_t num_q_heads, int32_t num_kv_heads,
+                                           int32_t head_dim, int32_t pt_cols, int32_t page_size);
+
+int qattn_prefix_quant_fwd(const void *q, const int64_t q_stride[3],
+                           const void *k_cache, const void *v_cache, const int64_t cache_stride[4],
+                           const void *k_scale, const void *v_scale, const int64_t scale_stride[4],
+                           const int32_t *page_table, int32_t pt_cols, int32_t num_pages,
+                           int32_t page_size, const int32_t *context_lens,
+                           void *o, const int64_t o_stride[3],
+                           float *lse, const int64_t lse_stride[2],
+                           const int32_t *cu_seqlens, int32_t batch, int32_t max_seqlen,
+                           int64_t total_tokens, int32_t num_q_heads, int32_t num_kv_heads,
+                           int32_t head_dim, float scale, int32_t dtype, int32_t bits, void *workspace,
+                           int64_t workspace_size, void *stream);
 
 /*
  * Two-state softmax merge.

@@ -10,6 +10,13 @@ from .paged_kv import (  # noqa: F401
     copy_kv_pages,
     prefix_attention_paged,
 )
+from .quantized_kv import (  # noqa: F401
+    QuantizedKV,
+    append_quantized_kv,
+    prefix_attention_quantized,
+    quantized_kv_cache,
+    read_quantized_kv,
+)
 from .ragged_attn import (  # noqa: F401
     ancestor_table,
     build_paged_kv,

@@ -29,6 +29,7 @@ QATTN_ERR_LAYOUT = -4
 
 DTYPE_F16 = 0
 DTYPE_BF16 = 1
+DTYPE_U8 = 2
 ALGO_AUTO, ALGO_GATHER, ALGO_SUBTREE = 0, 1, 2
 
 # Every symbol declared in include/qattn.h, with its ctypes signature.
@@ -88,6 +89,16 @@ SIGNATURES = {
         _p, _i64p, _p, _i64p, _i32, _p, _i32, _i32, _i32, _p, _p, _i32, _p, _i32, _i32, _i32, _i32, _p]),
     "qattn_kv_copy_pages": (C.c_int, [
         _p, _i64p, _p, _i64p, _i32, _i32, _i32, _p, _p, _i32, _i32, _i32, _i32, _p]),
+    "qattn_quant_append": (C.c_int, [
+        _p, _i64p, _p, _i64p, _p, _p, _i64p, _p, _p, _i64p, _p, _i32, _i32, _i32, _p, _p, _p,
+        _i32, _i32, _i64, _i32, _i32, _i32, _i32, _p]),
+    "qattn_quant_read": (C.c_int, [
+        _p, _p, _i64p, _p, _p, _i64p, _p, _i32, _i32, _i32, _p, _p, _i64p, _p, _i64p, _p,
+        _i32, _i32, _i64, _i32, _i32, _i32, _i32, _p]),
+    "qattn_prefix_quant_workspace_bytes": (C.c_int64, [_i32, _i32, _i64, _i32, _i32, _i32, _i32, _i32]),
+    "qattn_prefix_quant_fwd": (C.c_int, [
+        _p, _i64p, _p, _p, _i64p, _p, _p, _i64p, _p, _i32, _i32, _i32, _p, _p, _i64p, _p, _i64p,
+        _p, _i32, _i32, _i64, _i32, _i32, _i32, _f32, _i32, _i32, _p, _i64, _p]),
     "qattn_lse_merge": (C.c_int, [
         _p, _i64p, _p, _i64p, _p, _i64p, _p, _i64p, _p, _i64p,
         _i32, _i32, _i32, _i32, _i32, _p]),

@@ -25,8 +25,8 @@ CSRC = os.path.join(PKG_DIR, "csrc")
 LIB_PATH = os.path.join(PKG_DIR, "libqattn.so")
 OBJ_DIR = os.path.join(PKG_DIR, "_build")
 SOURCES = ["tree_attn.hip", "subtree_stream.hip", "prefix_attn.hip", "paged_attn.hip", "prompt_attn.hip",
-           "kv_pages.hip"]
-HEADERS = ["qattn_common.h", "qattn_device.h", "kv_tiles.h", "dense_tiles.h", "tree_walk.h"]
+           "kv_pages.hip", "quant_pages.hip", "quant_attn.hip"]
+HEADERS = ["qattn_common.h", "qattn_device.h", "kv_tiles.h", "dense_tiles.h", "paged_work.h", "quant_format.h", "tree_walk.h"]
 CALLS_SOURCE = "calls.cpp"
 CALLS_PATH = os.path.join(PKG_DIR, "_calls.so")
 ARCH = os.environ.get("QATTN_ARCH", "gfx950")

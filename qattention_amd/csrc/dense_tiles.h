@@ -356,20 +356,29 @@ struct DenseTile {
         }
     }
 
+    // First head dim of chunk j of d-tile dt (8 dims).  QUARTERS: rows whose chunks
+    // lie in LDS a quarter row apart, chunk c at place c % DT * 4 + c / DT.
+    template <bool QUARTERS>
+    static constexpr int dim_of(int dt, int j) {
+        return QUARTERS ? 8 * (j * DT + dt) : 32 * dt + 8 * j;
+    }
+
     // Stores the numerator as the fp32 row at acc.
+    template <bool QUARTERS = false>
     static __device__ __forceinline__ void store_state(const f16v_t (&oacc)[DT], float* acc) {
         acc += 4 * ((threadIdx.x >> 5) & 1);
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-                *reinterpret_cast<float4*>(acc + 32 * dt + 8 * j) = make_float4(
+                *reinterpret_cast<float4*>(acc + dim_of<QUARTERS>(dt, j)) = make_float4(
                     oacc[dt][4 * j], oacc[dt][4 * j + 1], oacc[dt][4 * j + 2], oacc[dt][4 * j + 3]);
     }
 
     // Stores oacc * inv as the row at orow: a lane pair (l, l + 32) holds dims
     // 8 j + 0 .. 3 and 8 j + 4 .. 7 of its query; a half-wave exchange of
     // neighbouring groups gives each lane 16 contiguous bytes.
+    template <bool QUARTERS = false>
     static __device__ __forceinline__ void store_row(const f16v_t (&oacc)[DT], float inv, uint16_t* orow, bool valid) {
         const int hl = (threadIdx.x >> 5) & 1;
 #pragma unroll
@@ -389,7 +398,7 @@ struct DenseTile {
                 auto b = __builtin_amdgcn_permlane32_swap(w[0][1], w[1][1], false, false);
                 // lanes 0-31: group j (own half, other half), lanes 32-63: group j + 1
                 if (valid)
-                    st16(orow + 32 * dt + 8 * (j + hl),
+                    st16(orow + dim_of<QUARTERS>(dt, j) + dim_of<QUARTERS>(0, 1) * hl,
                          Vec16{{(uint32_t)a[0], (uint32_t)b[0], (uint32_t)a[1], (uint32_t)b[1]}});
             }
         }

@@ -2,12 +2,14 @@
 // tokens into the pages behind each context, the rows of an accepted draft
 // path together, whole pages to other pages.
 //
-// All three only move 16-byte chunks: what bounds a large call is HBM (each
+// All three only move chunks of 16 bytes: what bounds a large call is HBM (each
 // byte read and written once), a small one its launch and one chain of
 // dependent loads (sequence offsets, context length, page, row).  A row is
 // addressed as page * stride_page + slot * stride_slot + head * stride_head
 // in 64 bits, so caches of any size work; positions inside a sequence are 32
-// bits (the host checks pt_cols * page_size).
+// bits (the host checks pt_cols * page_size).  compact and copy also move caches
+// of bytes (the elements and scales of quantised rows), in chunks of 4 bytes or
+// one where their rows are no whole 16-byte chunks.
 #include <algorithm>
 
 #include "qattn_common.h"
@@ -18,17 +20,19 @@ namespace qattn {
 constexpr int kMoveThreads = 256;
 
 struct PageParams {
-    uint16_t* kc;
-    uint16_t* vc;
+    char* kc;
+    char* vc;
+    // in bytes
     int64_t sk_layer, sk_page, sk_slot, sk_head;
     int64_t sv_layer, sv_page, sv_slot, sv_head;
     const int32_t* table;  // [B, pt_cols]
     const int32_t* ctx;    // [B]
     int32_t* new_lens;     // [B]
     int32_t pt_cols, num_pages, page_size, capacity;  // capacity: pt_cols * page_size
-    int32_t B, chunks;                                // chunks: 16-byte chunks of one token's K row (all heads)
+    int32_t B, chunks;                                // chunks of one token's K row (all heads)
     Divider pdiv, cdiv;                               // page_size, chunks
     int32_t dvshift;                                  // chunks of one head's row: 1 << dvshift
+    int32_t unit;                                     // bytes of a chunk
 };
 
 // Loads and stores of append and copy, past the caches where they can be: for
@@ -48,7 +52,29 @@ __device__ __forceinline__ void st16_once(void* p, const Vec16& v) {
     __builtin_nontemporal_store(x, reinterpret_cast<u4_t*>(p));
 }
 
-// Element offset of position pos of sequence seq (head 0) in K and V, or
+// A chunk, through the caches (compact) or past them.
+template <typename U>
+__device__ __forceinline__ U ld_chunk(const char* p) {
+    if constexpr (sizeof(U) == 16) return ld16(p);
+    else return *reinterpret_cast<const U*>(p);
+}
+template <typename U>
+__device__ __forceinline__ void st_chunk(char* p, const U& x) {
+    if constexpr (sizeof(U) == 16) st16(p, x);
+    else *reinterpret_cast<U*>(p) = x;
+}
+template <typename U>
+__device__ __forceinline__ U ld_chunk_once(const char* p) {
+    if constexpr (sizeof(U) == 16) return ld16_once(p);
+    else return __builtin_nontemporal_load(reinterpret_cast<const U*>(p));
+}
+template <typename U>
+__device__ __forceinline__ void st_chunk_once(char* p, const U& x) {
+    if constexpr (sizeof(U) == 16) st16_once(p, x);
+    else __builtin_nontemporal_store(x, reinterpret_cast<U*>(p));
+}
+
+// Byte offset of position pos of sequence seq (head 0) in K and V, or
 // false where its page does not exist.
 __device__ __forceinline__ bool slot_of(const PageParams& p, int seq, int32_t pos, int64_t& ko, int64_t& vo) {
     const int32_t col = divide(pos, p.pdiv);
@@ -91,7 +117,6 @@ __device__ __forceinline__ int32_t new_rows(const AppendParams& p, int seq, int3
 }
 
 template <bool PACKED>
-
 __global__ __launch_bounds__(kMoveThreads) void kv_append_kernel(AppendParams p) {
     const PageParams& g = p.pg;
     __shared__ int32_t at_seq[PACKED ? kMaxRows : 1], at_pos[PACKED ? kMaxRows : 1];  // the rows' sequences, positions
@@ -139,18 +164,18 @@ __global__ __launch_bounds__(kMoveThreads) void kv_append_kernel(AppendParams p)
             if (ok[u]) {
                 const int32_t row = divide(e, g.cdiv);
                 const int32_t rest = e - row * g.chunks;
-                const int32_t h = rest >> g.dvshift, c = 8 * (rest & ((1 << g.dvshift) - 1));
+                const int32_t h = rest >> g.dvshift, c = rest & ((1 << g.dvshift) - 1);
                 const int64_t t = (int64_t)s0 + first + row;
-                kv[u] = ld16_once(p.k + t * p.sk_t + h * p.sk_h + c);
-                vv[u] = ld16_once(p.v + t * p.sv_t + h * p.sv_h + c);
+                kv[u] = ld16_once(p.k + t * p.sk_t + h * p.sk_h + 8 * c);
+                vv[u] = ld16_once(p.v + t * p.sv_t + h * p.sv_h + 8 * c);
                 if constexpr (PACKED) {
                     seq = at_seq[row];
                     ok[u] = seq >= 0 && slot_of(g, seq, at_pos[row], ko[u], vo[u]);
                 } else {
                     ok[u] = slot_of(g, seq, ctx + first + row, ko[u], vo[u]);
                 }
-                ko[u] += h * g.sk_head + c;
-                vo[u] += h * g.sv_head + c;
+                ko[u] += h * g.sk_head + 16 * c;
+                vo[u] += h * g.sv_head + 16 * c;
             }
         }
 #pragma unroll
@@ -165,7 +190,7 @@ __global__ __launch_bounds__(kMoveThreads) void kv_append_kernel(AppendParams p)
 
 // ---------------------------------------------------------------------------
 // compact: workgroup (layer, sequence, run of 2 * chunks K and V chunks); a
-// thread owns one 16-byte column of the sequence's rows and moves it down the
+// thread owns one chunk's column of the sequence's rows and moves it down the
 // path, kStep rows requested before the first is stored.  The path is
 // strictly increasing, so node j >= j: a row is read before any row at or
 // above it is written, and threads share no byte.
@@ -189,6 +214,7 @@ __device__ __forceinline__ int64_t from_lane(int64_t x, int i) {
     return (int64_t)((uint64_t)hi << 32 | lo);
 }
 
+template <typename U>
 __global__ __launch_bounds__(kMoveThreads) void kv_compact_kernel(CompactParams p) {
     const PageParams& g = p.pg;
     const int r0 = divide(blockIdx.x, p.ptdiv);
@@ -202,8 +228,8 @@ __global__ __launch_bounds__(kMoveThreads) void kv_compact_kernel(CompactParams 
     const bool is_v = e >= g.chunks;
     const bool live = e < 2 * g.chunks;
     const int32_t rest = is_v ? e - g.chunks : e;
-    const int32_t h = rest >> g.dvshift, c = 8 * (rest & ((1 << g.dvshift) - 1));
-    uint16_t* const base = is_v ? g.vc + layer * g.sv_layer + h * g.sv_head + c
+    const int32_t h = rest >> g.dvshift, c = (int)sizeof(U) * (rest & ((1 << g.dvshift) - 1));
+    char* const base = is_v ? g.vc + layer * g.sv_layer + h * g.sv_head + c
                                 : g.kc + layer * g.sk_layer + h * g.sk_head + c;
     constexpr int kStep = 8;
     int32_t count = 0, last = -1;
@@ -223,19 +249,19 @@ __global__ __launch_bounds__(kMoveThreads) void kv_compact_kernel(CompactParams 
         }
         const uint64_t moves = __ballot(have);
         for (int j = 0; j < n; j += kStep) {
-            Vec16 x[kStep];
+            U x[kStep];
 #pragma unroll
             for (int u = 0; u < kStep; ++u) {
                 if (j + u < n && moves >> (j + u) & 1) {
                     const int64_t k = from_lane(ks, j + u), v = from_lane(vs, j + u);
-                    if (live) x[u] = ld16(base + (is_v ? v : k));
+                    if (live) x[u] = ld_chunk<U>(base + (is_v ? v : k));
                 }
             }
 #pragma unroll
             for (int u = 0; u < kStep; ++u) {
                 if (j + u < n && moves >> (j + u) & 1) {
                     const int64_t k = from_lane(kd, j + u), v = from_lane(vd, j + u);
-                    if (live) st16(base + (is_v ? v : k), x[u]);
+                    if (live) st_chunk<U>(base + (is_v ? v : k), x[u]);
                 }
             }
         }
@@ -247,18 +273,19 @@ __global__ __launch_bounds__(kMoveThreads) void kv_compact_kernel(CompactParams 
 }
 
 // ---------------------------------------------------------------------------
-// copy: workgroup (layer, pair of pages, run of 16-byte chunks of the page)
+// copy: workgroup (layer, pair of pages, run of chunks of the page)
 // ---------------------------------------------------------------------------
 struct CopyParams {
     PageParams pg;
     const int32_t* src;
     const int32_t* dst;
-    int32_t n, page_chunks, parts;  // page_chunks: 16-byte chunks of one K page
+    int32_t n, page_chunks, parts;  // page_chunks: chunks of one K page
     Divider ptdiv, ndiv;            // parts, n
 };
 
 constexpr int kCopyU = 2;
 
+template <typename U>
 __global__ __launch_bounds__(kMoveThreads) void kv_copy_kernel(CopyParams p) {
     const PageParams& g = p.pg;
     const int r0 = divide(blockIdx.x, p.ptdiv);
@@ -267,11 +294,11 @@ __global__ __launch_bounds__(kMoveThreads) void kv_copy_kernel(CopyParams p) {
     const int i = r0 - layer * p.n;
     const int32_t a = p.src[i], b = p.dst[i];
     if ((uint32_t)a >= (uint32_t)g.num_pages || (uint32_t)b >= (uint32_t)g.num_pages || a == b) return;
-    const uint16_t* ks = g.kc + layer * g.sk_layer + a * g.sk_page;
-    const uint16_t* vs = g.vc + layer * g.sv_layer + a * g.sv_page;
-    uint16_t* kd = g.kc + layer * g.sk_layer + b * g.sk_page;
-    uint16_t* vd = g.vc + layer * g.sv_layer + b * g.sv_page;
-    Vec16 kv[kCopyU], vv[kCopyU];
+    const char* ks = g.kc + layer * g.sk_layer + a * g.sk_page;
+    const char* vs = g.vc + layer * g.sv_layer + a * g.sv_page;
+    char* kd = g.kc + layer * g.sk_layer + b * g.sk_page;
+    char* vd = g.vc + layer * g.sv_layer + b * g.sv_page;
+    U kv[kCopyU], vv[kCopyU];
     int64_t ko[kCopyU], vo[kCopyU];
 #pragma unroll
     for (int u = 0; u < kCopyU; ++u) {
@@ -279,18 +306,18 @@ __global__ __launch_bounds__(kMoveThreads) void kv_copy_kernel(CopyParams p) {
         if (e < p.page_chunks) {
             const int32_t slot = divide(e, g.cdiv);
             const int32_t rest = e - slot * g.chunks;
-            const int32_t h = rest >> g.dvshift, c = 8 * (rest & ((1 << g.dvshift) - 1));
+            const int32_t h = rest >> g.dvshift, c = (int)sizeof(U) * (rest & ((1 << g.dvshift) - 1));
             ko[u] = slot * g.sk_slot + h * g.sk_head + c;
             vo[u] = slot * g.sv_slot + h * g.sv_head + c;
-            kv[u] = ld16_once(ks + ko[u]);
-            vv[u] = ld16_once(vs + vo[u]);
+            kv[u] = ld_chunk_once<U>(ks + ko[u]);
+            vv[u] = ld_chunk_once<U>(vs + vo[u]);
         }
     }
 #pragma unroll
     for (int u = 0; u < kCopyU; ++u) {
         if ((part * kCopyU + u) * kMoveThreads + (int32_t)threadIdx.x < p.page_chunks) {
-            st16_once(kd + ko[u], kv[u]);
-            st16_once(vd + vo[u], vv[u]);
+            st_chunk_once<U>(kd + ko[u], kv[u]);
+            st_chunk_once<U>(vd + vo[u], vv[u]);
         }
     }
 }
@@ -301,13 +328,15 @@ __global__ __launch_bounds__(kMoveThreads) void kv_copy_kernel(CopyParams p) {
 // Checks and fills what the three calls share.  stride: {layer, page, slot,
 // head, dim}.
 static int fill_pages(PageParams& p, void* kc, const int64_t* ks, void* vc, const int64_t* vs, int32_t num_layers,
-                      int32_t num_pages, int32_t page_size, int32_t hkv, int32_t head_dim, int32_t dtype) {
-    if (dtype != QATTN_DTYPE_F16 && dtype != QATTN_DTYPE_BF16) {
-        set_error("dtype %d is not fp16 (0) or bf16 (1)", dtype);
+                      int32_t num_pages, int32_t page_size, int32_t hkv, int32_t head_dim, int32_t dtype,
+                      bool bytes = false) {
+    const bool u8 = bytes && dtype == QATTN_DTYPE_U8;
+    if (dtype != QATTN_DTYPE_F16 && dtype != QATTN_DTYPE_BF16 && !u8) {
+        set_error("dtype %d is not fp16 (0) or bf16 (1)%s", dtype, bytes ? " or bytes (2)" : "");
         return QATTN_ERR_DTYPE;
     }
-    if (head_dim != 32 && head_dim != 64 && head_dim != 128) {
-        set_error("head_dim %d not in {32, 64, 128}", head_dim);
+    if (u8 ? head_dim < 1 || head_dim > 1024 : head_dim != 32 && head_dim != 64 && head_dim != 128) {
+        set_error("head_dim %d not in %s", head_dim, u8 ? "[1, 1024]" : "{32, 64, 128}");
         return QATTN_ERR_HEAD_DIM;
     }
     if (num_layers < 0 || num_pages < 0 || page_size < 1 || hkv < 1 || hkv > (1 << 16)) {
@@ -319,29 +348,54 @@ static int fill_pages(PageParams& p, void* kc, const int64_t* ks, void* vc, cons
         set_error("null stride array");
         return QATTN_ERR_ARG;
     }
-    p = PageParams{};
-    p.chunks = hkv * (head_dim / 8);
-    if ((int64_t)page_size * p.chunks >= (int64_t(1) << 30)) {
-        set_error("a page of %d rows of %d heads is too large", page_size, hkv);
-        return QATTN_ERR_ARG;
-    }
     if ((num_layers > 0 && num_pages > 0) && (!kc || !vc)) {
         set_error("null cache pointer");
         return QATTN_ERR_ARG;
     }
-    if (!row_aligned(kc, ks, 4) || !row_aligned(vc, vs, 4)) {
-        set_error("k/v cache rows must be 16-byte aligned with stride_dim 1");
-        return QATTN_ERR_LAYOUT;
+    p = PageParams{};
+    const int64_t size = u8 ? 1 : 2;
+    int64_t row = head_dim * size;  // bytes that lie together
+    int32_t heads = hkv;
+    if (u8) {
+        if (ks[4] != 1 || vs[4] != 1) {
+            set_error("k/v cache rows of bytes must have stride_dim 1");
+            return QATTN_ERR_LAYOUT;
+        }
+        if (hkv == 1 || (ks[3] == row && vs[3] == row)) row *= hkv, heads = 1;
+        uint64_t all = (uint64_t)row | (uintptr_t)kc | (uintptr_t)vc;
+        for (int i = 0; i < (heads > 1 ? 4 : 3); ++i) all |= (uint64_t)ks[i] | (uint64_t)vs[i];
+        p.unit = all % 16 == 0 ? 16 : all % 4 == 0 ? 4 : 1;
+    } else {
+        if (!row_aligned(kc, ks, 4) || !row_aligned(vc, vs, 4)) {
+            set_error("k/v cache rows must be 16-byte aligned with stride_dim 1");
+            return QATTN_ERR_LAYOUT;
+        }
+        p.unit = 16;
     }
-    p.kc = (uint16_t*)kc;
-    p.vc = (uint16_t*)vc;
-    p.sk_layer = ks[0], p.sk_page = ks[1], p.sk_slot = ks[2], p.sk_head = ks[3];
-    p.sv_layer = vs[0], p.sv_page = vs[1], p.sv_slot = vs[2], p.sv_head = vs[3];
+    const int32_t per = (int32_t)(row / p.unit);
+    p.dvshift = 30;  // (one run of bytes per token: head 0)
+    if (heads > 1) {
+        p.dvshift = 0;
+        while ((1 << p.dvshift) < per) ++p.dvshift;
+        if ((1 << p.dvshift) != per) {
+            set_error("rows of %d bytes that do not lie together: not a power of two of %d-byte chunks", head_dim,
+                      p.unit);
+            return QATTN_ERR_LAYOUT;
+        }
+    }
+    p.chunks = heads * per;
+    if ((int64_t)page_size * p.chunks >= (int64_t(1) << 30)) {
+        set_error("a page of %d rows of %d heads is too large", page_size, hkv);
+        return QATTN_ERR_ARG;
+    }
+    p.kc = (char*)kc;
+    p.vc = (char*)vc;
+    p.sk_layer = size * ks[0], p.sk_page = size * ks[1], p.sk_slot = size * ks[2], p.sk_head = size * ks[3];
+    p.sv_layer = size * vs[0], p.sv_page = size * vs[1], p.sv_slot = size * vs[2], p.sv_head = size * vs[3];
     p.num_pages = num_pages;
     p.page_size = page_size;
     p.pdiv = make_divider(page_size);
     p.cdiv = make_divider(p.chunks);
-    p.dvshift = head_dim == 32 ? 2 : head_dim == 64 ? 3 : 4;
     return QATTN_OK;
 }
 
@@ -437,7 +491,7 @@ int qattn_kv_compact(void* k_cache, const int64_t kc_stride[5], void* v_cache, c
     clear_error();
     CompactParams p{};
     int rc = fill_pages(p.pg, k_cache, kc_stride, v_cache, vc_stride, num_layers, num_pages, page_size, num_kv_heads,
-                        head_dim, dtype);
+                        head_dim, dtype, true);
     if (rc) return rc;
     rc = fill_table(p.pg, page_table, pt_cols, context_lens, new_lens, batch);
     if (rc) return rc;
@@ -453,7 +507,10 @@ int qattn_kv_compact(void* k_cache, const int64_t kc_stride[5], void* v_cache, c
     p.bdiv = make_divider(batch);
     const int grid = grid_of((int64_t)num_layers * batch * p.parts);
     if (grid < 0) return QATTN_ERR_ARG;
-    hipLaunchKernelGGL(kv_compact_kernel, dim3(grid), dim3(kMoveThreads), 0, (hipStream_t)stream, p);
+    const auto kernel = p.pg.unit == 16  ? kv_compact_kernel<Vec16>
+                        : p.pg.unit == 4 ? kv_compact_kernel<uint32_t>
+                                         : kv_compact_kernel<uint8_t>;
+    hipLaunchKernelGGL(kernel, dim3(grid), dim3(kMoveThreads), 0, (hipStream_t)stream, p);
     return launch_status("kv_compact_kernel");
 }
 
@@ -464,7 +521,7 @@ int qattn_kv_copy_pages(void* k_cache, const int64_t kc_stride[5], void* v_cache
     clear_error();
     CopyParams p{};
     const int rc = fill_pages(p.pg, k_cache, kc_stride, v_cache, vc_stride, num_layers, num_pages, page_size,
-                              num_kv_heads, head_dim, dtype);
+                              num_kv_heads, head_dim, dtype, true);
     if (rc) return rc;
     if (n < 0 || (n > 0 && (!src_pages || !dst_pages))) {
         set_error("bad page list (n=%d)", n);
@@ -480,7 +537,10 @@ int qattn_kv_copy_pages(void* k_cache, const int64_t kc_stride[5], void* v_cache
     p.ndiv = make_divider(n);
     const int grid = grid_of((int64_t)num_layers * n * p.parts);
     if (grid < 0) return QATTN_ERR_ARG;
-    hipLaunchKernelGGL(kv_copy_kernel, dim3(grid), dim3(kMoveThreads), 0, (hipStream_t)stream, p);
+    const auto kernel = p.pg.unit == 16  ? kv_copy_kernel<Vec16>
+                        : p.pg.unit == 4 ? kv_copy_kernel<uint32_t>
+                                         : kv_copy_kernel<uint8_t>;
+    hipLaunchKernelGGL(kernel, dim3(grid), dim3(kMoveThreads), 0, (hipStream_t)stream, p);
     return launch_status("kv_copy_kernel");
 }
 

@@ -174,6 +174,11 @@ bool row_aligned(const void* ptr, const int64_t* st, int n_outer);
 int check_common(int32_t dtype, int32_t head_dim, int32_t batch, int32_t max_seqlen, int64_t total_tokens,
                  int32_t hq, int32_t hkv, int32_t max_depth);
 int launch_status(const char* what);
+// The cache of the calls over 4 or 8 bits (quant_pages.hip): strides in bytes
+// {page, slot, head, byte}, K and V alike.
+int check_quant(const void* kc, const void* vc, const int64_t* cs, const void* ks, const void* vs, const int64_t* ss,
+                int32_t pt_cols, int32_t num_pages, int32_t page_size, int32_t hkv, int32_t head_dim, int32_t dtype,
+                int32_t bits);
 int fill_tree_params(TreeParams& p, const void* q, const int64_t* qs, const void* k, const int64_t* ks,
                      const void* v, const int64_t* vs, void* o, const int64_t* os, float* lse, const int64_t* lss,
                      const int32_t* cu, int32_t batch, int32_t max_seqlen, int64_t total_tokens, int32_t hq,

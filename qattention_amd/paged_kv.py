@@ -54,6 +54,8 @@ def _int32(t: torch.Tensor, device) -> torch.Tensor:
 def _check_caches(K_cache, V_cache, dims: Tuple[int, ...]) -> tuple:
     """Caches that a call writes in place: no copy can stand in for them.
     Returns their addresses and 5 strides {layer, page, slot, head, dim} each."""
+    if K_cache.dtype is torch.uint8:
+        return _check_bytes(K_cache, V_cache, dims)
     if K_cache.dim() not in dims or K_cache.shape != V_cache.shape:
         raise ValueError(f"caches must be {' or '.join(f'{d}-D' for d in dims)} and of one shape (got "
                          f"{tuple(K_cache.shape)}, {tuple(V_cache.shape)})")
@@ -71,6 +73,28 @@ def _check_caches(K_cache, V_cache, dims: Tuple[int, ...]) -> tuple:
         if k == v:
             raise ValueError("K_cache and V_cache are the same memory")
     return k, ks, v, vs
+
+
+def _check_bytes(K_cache, V_cache, dims: Tuple[int, ...]) -> tuple:
+    """_check_caches for caches of bytes (a quantised cache's elements, or its scales)."""
+    if K_cache.dim() not in dims or K_cache.shape != V_cache.shape or V_cache.dtype is not torch.uint8:
+        raise ValueError(f"caches must be {' or '.join(f'{d}-D' for d in dims)}, of one shape and type (got "
+                         f"{tuple(K_cache.shape)}, {V_cache.dtype} {tuple(V_cache.shape)})")
+    width = K_cache.shape[-1]
+    for c in (K_cache, V_cache):
+        if c.stride(-1) != 1 and width > 1:
+            raise ValueError(f"cache rows of strides {tuple(c.stride())} are no runs of bytes")
+        if any(st == 0 and n > 1 for st, n in zip(c.stride(), c.shape)):
+            raise ValueError("cache rows overlap (a stride of 0)")
+    k, v = K_cache.data_ptr(), V_cache.data_ptr()
+    if k == v and K_cache.numel():
+        raise ValueError("K_cache and V_cache are the same memory")
+    ks, vs = (_lib.cache_layout(c.stride()[:-1] + (1,))[0] for c in (K_cache, V_cache))
+    return k, ks, v, vs
+
+
+def _cache_code(cache) -> int:
+    return _lib.DTYPE_U8 if cache.dtype is torch.uint8 else _dtype_code(cache)
 
 
 def _table(page_table, B: int, device) -> torch.Tensor:
@@ -217,7 +241,8 @@ def compact_paged_kv(
     accepted[s, j]) moves to position context_lens[s] + j, in every layer.
 
     K_cache, V_cache: [layers, pages, page_size, Hkv, D] or one layer's [pages,
-    page_size, Hkv, D]; accepted: int32 [B, P], strictly increasing along a path
+    page_size, Hkv, D], fp16, bf16 or the bytes of a quantised cache (its elements,
+    or its scales); accepted: int32 [B, P], strictly increasing along a path
     (breadth-first order has ancestors before descendants), -1 behind its end; a
     path ends before the first entry that is not above its predecessor or that
     the table has no column for.  Returns the lengths afterwards, context plus
@@ -240,7 +265,7 @@ def compact_paged_kv(
     layers = K_cache.shape[0] if K_cache.dim() == 5 else 1
     _launch(idx, "qattn_kv_compact", _lib.lib().qattn_kv_compact,
             kc, kcs, vc, vcs, layers, pt.data_ptr(), pt.shape[1], num_pages, page_size, ctx.data_ptr(),
-            path.data_ptr(), path.shape[1], new.data_ptr(), B, Hkv, D, _dtype_code(K_cache))
+            path.data_ptr(), path.shape[1], new.data_ptr(), B, Hkv, D, _cache_code(K_cache))
     return new
 
 
@@ -281,7 +306,7 @@ def copy_kv_pages(K_cache: torch.Tensor, V_cache: torch.Tensor, src_pages: _Page
     forked sequence, pages gathered to free others).
 
     K_cache, V_cache: [layers, pages, page_size, Hkv, D] or one layer's [pages,
-    page_size, Hkv, D].  The copies run side by side, so no page may be the
+    page_size, Hkv, D], fp16, bf16 or the bytes of a quantised cache.  The copies run side by side, so no page may be the
     destination of two or the destination of one and the source of another:
     lists on the host are checked for that (ValueError); of lists on the GPU,
     pairs with a page outside the cache are passed over, the rest is the
@@ -299,4 +324,4 @@ def copy_kv_pages(K_cache: torch.Tensor, V_cache: torch.Tensor, src_pages: _Page
     layers = K_cache.shape[0] if K_cache.dim() == 5 else 1
     _launch(idx, "qattn_kv_copy_pages", _lib.lib().qattn_kv_copy_pages,
             kc, kcs, vc, vcs, layers, num_pages, page_size, src.data_ptr(), dst.data_ptr(), src.shape[0], Hkv, D,
-            _dtype_code(K_cache))
+            _cache_code(K_cache))
