@@ -537,7 +537,8 @@ int qattn_quant_read(const void *k_cache, const void *v_cache, const int64_t cac
  */
 int64_t qattn_prefix_quant_workspace_bytes(int32_t batch, int32_t max_seqlen, int64_t total_tokens,
                                            int32_t num_q_heads, int32_t num_kv_heads,
-                                           int32_t head_dim, int32_t pt_cols, int32_t page_size);
+                                           int32_t head_dim, int32_t pt_cols, int32_t page_size,
+                                           int32_t bits);
 
 int qattn_prefix_quant_fwd(const void *q, const int64_t q_stride[3],
                            const void *k_cache, const void *v_cache, const int64_t cache_stride[4],

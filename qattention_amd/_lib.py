@@ -95,7 +95,7 @@ SIGNATURES = {
     "qattn_quant_read": (C.c_int, [
         _p, _p, _i64p, _p, _p, _i64p, _p, _i32, _i32, _i32, _p, _p, _i64p, _p, _i64p, _p,
         _i32, _i32, _i64, _i32, _i32, _i32, _i32, _p]),
-    "qattn_prefix_quant_workspace_bytes": (C.c_int64, [_i32, _i32, _i64, _i32, _i32, _i32, _i32, _i32]),
+    "qattn_prefix_quant_workspace_bytes": (C.c_int64, [_i32, _i32, _i64, _i32, _i32, _i32, _i32, _i32, _i32]),
     "qattn_prefix_quant_fwd": (C.c_int, [
         _p, _i64p, _p, _p, _i64p, _p, _p, _i64p, _p, _i32, _i32, _i32, _p, _p, _i64p, _p, _i64p,
         _p, _i32, _i32, _i64, _i32, _i32, _i32, _f32, _i32, _i32, _p, _i64, _p]),
@@ -110,6 +110,9 @@ _calls = None
 # What _calls.bind takes, in its order.
 _BOUND = ("qattn_prompt_workspace_bytes", "qattn_prompt_fwd", "qattn_prefix_paged_workspace_bytes",
           "qattn_prefix_paged_fwd", "qattn_kv_append", "qattn_kv_compact", "qattn_kv_copy_pages")
+# What _calls.bind_quantized takes.
+_BOUND_QUANTIZED = ("qattn_prefix_quant_workspace_bytes", "qattn_prefix_quant_fwd", "qattn_quant_append",
+                    "qattn_quant_read")
 
 
 class QAttnError(RuntimeError):
@@ -153,10 +156,12 @@ def calls():
             warnings.warn(f"serving calls go through Python (4 to 8 us more each): {e}; build the call module with "
                           "`python -m qattention_amd.build`", RuntimeWarning)
             _calls = types.SimpleNamespace(**dict.fromkeys(
-                ("prompt", "paged", "append", "compact", "copy", "set_ready"), _not_here))
+                ("prompt", "paged", "append", "compact", "copy", "quant_append", "quant_read", "quant_paged",
+                 "set_ready"), _not_here))
             return _calls
         module.bind(*(C.cast(getattr(L, name), _p).value for name in _BOUND),
                     torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream)
+        module.bind_quantized(*(C.cast(getattr(L, name), _p).value for name in _BOUND_QUANTIZED))
         for idx in _initialised:
             module.set_ready(idx)
         _calls = module

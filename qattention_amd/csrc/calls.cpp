@@ -14,8 +14,10 @@
 #include <Python.h>
 
 #include <ATen/Functions.h>
+#include <torch/csrc/Dtype.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <algorithm>
 #include <cmath>
 
 namespace {
@@ -41,6 +43,20 @@ using Compact = int (*)(void*, const int64_t*, void*, const int64_t*, int32_t, c
 using Copy = int (*)(void*, const int64_t*, void*, const int64_t*, int32_t, int32_t, int32_t, const int32_t*,
                      const int32_t*, int32_t, int32_t, int32_t, int32_t, void*);
 
+using QuantWs = int64_t (*)(int32_t, int32_t, int64_t, int32_t, int32_t, int32_t, int32_t, int32_t, int32_t);
+using Quant = int (*)(const void*, const int64_t*, const void*, const void*, const int64_t*, const void*, const void*,
+                      const int64_t*, const int32_t*, int32_t, int32_t, int32_t, const int32_t*, void*, const int64_t*,
+                      float*, const int64_t*, const int32_t*, int32_t, int32_t, int64_t, int32_t, int32_t, int32_t,
+                      float, int32_t, int32_t, void*, int64_t, void*);
+using QuantAppend = int (*)(const void*, const int64_t*, const void*, const int64_t*, void*, void*, const int64_t*,
+                            void*, void*, const int64_t*, const int32_t*, int32_t, int32_t, int32_t, const int32_t*,
+                            int32_t*, const int32_t*, int32_t, int32_t, int64_t, int32_t, int32_t, int32_t, int32_t,
+                            void*);
+using QuantRead = int (*)(const void*, const void*, const int64_t*, const void*, const void*, const int64_t*,
+                          const int32_t*, int32_t, int32_t, int32_t, const int32_t*, void*, const int64_t*, void*,
+                          const int64_t*, const int32_t*, int32_t, int32_t, int64_t, int32_t, int32_t, int32_t, int32_t,
+                          void*);
+
 PromptWs prompt_ws;
 Prompt prompt_fwd;
 PagedWs paged_ws;
@@ -48,6 +64,10 @@ Paged paged_fwd;
 Append kv_append;
 Compact kv_compact;
 Copy kv_copy;
+QuantWs quant_ws;
+Quant quant_fwd;
+QuantAppend quant_append_rows;
+QuantRead quant_read_rows;
 PyObject *current_device, *current_stream;  // torch._C functions
 uint64_t ready;                             // bit d: qattn_init ran on device d
 
@@ -124,6 +144,44 @@ int64_t* strides5(const Tensor& t, int64_t (&st)[5]) {
     for (int i = 0; i < 4; ++i) st[i + 1] = s[i + all];
     return st;
 }
+
+// A quantised cache (a tuple of K, V, K_scale, V_scale) that the library reads as it is.
+struct Quantized {
+    const Tensor *K, *V, *Ks, *Vs;
+    int32_t pages, page_size, heads, dim, bits;
+    int64_t cs[4], ss[4];
+
+    bool take(Call& c, PyObject* o, bool written) {
+        if (!PyTuple_Check(o) || PyTuple_GET_SIZE(o) != 4) return false;
+        const Tensor** at[4] = {&K, &V, &Ks, &Vs};
+        for (int i = 0; i < 4; ++i) {
+            if (!c.plain(PyTuple_GET_ITEM(o, i), *at[i])) return false;
+            const Tensor& t = **at[i];
+            if (t.scalar_type() != at::kByte || t.dim() != 4 || !t.numel()) return false;
+        }
+        for (int i = 0; i < 3; ++i)
+            if (K->size(i) != Ks->size(i) || K->size(i) > kInt) return false;
+        const int64_t D = 32 * Ks->size(3), width = K->size(3);
+        if ((D != 32 && D != 64 && D != 128) || (8 * width != 4 * D && 8 * width != 8 * D)) return false;
+        if (!pair(*K, *V, 16, written, cs) || !pair(*Ks, *Vs, D / 32, written, ss)) return false;
+        pages = (int32_t)K->size(0), page_size = (int32_t)K->size(1), heads = (int32_t)K->size(2), dim = (int32_t)D;
+        bits = (int32_t)(8 * width / D);
+        return true;
+    }
+
+private:
+    // Two tensors laid out alike in rows on `unit`-byte boundaries, if written each in
+    // memory of its own.
+    static bool pair(const Tensor& a, const Tensor& b, int64_t unit, bool written, int64_t (&st)[4]) {
+        const auto s = a.strides();
+        if (a.sizes() != b.sizes() || s != b.strides() || (s[3] != 1 && a.size(3) > 1)) return false;
+        const uintptr_t x = (uintptr_t)a.data_ptr(), y = (uintptr_t)b.data_ptr();
+        if ((s[0] | s[1] | s[2]) & (unit - 1) || (x | y) & (uintptr_t)(unit - 1)) return false;
+        if (written && (x == y || !s[0] || !s[1] || !s[2])) return false;
+        st[0] = s[0], st[1] = s[1], st[2] = s[2], st[3] = 1;
+        return true;
+    }
+};
 
 // An int argument in [0, 2^31); false for anything else.
 bool small_int(PyObject* o, int32_t& v) {
@@ -346,21 +404,123 @@ PyObject* copy(PyObject*, PyObject* const* a, Py_ssize_t n) {
     });
 }
 
+// quant_append(K, V, cache, page_table, context_lens, cu_seqlens, max_seqlen)
+PyObject* quant_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        Call c;
+        Quantized q;
+        const Tensor *K, *V, *table, *ctx;
+        if (n != 7 || !quant_fwd || !c.rows(a[0], 3, K) || !c.rows(a[1], 3, V) || !q.take(c, a[2], true) ||
+            !c.ints(a[3], 2, table) || !c.ints(a[4], 1, ctx))
+            return none();
+        const int64_t T = K->size(0), B = ctx->size(0);
+        const int32_t* cu;
+        int32_t ms;
+        if (K->sizes() != V->sizes() || K->size(1) != q.heads || K->size(2) != q.dim || table->size(0) < B ||
+            T > kInt || B > kInt || table->size(1) > kInt || !offsets(c, a[5], a[6], T, B, cu, ms) || !c.here())
+            return none();
+        Tensor after;
+        const int rc = [&] {
+            Unlocked others;
+            after = at::empty_like(*ctx);
+            return quant_append_rows(K->data_ptr(), K->strides().data(), V->data_ptr(), V->strides().data(),
+                                     q.K->data_ptr(), q.V->data_ptr(), q.cs, q.Ks->data_ptr(), q.Vs->data_ptr(), q.ss,
+                                     table->data_ptr<int32_t>(), (int32_t)table->size(1), q.pages, q.page_size,
+                                     ctx->data_ptr<int32_t>(), after.data_ptr<int32_t>(), cu, (int32_t)B, ms, T,
+                                     q.heads, q.dim, c.code(), q.bits, c.stream);
+        }();
+        return rc ? none() : THPVariable_Wrap(after);
+    });
+}
+
+// quant_read(cache, page_table, starts, cu_seqlens, max_seqlen, total_tokens, dtype)
+PyObject* quant_read(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        Call c;
+        Quantized q;
+        const Tensor *table, *start;
+        if (n != 7 || !quant_fwd || !q.take(c, a[0], false) || !c.ints(a[1], 2, table) || !c.ints(a[2], 1, start) ||
+            !THPDtype_Check(a[6]))
+            return none();
+        c.type = reinterpret_cast<THPDtype*>(a[6])->scalar_type;
+        const int64_t B = start->size(0);
+        const int32_t* cu;
+        int32_t ms, T = (int32_t)std::min(B, kInt);
+        if ((c.type != at::kHalf && c.type != at::kBFloat16) || table->size(0) < B || B > kInt ||
+            table->size(1) > kInt || !offsets(c, a[3], a[4], B, B, cu, ms) ||
+            !(cu ? small_int(a[5], T) : a[5] == Py_None || (small_int(a[5], T) && T == B)) || !c.here())
+            return none();
+        Tensor K, V;
+        const int rc = [&] {
+            Unlocked others;
+            K = at::empty({T, q.heads, q.dim}, c.options(c.type));
+            V = at::empty({T, q.heads, q.dim}, c.options(c.type));
+            return quant_read_rows(q.K->data_ptr(), q.V->data_ptr(), q.cs, q.Ks->data_ptr(), q.Vs->data_ptr(), q.ss,
+                                   table->data_ptr<int32_t>(), (int32_t)table->size(1), q.pages, q.page_size,
+                                   start->data_ptr<int32_t>(), K.data_ptr(), K.strides().data(), V.data_ptr(),
+                                   V.strides().data(), cu, (int32_t)B, ms, T, q.heads, q.dim, c.code(), q.bits,
+                                   c.stream);
+        }();
+        return rc ? none() : wrap(K, V, true);
+    });
+}
+
+// quant_paged(Q, cache, page_table, context_lens, cu_seqlens, max_seqlen, return_lse)
+PyObject* quant_paged(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        Call c;
+        Quantized q;
+        const Tensor *Q, *table, *ctx;
+        if (n != 7 || !quant_fwd || !c.rows(a[0], 3, Q) || !q.take(c, a[1], false) || !c.ints(a[2], 2, table) ||
+            !c.ints(a[3], 1, ctx) || !PyBool_Check(a[6]))
+            return none();
+        const int64_t T = Q->size(0), Hq = Q->size(1), B = ctx->size(0);
+        const int32_t* cu;
+        int32_t ms;
+        if (Q->size(2) != q.dim || Hq % q.heads || table->size(0) < B || T > kInt || Hq > kInt || B > kInt ||
+            table->size(1) > kInt || !offsets(c, a[4], a[5], T, B, cu, ms) || !c.here())
+            return none();
+        const bool want = a[6] == Py_True;
+        const int32_t cols = (int32_t)table->size(1);
+        Tensor O, LSE;
+        const int rc = [&] {
+            Unlocked others;
+            const int64_t bytes = quant_ws((int32_t)B, ms, T, (int32_t)Hq, q.heads, q.dim, cols, q.page_size, q.bits);
+            if (!outputs(c, *Q, want, O, LSE)) return -1;
+            Tensor ws;
+            if (bytes) ws = at::empty({bytes}, c.options(at::kByte));
+            return quant_fwd(Q->data_ptr(), Q->strides().data(), q.K->data_ptr(), q.V->data_ptr(), q.cs,
+                             q.Ks->data_ptr(), q.Vs->data_ptr(), q.ss, table->data_ptr<int32_t>(), cols, q.pages,
+                             q.page_size, ctx->data_ptr<int32_t>(), O.data_ptr(), O.strides().data(),
+                             want ? LSE.data_ptr<float>() : nullptr, want ? LSE.strides().data() : nullptr, cu,
+                             (int32_t)B, ms, T, (int32_t)Hq, q.heads, q.dim, (float)(1.0 / std::sqrt((double)q.dim)),
+                             c.code(), q.bits, bytes ? ws.data_ptr() : nullptr, bytes, c.stream);
+        }();
+        return rc ? none() : wrap(O, LSE, want);
+    });
+}
+
+// n addresses of entry points; false with an error set where one is none.
+bool addresses(PyObject* const* a, int n, void** at) {
+    for (int i = 0; i < n; ++i) {
+        at[i] = PyLong_AsVoidPtr(a[i]);
+        if (!at[i]) {
+            if (!PyErr_Occurred()) PyErr_SetString(PyExc_ValueError, "null entry point");
+            return false;
+        }
+    }
+    return true;
+}
+
 // bind(addresses of the seven entry points, torch's current-device and
 // current-raw-stream functions)
 PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    void* at[7];
     if (n != 9) {
         PyErr_SetString(PyExc_TypeError, "bind takes seven addresses and two functions");
         return nullptr;
     }
-    void* at[7];
-    for (int i = 0; i < 7; ++i) {
-        at[i] = PyLong_AsVoidPtr(a[i]);
-        if (!at[i]) {
-            if (!PyErr_Occurred()) PyErr_SetString(PyExc_ValueError, "null entry point");
-            return nullptr;
-        }
-    }
+    if (!addresses(a, 7, at)) return nullptr;
     prompt_ws = (PromptWs)at[0], prompt_fwd = (Prompt)at[1], paged_ws = (PagedWs)at[2], paged_fwd = (Paged)at[3];
     kv_append = (Append)at[4], kv_compact = (Compact)at[5], kv_copy = (Copy)at[6];
     Py_INCREF(a[7]);
@@ -368,6 +528,19 @@ PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
     Py_XDECREF(current_device);
     Py_XDECREF(current_stream);
     current_device = a[7], current_stream = a[8];
+    return none();
+}
+
+// bind_quantized(addresses of the four entry points over a quantised cache)
+PyObject* bind_quantized(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    void* at[4];
+    if (n != 4) {
+        PyErr_SetString(PyExc_TypeError, "bind_quantized takes four addresses");
+        return nullptr;
+    }
+    if (!addresses(a, 4, at)) return nullptr;
+    quant_ws = (QuantWs)at[0], quant_fwd = (Quant)at[1], quant_append_rows = (QuantAppend)at[2];
+    quant_read_rows = (QuantRead)at[3];
     return none();
 }
 
@@ -380,9 +553,9 @@ PyObject* set_ready(PyObject*, PyObject* d) {
 }
 
 #define FAST(name) {#name, (PyCFunction)(void (*)(void))name, METH_FASTCALL, nullptr}
-PyMethodDef methods[] = {FAST(prompt), FAST(paged),  FAST(append), FAST(compact),
-                         FAST(copy),   FAST(bind),   {"set_ready", set_ready, METH_O, nullptr},
-                         {nullptr, nullptr, 0, nullptr}};
+PyMethodDef methods[] = {FAST(prompt),       FAST(paged),      FAST(append),      FAST(compact), FAST(copy),
+                         FAST(quant_append), FAST(quant_read), FAST(quant_paged), FAST(bind), FAST(bind_quantized),
+                         {"set_ready", set_ready, METH_O, nullptr}, {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_calls", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

@@ -261,7 +261,9 @@ __global__ __launch_bounds__(64 * NW)
             __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
         }
 
-        join_waves<T, D, QB, NW, HW>(p, sh, part, query_of, m_run, l_run, oacc, vlds, ml, [](int ch) { return ch; });
+        join_waves<T, D, QB, NW, HW>(
+            p, sh, part, query_of, m_run, l_run, oacc, vlds, ml, [](int ch) { return ch; }, HW,
+            [&](int r) { return wave / WPH * ROWS + r; });
         __syncthreads();  // the LDS is free for the next item
         sh.u += STREAM ? b1 - b0 : 1;
     }

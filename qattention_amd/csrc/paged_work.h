@@ -99,8 +99,8 @@ struct Runs {
 };
 
 // This workgroup's run [u, end): the sequence that holds u and its first unit.
-// Workgroup 0 leaves the sequences' first units to the merge.  Every thread
-// calls it; false: no unit.
+// Workgroup 0 leaves the sequences' first units to the merge.  Every one of the
+// workgroup's NT threads calls it; false: no unit.
 struct Share {
     int32_t u, end, start, seq, seq_base, total;
     SeqWork sw;  // of seq
@@ -109,8 +109,9 @@ __device__ __forceinline__ bool no_share(const PagedParams& p, int wg) {
     if (p.cuts && threadIdx.x == 0) p.cuts[wg] = RunStart{};
     return false;
 }
+template <int NT = kPagedThreads>
 __device__ __forceinline__ bool find_share(const PagedParams& p, Share& sh) {
-    __shared__ int32_t sums[4];
+    __shared__ int32_t sums[NT / 64];
     __shared__ int32_t found[2];
     __shared__ SeqWork found_work;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -163,7 +164,7 @@ __device__ __forceinline__ bool find_share(const PagedParams& p, Share& sh) {
         int32_t before = 0;
         sum = 0;
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
+        for (int w = 0; w < NT / 64; ++w) {
             before += w < wave ? sums[w] : 0;
             sum += sums[w];
         }
@@ -171,7 +172,7 @@ __device__ __forceinline__ bool find_share(const PagedParams& p, Share& sh) {
     };
     int32_t total = 0, mine = 0, excl = 0;
     SeqWork work{};
-    for (int c = 0; c < p.B; c += kPagedThreads) {
+    for (int c = 0; c < p.B; c += NT) {
         int32_t sum;
         if (c + tid < p.B) work = seq_work(p, c + tid);
         mine = c + tid < p.B ? work.units(p.groups) : 0;
@@ -186,11 +187,11 @@ __device__ __forceinline__ bool find_share(const PagedParams& p, Share& sh) {
     sh.u = sh.start = runs.first(wg);
     sh.end = runs.first(wg + 1);
     sh.total = total;
-    if (p.B <= kPagedThreads) {
+    if (p.B <= NT) {
         if (sh.u >= excl && sh.u < excl + mine) found[0] = tid, found[1] = excl, found_work = work;
     } else {
         int32_t before = 0;
-        for (int c = 0; c < p.B; c += kPagedThreads) {
+        for (int c = 0; c < p.B; c += NT) {
             int32_t sum;
             if (c + tid < p.B) work = seq_work(p, c + tid);
             mine = c + tid < p.B ? work.units(p.groups) : 0;
@@ -248,14 +249,16 @@ __device__ __forceinline__ SeqWork next_part(const PagedParams& p, Share& sh, Pa
 // The states of a workgroup's NW waves (NW / HW for each of HW kv heads, 16 QB
 // rows each) joined row block by row block: the part's output, or its state in
 // the workspace.  oacc element i of tile dt is row l16, column 16 dt + 4 lq + i;
-// column chunk ch (8 columns) holds head dims 8 dims_of(ch) .. + 7.  lds: NW x 32 x D
-// elements of 16 bits that no wave uses any more after the first barrier.
+// column chunk ch (8 columns) holds head dims 8 dims_of(ch) .. + 7; row r's state lies
+// at row state_of(r) of its part's in the workspace.  lds: NW x 32 x D elements of 16
+// bits that no wave uses any more after the first barrier.
 // ---------------------------------------------------------------------------
-template <typename T, int D, int QB, int NW, int HW, class Query, class Dims>
+template <typename T, int D, int QB, int NW, int HW, class Query, class Dims, class State>
 __device__ __forceinline__ void join_waves(const PagedParams& p, const Share& sh, const Part& part, Query query_of,
                                            const float (&m_run)[QB], float (&l_run)[QB], const f4_t (&oacc)[QB][D / 16],
-                                           uint16_t* lds, float (&ml)[2][NW][16 * QB], Dims dims_of) {
-    constexpr int ND = D / 16, DV = D / 8, WBLK = 32 * D, ROWS = 16 * QB, WPH = NW / HW;
+                                           uint16_t* lds, float (&ml)[2][NW][16 * QB], Dims dims_of, int heads,
+                                           State state_of) {
+    constexpr int DV = D / 8, ND = D / 16, WBLK = 32 * D, ROWS = 16 * QB, WPH = NW / HW;
     const int tid = threadIdx.x;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int lane = tid & 63;
@@ -285,7 +288,7 @@ __device__ __forceinline__ void join_waves(const PagedParams& p, const Share& sh
         for (int row = ht / DV; row < 16; row += PASS) {
             int64_t qrow;
             int qh;
-            if (!query_of(16 * q + row, qrow, qh)) break;
+            if (!query_of(16 * q + row, qrow, qh)) continue;
             float m = -INFINITY, l = 0.f, acc[8] = {};
 #pragma unroll
             for (int w = 0; w < WPH; ++w) m = fmaxf(m, ml[0][hw + w][16 * q + row]);
@@ -306,7 +309,7 @@ __device__ __forceinline__ void join_waves(const PagedParams& p, const Share& sh
                 st16(p.o + qrow * p.so_t + qh * p.so_h + dim, pack8<T>(acc));
                 if (p.lse && ch == 0) p.lse[qrow * p.sl_t + qh * p.sl_h] = (mc + fast_log2(l)) * kLn2;
             } else {
-                const int64_t r = (part_slot(sh) * HW + wave / WPH) * ROWS + 16 * q + row;
+                const int64_t r = part_slot(sh) * heads * ROWS + state_of(16 * q + row);
                 if (ch == 0) {
                     p.part_m[r] = m * p.scale_log2;
                     p.part_l[r] = l;
@@ -460,11 +463,12 @@ __global__ __launch_bounds__(kPagedThreads) void paged_merge_kernel(PagedParams 
 // Host side
 // ---------------------------------------------------------------------------
 // Kernel of a call: row blocks of a tile (0: the wide kernel), log2 of its rows
-// and of a unit's keys, kv heads of a workgroup, workgroups per CU, and whether
-// every item is one workgroup's.
+// and of a unit's keys, kv heads of a workgroup, workgroups per CU, whether every
+// item is one workgroup's.
 struct PagedShape {
     int qb, row_shift, key_shift, heads, per_cu;
     bool items;
+    int wave_heads;  // quantised caches: kv heads of a wave
 };
 
 struct PagedSpace {
@@ -626,7 +630,7 @@ static int paged_setup(PagedParams& p, PagedPlan& plan, ShapeOf shape_of, const 
     p.key_shift = plan.shape.key_shift;
     p.groupdiv = make_divider(p.groups);
     p.tilediv = make_divider(plan.tiles);
-    p.head_shift = p.heads == 4 ? 2 : p.heads == 2 ? 1 : 0;
+    p.head_shift = __builtin_ctz((unsigned)p.heads);
     p.pdiv = make_divider(page_size);
     p.gdiv = make_divider(p.group);
     p.scale_log2 = scale * kLog2e;

@@ -20,28 +20,39 @@ namespace qattn {
 
 struct QuantParams : PagedParams {
     const uint8_t *ks, *vs;              // scales; K and V share all strides
-    int64_t ss_page, ss_slot, ss_head;   // bytes
+    int64_t ss_head;                     // bytes
+    // of a page and a slot, in 16-byte units of the elements and in rows of the scales
+    // (a row's offset, kv head aside, is 32 bits wide)
+    uint32_t row_page, row_slot, scale_page, scale_slot;
 };
 
-// N words at p (aligned to their size, up to 16 bytes).
-template <int N>
+typedef uint32_t w2_t __attribute__((ext_vector_type(2)));
+typedef uint32_t w4_t __attribute__((ext_vector_type(4)));
+
+// N words at p (aligned to their size, up to 16 bytes).  ONCE: past the caches.
+template <bool ONCE = false, int N>
 __device__ __forceinline__ void ld_words(uint32_t (&w)[N], const char* p) {
+    auto ld = [](auto* at) { return ONCE ? __builtin_nontemporal_load(at) : *at; };
     if constexpr (N == 1) {
-        w[0] = *reinterpret_cast<const uint32_t*>(p);
+        w[0] = ld(reinterpret_cast<const uint32_t*>(p));
     } else if constexpr (N == 2) {
-        const uint2 x = *reinterpret_cast<const uint2*>(p);
-        w[0] = x.x, w[1] = x.y;
+        const w2_t x = ld(reinterpret_cast<const w2_t*>(p));
+        w[0] = x[0], w[1] = x[1];
     } else {
 #pragma unroll
         for (int i = 0; i < N; i += 4) {
-            const Vec16 x = ld16(p + 4 * i);
+            const w4_t x = ld(reinterpret_cast<const w4_t*>(p + 4 * i));
 #pragma unroll
-            for (int j = 0; j < 4; ++j) w[i + j] = x.w[j];
+            for (int j = 0; j < 4; ++j) w[i + j] = x[j];
         }
     }
 }
 
-// One head's N scales at p, one byte each.
+__device__ __forceinline__ uint32_t lds_at(const void* p) {
+    return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void*)p;
+}
+
+// N scales at p, one byte each (aligned to N), the first in the low byte.
 template <int N>
 __device__ __forceinline__ uint32_t ld_scales(const char* p) {
     if constexpr (N == 4) return *reinterpret_cast<const uint32_t*>(p);
@@ -49,52 +60,98 @@ __device__ __forceinline__ uint32_t ld_scales(const char* p) {
     else return *reinterpret_cast<const uint8_t*>(p);
 }
 
+// Word i of head h's operand from the loads x of a key tile: lanes g COLS .. of every
+// 16 from load (g - h) % NH, whose lanes h COLS .. hold the head's words, turned by the
+// groups in between.  (DPP: row_ror moves lane i to i + n; a bank is four lanes.)
+template <int NH, int N>
+__device__ __forceinline__ uint32_t turn_in(const uint32_t (&x)[NH][N], int i, int h) {
+    static_assert(NH == 1 || NH == 2 || NH == 4, "groups of lanes");
+    int w = (int)x[0][i];
+    if constexpr (NH == 2) {
+        w = h ? __builtin_amdgcn_update_dpp(w, (int)x[1][i], 0x128, 0xF, 0x3, false)
+              : __builtin_amdgcn_update_dpp(w, (int)x[1][i], 0x128, 0xF, 0xC, false);
+    } else if constexpr (NH == 4) {
+        // load j into group (h + j) % 4
+#define QATTN_TURN(J)                                                                                   \
+    w = h == 0   ? __builtin_amdgcn_update_dpp(w, (int)x[J][i], 0x120 + 4 * J, 0xF, 1 << (J) % 4, false)     \
+        : h == 1 ? __builtin_amdgcn_update_dpp(w, (int)x[J][i], 0x120 + 4 * J, 0xF, 1 << (1 + J) % 4, false) \
+        : h == 2 ? __builtin_amdgcn_update_dpp(w, (int)x[J][i], 0x120 + 4 * J, 0xF, 1 << (2 + J) % 4, false) \
+                 : __builtin_amdgcn_update_dpp(w, (int)x[J][i], 0x120 + 4 * J, 0xF, 1 << (3 + J) % 4, false)
+        QATTN_TURN(1);
+        QATTN_TURN(2);
+        QATTN_TURN(3);
+#undef QATTN_TURN
+    }
+    return (uint32_t)w;
+}
+
 // ---------------------------------------------------------------------------
 // Few rows (16 QB per tile).  The waves' split, the products and the softmax are
 // the 16-bit kernel's: per step a wave forms S^T = K Q^T and O^T += V^T P^T for 32
-// keys of its own.  What differs is the way in:
+// keys of its own, and nothing is shared between the waves but a head's last join.
+// What differs is the way in:
 //   K  A lane's operand words are a quarter of a key row, contiguous: lane (l16, lq)
 //      takes dims D/4 lq .. of key l16, k-step c the 8 from D/4 lq + 8 c on (Q^T is
 //      read in that order, which is free), so a quarter has one scale.
-//   V  A lane widens 16 (or 8) bytes of a row and stores them to the wave's LDS block
+//   V  A lane widens 16 (or 8) bytes of a row and stores them to the head's LDS block
 //      as 16-byte chunks; chunk i of lane part ch lies at place i LPR + ch, so that
 //      the lanes of a row write side by side.  O's columns come out in that order and
 //      are put back where they are stored.
-//   scales  One load per step: lane j that of K's key j (j < 32) or V's key j - 32;
-//      lane exchanges hand them out.
+//   scales  A lane loads a word of one token's (K's and V's); lane exchanges hand the
+//      words out.
+// and the number of heads: a wave takes NH kv heads whose rows lie side by side in a
+// token, 128 bytes where they reach, and each load takes whole tokens: a 64-byte row by
+// itself is half a line, fetched again for the other half (64 x 5300-16000 tokens, 4
+// bits, heads of 128: 259 us with one head per wave, 154 with two, 143 of them the bare
+// loads; with whole lines per load, past the caches, the bare loads take 121).
+//   columns  Each head has COLS = 16 / NH of the 16 columns of one S^T, put together
+//      from the heads' products with all columns of Q^T, so that the softmax is paid
+//      once for NH heads; P^T as it is serves every head's product with V (a head's
+//      columns of the others' products are not read, and no column touches another).
+//   rows  Load j of a key tile holds tokens COLS j .. + COLS - 1, lanes h COLS .. their
+//      rows of head h.  Head h's operand has them in its lanes g COLS .. from load (g -
+//      h) % NH, turned by (g - h) COLS lanes (DPP): its row r is token turned(r, -h),
+//      where turned(r, x) moves r's group of COLS by x groups.  V's rows of head h are
+//      stored in the same order, and its columns' masks read so.
 // ---------------------------------------------------------------------------
 constexpr int kNarrowWaves = 4;             // waves of a STREAM workgroup
 constexpr int kItemWaves = 8;               // waves of a workgroup per item
+constexpr int kAhead = 3;                   // V operands read ahead of their product
 
-constexpr int quant_waves(int d, int qb) { return d == 128 ? (qb > 1 ? 2 : 3) : 4; }
+constexpr int quant_waves(int d, int qb, int nh) { return d == 128 || nh > 1 ? 2 : qb > 1 ? 3 : 4; }
 
-template <typename T, int D, int BITS, int QB, int NW, int HW, bool STREAM>
+// NW waves for G sets of NH kv heads.
+template <typename T, int D, int BITS, int QB, int NW, int NH, int G, bool STREAM>
 __global__ __launch_bounds__(64 * NW)
-    __attribute__((amdgpu_waves_per_eu(quant_waves(D, QB)))) void quant_attn_kernel(QuantParams p) {
+    __attribute__((amdgpu_waves_per_eu(quant_waves(D, QB, NH)))) void quant_attn_kernel(QuantParams p) {
     constexpr int NC = D / 32;              // k-steps of S^T over the head dim
     constexpr int ND = D / 16;              // d-tiles of O^T
     constexpr int DV = D / 8;               // 16-byte chunks per widened row
     constexpr int NS = D / kQuantBlock;     // scales per row
+    constexpr int SW = (NH * NS + 3) / 4;   // words of a token's scales (K's or V's)
     constexpr int KW = D * BITS / 128;      // words of a quarter row
     constexpr int RB = D * BITS / 8;        // bytes of a row
     constexpr int VB = RB / 2 < 16 ? RB / 2 : 16;  // bytes of V per lane and load
     constexpr int LPR = RB / VB;            // lanes per V row
-    constexpr int RPI = 64 / LPR;           // V rows per load
-    constexpr int NV = 32 / RPI;            // V loads per lane and step
+    constexpr int TPI = 64 / (NH * LPR);    // tokens per V load
+    constexpr int NV = 32 / TPI;            // V loads per lane and step
     constexpr int SUB = VB / BITS;          // chunks of 8 elements per load
-    constexpr int WBLK = 32 * D;            // elements of a wave's V block
+    constexpr int WBLK = 32 * D;            // elements of a head's V block
     constexpr int ROWS = 16 * QB;
-    constexpr int WPH = NW / HW;            // waves of a kv head
+    constexpr int COLS = 16 / NH;           // columns of a head
+    constexpr int WPH = NW / G;             // waves of a set of heads
     constexpr int KEYS = 32 * WPH;          // of a unit
-    static_assert(LPR * SUB == DV && NV * RPI == 32 && NC * BITS / 4 == KW, "a step is 32 rows");
+    constexpr bool ONCE = NH * RB >= 128;   // a load's tokens are whole lines: past the caches
+    static_assert(LPR * SUB == DV && NV * TPI == 32 && TPI % 8 == 0 && NC * BITS / 4 == KW, "a step is 32 rows");
+    static_assert(NH == 1 || (QB == 1 && NH * RB <= 128), "one tile of columns");
     // The waves' V blocks; after the key loop, the waves' numerators of one
-    // row block (NW x 16 rows x D floats, the same size).
-    __shared__ __attribute__((aligned(1024))) uint16_t vlds[NW * WBLK];
+    // row block (NW x 16 rows x D floats, the size of one head's).
+    __shared__ __attribute__((aligned(4096))) uint16_t vlds[NW * NH * WBLK];  // (16 rows: bits of an address)
     __shared__ float ml[2][NW][ROWS];
 
     Share sh{};
     if constexpr (STREAM) {
-        if (!find_share(p, sh)) return;
+        if (!find_share<64 * NW>(p, sh)) return;
     } else {
         sh.end = 1;  // one part: the item
     }
@@ -104,11 +161,23 @@ __global__ __launch_bounds__(64 * NW)
     const int l16 = lane & 15, lq = lane >> 4;
 
     // wave-private V block: chunk c of row r at c ^ kv_swz(r)
-    uint16_t* const vblk = vlds + wave * WBLK;
+    // (byte addresses; the others are these with bits flipped.  hide() keeps the compiler
+    // from holding a register for each, which spills.)
+    const uint32_t vblk = lds_at(vlds + wave * NH * WBLK);
     const int vr = 4 * lq + (l16 >> 2);
-    const int vaddr0 = vr * D + 8 * (((l16 & 3) >> 1) ^ kv_swz(vr, DV)) + 4 * (l16 & 1);
-    const int kshift = 8 * (lq * NS / 4);                               // the lane's scale in a word of them
-    const int vshift = 8 * ((lane % LPR) * (VB * 8 / BITS) / kQuantBlock);
+    uint32_t vget = vblk + 2 * (vr * D + 8 * (((l16 & 3) >> 1) ^ kv_swz(vr, DV)) + 4 * (l16 & 1));
+    // The lane's token in V's load 0 (+ n TPI) and head there: with four lanes per row
+    // neighbouring quads take rows two apart, whose swizzles keep their stores in
+    // different banks.
+    const int vj = lane / LPR % TPI, vhead = lane / (LPR * TPI);
+    const int vtok = LPR == 4 ? (vj & ~3) | (vj & 1) << 1 | (vj >> 1 & 1) : vj;
+    auto turned = [](int r, int x) { return (r & ~15) | ((r / COLS + x) * COLS & 15) | r % COLS; };
+    const int vrow = turned(vtok, vhead);
+    uint32_t vput = vblk + 2 * (WBLK * vhead + vrow * D + 8 * (lane % LPR ^ kv_swz(vrow, DV)));
+    auto hide = [&] { asm volatile("" : "+v"(vget), "+v"(vput)); };
+    // the lane's scale in a word of them
+    const int kshift = 8 * (lq * NS / 4);
+    const int vshift = 8 * (vhead * NS % 4 + (lane % LPR) * (VB * 8 / BITS) / kQuantBlock);
 
     while (sh.u < sh.end) {
         Part part;
@@ -125,16 +194,18 @@ __global__ __launch_bounds__(64 * NW)
             part.b0 = 0, part.b1 = sw.blocks, part.whole = true;
         }
         const int tile = part.tile, b0 = part.b0, b1 = part.b1, ctx = sw.ctx;
-        const int kvh = part.group * HW + wave / WPH;
+        const int kvh = (part.group * G + wave / WPH) * NH;  // the wave's first head
 
+        // column r of the wave's tile: a row of head kvh + r / COLS (all of the tile's
+        // rows, where the wave has one head)
         auto query_of = [&](int r, int64_t& qrow, int& qh) {
-            const int rr = tile * 16 * QB + r;
+            const int rr = NH == 1 ? tile * 16 * QB + r : r % COLS;
             const int tok = divide(rr, p.gdiv);
-            qh = kvh * p.group + (rr - tok * p.group);
+            qh = (kvh + (NH == 1 ? 0 : r / COLS)) * p.group + (rr - tok * p.group);
             qrow = (int64_t)sw.s0 + tok;
             return rr < sw.rows;
         };
-        // Q^T operand of k-step c: dims D/4 lq + 8 c .. + 7 of row 16 b + l16
+        // Q^T operand of k-step c: dims D/4 lq + 8 c .. + 7 of the lane's column
         Vec16 qf[QB][NC];
 #pragma unroll
         for (int b = 0; b < QB; ++b) {
@@ -149,111 +220,142 @@ __global__ __launch_bounds__(64 * NW)
             }
         }
         float m_run[QB], l_run[QB];
-        f4_t oacc[QB][ND];
+        f4_t oacc[QB * NH][ND];
 #pragma unroll
-        for (int b = 0; b < QB; ++b) {
-            m_run[b] = -INFINITY;
-            l_run[b] = 0.f;
+        for (int b = 0; b < QB * NH; ++b)
 #pragma unroll
             for (int i = 0; i < ND; ++i) oacc[b][i] = f4_t{0.f, 0.f, 0.f, 0.f};
-        }
-        const char* const kb = (const char*)(p.kc + kvh * p.sk_head) + 4 * KW * lq;
-        const char* const vb = (const char*)(p.vc + kvh * p.sk_head) + VB * (lane % LPR);
-        const char* const sb = (const char*)(lane < 32 ? p.ks : p.vs) + kvh * p.ss_head;
+#pragma unroll
+        for (int b = 0; b < QB; ++b) m_run[b] = -INFINITY, l_run[b] = 0.f;
+        const char* const kb = (const char*)(p.kc + kvh * p.sk_head) + RB * (l16 / COLS) + 4 * KW * lq;
+        const char* const vb = (const char*)(p.vc + kvh * p.sk_head) + RB * vhead + VB * (lane % LPR);
+        // one word per token: lanes 0 .. 31 K's, 32 .. 63 V's; two: K's, then V's, lanes
+        // 32 .. 63 the second
+        const char* const sb = (const char*)(SW == 2 || lane < 32 ? p.ks : p.vs) + kvh * p.ss_head + (SW == 2 ? lane / 32 * 4 : 0);
+        const char* const sb2 = (const char*)p.vs + kvh * p.ss_head + lane / 32 * 4;
         const int32_t* const pt = p.table + (int64_t)sh.seq * p.pt_cols;
 
-        // key lane % 32 of step b: its page (asked for without waiting for the
-        // context's length), or -1 past the table
+        // key lane % 32 of step b, and its page (within the table: what lies past the
+        // context is not used)
         auto key_at = [&](int b) { return KEYS * b + 32 * (wave % WPH) + (lane & 31); };
-        auto page_of = [&](int b) {
-            const int pos = key_at(b);
-            return pos < p.capacity ? pt[divide(pos, p.pdiv)] : -1;
+        auto page_at = [&](int b) { return pt[divide(min(key_at(b), p.capacity - 1), p.pdiv)]; };
+        // x of the lane at byte 4 * lane
+        auto from = [](uint32_t x, int at) { return (uint32_t)__builtin_amdgcn_ds_bpermute(at, (int)x); };
+        const int klane = 4 * (l16 % COLS), vlane = 4 * vtok;
+        const int vslane = vlane + (SW == 2 ? 128 * (vhead * NS / 4) : 128);
+        // A step's loads, requested two steps ahead.  Keys that do not exist, and those
+        // of steps past the part, read the cache's first row and count for nothing.
+        struct Raw {
+            uint32_t k[2][NH][KW], v[NV][VB / 4], s[SW];
+            uint32_t have;  // bit j: key j of the step exists
         };
-        // the step's loads.  Keys that do not exist read the cache's first row and
-        // count for nothing below.
-        uint32_t kx[2][KW], vx[NV][VB / 4], sx = 0;
-        uint32_t have = 0;  // bit j: key j of the step exists
-        auto issue = [&](int b, int page) {
+        auto issue = [&](Raw& r, int b, int page) {
             const int pos = key_at(b);
-            const bool ok = (uint32_t)page < (uint32_t)p.num_pages && pos < ctx;
-            have = (uint32_t)__ballot(ok);
+            const bool ok = (uint32_t)page < (uint32_t)p.num_pages && pos < ctx && b < b1;
+            r.have = (uint32_t)__ballot(ok);
             const int slot = pos - divide(pos, p.pdiv) * p.page_size;
-            // row offsets in 16-byte units, scales in rows of them (below 2^32:
-            // checked on the host)
-            const uint32_t off = ok ? (uint32_t)((page * p.sk_page + slot * p.sk_slot) >> 3) : 0u;
-            const uint32_t so = ok ? (uint32_t)((uint64_t)(page * p.ss_page + slot * p.ss_slot) / NS) : 0u;
-            sx = ld_scales<NS>(sb + NS * (uint64_t)so);
+            // row offsets in 16-byte units, scales in rows of them (both below 2^32)
+            const uint32_t off = ok ? (uint32_t)page * p.row_page + (uint32_t)slot * p.row_slot : 0u;
+            const uint32_t so = ok ? (uint32_t)page * p.scale_page + (uint32_t)slot * p.scale_slot : 0u;
+            uint32_t ko[2][NH], vo[NV];
 #pragma unroll
             for (int t = 0; t < 2; ++t)
-                ld_words(kx[t], kb + 16 * (uint64_t)(uint32_t)__shfl((int)off, 16 * t + l16));
+#pragma unroll
+                for (int j = 0; j < NH; ++j) ko[t][j] = from(off, klane + 64 * t + 4 * COLS * j);
+#pragma unroll
+            for (int n = 0; n < NV; ++n) vo[n] = from(off, vlane + 4 * TPI * n);
+            r.s[0] = ld_scales<SW == 2 ? 4 : NH * NS>(sb + NS * (uint64_t)so);
+            if constexpr (SW == 2) r.s[1] = ld_scales<4>(sb2 + NS * (uint64_t)so);
+#pragma unroll
+            for (int n = 0; n < NV; ++n) ld_words<ONCE>(r.v[n], vb + 16 * (uint64_t)vo[n]);
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int j = 0; j < NH; ++j) ld_words<ONCE>(r.k[t][j], kb + 16 * (uint64_t)ko[t][j]);
+            // (requests keep their order, so that a wait for one step's is no wait for the next one's)
+            __builtin_amdgcn_sched_barrier(0);
+        };
+        int page = 0;  // of the step after the next
+        auto step = [&](Raw& r, int b) {
+            hide();
+            const int after = page_at(b + 3);  // (ahead of the loads that it does not wait for)
+            const uint32_t mask = r.have;
+            // scales of the lane's V rows, and of the rows of K's operands
+            float vscale[NV], kscale[2][NH];
 #pragma unroll
             for (int n = 0; n < NV; ++n)
-                ld_words(vx[n], vb + 16 * (uint64_t)(uint32_t)__shfl((int)off, n * RPI + lane / LPR));
-        };
-        int page = page_of(b0);
-        int next = page_of(b0 + 1);
-        if (ctx > 0) issue(b0, page);  // (no context: nothing to read, maybe no cache)
-        for (int b = b0; b < b1; ++b) {
-            const uint32_t mask = have, scales = sx;
-            auto scale_at = [&](int from, int shift) {
-                return scale_of((uint32_t)__shfl((int)scales, from) >> shift & 255u);
-            };
+                vscale[n] = scale_of(from(r.s[SW - 1], vslane + 4 * TPI * n) >> vshift & 255u);
+#pragma unroll
+            for (int h = 0; h < NH; ++h)
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+                    kscale[t][h] = scale_of(from(r.s[0], 4 * turned(l16, NH - h) + 64 * t + 128 * (h * NS / 4)) >>
+                                                (8 * (h * NS % 4) + kshift) & 255u);
             // V to LDS; rows of keys that do not exist as zeros (weight 0
             // times what lies there could be NaN)
+            if (mask != 0xffffffffu) {
+                const uint32_t mine = mask >> vtok;
 #pragma unroll
-            for (int n = 0; n < NV; ++n) {
-                const int r = n * RPI + lane / LPR;
-                float s = scale_at(32 + r, vshift);
-                if (mask != 0xffffffffu && !(mask >> r & 1)) {
-                    s = 1.f;
+                for (int n = 0; n < NV; ++n) {
+                    const bool there = mine >> (n * TPI) & 1;
+                    vscale[n] = there ? vscale[n] : 1.f;
 #pragma unroll
-                    for (int i = 0; i < VB / 4; ++i) vx[n][i] = 0;
+                    for (int i = 0; i < VB / 4; ++i) r.v[n][i] = there ? r.v[n][i] : 0u;
                 }
-#pragma unroll
-                for (int i = 0; i < SUB; ++i)
-                    st16(vblk + r * D + 8 * ((i * LPR + lane % LPR) ^ kv_swz(r, DV)),
-                         widen8<T, BITS>(vx[n] + i * (BITS / 4), s));
             }
-            uint32_t kf[2][KW];
-            float kscale[2];
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                kscale[t] = scale_at(16 * t + l16, kshift);
+            for (int n = 0; n < NV; ++n)
 #pragma unroll
-                for (int i = 0; i < KW; ++i) kf[t][i] = kx[t][i];
-            }
-            if (b + 1 < b1) {
-                page = next;
-                next = page_of(b + 2);
-                issue(b + 1, page);
-            }
-            if (mask == 0) continue;  // none of the wave's keys exists
+                for (int i = 0; i < SUB; ++i) {
+                    // (of 8 tokens per load, those of odd loads lie 8 rows further or before)
+                    constexpr int ODD = TPI % 16;
+                    const uint32_t at = (vput ^ (16 * (LPR * i) ^ (n % 2 ? 16 * kv_swz(ODD, DV) ^ 2 * D * ODD : 0))) +
+                                        2 * D * (TPI * n / 16 * 16);
+                    const Vec16 x = widen8<T, BITS>(r.v[n] + i * (BITS / 4), vscale[n]);
+                    *(__attribute__((address_space(3))) w4_t*)(uintptr_t)at = w4_t{x.w[0], x.w[1], x.w[2], x.w[3]};
+                }
+            // scores: every head's K with all columns, each column from its own head (no
+            // zeros in the other columns: 0 times what is no number is none either)
+            f4_t s[QB][2];
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int h = 0; h < NH; ++h) {
+                    uint32_t kw[KW];
+#pragma unroll
+                    for (int i = 0; i < KW; ++i) kw[i] = turn_in<NH>(r.k[t], i, h);
+                    f4_t x[QB];
+#pragma unroll
+                    for (int q = 0; q < QB; ++q) x[q] = f4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int c = 0; c < NC; ++c) {
+                        const Vec16 k = widen8<T, BITS>(kw + c * (BITS / 4), kscale[t][h]);
+#pragma unroll
+                        for (int q = 0; q < QB; ++q) x[q] = MfmaOps<T>::mma(k, qf[q][c], x[q]);
+                    }
+#pragma unroll
+                    for (int q = 0; q < QB; ++q)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) s[q][t][i] = h == 0 || l16 / COLS == h ? x[q][i] : s[q][t][i];
+                }
+            issue(r, b + 2, page);
+            page = after;
             __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
             __builtin_amdgcn_wave_barrier();
             __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-            f4_t s[QB][2];
-#pragma unroll
-            for (int t = 0; t < 2; ++t) {
-#pragma unroll
-                for (int q = 0; q < QB; ++q) s[q][t] = f4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int c = 0; c < NC; ++c) {
-                    const Vec16 k = widen8<T, BITS>(kf[t] + c * (BITS / 4), kscale[t]);
-#pragma unroll
-                    for (int q = 0; q < QB; ++q) s[q][t] = MfmaOps<T>::mma(k, qf[q][c], s[q][t]);
-                }
-            }
             Vec16 pf[QB];
             float alpha[QB];
 #pragma unroll
             for (int q = 0; q < QB; ++q) {
-                // lane: keys 16 t + 4 lq + i of row l16
+                // lane: rows 16 t + 4 lq + i of column l16
                 if (mask != 0xffffffffu) {
+                    uint32_t mine = mask >> turned(4 * lq, NH - l16 / COLS);
+                    asm volatile("" : "+v"(mine));  // (eight tests of one word, no eight lane masks)
 #pragma unroll
                     for (int t = 0; t < 2; ++t)
 #pragma unroll
                         for (int i = 0; i < 4; ++i)
-                            if (!(mask >> (16 * t + 4 * lq + i) & 1)) s[q][t][i] = -INFINITY;
+                            if (!(mine >> (16 * t + i) & 1)) s[q][t][i] = -INFINITY;
                 }
                 float mb = -INFINITY;
 #pragma unroll
@@ -289,26 +391,69 @@ __global__ __launch_bounds__(64 * NW)
 #pragma unroll
                 for (int q = 0; q < QB; ++q)
 #pragma unroll
-                    for (int dt = 0; dt < ND; ++dt) oacc[q][dt] *= alpha[q];
-            }
+                    for (int h = 0; h < NH; ++h)
 #pragma unroll
-            for (int dt = 0; dt < ND; ++dt) {
+                        for (int dt = 0; dt < ND; ++dt) oacc[q + h][dt] *= alpha[q];
+            }
+            auto v_operand = [&](int i) {  // d-tile i % ND of head i / ND
                 typedef short v4s __attribute__((ext_vector_type(4)));
                 typedef __attribute__((address_space(3))) v4s* lds_v4s;
-                uint16_t* a = vblk + (vaddr0 ^ (16 * dt));
-                const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s)a);
-                const v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s)(a + 16 * D));
+                const uint32_t a = (vget ^ (32 * (i % ND))) + 2 * WBLK * (i / ND);
+                const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s)(uintptr_t)a);
+                const v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s)(uintptr_t)(a + 32 * D));
                 const uint2 l2 = __builtin_bit_cast(uint2, lo), h2 = __builtin_bit_cast(uint2, hi);
-                const Vec16 va{{l2.x, l2.y, h2.x, h2.y}};
+                return Vec16{{l2.x, l2.y, h2.x, h2.y}};
+            };
+            constexpr int NT = NH * ND, AHEAD = NT < kAhead ? NT : kAhead;
+            Vec16 va[AHEAD];
 #pragma unroll
-                for (int q = 0; q < QB; ++q) oacc[q][dt] = MfmaOps<T>::mma(va, pf[q], oacc[q][dt]);
+            for (int i = 0; i < AHEAD; ++i) va[i] = v_operand(i);
+#pragma unroll
+            for (int i = 0; i < NT; ++i) {
+                const Vec16 v = va[i % AHEAD];
+#pragma unroll
+                for (int q = 0; q < QB; ++q)
+                    oacc[q + i / ND][i % ND] = MfmaOps<T>::mma(v, pf[q], oacc[q + i / ND][i % ND]);
+                if (i + AHEAD < NT) va[i % AHEAD] = v_operand(i + AHEAD);
+                __builtin_amdgcn_sched_barrier(0);
             }
             __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
             __builtin_amdgcn_wave_barrier();  // the block's reads come before the next step's writes
             __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        };
+        if (ctx > 0) {  // (no context: nothing to read, maybe no cache)
+            Raw r0, r1;
+            const int first = page_at(b0), second = page_at(b0 + 1);
+            page = page_at(b0 + 2);
+            __builtin_amdgcn_sched_barrier(0);
+            issue(r0, b0, first);
+            issue(r1, b0 + 1, second);
+            for (int b = b0;;) {
+                step(r0, b);
+                if (++b >= b1) break;
+                step(r1, b);
+                if (++b >= b1) break;
+            }
         }
-        join_waves<T, D, QB, NW, HW>(p, sh, part, query_of, m_run, l_run, oacc, vlds, ml,
-                                     [](int ch) { return ch % LPR * SUB + ch / LPR; });
+        auto dims_of = [](int ch) { return ch % LPR * SUB + ch / LPR; };
+        auto state_of = [&](int r) {
+            return (wave / WPH * NH + (NH == 1 ? 0 : r / COLS)) * ROWS + (NH == 1 ? r : r % COLS);
+        };
+        if constexpr (NH > 1) {
+            // each column of the head that it belongs to
+            f4_t own[1][ND];
+#pragma unroll
+            for (int dt = 0; dt < ND; ++dt) {
+                own[0][dt] = oacc[0][dt];
+#pragma unroll
+                for (int h = 1; h < NH; ++h)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) own[0][dt][i] = l16 / COLS == h ? oacc[h][dt][i] : own[0][dt][i];
+            }
+            join_waves<T, D, 1, NW, G>(p, sh, part, query_of, m_run, l_run, own, vlds, ml, dims_of, NH * G, state_of);
+        } else {
+            join_waves<T, D, QB, NW, G>(p, sh, part, query_of, m_run, l_run, oacc, vlds, ml, dims_of, NH * G, state_of);
+        }
         __syncthreads();  // the LDS is free for the next item
         sh.u += STREAM ? b1 - b0 : 1;
     }
@@ -372,8 +517,8 @@ struct QuantKeys {
             const int slot = pos - col * p.page_size;
             const bool ok = (uint32_t)page < (uint32_t)p.num_pages;
             // (keys that do not exist read the cache's first row)
-            t.row[i][lane] = ok ? (uint32_t)((page * p.sk_page + slot * p.sk_slot) >> 3) : 0u;
-            t.scale[i][lane] = ok ? (uint32_t)((uint64_t)(page * p.ss_page + slot * p.ss_slot) / NS) : 0u;
+            t.row[i][lane] = ok ? (uint32_t)page * p.row_page + (uint32_t)slot * p.row_slot : 0u;
+            t.scale[i][lane] = ok ? (uint32_t)page * p.scale_page + (uint32_t)slot * p.scale_slot : 0u;
             const uint64_t have = __ballot(ok);
             if (lane == 0) t.have[i] = have;
         }
@@ -526,36 +671,55 @@ __global__ __launch_bounds__(kPagedThreads) __attribute__((amdgpu_waves_per_eu(2
 // ---------------------------------------------------------------------------
 // Host side
 // ---------------------------------------------------------------------------
-static PagedShape quant_shape(int64_t max_rows, int64_t pairs, int hkv, int64_t capacity, int head_dim) {
-    const int steps = pairs >= 128 ? 4 : 2;
-    if (max_rows <= 16 && capacity <= steps * 32 * kItemWaves && pairs <= 256) return {1, 4, 8, 1, 1, true};
+// Largest power of two up to `most` that divides n.
+static int pow2_part(int n, int most) {
+    int g = 1;
+    while (2 * g <= most && n % (2 * g) == 0) g *= 2;
+    return g;
+}
+
+// together: the heads of a token lie side by side, elements and scales.
+static PagedShape quant_shape(int bits, bool together, int64_t max_rows, int64_t pairs, int hkv, int64_t capacity,
+                              int head_dim) {
+    const int steps = (bits == 4 ? pairs <= 128 : pairs >= 64) ? 4 : 2;
+    if (max_rows <= 16 && capacity <= steps * 32 * kItemWaves && pairs <= 256) return {1, 4, 8, 1, 1, true, 1};
     if (max_rows <= 32) {
-        const int qb = max_rows <= 16 ? 1 : 2;
-        const int per_cu = quant_waves(head_dim, qb);
-        int heads = hkv % 4 == 0 ? 4 : hkv % 2 == 0 ? 2 : 1;
-        const int64_t work = pairs * ((capacity + 127) / 128);
-        if (max_rows > 8 || pairs / heads * 16 < 256 * per_cu || work < 16 * 256 * per_cu) heads = 1;
-        return {qb, qb == 1 ? 4 : 5, heads == 4 ? 5 : heads == 2 ? 6 : 7, heads, per_cu, false};
+        const int qb = max_rows <= 16 ? 1 : 2, row_bytes = head_dim * bits / 8;
+        int nh = 1;
+        while (together && nh < 4 && 2 * nh * row_bytes <= 128 && max_rows * 2 * nh <= 16 && hkv % (2 * nh) == 0) nh *= 2;
+        int per_cu = quant_waves(head_dim, qb, nh);
+        int g = max_rows <= 16 ? pow2_part(hkv / nh, kNarrowWaves) : 1;
+        if (pairs / (nh * g) * ((capacity + 31) / 32) < (nh > 1 ? 16 : 8) * 256 * per_cu) g = 1;
+        if (nh > 1 && g == 1) per_cu = 1;
+        return {qb, qb == 1 ? 4 : 5, 7 - __builtin_ctz((unsigned)g), nh * g, per_cu, false, nh};
     }
-    return {0, 7, 6, 1, 2, false};
+    return {0, 7, 6, 1, 2, false, 1};
 }
 
 template <typename T, int D, int BITS>
 static int launch_quant(const QuantParams& p, const PagedShape& sh, hipStream_t st) {
     const dim3 grid(p.nwg), block(kPagedThreads);
     if (sh.items) {
-        hipLaunchKernelGGL((quant_attn_kernel<T, D, BITS, 1, kItemWaves, 1, false>),
+        hipLaunchKernelGGL((quant_attn_kernel<T, D, BITS, 1, kItemWaves, 1, 1, false>),
                            dim3((uint32_t)(p.B * p.tiles * p.Hkv)), dim3(64 * kItemWaves), 0, st, p);
         return launch_status("quant_attn_kernel, a workgroup per item");
     }
-#define QATTN_NARROW(QB, HW) \
-    hipLaunchKernelGGL((quant_attn_kernel<T, D, BITS, QB, kNarrowWaves, HW, true>), grid, block, 0, st, p)
-    switch (8 * sh.qb + sh.heads) {
-        case 8 + 1: QATTN_NARROW(1, 1); break;
-        case 8 + 2: QATTN_NARROW(1, 2); break;
-        case 8 + 4: QATTN_NARROW(1, 4); break;
-        case 16 + 1: QATTN_NARROW(2, 1); break;
-        default: hipLaunchKernelGGL((quant_wide_kernel<T, D, BITS>), grid, block, 0, st, p);
+    constexpr int NH2 = D * BITS / 8 <= 64 ? 2 : 1, NH4 = D * BITS / 8 <= 32 ? 4 : NH2;
+#define QATTN_NARROW(QB, NH, G) \
+    hipLaunchKernelGGL((quant_attn_kernel<T, D, BITS, QB, kNarrowWaves, NH, G, true>), grid, block, 0, st, p)
+    const int sets = sh.heads / sh.wave_heads;
+    switch (sh.qb == 0 ? 0 : sh.qb == 2 ? 1 : 10 * sh.wave_heads + sets) {
+        case 0: hipLaunchKernelGGL((quant_wide_kernel<T, D, BITS>), grid, block, 0, st, p); break;
+        case 1: QATTN_NARROW(2, 1, 1); break;
+        case 11: QATTN_NARROW(1, 1, 1); break;
+        case 12: QATTN_NARROW(1, 1, 2); break;
+        case 14: QATTN_NARROW(1, 1, 4); break;
+        case 21: QATTN_NARROW(1, NH2, 1); break;
+        case 22: QATTN_NARROW(1, NH2, 2); break;
+        case 24: QATTN_NARROW(1, NH2, 4); break;
+        case 41: QATTN_NARROW(1, NH4, 1); break;
+        case 42: QATTN_NARROW(1, NH4, 2); break;
+        default: QATTN_NARROW(1, NH4, 4);
     }
 #undef QATTN_NARROW
     const int rc = launch_status(sh.qb ? "quant_attn_kernel" : "quant_wide_kernel");
@@ -577,9 +741,14 @@ extern "C" {
 
 int64_t qattn_prefix_quant_workspace_bytes(int32_t batch, int32_t max_seqlen, int64_t total_tokens,
                                            int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
-                                           int32_t pt_cols, int32_t page_size) {
-    return paged_workspace(quant_shape, batch, max_seqlen, total_tokens, num_q_heads, num_kv_heads, head_dim, pt_cols,
-                           page_size);
+                                           int32_t pt_cols, int32_t page_size, int32_t bits) {
+    // (for heads side by side or not: the call knows the strides)
+    int64_t most = 0;
+    for (bool together : {false, true})
+        most = std::max(most, paged_workspace([=](auto... a) { return quant_shape(bits, together, a...); }, batch,
+                                              max_seqlen, total_tokens, num_q_heads, num_kv_heads, head_dim, pt_cols,
+                                              page_size));
+    return most;
 }
 
 int qattn_prefix_quant_fwd(const void* q, const int64_t q_stride[3], const void* k_cache, const void* v_cache,
@@ -597,12 +766,16 @@ int qattn_prefix_quant_fwd(const void* q, const int64_t q_stride[3], const void*
     QuantParams p{};
     PagedPlan plan;
     const int64_t half[4] = {cache_stride[0] / 2, cache_stride[1] / 2, cache_stride[2] / 2, 1};
-    rc = paged_setup(p, plan, quant_shape, q, q_stride, k_cache, half, v_cache, half, page_table, pt_cols, num_pages,
-                     page_size, context_lens, o, o_stride, lse, lse_stride, cu_seqlens, batch, max_seqlen,
-                     total_tokens, num_q_heads, num_kv_heads, head_dim, scale, dtype, workspace, workspace_size);
-    if (rc || plan.nothing) return rc;
-    const int64_t unit = head_dim / kQuantBlock;
+    // (what a wave of several heads loads at once: 128 bytes of elements, 32 / bits of scales)
+    const int64_t unit = head_dim / kQuantBlock, sides = 32 / bits;
     const int64_t* ss = scale_stride;
+    const bool together = cache_stride[2] == head_dim * bits / 8 && ss[2] == unit && (ss[0] | ss[1]) % sides == 0 &&
+                          ((uintptr_t)k_scale | (uintptr_t)v_scale) % sides == 0;
+    rc = paged_setup(p, plan, [=](auto... a) { return quant_shape(bits, together, a...); }, q, q_stride, k_cache, half,
+                     v_cache, half, page_table, pt_cols, num_pages, page_size, context_lens, o, o_stride, lse,
+                     lse_stride, cu_seqlens, batch, max_seqlen, total_tokens, num_q_heads, num_kv_heads, head_dim,
+                     scale, dtype, workspace, workspace_size);
+    if (rc || plan.nothing) return rc;
     // a row's scales are found by a 32-bit offset in rows of them
     if (pt_cols > 0 && num_pages > 0 &&
         (ss[0] < 0 || ss[1] < 0 || ss[0] > (int64_t(1) << 40) || ss[1] > (int64_t(1) << 32) ||
@@ -611,7 +784,12 @@ int qattn_prefix_quant_fwd(const void* q, const int64_t q_stride[3], const void*
         return QATTN_ERR_LAYOUT;
     }
     p.ks = (const uint8_t*)k_scale, p.vs = (const uint8_t*)v_scale;
-    p.ss_page = ss[0], p.ss_slot = ss[1], p.ss_head = ss[2];
+    p.ss_head = ss[2];
+    // (one page, one slot: the stride is not used)
+    p.row_page = num_pages > 1 ? (uint32_t)(half[0] / 8) : 0u;
+    p.row_slot = page_size > 1 ? (uint32_t)(half[1] / 8) : 0u;
+    p.scale_page = num_pages > 1 ? (uint32_t)(ss[0] / unit) : 0u;
+    p.scale_slot = page_size > 1 ? (uint32_t)(ss[1] / unit) : 0u;
     hipStream_t st = (hipStream_t)stream;
     if (dtype == QATTN_DTYPE_F16)
         return bits == 4 ? launch_quant<F16, 4>(p, plan.shape, head_dim, st)

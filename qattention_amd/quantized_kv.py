@@ -134,6 +134,9 @@ def append_quantized_kv(
     end at the format's largest (6, 448).  A block with an infinity or a NaN is NaN.
     Positions, pages and lengths are append_paged_kv's; returns the lengths
     afterwards, int32 [B] on the device."""
+    new = _lib.calls().quant_append(K, V, cache, page_table, context_lens, cu_seqlens, max_seqlen)
+    if new is not None:
+        return new
     num_pages, page_size, Hkv, D, bits, at = _check_cache(cache, written=True)
     assert K.dtype in _SUPPORTED and V.dtype == K.dtype, f"Inputs must be fp16 or bf16 (got {K.dtype}, {V.dtype})"
     idx = _device_index(K, V, *cache)
@@ -173,6 +176,9 @@ def read_quantized_kv(
     no sequence are not written.  Values are exact in bf16, and in fp16 where they lie
     in its range (as those written from fp16 rows do; larger ones become infinities).
     Returns K, V [total_tokens, Hkv, D]."""
+    out = _lib.calls().quant_read(cache, page_table, starts, cu_seqlens, max_seqlen, total_tokens, dtype)
+    if out is not None:
+        return out
     num_pages, page_size, Hkv, D, bits, at = _check_cache(cache, written=False)
     if dtype not in _SUPPORTED:
         raise ValueError(f"dtype must be fp16 or bf16 (got {dtype})")
@@ -211,6 +217,9 @@ def prefix_attention_quantized(
     range, as those written from fp16 rows do.  The elements span less than 64 GiB, the
     scales less than 2^32 rows (QAttnError otherwise).  A block whose scale is no number
     makes the rows that attend it NaN."""
+    out = _lib.calls().quant_paged(Q, cache, page_table, context_lens, cu_seqlens, max_seqlen, return_lse)
+    if out is not None:
+        return out
     num_pages, page_size, Hkv, D, bits, at = _check_cache(cache, written=False)
     assert Q.dtype in _SUPPORTED, f"Inputs must be fp16 or bf16 (got {Q.dtype})"
     idx = _device_index(Q, *cache)
@@ -228,7 +237,7 @@ def prefix_attention_quantized(
     LSE = torch.empty(T, Hq, dtype=torch.float32, device=device) if return_lse else None
     L = _lib.lib()
     cols = pt.shape[1]
-    ws_bytes = L.qattn_prefix_quant_workspace_bytes(B, ms, T, Hq, Hkv, D, cols, page_size)
+    ws_bytes = L.qattn_prefix_quant_workspace_bytes(B, ms, T, Hq, Hkv, D, cols, page_size, bits)
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=device) if ws_bytes else None
     _launch(idx, "qattn_prefix_quant_fwd", L.qattn_prefix_quant_fwd,
             q, qs, *at, pt.data_ptr(), cols, num_pages, page_size, ctx.data_ptr(), o, os_, _lib.ptr(LSE),

@@ -98,6 +98,7 @@ def test_one_token(ctx, ps, Hq, Hkv, D, dtype, bits):
 @pytest.mark.parametrize("dtype", [FP16, BF16])
 @pytest.mark.parametrize("B,ctx,Hq,Hkv,D", [
     (70, 900, 32, 8, 128), (33, 2100, 8, 2, 64), (300, 130, 4, 4, 32), (20, 5000, 32, 4, 128), (64, 1900, 16, 16, 128),
+    (64, 5000, 16, 8, 128), (60, 7000, 16, 8, 64), (64, 9000, 8, 8, 32), (40, 3000, 16, 2, 128), (50, 4000, 8, 2, 32),
 ])
 def test_batches(B, ctx, Hq, Hkv, D, dtype, bits):
     """Contexts of ragged lengths, cut between workgroups, several kv heads each."""
@@ -183,20 +184,21 @@ def test_missing_pages_and_lengths_past_the_table(n, bits):
 
 
 @pytest.mark.parametrize("bits", [4, 8])
-@pytest.mark.parametrize("n", [1, 5, 50])
-def test_no_numbers(n, bits):
+@pytest.mark.parametrize("n,ctx", [(1, [200, 300]), (5, [200, 300]), (50, [200, 300]), (1, [1500, 2900]),
+                                   (1, [130] + 39 * [6000])])
+def test_no_numbers(n, ctx, bits):
     """A block without a number makes the rows that attend it NaN, of its own head and
     sequence alone."""
     from qattention_amd import prefix_attention_quantized
-    ctx = [200, 300]
+    B = len(ctx)
     for name, part in (("K_scale", 0), ("V_scale", 1)):
         cache, table, lens, rows = context(ctx, 16, 2, 128, bits, 91)
         getattr(cache, name)[int(table[0, 100 // 16]), 100 % 16, 1, 2] = 255
-        Q = queries(2 * n, 8, 128, FP16, 92)
-        say("no numbers", n, bits, name)
-        cu = torch.arange(0, 2 * n + 1, n, dtype=torch.int32, device=DEV)
+        Q = queries(B * n, 8, 128, FP16, 92)
+        say("no numbers", n, ctx[:2], bits, name)
+        cu = torch.arange(0, B * n + 1, n, dtype=torch.int32, device=DEV)
         O, L = prefix_attention_quantized(Q, cache, table, lens, cu, max_seqlen=n)
-        o, lse, to, tl = reference(Q, rows, [n, n])
+        o, lse, to, tl = reference(Q, rows, [n] * B)
         bad = torch.zeros_like(O, dtype=torch.bool)
         if part == 0:
             bad[:n, 4:] = True
