@@ -506,7 +506,7 @@ struct QuantKeys {
         vbase = (const char*)(p.vc + (int64_t)kvh * p.sk_head) + 4 * KW * qd;
         ksbase = (const char*)p.ks + kvh * p.ss_head + qd * NS / 4;
         vsbase = (const char*)p.vs + kvh * p.ss_head + qd * NS / 4;
-        lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void*)smem;
+        lds0 = lds_at(smem);
         put = 2 * D * row + 16 * (qd ^ kv_swz32(row, DV));
         __syncthreads();  // the table's and the buffers' last readers are done
         for (int i = wave; i < n; i += 4) {
@@ -534,54 +534,54 @@ struct QuantKeys {
         ld_words(r, base + 16 * (uint64_t)tab->row[b][row]);
         c = *reinterpret_cast<const uint8_t*>(sbase + NS * (uint64_t)tab->scale[b][row]);
     }
-    // Piece n of block j's quarter to the buffer at dst.  A key that does not exist
-    // is zeros.
-    __device__ __forceinline__ void store(int j, int n, const uint32_t (&r)[KW], uint32_t c, uint32_t dst) const {
-        uint32_t w[W];
-        float s = scale_of(c);
-#pragma unroll
-        for (int i = 0; i < W; ++i) w[i] = r[n * W + i];
+    // A key of block j that does not exist is zeros.  (Once per block: a test at each
+    // piece cut the loop into 8 basic blocks more.)
+    __device__ __forceinline__ void drop(int j, uint32_t (&r)[KW], uint32_t& c) const {
         const int b = min(j, nb - 1);
         if (__builtin_expect(bad >> b & 1, 0)) {
             if (!(tab->have[b] >> row & 1)) {
-                s = 1.f;
+                c = 127;
 #pragma unroll
-                for (int i = 0; i < W; ++i) w[i] = 0;
+                for (int i = 0; i < KW; ++i) r[i] = 0;
             }
         }
-        typedef uint32_t v4u __attribute__((ext_vector_type(4)));
-        const Vec16 x = widen8<T, BITS>(w, s);
-        *(__attribute__((address_space(3))) v4u*)(uintptr_t)(dst + (put ^ (64 * n))) = v4u{x.w[0], x.w[1], x.w[2], x.w[3]};
+    }
+    // Piece n of the quarter to the buffer at dst.
+    __device__ __forceinline__ void store(int n, const uint32_t (&r)[KW], uint32_t c, uint32_t dst) const {
+        const Vec16 x = widen8<T, BITS>(r + n * W, scale_of(c));
+        *(__attribute__((address_space(3))) w4_t*)(uintptr_t)(dst + (put ^ (64 * n))) = w4_t{x.w[0], x.w[1], x.w[2], x.w[3]};
     }
     struct Dma {
         const QuantKeys& src;
         int j;
         __device__ __forceinline__ void k(int buf, int n) {
-            src.store(j + 3, n, src.rk, src.ck, src.lds0 + 2 * buf * BLK);
+            if (n == 0) src.drop(j + 3, src.rk, src.ck);
+            src.store(n, src.rk, src.ck, src.lds0 + 2 * buf * BLK);
             if (n == NI - 1) src.fetch(j + 4, src.kbase, src.ksbase, src.rk, src.ck);
         }
         __device__ __forceinline__ void v(int buf, int n) {
-            src.store(j + 1, n, src.rv, src.cv, src.lds0 + 2 * (2 + buf) * BLK);
+            if (n == 0) src.drop(j + 1, src.rv, src.cv);
+            src.store(n, src.rv, src.cv, src.lds0 + 2 * (2 + buf) * BLK);
             if (n == NI - 1) src.fetch(j + 2, src.vbase, src.vsbase, src.rv, src.cv);
         }
     };
     __device__ __forceinline__ Dma dma(int j) const { return Dma{*this, j}; }
-    static __device__ __forceinline__ uint32_t lds_of(const uint16_t* buf) {
-        return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void*)buf;
-    }
     // Blocks 0 to 2, before the loop.
     __device__ __forceinline__ void load_k(int j, uint16_t* buf) const {
+        if (j == 1) drop(1, r1, c1);
+        else drop(j, rk, ck);
 #pragma unroll
         for (int n = 0; n < NI; ++n) {
-            if (j == 1) store(1, n, r1, c1, lds_of(buf));
-            else store(j, n, rk, ck, lds_of(buf));
+            if (j == 1) store(n, r1, c1, lds_at(buf));
+            else store(n, rk, ck, lds_at(buf));
         }
         if (j == 0) fetch(2, kbase, ksbase, rk, ck);
         if (j == 2) fetch(3, kbase, ksbase, rk, ck);
     }
     __device__ __forceinline__ void load_v(int j, uint16_t* buf) const {
+        drop(j, rv, cv);
 #pragma unroll
-        for (int n = 0; n < NI; ++n) store(j, n, rv, cv, lds_of(buf));
+        for (int n = 0; n < NI; ++n) store(n, rv, cv, lds_at(buf));
         fetch(j + 1, vbase, vsbase, rv, cv);
     }
     __device__ __forceinline__ void mask(int j, f16v_t (&s)[2]) const {
@@ -669,6 +669,73 @@ __global__ __launch_bounds__(kPagedThreads) __attribute__((amdgpu_waves_per_eu(2
 }
 
 // ---------------------------------------------------------------------------
+// Joins the parts of the wide kernel's cut items: SUB workgroups per run, for the item
+// that the run starts inside (the first such run joins it), D / 8 lanes per row, kParts
+// states in flight.  Where nothing is cut a workgroup ends on its first load: a wave
+// per row of the call instead looked for nothing for 21 us of a chunk's 237 (2 x 1009
+// tokens over 6007).  A run's states are read on the XCD that wrote them.
+// ---------------------------------------------------------------------------
+constexpr int kParts = 4;
+
+template <int D>
+constexpr int kJoinRows = 4 * 64 / (D / 8);  // of a workgroup
+
+template <typename T, int D>
+__global__ __launch_bounds__(kPagedThreads) void quant_join_kernel(PagedParams p) {
+    constexpr int LPR = D / 8, SUB = DenseTile<T, D>::kBM / kJoinRows<D>;
+    const int per = p.nwg >> 3, in = blockIdx.x >> 3;
+    const int w = (blockIdx.x & 7) * per + in / SUB;
+    const RunStart c = p.cuts[w];
+    if (c.b0 == 0) return;
+    const Runs runs(c.total, p.nwg, p.least);
+    const int32_t a = c.first;
+    if (w > 0 && runs.first(w - 1) > a) return;
+    const int rr = in % SUB * kJoinRows<D> + threadIdx.x / LPR, ch = threadIdx.x % LPR;
+    const int in_seq = (c.tile << p.row_shift) + rr;
+    if (in_seq >= c.rows) return;
+    const int w0 = runs.of(a), w1 = runs.of(a + c.blocks - 1) + 1;
+    float m = -INFINITY, l = 0.f, acc[8] = {};
+    for (int v = w0; v < w1; v += kParts) {
+        float mi[kParts], li[kParts];
+        float4 x[kParts], y[kParts];
+#pragma unroll
+        for (int u = 0; u < kParts; ++u) {
+            // (past the last part: the last one again, with a weight of 0)
+            const int ww = min(v + u, w1 - 1);
+            const int64_t row = ((2 * (int64_t)ww + (runs.first(ww) >= a ? 0 : 1)) << p.row_shift) + rr;
+            mi[u] = v + u < w1 ? p.part_m[row] : -INFINITY;
+            li[u] = v + u < w1 ? p.part_l[row] : 0.f;
+            const float4* from = reinterpret_cast<const float4*>(p.part_acc + row * D + 8 * ch);
+            x[u] = from[0], y[u] = from[1];
+        }
+        float mn = m;
+#pragma unroll
+        for (int u = 0; u < kParts; ++u) mn = fmaxf(mn, mi[u]);
+        const float mc = mn == -INFINITY ? 0.f : mn, old = fast_exp2(m - mc);
+        l *= old;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) acc[i] *= old;
+#pragma unroll
+        for (int u = 0; u < kParts; ++u) {
+            if (v + u >= w1) break;
+            const float f = fast_exp2(mi[u] - mc);
+            l += f * li[u];
+            acc[0] += f * x[u].x, acc[1] += f * x[u].y, acc[2] += f * x[u].z, acc[3] += f * x[u].w;
+            acc[4] += f * y[u].x, acc[5] += f * y[u].y, acc[6] += f * y[u].z, acc[7] += f * y[u].w;
+        }
+        m = mn;
+    }
+    const int tok = divide(in_seq, p.gdiv);
+    const int qh = c.group * p.group + (in_seq - tok * p.group);
+    const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) acc[i] = in_range<T>(acc[i] * inv);
+    const int64_t qrow = (int64_t)c.s0 + tok;
+    st16(p.o + qrow * p.so_t + qh * p.so_h + 8 * ch, pack8<T>(acc));
+    if (p.lse && ch == 0) p.lse[qrow * p.sl_t + qh * p.sl_h] = ((m == -INFINITY ? 0.f : m) + fast_log2(l)) * kLn2;
+}
+
+// ---------------------------------------------------------------------------
 // Host side
 // ---------------------------------------------------------------------------
 // Largest power of two up to `most` that divides n.
@@ -694,6 +761,14 @@ static PagedShape quant_shape(int bits, bool together, int64_t max_rows, int64_t
         return {qb, qb == 1 ? 4 : 5, 7 - __builtin_ctz((unsigned)g), nh * g, per_cu, false, nh};
     }
     return {0, 7, 6, 1, 2, false, 1};
+}
+
+// Whether the wide kernel's cut items are joined by quant_join_kernel: not where an item
+// is cut into more than 16 parts, which four waves per row read faster (one context of
+// 60000, 10 tokens: 52.8 us against 66.2; 60 tokens 101 and 103; 4 x 60 over 10240 72.4
+// and 71.7; 64 x 16 over 300 34.3 and 25.7).
+static bool by_runs(const PagedParams& p, const PagedShape& sh) {
+    return sh.qb == 0 && (int64_t)p.B * p.Hkv * p.tiles * 16 >= p.nwg;
 }
 
 template <typename T, int D, int BITS>
@@ -723,7 +798,10 @@ static int launch_quant(const QuantParams& p, const PagedShape& sh, hipStream_t 
     }
 #undef QATTN_NARROW
     const int rc = launch_status(sh.qb ? "quant_attn_kernel" : "quant_wide_kernel");
-    return rc ? rc : launch_merge<T, D>(p, st);
+    if (rc) return rc;
+    if (!by_runs(p, sh)) return launch_merge<T, D>(p, st);
+    hipLaunchKernelGGL((quant_join_kernel<T, D>), dim3(p.nwg * (DenseTile<T, D>::kBM / kJoinRows<D>)), block, 0, st, p);
+    return launch_status("quant_join_kernel");
 }
 
 template <typename T, int BITS>
@@ -783,6 +861,8 @@ int qattn_prefix_quant_fwd(const void* q, const int64_t q_stride[3], const void*
         set_error("scale strides must be non-negative and a cache's scales span less than 2^32 rows");
         return QATTN_ERR_LAYOUT;
     }
+    if (by_runs(p, plan.shape))
+        p.cuts = (RunStart*)((char*)workspace + paged_space(batch, plan.nwg, plan.shape, head_dim).cuts);
     p.ks = (const uint8_t*)k_scale, p.vs = (const uint8_t*)v_scale;
     p.ss_head = ss[2];
     // (one page, one slot: the stride is not used)
