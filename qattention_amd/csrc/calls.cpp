@@ -102,9 +102,15 @@ struct Call {
         for (size_t i = 0; i + 1 < st.size(); ++i) outer |= st[i];
         return st.back() == 1 && !(outer & 7) && !((uintptr_t)t.data_ptr() & 15);
     }
+    // Runs of bytes of a quantised cache.
+    bool bytes(PyObject* o, int64_t dim, const Tensor*& t) {
+        type = at::kByte;
+        return plain(o, t) && t->dim() == dim && t->numel() && t->scalar_type() == at::kByte && t->strides().back() == 1;
+    }
     // Caches that are written: of one shape, no stride of 0, not the same memory.
-    bool caches(PyObject* ok, PyObject* ov, int64_t dim, const Tensor*& k, const Tensor*& v) {
-        if (!rows(ok, dim, k) || !rows(ov, dim, v) || k->sizes() != v->sizes() || k->data_ptr() == v->data_ptr())
+    bool caches(PyObject* ok, PyObject* ov, int64_t dim, const Tensor*& k, const Tensor*& v, bool u8 = false) {
+        if (!(u8 ? bytes(ok, dim, k) && bytes(ov, dim, v) : rows(ok, dim, k) && rows(ov, dim, v)) ||
+            k->sizes() != v->sizes() || k->data_ptr() == v->data_ptr())
             return false;
         for (const Tensor* t : {k, v})
             for (int64_t s : t->strides())
@@ -131,7 +137,8 @@ struct Call {
         if (PyErr_Occurred()) return PyErr_Clear(), false;
         return true;
     }
-    int32_t code() const { return type == at::kHalf ? 0 : 1; }
+    // QATTN_DTYPE_F16, _BF16, _U8
+    int32_t code() const { return type == at::kHalf ? 0 : type == at::kByte ? 2 : 1; }
     at::TensorOptions options(at::ScalarType t) const {
         return at::TensorOptions().dtype(t).device(at::Device(at::kCUDA, (at::DeviceIndex)device));
     }
@@ -357,7 +364,8 @@ PyObject* compact(PyObject*, PyObject* const* a, Py_ssize_t n) {
         const Tensor *Kc, *Vc, *table, *ctx, *path;
         if (n != 5 || !THPVariable_CheckExact(a[0])) return none();
         const int64_t dim = THPVariable_Unpack(a[0]).dim();
-        if ((dim != 4 && dim != 5) || !c.caches(a[0], a[1], dim, Kc, Vc) || !c.ints(a[2], 2, table) ||
+        const bool u8 = THPVariable_Unpack(a[0]).scalar_type() == at::kByte;
+        if ((dim != 4 && dim != 5) || !c.caches(a[0], a[1], dim, Kc, Vc, u8) || !c.ints(a[2], 2, table) ||
             !c.ints(a[3], 1, ctx) || !c.ints(a[4], 2, path))
             return none();
         const int64_t B = ctx->size(0);
@@ -387,7 +395,8 @@ PyObject* copy(PyObject*, PyObject* const* a, Py_ssize_t n) {
         const Tensor *Kc, *Vc, *src, *dst;
         if (n != 4 || !THPVariable_CheckExact(a[0])) return none();
         const int64_t dim = THPVariable_Unpack(a[0]).dim();
-        if ((dim != 4 && dim != 5) || !c.caches(a[0], a[1], dim, Kc, Vc) || !c.ints(a[2], 1, src) ||
+        const bool u8 = THPVariable_Unpack(a[0]).scalar_type() == at::kByte;
+        if ((dim != 4 && dim != 5) || !c.caches(a[0], a[1], dim, Kc, Vc, u8) || !c.ints(a[2], 1, src) ||
             !c.ints(a[3], 1, dst) || src->size(0) != dst->size(0) || src->size(0) > kInt || !c.here())
             return none();
         int64_t ks[5], vs[5];

@@ -85,6 +85,8 @@ def quantized_kv_cache(
 def _check_cache(cache, written: bool):
     """The sizes of one layer's cache: (num_pages, page_size, Hkv, D, bits, addresses and
     strides of elements and of scales as the library takes them)."""
+    if not isinstance(cache, tuple) or len(cache) != 4 or not all(isinstance(t, torch.Tensor) for t in cache):
+        raise ValueError("cache must be a QuantizedKV (or such a tuple) of four tensors")
     K, V, Ks, Vs = cache
     for t in (K, V, Ks, Vs):
         if t.dtype is not torch.uint8 or t.dim() != 4:

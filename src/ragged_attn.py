@@ -5,6 +5,13 @@ from qattention_amd.paged_kv import (  # noqa: F401
     copy_kv_pages,
     prefix_attention_paged,
 )
+from qattention_amd.quantized_kv import (  # noqa: F401
+    QuantizedKV,
+    append_quantized_kv,
+    prefix_attention_quantized,
+    quantized_kv_cache,
+    read_quantized_kv,
+)
 from qattention_amd.ragged_attn import *  # noqa: F401,F403
 from qattention_amd.ragged_attn import (  # noqa: F401
     ancestor_table,
