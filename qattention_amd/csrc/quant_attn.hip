@@ -102,8 +102,9 @@ __device__ __forceinline__ uint32_t turn_in(const uint32_t (&x)[NH][N], int i, i
 // and the number of heads: a wave takes NH kv heads whose rows lie side by side in a
 // token, 128 bytes where they reach, and each load takes whole tokens: a 64-byte row by
 // itself is half a line, fetched again for the other half (64 x 5300-16000 tokens, 4
-// bits, heads of 128: 259 us with one head per wave, 154 with two, 143 of them the bare
-// loads; with whole lines per load, past the caches, the bare loads take 121).
+// bits, 8 heads of 128, 731 MB: 259 us with one head per wave, 154 with two, 143 of them
+// the bare loads; with whole lines per load 150, the loads past the caches 142, columns
+// chosen and not zeroed 131, where the bare loads take 121: 5.6 TB/s).
 //   columns  Each head has COLS = 16 / NH of the 16 columns of one S^T, put together
 //      from the heads' products with all columns of Q^T, so that the softmax is paid
 //      once for NH heads; P^T as it is serves every head's product with V (a head's
@@ -113,11 +114,15 @@ __device__ __forceinline__ uint32_t turn_in(const uint32_t (&x)[NH][N], int i, i
 //      h) % NH, turned by (g - h) COLS lanes (DPP): its row r is token turned(r, -h),
 //      where turned(r, x) moves r's group of COLS by x groups.  V's rows of head h are
 //      stored in the same order, and its columns' masks read so.
+// Loads run two steps ahead of their use in registers (three steps: the third spills,
+// 167 us became 197; dealing whole lines out through LDS instead: 147-157).
 // ---------------------------------------------------------------------------
 constexpr int kNarrowWaves = 4;             // waves of a STREAM workgroup
 constexpr int kItemWaves = 8;               // waves of a workgroup per item
 constexpr int kAhead = 3;                   // V operands read ahead of their product
 
+// Waves per SIMD that the registers are bounded for: what holds two steps' loads of two
+// heads, or of 128 dims, does not fit a third of them.
 constexpr int quant_waves(int d, int qb, int nh) { return d == 128 || nh > 1 ? 2 : qb > 1 ? 3 : 4; }
 
 // NW waves for G sets of NH kv heads.
@@ -231,7 +236,8 @@ __global__ __launch_bounds__(64 * NW)
         const char* const vb = (const char*)(p.vc + kvh * p.sk_head) + RB * vhead + VB * (lane % LPR);
         // one word per token: lanes 0 .. 31 K's, 32 .. 63 V's; two: K's, then V's, lanes
         // 32 .. 63 the second
-        const char* const sb = (const char*)(SW == 2 || lane < 32 ? p.ks : p.vs) + kvh * p.ss_head + (SW == 2 ? lane / 32 * 4 : 0);
+        const char* const sb = (const char*)(SW == 2 || lane < 32 ? p.ks : p.vs) + kvh * p.ss_head +
+                               (SW == 2 ? lane / 32 * 4 : 0);
         const char* const sb2 = (const char*)p.vs + kvh * p.ss_head + lane / 32 * 4;
         const int32_t* const pt = p.table + (int64_t)sh.seq * p.pt_cols;
 
@@ -468,9 +474,12 @@ __global__ __launch_bounds__(64 * NW)
 // quarter qd lies at place 4 n + qd of its row (a quarter-row's writes side by
 // side, no bank twice), which orders the dims of S's products (Q is read alike) and
 // of O's columns (put back where they are stored).
+// 2 x 1009 tokens over 6007, 8 bits, 8 heads of 128 for 32: 218 us, 0.91 PFLOP/s (a
+// library product of 8192^3: 1.23), 223 over 16 bits; 4 x 60 over 10240, 4 bits: 67,
+// 15 of them the first loads and the states of the 512 workgroups' cut items.
 // ---------------------------------------------------------------------------
 constexpr int kWideKeys = 64;
-constexpr int kTable = 24;
+constexpr int kTable = 24;  // blocks whose keys are looked up at once: the LDS that the buffers leave two workgroups
 
 struct QuantTable {
     uint32_t row[kTable][kWideKeys];    // offsets in 16-byte units
@@ -549,7 +558,8 @@ struct QuantKeys {
     // Piece n of the quarter to the buffer at dst.
     __device__ __forceinline__ void store(int n, const uint32_t (&r)[KW], uint32_t c, uint32_t dst) const {
         const Vec16 x = widen8<T, BITS>(r + n * W, scale_of(c));
-        *(__attribute__((address_space(3))) w4_t*)(uintptr_t)(dst + (put ^ (64 * n))) = w4_t{x.w[0], x.w[1], x.w[2], x.w[3]};
+        *(__attribute__((address_space(3))) w4_t*)(uintptr_t)(dst + (put ^ (64 * n))) =
+            w4_t{x.w[0], x.w[1], x.w[2], x.w[3]};
     }
     struct Dma {
         const QuantKeys& src;
@@ -746,6 +756,25 @@ static int pow2_part(int n, int most) {
 }
 
 // together: the heads of a token lie side by side, elements and scales.
+//
+// The choices, each with both sides measured (us a call, graphs of calls on caches that
+// no call before left in the chip's; 32 q heads for 8 kv heads of 128 where nothing else
+// is said):
+//   A workgroup per item (8 waves, nothing joined by a second launch) or runs: up to 4
+//   steps per wave where the items are few enough for 4 bits (2 x 731: 8.4, runs 9.6; 8 x
+//   1000: 9.6, 11.7; but 32 x 1000: 17.7, 16.9; past 4 steps 1 x 2000: 14.1, 9.7, 8 x
+//   2000: 15.8, 13.0) or many enough for 8 (8 x 1000: 11.3, 12.5; 32 x 1000: 20.9, 25.4;
+//   but 2 x 900: 15.7, 10.1), else up to 2.
+//   Heads of a wave (nh): as many as fill a 128-byte line (see above).
+//   Sets of heads of a workgroup (g), each to one wave, or all four waves on one set's
+//   keys (g = 1): the first saves the waves' join, the second has more and shorter parts.
+//   One head per wave takes sets from 8 steps per wave on, 8 bits: 48 x 4000-12001: 146,
+//   g = 1 176; 32 x 4000: 67, 74; 16 x 4000: 43, 42.  Several heads per wave from 16 on,
+//   4 bits: 64 x 5300-16000: 154, g = 1 171; 8 x 8000 with 32 kv heads: 77, 84; below,
+//   1 x 131072: 54.5, 43.4; 32 x 4000: 44.8, 42.0; 1 x 131072 with 4 heads of 64: 29.1, 24.2.
+//   Workgroups per CU with several heads per wave and g = 1: one (1 x 30000: 23.5, two
+//   25.1; 32 x 2000: 28.5, 30.2; 4 x 20000 with heads of 64: 25.6, 28.8): a wave's start
+//   and the join of twice the parts cost more than the second workgroup hides.
 static PagedShape quant_shape(int bits, bool together, int64_t max_rows, int64_t pairs, int hkv, int64_t capacity,
                               int head_dim) {
     const int steps = (bits == 4 ? pairs <= 128 : pairs >= 64) ? 4 : 2;
@@ -753,7 +782,8 @@ static PagedShape quant_shape(int bits, bool together, int64_t max_rows, int64_t
     if (max_rows <= 32) {
         const int qb = max_rows <= 16 ? 1 : 2, row_bytes = head_dim * bits / 8;
         int nh = 1;
-        while (together && nh < 4 && 2 * nh * row_bytes <= 128 && max_rows * 2 * nh <= 16 && hkv % (2 * nh) == 0) nh *= 2;
+        while (together && nh < 4 && 2 * nh * row_bytes <= 128 && max_rows * 2 * nh <= 16 && hkv % (2 * nh) == 0)
+            nh *= 2;
         int per_cu = quant_waves(head_dim, qb, nh);
         int g = max_rows <= 16 ? pow2_part(hkv / nh, kNarrowWaves) : 1;
         if (pairs / (nh * g) * ((capacity + 31) / 32) < (nh > 1 ? 16 : 8) * 256 * per_cu) g = 1;

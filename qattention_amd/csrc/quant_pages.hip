@@ -4,8 +4,11 @@
 //
 // A thread has 8 elements of K and of V at a time, a quad of lanes a block of 32
 // with its scale.  Both directions are bound by HBM in large calls (16 bits per
-// element on one side, 4.25 or 8.25 on the other) and by their launch and one
-// chain of dependent loads (offsets, context length, page, row) in small ones.
+// element on one side, 4.25 or 8.25 on the other: 8 x 4003 rows of 8 heads of 128
+// in 4 bits, 166 MB, are written in 31.5 us, 5.3 TB/s, what a copy reaches; 16
+// contexts of 10007 read back, 835 MB, in 144) and by their launch and one chain of
+// dependent loads (offsets, context length, page, row) in small ones (32 x 1 rows:
+// 2.7 and 2.5 us).
 #include <algorithm>
 
 #include "qattn_common.h"
@@ -54,7 +57,13 @@ __device__ __forceinline__ int32_t rows_of(const QuantPageParams& p, int seq, in
 // The workgroup's packed rows: first + r, r < count, of sequence seq(r) at
 // position pos(r).  PACKED: `rows` rows of whichever sequences (seq -1: of none);
 // otherwise a run of one sequence's rows.
-constexpr int kUnits = 2;                                   // chunks of K and of V per thread and round
+// Chunks of K and of V per thread and round.  (Two keep more loads in flight, 16 x 10007
+// rows read back: 144 us, with one 151, with four 151.  Calls of fewer than kFull
+// workgroups get half the rows per workgroup and leave the second chunk out: append 1 x
+// 731: 3.2 us, with two 4.1; 63 x 1 and one of 2000: 5.3, 5.8; from there on the other
+// way round, 7 x 1 and one of 8000: 11.9, 11.1.)
+constexpr int kUnits = 2;
+constexpr int kFull = 1024;
 constexpr int kMaxRows = kUnits * kRowThreads / 4;          // of a workgroup: 4 chunks a row at least
 template <bool PACKED, bool APPEND>
 struct WorkRows {
@@ -313,14 +322,18 @@ static int fill_quant(QuantPageParams& p, const void* kc, const void* vc, const 
     p.max_seqlen = (int32_t)std::min<int64_t>(cu ? max_seqlen : 1, total_tokens);
     p.chunks = hkv * (head_dim / 8);
     p.dvshift = head_dim == 32 ? 2 : head_dim == 64 ? 3 : 4;
-    p.rows = std::max(1, kUnits * kRowThreads / p.chunks);
+    const bool full = total_tokens * p.chunks >= (int64_t)kFull * kUnits * kRowThreads;
+    p.rows = std::max(1, (full ? kUnits : 1) * kRowThreads / p.chunks);
     p.pdiv = make_divider(page_size);
     p.cdiv = make_divider(p.chunks);
     return QATTN_OK;
 }
 
 // Workgroups of one sequence's rows each, or of packed rows, of whichever
-// sequences, where most sequences are far shorter than the longest.
+// sequences, where most sequences are far shorter than the longest.  (Packed ones
+// look every sequence up: append 32 x 1 rows 3.7 us, by sequences 2.7; 8 x 4003 36.9
+// and 33.3.  By sequences most workgroups find nothing: 63 x 1 and one of 2000 16.0,
+// packed 5.8; 7 x 1 and one of 8000 15.3 and 11.1; 31 x 1 and one of 300 4.4 and 3.9.)
 static int row_grid(QuantPageParams& p, int32_t longest, bool& packed, uint32_t& grid) {
     p.runs = std::max(1, (int32_t)(((int64_t)longest + p.rows - 1) / p.rows));
     p.rdiv = make_divider(p.runs);
