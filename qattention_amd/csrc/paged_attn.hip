@@ -262,7 +262,7 @@ __global__ __launch_bounds__(64 * NW)
         }
 
         join_waves<T, D, QB, NW, HW>(
-            p, sh, part, query_of, m_run, l_run, oacc, vlds, ml, [](int ch) { return ch; }, HW,
+            p, sh, part, query_of, m_run, l_run, oacc, vlds, ml, [](int ch) { return ch; }, HW * ROWS,
             [&](int r) { return wave / WPH * ROWS + r; });
         __syncthreads();  // the LDS is free for the next item
         sh.u += STREAM ? b1 - b0 : 1;

@@ -251,14 +251,14 @@ __device__ __forceinline__ SeqWork next_part(const PagedParams& p, Share& sh, Pa
 // the workspace.  oacc element i of tile dt is row l16, column 16 dt + 4 lq + i;
 // column chunk ch (8 columns) holds head dims 8 dims_of(ch) .. + 7; row r's state lies
 // at row state_of(r) of its part's in the workspace.  lds: NW x 32 x D elements of 16
-// bits that no wave uses any more after the first barrier.
+// bits that no wave uses any more after the first barrier.  part_rows: rows of a part.
 // ---------------------------------------------------------------------------
 template <typename T, int D, int QB, int NW, int HW, class Query, class Dims, class State>
 __device__ __forceinline__ void join_waves(const PagedParams& p, const Share& sh, const Part& part, Query query_of,
                                            const float (&m_run)[QB], float (&l_run)[QB], const f4_t (&oacc)[QB][D / 16],
-                                           uint16_t* lds, float (&ml)[2][NW][16 * QB], Dims dims_of, int heads,
+                                           uint16_t* lds, float (&ml)[2][NW][16 * QB], Dims dims_of, int part_rows,
                                            State state_of) {
-    constexpr int DV = D / 8, ND = D / 16, WBLK = 32 * D, ROWS = 16 * QB, WPH = NW / HW;
+    constexpr int DV = D / 8, ND = D / 16, WBLK = 32 * D, WPH = NW / HW;
     const int tid = threadIdx.x;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int lane = tid & 63;
@@ -309,7 +309,7 @@ __device__ __forceinline__ void join_waves(const PagedParams& p, const Share& sh
                 st16(p.o + qrow * p.so_t + qh * p.so_h + dim, pack8<T>(acc));
                 if (p.lse && ch == 0) p.lse[qrow * p.sl_t + qh * p.sl_h] = (mc + fast_log2(l)) * kLn2;
             } else {
-                const int64_t r = part_slot(sh) * heads * ROWS + state_of(16 * q + row);
+                const int64_t r = part_slot(sh) * part_rows + state_of(16 * q + row);
                 if (ch == 0) {
                     p.part_m[r] = m * p.scale_log2;
                     p.part_l[r] = l;

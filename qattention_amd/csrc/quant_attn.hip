@@ -105,10 +105,11 @@ __device__ __forceinline__ uint32_t turn_in(const uint32_t (&x)[NH][N], int i, i
 // bits, 8 heads of 128, 731 MB: 259 us with one head per wave, 154 with two, 143 of them
 // the bare loads; with whole lines per load 150, the loads past the caches 142, columns
 // chosen and not zeroed 131, where the bare loads take 121: 5.6 TB/s).
-//   columns  Each head has COLS = 16 / NH of the 16 columns of one S^T, put together
-//      from the heads' products with all columns of Q^T, so that the softmax is paid
-//      once for NH heads; P^T as it is serves every head's product with V (a head's
-//      columns of the others' products are not read, and no column touches another).
+//   columns  Where a head's rows fit, each head has COLS = 16 / NH of the 16 columns of
+//      one S^T, put together from the heads' products with all columns of Q^T, so that the
+//      softmax is paid once for NH heads; P^T as it is serves every head's product with V
+//      (a head's columns of the others' products are not read, and no column touches
+//      another).  Otherwise two heads have a tile each.
 //   rows  Load j of a key tile holds tokens COLS j .. + COLS - 1, lanes h COLS .. their
 //      rows of head h.  Head h's operand has them in its lanes g COLS .. from load (g -
 //      h) % NH, turned by (g - h) COLS lanes (DPP): its row r is token turned(r, -h),
@@ -125,7 +126,8 @@ constexpr int kAhead = 3;                   // V operands read ahead of their pr
 // heads, or of 128 dims, does not fit a third of them.
 constexpr int quant_waves(int d, int qb, int nh) { return d == 128 || nh > 1 ? 2 : qb > 1 ? 3 : 4; }
 
-// NW waves for G sets of NH kv heads.
+// NW waves for G sets of NH kv heads.  (NH > 1: QB = 1 is one tile of columns for all of
+// them, QB = NH a tile each.)
 template <typename T, int D, int BITS, int QB, int NW, int NH, int G, bool STREAM>
 __global__ __launch_bounds__(64 * NW)
     __attribute__((amdgpu_waves_per_eu(quant_waves(D, QB, NH)))) void quant_attn_kernel(QuantParams p) {
@@ -142,17 +144,20 @@ __global__ __launch_bounds__(64 * NW)
     constexpr int NV = 32 / TPI;            // V loads per lane and step
     constexpr int SUB = VB / BITS;          // chunks of 8 elements per load
     constexpr int WBLK = 32 * D;            // elements of a head's V block
-    constexpr int ROWS = 16 * QB;
-    constexpr int COLS = 16 / NH;           // columns of a head
+    constexpr bool OWN = NH > 1 && QB == NH;  // a tile of columns per head
+    constexpr int ROWS = NH > 1 ? 16 : 16 * QB;  // of an item
+    constexpr int COLS = 16 / NH;           // tokens of a K load; columns of a head, where heads share a tile
+    constexpr int HC = OWN ? 16 : COLS;     // columns of a head
+    constexpr int NO = OWN ? NH : QB * NH;  // tiles of O^T
     constexpr int WPH = NW / G;             // waves of a set of heads
     constexpr int KEYS = 32 * WPH;          // of a unit
     constexpr bool ONCE = NH * RB >= 128;   // a load's tokens are whole lines: past the caches
     static_assert(LPR * SUB == DV && NV * TPI == 32 && TPI % 8 == 0 && NC * BITS / 4 == KW, "a step is 32 rows");
-    static_assert(NH == 1 || (QB == 1 && NH * RB <= 128), "one tile of columns");
+    static_assert(NH == 1 || ((QB == 1 || OWN) && NH * RB <= 128), "one tile of columns, or one per head");
     // The waves' V blocks; after the key loop, the waves' numerators of one
     // row block (NW x 16 rows x D floats, the size of one head's).
     __shared__ __attribute__((aligned(4096))) uint16_t vlds[NW * NH * WBLK];  // (16 rows: bits of an address)
-    __shared__ float ml[2][NW][ROWS];
+    __shared__ float ml[2][NW][16 * QB];
 
     Share sh{};
     if constexpr (STREAM) {
@@ -201,12 +206,12 @@ __global__ __launch_bounds__(64 * NW)
         const int tile = part.tile, b0 = part.b0, b1 = part.b1, ctx = sw.ctx;
         const int kvh = (part.group * G + wave / WPH) * NH;  // the wave's first head
 
-        // column r of the wave's tile: a row of head kvh + r / COLS (all of the tile's
+        // column r of the wave's tiles: a row of head kvh + r / HC (all of the tiles'
         // rows, where the wave has one head)
         auto query_of = [&](int r, int64_t& qrow, int& qh) {
-            const int rr = NH == 1 ? tile * 16 * QB + r : r % COLS;
+            const int rr = NH == 1 ? tile * 16 * QB + r : r % HC;
             const int tok = divide(rr, p.gdiv);
-            qh = (kvh + (NH == 1 ? 0 : r / COLS)) * p.group + (rr - tok * p.group);
+            qh = (kvh + (NH == 1 ? 0 : r / HC)) * p.group + (rr - tok * p.group);
             qrow = (int64_t)sw.s0 + tok;
             return rr < sw.rows;
         };
@@ -225,9 +230,9 @@ __global__ __launch_bounds__(64 * NW)
             }
         }
         float m_run[QB], l_run[QB];
-        f4_t oacc[QB * NH][ND];
+        f4_t oacc[NO][ND];
 #pragma unroll
-        for (int b = 0; b < QB * NH; ++b)
+        for (int b = 0; b < NO; ++b)
 #pragma unroll
             for (int i = 0; i < ND; ++i) oacc[b][i] = f4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -320,8 +325,9 @@ __global__ __launch_bounds__(64 * NW)
                     const Vec16 x = widen8<T, BITS>(r.v[n] + i * (BITS / 4), vscale[n]);
                     *(__attribute__((address_space(3))) w4_t*)(uintptr_t)at = w4_t{x.w[0], x.w[1], x.w[2], x.w[3]};
                 }
-            // scores: every head's K with all columns, each column from its own head (no
-            // zeros in the other columns: 0 times what is no number is none either)
+            // scores: every head's K with its own tile of columns; where heads share one, with
+            // all columns, each column from its own head (no zeros in the other columns: 0
+            // times what is no number is none either)
             f4_t s[QB][2];
 #pragma unroll
             for (int t = 0; t < 2; ++t)
@@ -337,12 +343,16 @@ __global__ __launch_bounds__(64 * NW)
                     for (int c = 0; c < NC; ++c) {
                         const Vec16 k = widen8<T, BITS>(kw + c * (BITS / 4), kscale[t][h]);
 #pragma unroll
-                        for (int q = 0; q < QB; ++q) x[q] = MfmaOps<T>::mma(k, qf[q][c], x[q]);
+                        for (int q = 0; q < QB; ++q)
+                            if (!OWN || q == h) x[q] = MfmaOps<T>::mma(k, qf[q][c], x[q]);
                     }
 #pragma unroll
-                    for (int q = 0; q < QB; ++q)
+                    for (int q = 0; q < QB; ++q) {
+                        if (OWN && q != h) continue;
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) s[q][t][i] = h == 0 || l16 / COLS == h ? x[q][i] : s[q][t][i];
+                        for (int i = 0; i < 4; ++i)
+                            s[q][t][i] = OWN || h == 0 || l16 / COLS == h ? x[q][i] : s[q][t][i];
+                    }
                 }
             issue(r, b + 2, page);
             page = after;
@@ -355,7 +365,7 @@ __global__ __launch_bounds__(64 * NW)
             for (int q = 0; q < QB; ++q) {
                 // lane: rows 16 t + 4 lq + i of column l16
                 if (mask != 0xffffffffu) {
-                    uint32_t mine = mask >> turned(4 * lq, NH - l16 / COLS);
+                    uint32_t mine = mask >> turned(4 * lq, NH - (OWN ? q : l16 / COLS));
                     asm volatile("" : "+v"(mine));  // (eight tests of one word, no eight lane masks)
 #pragma unroll
                     for (int t = 0; t < 2; ++t)
@@ -395,11 +405,9 @@ __global__ __launch_bounds__(64 * NW)
             for (int q = 0; q < QB; ++q) moved |= alpha[q] != 1.f;
             if (__any(moved)) {
 #pragma unroll
-                for (int q = 0; q < QB; ++q)
+                for (int o = 0; o < NO; ++o)
 #pragma unroll
-                    for (int h = 0; h < NH; ++h)
-#pragma unroll
-                        for (int dt = 0; dt < ND; ++dt) oacc[q + h][dt] *= alpha[q];
+                    for (int dt = 0; dt < ND; ++dt) oacc[o][dt] *= alpha[QB == 1 ? 0 : o];
             }
             auto v_operand = [&](int i) {  // d-tile i % ND of head i / ND
                 typedef short v4s __attribute__((ext_vector_type(4)));
@@ -418,8 +426,11 @@ __global__ __launch_bounds__(64 * NW)
             for (int i = 0; i < NT; ++i) {
                 const Vec16 v = va[i % AHEAD];
 #pragma unroll
-                for (int q = 0; q < QB; ++q)
-                    oacc[q + i / ND][i % ND] = MfmaOps<T>::mma(v, pf[q], oacc[q + i / ND][i % ND]);
+                for (int q = 0; q < QB; ++q) {
+                    if (OWN && q != i / ND) continue;
+                    const int o = OWN ? q : q + i / ND;
+                    oacc[o][i % ND] = MfmaOps<T>::mma(v, pf[q], oacc[o][i % ND]);
+                }
                 if (i + AHEAD < NT) va[i % AHEAD] = v_operand(i + AHEAD);
                 __builtin_amdgcn_sched_barrier(0);
             }
@@ -443,9 +454,9 @@ __global__ __launch_bounds__(64 * NW)
         }
         auto dims_of = [](int ch) { return ch % LPR * SUB + ch / LPR; };
         auto state_of = [&](int r) {
-            return (wave / WPH * NH + (NH == 1 ? 0 : r / COLS)) * ROWS + (NH == 1 ? r : r % COLS);
+            return (wave / WPH * NH + (NH == 1 ? 0 : r / HC)) * ROWS + (NH == 1 ? r : r % HC);
         };
-        if constexpr (NH > 1) {
+        if constexpr (NH > 1 && !OWN) {
             // each column of the head that it belongs to
             f4_t own[1][ND];
 #pragma unroll
@@ -456,9 +467,9 @@ __global__ __launch_bounds__(64 * NW)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) own[0][dt][i] = l16 / COLS == h ? oacc[h][dt][i] : own[0][dt][i];
             }
-            join_waves<T, D, 1, NW, G>(p, sh, part, query_of, m_run, l_run, own, vlds, ml, dims_of, NH * G, state_of);
+            join_waves<T, D, 1, NW, G>(p, sh, part, query_of, m_run, l_run, own, vlds, ml, dims_of, NH * G * ROWS, state_of);
         } else {
-            join_waves<T, D, QB, NW, G>(p, sh, part, query_of, m_run, l_run, oacc, vlds, ml, dims_of, NH * G, state_of);
+            join_waves<T, D, QB, NW, G>(p, sh, part, query_of, m_run, l_run, oacc, vlds, ml, dims_of, NH * G * ROWS, state_of);
         }
         __syncthreads();  // the LDS is free for the next item
         sh.u += STREAM ? b1 - b0 : 1;
@@ -772,6 +783,10 @@ static int pow2_part(int n, int most) {
 //   g = 1 176; 32 x 4000: 67, 74; 16 x 4000: 43, 42.  Several heads per wave from 16 on,
 //   4 bits: 64 x 5300-16000: 154, g = 1 171; 8 x 8000 with 32 kv heads: 77, 84; below,
 //   1 x 131072: 54.5, 43.4; 32 x 4000: 44.8, 42.0; 1 x 131072 with 4 heads of 64: 29.1, 24.2.
+//   9 .. 16 rows: two heads with a tile of columns each where several sets get 8 steps per
+//   wave (48 with heads of 128, whose registers spill), else one head, 4 tokens, 4 bits: 64
+//   x 16000 with heads of 64 148, one head 183; 40 x 8000 of 64 63, 67, of 32 44, 54; 24 x
+//   8000 of 64 in 8 bits 58, 67; of 128 64 x 5300-16000 167, 182, but 24 x 16000 114, 112.
 //   Workgroups per CU with several heads per wave and g = 1: one (1 x 30000: 23.5, two
 //   25.1; 32 x 2000: 28.5, 30.2; 4 x 20000 with heads of 64: 25.6, 28.8): a wave's start
 //   and the join of twice the parts cost more than the second workgroup hides.
@@ -784,11 +799,19 @@ static PagedShape quant_shape(int bits, bool together, int64_t max_rows, int64_t
         int nh = 1;
         while (together && nh < 4 && 2 * nh * row_bytes <= 128 && max_rows * 2 * nh <= 16 && hkv % (2 * nh) == 0)
             nh *= 2;
-        int per_cu = quant_waves(head_dim, qb, nh);
-        int g = max_rows <= 16 ? pow2_part(hkv / nh, kNarrowWaves) : 1;
-        if (pairs / (nh * g) * ((capacity + 31) / 32) < (nh > 1 ? 16 : 8) * 256 * per_cu) g = 1;
+        bool own = together && nh == 1 && qb == 1 && 2 * row_bytes <= 128 && hkv % 2 == 0;
+        int per_cu, g;
+        for (;; own = false) {
+            const int n = own ? 2 : nh;
+            per_cu = quant_waves(head_dim, qb, n);
+            g = max_rows <= 16 ? pow2_part(hkv / n, kNarrowWaves) : 1;
+            const int least = own ? (head_dim == 128 ? 48 : 8) : n > 1 ? 16 : 8;
+            if (pairs / (n * g) * ((capacity + 31) / 32) < least * 256 * per_cu) g = 1;
+            if (!own || g > 1) break;
+        }
+        if (own) nh = 2;
         if (nh > 1 && g == 1) per_cu = 1;
-        return {qb, qb == 1 ? 4 : 5, 7 - __builtin_ctz((unsigned)g), nh * g, per_cu, false, nh};
+        return {own ? 2 : qb, qb == 1 ? 4 : 5, 7 - __builtin_ctz((unsigned)g), nh * g, per_cu, false, nh};
     }
     return {0, 7, 6, 1, 2, false, 1};
 }
@@ -813,17 +836,19 @@ static int launch_quant(const QuantParams& p, const PagedShape& sh, hipStream_t 
 #define QATTN_NARROW(QB, NH, G) \
     hipLaunchKernelGGL((quant_attn_kernel<T, D, BITS, QB, kNarrowWaves, NH, G, true>), grid, block, 0, st, p)
     const int sets = sh.heads / sh.wave_heads;
-    switch (sh.qb == 0 ? 0 : sh.qb == 2 ? 1 : 10 * sh.wave_heads + sets) {
+    switch (sh.qb == 0 ? 0 : 100 * sh.qb + 10 * sh.wave_heads + sets) {
         case 0: hipLaunchKernelGGL((quant_wide_kernel<T, D, BITS>), grid, block, 0, st, p); break;
-        case 1: QATTN_NARROW(2, 1, 1); break;
-        case 11: QATTN_NARROW(1, 1, 1); break;
-        case 12: QATTN_NARROW(1, 1, 2); break;
-        case 14: QATTN_NARROW(1, 1, 4); break;
-        case 21: QATTN_NARROW(1, NH2, 1); break;
-        case 22: QATTN_NARROW(1, NH2, 2); break;
-        case 24: QATTN_NARROW(1, NH2, 4); break;
-        case 41: QATTN_NARROW(1, NH4, 1); break;
-        case 42: QATTN_NARROW(1, NH4, 2); break;
+        case 211: QATTN_NARROW(2, 1, 1); break;
+        case 222: QATTN_NARROW(NH2, NH2, 2); break;
+        case 224: QATTN_NARROW(NH2, NH2, 4); break;
+        case 111: QATTN_NARROW(1, 1, 1); break;
+        case 112: QATTN_NARROW(1, 1, 2); break;
+        case 114: QATTN_NARROW(1, 1, 4); break;
+        case 121: QATTN_NARROW(1, NH2, 1); break;
+        case 122: QATTN_NARROW(1, NH2, 2); break;
+        case 124: QATTN_NARROW(1, NH2, 4); break;
+        case 141: QATTN_NARROW(1, NH4, 1); break;
+        case 142: QATTN_NARROW(1, NH4, 2); break;
         default: QATTN_NARROW(1, NH4, 4);
     }
 #undef QATTN_NARROW

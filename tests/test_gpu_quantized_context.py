@@ -184,6 +184,44 @@ def test_missing_pages_and_lengths_past_the_table(n, bits):
 
 
 @pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("dtype", [FP16, BF16])
+@pytest.mark.parametrize("B,ctx,n,Hq,Hkv,D", [
+    (24, 8000, 4, 32, 8, 64), (40, 8000, 5, 8, 4, 64), (64, 9000, 12, 4, 4, 32), (33, 7000, 3, 16, 4, 32),
+    (66, 14000, 5, 16, 8, 128), (64, 14000, 13, 4, 4, 128), (24, 8000, 16, 6, 6, 64),
+])
+def test_short_drafts_over_long_contexts(B, ctx, n, Hq, Hkv, D, dtype, bits):
+    """9 to 16 rows: heads in tiles of their own.  Most sequences read the same pages, to
+    lengths of their own; the first one's hold a block without a number in K and in V."""
+    from qattention_amd import prefix_attention_quantized
+    own = 777
+    cache, table, _, rows = context([own, ctx, ctx - 1000], 16, Hkv, D, bits, 600 + B + D)
+    table = table[torch.tensor([0] + [1 + s % 2 for s in range(1, B)], device=DEV)].contiguous()
+    lens = [own] + [ctx - 1000 - (37 * s * s) % (ctx // 2) if s % 9 else s % 4 for s in range(1, B)]
+    toks = [n] + [n - s % 3 if s % 7 else 0 for s in range(1, B)]
+    cache.K_scale[int(table[0, 100 // 16]), 100 % 16, 1, 0] = 255
+    cache.V_scale[int(table[0, 200 // 16]), 200 % 16, 0, 0] = 255
+    Q = queries(sum(toks), Hq, D, dtype, 601)
+    say("drafts", B, ctx, n, Hq, Hkv, D, dtype, bits)
+    n_ctx = torch.tensor(lens, dtype=torch.int32, device=DEV)
+    O, L = prefix_attention_quantized(Q, cache, table, n_ctx, offsets(toks))
+    kv = [rows[0]] + [tuple(x[:m] for x in rows[1 + s % 2]) for s, m in zip(range(1, B), lens[1:])]
+    o, lse, to, tl = reference(Q, kv, toks)
+    g = Hq // Hkv
+    bad = torch.zeros_like(O, dtype=torch.bool)
+    bad[:n, g:2 * g] = True     # (K of head 1)
+    bad[:n, :g, :32] = True     # (V of head 0)
+    assert torch.equal(torch.isnan(O), bad)
+    bad_lse = torch.zeros_like(L, dtype=torch.bool)
+    bad_lse[:n, g:2 * g] = True
+    assert torch.equal(torch.isnan(L), bad_lse)
+    some = ~bad[..., 0]
+    check(O.masked_fill(bad, 0), L.masked_fill(bad_lse, 0),
+          (o.masked_fill(bad, 0), lse.masked_fill(bad_lse, 0), to.masked_fill(bad, 0), tl.masked_fill(bad_lse, 0)))
+    again = prefix_attention_quantized(Q, cache, table, n_ctx, offsets(toks))
+    assert torch.equal(again[0][some], O[some]) and torch.equal(again[1][some], L[some])
+
+
+@pytest.mark.parametrize("bits", [4, 8])
 @pytest.mark.parametrize("n,ctx", [(1, [200, 300]), (5, [200, 300]), (50, [200, 300]), (1, [1500, 2900]),
                                    (1, [130] + 39 * [6000])])
 def test_no_numbers(n, ctx, bits):
