@@ -105,7 +105,8 @@ struct Call {
     // Runs of bytes of a quantised cache.
     bool bytes(PyObject* o, int64_t dim, const Tensor*& t) {
         type = at::kByte;
-        return plain(o, t) && t->dim() == dim && t->numel() && t->scalar_type() == at::kByte && t->strides().back() == 1;
+        return plain(o, t) && t->dim() == dim && t->numel() && t->scalar_type() == at::kByte &&
+               t->strides().back() == 1;
     }
     // Caches that are written: of one shape, no stride of 0, not the same memory.
     bool caches(PyObject* ok, PyObject* ov, int64_t dim, const Tensor*& k, const Tensor*& v, bool u8 = false) {

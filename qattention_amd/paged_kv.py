@@ -306,9 +306,9 @@ def copy_kv_pages(K_cache: torch.Tensor, V_cache: torch.Tensor, src_pages: _Page
     forked sequence, pages gathered to free others).
 
     K_cache, V_cache: [layers, pages, page_size, Hkv, D] or one layer's [pages,
-    page_size, Hkv, D], fp16, bf16 or the bytes of a quantised cache.  The copies run side by side, so no page may be the
-    destination of two or the destination of one and the source of another:
-    lists on the host are checked for that (ValueError); of lists on the GPU,
+    page_size, Hkv, D], fp16, bf16 or the bytes of a quantised cache.  The copies run
+    side by side, so no page may be the destination of two or the destination of one
+    and the source of another: lists on the host are checked for that (ValueError); of lists on the GPU,
     pairs with a page outside the cache are passed over, the rest is the
     caller's to keep."""
     if _lib.calls().copy(K_cache, V_cache, src_pages, dst_pages):
