@@ -485,7 +485,7 @@ __global__ __launch_bounds__(64 * NW)
 // quarter qd lies at place 4 n + qd of its row (a quarter-row's writes side by
 // side, no bank twice), which orders the dims of S's products (Q is read alike) and
 // of O's columns (put back where they are stored).
-// 2 x 1009 tokens over 6007, 8 bits, 8 heads of 128 for 32: 218 us, 0.91 PFLOP/s (a
+// 2 x 1009 tokens over 6007, 8 bits, 8 heads of 128 for 32: 202-211 us, 0.97 PFLOP/s (a
 // library product of 8192^3: 1.23), 223 over 16 bits; 4 x 60 over 10240, 4 bits: 67,
 // 15 of them the first loads and the states of the 512 workgroups' cut items.
 // ---------------------------------------------------------------------------
