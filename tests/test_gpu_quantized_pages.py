@@ -247,3 +247,34 @@ def test_moves_of_bytes():
         for k, v in ((cache.K, cache.V), (cache.K_scale, cache.V_scale)):
             qa.copy_kv_pages(k, v, src, dst)
         assert all(torch.equal(a, b) for a, b in zip(wide, want))
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+def test_offsets_past_32_bits(bits):
+    """Pages 5 GiB from the first one: written, moved, copied and read back."""
+    import qattention_amd as qa
+    ps, Hkv, D, n = 16, 2, 128, 40
+    widths = [Hkv * D * bits // 8] * 2 + [Hkv * D // 32] * 2
+    room = torch.empty((5 << 30) + (1 << 20), dtype=torch.uint8, device=DEV)
+    step = (5 << 30) // 4
+    cache = qa.QuantizedKV(*(room.as_strided((5, ps, Hkv, w // Hkv), (step, w, w // Hkv, 1), i << 16)
+                             for i, w in enumerate(widths)))
+    for t in cache:
+        t.zero_()
+    table = torch.tensor([[4, 0, 3]], dtype=torch.int32, device=DEV)
+    K, V = rows(n, Hkv, D, FP16, 20).to(DEV), rows(n, Hkv, D, FP16, 21).to(DEV)
+    zero = torch.zeros(1, dtype=torch.int32, device=DEV)
+    say("far", bits)
+    assert qa.append_quantized_kv(K, V, cache, table, zero, offsets([n])).tolist() == [n]
+    want = [quant64.decode(*quant64.encode(x, bits), bits).float().to(BF16) for x in (K, V)]
+    for x, w in zip(qa.read_quantized_kv(cache, table, zero, offsets([n]), dtype=BF16), want):
+        assert same(x.cpu(), w)
+    # rows 1, 33 and 39 to places 0, 1 and 2; then page 4 to page 1
+    path = torch.tensor([[1, 33, 39]], dtype=torch.int32, device=DEV)
+    for k, v in ((cache.K, cache.V), (cache.K_scale, cache.V_scale)):
+        assert qa.compact_paged_kv(k, v, table, zero, path).tolist() == [3]
+        qa.copy_kv_pages(k, v, [4], [1])
+    other = torch.tensor([[1]], dtype=torch.int32, device=DEV)
+    for t in (table, other):
+        for x, w in zip(qa.read_quantized_kv(cache, t, zero, offsets([ps]), dtype=BF16), want):
+            assert same(x.cpu(), torch.cat([w[[1, 33, 39]], w[3:ps]]))
