@@ -205,10 +205,20 @@ int qattn_debug_walk(int32_t *out);
 
 /*
  * Name of the last kernel that a call of this thread launched ("" before the
- * first; the group kernel's with its heads or lanes per slot), for tests of
- * the rules that choose one.
+ * first; the group kernel's with its heads or lanes per slot; a call over a
+ * quantised cache leaves its main kernel's, with the row tiles, heads and sets
+ * of heads that it was built for), for tests of the rules that choose one.
  */
 const char *qattn_debug_last_kernel(void);
+
+/*
+ * The name that qattn_prefix_quant_fwd with such arguments leaves there, without
+ * a launch ("": it launches nothing).  together: the heads of a token lie side by
+ * side, elements and scales.
+ */
+const char *qattn_debug_quant_kernel(int32_t batch, int32_t max_seqlen, int64_t total_tokens,
+                                     int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
+                                     int32_t pt_cols, int32_t page_size, int32_t bits, int32_t together);
 
 /*
  * Tree-verify attention with a prefix KV cache that every tree query attends

@@ -46,6 +46,7 @@ SIGNATURES = {
     "qattn_sched_info": (C.c_int, [_i64p]),
     "qattn_debug_walk": (C.c_int, [_p]),
     "qattn_debug_last_kernel": (C.c_char_p, []),
+    "qattn_debug_quant_kernel": (C.c_char_p, [_i32, _i32, _i64, _i32, _i32, _i32, _i32, _i32, _i32, _i32]),
     "qattn_tree_fwd": (C.c_int, [
         _p, _i64p, _p, _i64p, _p, _i64p, _p, _i64p, _p, _i64p,
         _p, _i32, _i32, _i64, _i32, _i32, _i32, _i32, _i32, _f32, _i32, _i32, _p]),

@@ -824,19 +824,41 @@ static bool by_runs(const PagedParams& p, const PagedShape& sh) {
     return sh.qb == 0 && (int64_t)p.B * p.Hkv * p.tiles * 16 >= p.nwg;
 }
 
+// The main kernel of a call by its name (qattn_debug_quant_kernel): 100 QB + 10 NH + G.
+static int form_of(const PagedShape& sh) {
+    return sh.qb == 0 ? 0 : 100 * sh.qb + 10 * sh.wave_heads + sh.heads / sh.wave_heads;
+}
+static const char* name_of(const PagedShape& sh) {
+    if (sh.items) return "quant_attn_kernel, a workgroup per item";
+    switch (form_of(sh)) {
+        case 0: return "quant_wide_kernel";
+        case 211: return "quant_attn_kernel, 2 tiles, 1 head";
+        case 222: return "quant_attn_kernel, 2 tiles, 2 heads, 2 sets";
+        case 224: return "quant_attn_kernel, 2 tiles, 2 heads, 4 sets";
+        case 111: return "quant_attn_kernel, 1 head";
+        case 112: return "quant_attn_kernel, 1 head, 2 sets";
+        case 114: return "quant_attn_kernel, 1 head, 4 sets";
+        case 121: return "quant_attn_kernel, 2 heads";
+        case 122: return "quant_attn_kernel, 2 heads, 2 sets";
+        case 124: return "quant_attn_kernel, 2 heads, 4 sets";
+        case 141: return "quant_attn_kernel, 4 heads";
+        case 142: return "quant_attn_kernel, 4 heads, 2 sets";
+        default: return "quant_attn_kernel, 4 heads, 4 sets";
+    }
+}
+
 template <typename T, int D, int BITS>
 static int launch_quant(const QuantParams& p, const PagedShape& sh, hipStream_t st) {
     const dim3 grid(p.nwg), block(kPagedThreads);
     if (sh.items) {
         hipLaunchKernelGGL((quant_attn_kernel<T, D, BITS, 1, kItemWaves, 1, 1, false>),
                            dim3((uint32_t)(p.B * p.tiles * p.Hkv)), dim3(64 * kItemWaves), 0, st, p);
-        return launch_status("quant_attn_kernel, a workgroup per item");
+        return launch_status(name_of(sh));
     }
     constexpr int NH2 = D * BITS / 8 <= 64 ? 2 : 1, NH4 = D * BITS / 8 <= 32 ? 4 : NH2;
 #define QATTN_NARROW(QB, NH, G) \
     hipLaunchKernelGGL((quant_attn_kernel<T, D, BITS, QB, kNarrowWaves, NH, G, true>), grid, block, 0, st, p)
-    const int sets = sh.heads / sh.wave_heads;
-    switch (sh.qb == 0 ? 0 : 100 * sh.qb + 10 * sh.wave_heads + sets) {
+    switch (form_of(sh)) {
         case 0: hipLaunchKernelGGL((quant_wide_kernel<T, D, BITS>), grid, block, 0, st, p); break;
         case 211: QATTN_NARROW(2, 1, 1); break;
         case 222: QATTN_NARROW(NH2, NH2, 2); break;
@@ -852,11 +874,16 @@ static int launch_quant(const QuantParams& p, const PagedShape& sh, hipStream_t 
         default: QATTN_NARROW(1, NH4, 4);
     }
 #undef QATTN_NARROW
-    const int rc = launch_status(sh.qb ? "quant_attn_kernel" : "quant_wide_kernel");
+    int rc = launch_status(name_of(sh));
     if (rc) return rc;
-    if (!by_runs(p, sh)) return launch_merge<T, D>(p, st);
-    hipLaunchKernelGGL((quant_join_kernel<T, D>), dim3(p.nwg * (DenseTile<T, D>::kBM / kJoinRows<D>)), block, 0, st, p);
-    return launch_status("quant_join_kernel");
+    if (by_runs(p, sh)) {
+        hipLaunchKernelGGL((quant_join_kernel<T, D>), dim3(p.nwg * (DenseTile<T, D>::kBM / kJoinRows<D>)), block, 0,
+                           st, p);
+        rc = launch_status("quant_join_kernel");
+    } else {
+        rc = launch_merge<T, D>(p, st);
+    }
+    return rc ? rc : launch_status(name_of(sh));  // (what a call is told apart by)
 }
 
 template <typename T, int BITS>
@@ -884,6 +911,16 @@ int64_t qattn_prefix_quant_workspace_bytes(int32_t batch, int32_t max_seqlen, in
     return most;
 }
 
+const char* qattn_debug_quant_kernel(int32_t batch, int32_t max_seqlen, int64_t total_tokens, int32_t num_q_heads,
+                                     int32_t num_kv_heads, int32_t head_dim, int32_t pt_cols, int32_t page_size,
+                                     int32_t bits, int32_t together) {
+    PagedPlan plan;
+    if (!paged_plan(plan, [=](auto... a) { return quant_shape(bits, together != 0, a...); }, batch, max_seqlen,
+                    total_tokens, num_q_heads, num_kv_heads, head_dim, pt_cols, page_size))
+        return "";
+    return name_of(plan.shape);
+}
+
 int qattn_prefix_quant_fwd(const void* q, const int64_t q_stride[3], const void* k_cache, const void* v_cache,
                            const int64_t cache_stride[4], const void* k_scale, const void* v_scale,
                            const int64_t scale_stride[4], const int32_t* page_table, int32_t pt_cols,
@@ -899,8 +936,12 @@ int qattn_prefix_quant_fwd(const void* q, const int64_t q_stride[3], const void*
     QuantParams p{};
     PagedPlan plan;
     const int64_t half[4] = {cache_stride[0] / 2, cache_stride[1] / 2, cache_stride[2] / 2, 1};
-    // (what a wave of several heads loads at once: 128 bytes of elements, 32 / bits of scales)
-    const int64_t unit = head_dim / kQuantBlock, sides = 32 / bits;
+    // What a wave of NH heads loads of a token's scales at once, words of NH unit bytes or of
+    // four, must be aligned; NH is a power of two that divides the heads.  (4 bits, heads of
+    // 32, 4 kv heads, whose tokens have 4 scales: 64 x 8000 x 4 tokens 37.5 us, one head per
+    // wave 40.1; 8 x 4000 11.0 and 11.9.)
+    const int64_t unit = head_dim / kQuantBlock;
+    const int64_t sides = std::min<int64_t>(4, (num_kv_heads & -num_kv_heads) * unit);
     const int64_t* ss = scale_stride;
     const bool together = cache_stride[2] == head_dim * bits / 8 && ss[2] == unit && (ss[0] | ss[1]) % sides == 0 &&
                           ((uintptr_t)k_scale | (uintptr_t)v_scale) % sides == 0;
