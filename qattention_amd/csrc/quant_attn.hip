@@ -772,10 +772,15 @@ static int pow2_part(int n, int most) {
 // no call before left in the chip's; 32 q heads for 8 kv heads of 128 where nothing else
 // is said):
 //   A workgroup per item (8 waves, nothing joined by a second launch) or runs: up to 4
-//   steps per wave where the items are few enough for 4 bits (2 x 731: 8.4, runs 9.6; 8 x
-//   1000: 9.6, 11.7; but 32 x 1000: 17.7, 16.9; past 4 steps 1 x 2000: 14.1, 9.7, 8 x
-//   2000: 15.8, 13.0) or many enough for 8 (8 x 1000: 11.3, 12.5; 32 x 1000: 20.9, 25.4;
-//   but 2 x 900: 15.7, 10.1), else up to 2.
+//   steps per wave, but up to 2 where rows are 128 bytes and the items no more than 64.  A
+//   workgroup draws some 22 bytes a ns however few there are, so two more steps take 3 us
+//   in rows of up to 64 bytes, about what the second launch and the states of runs take,
+//   but 6 in rows of 128; with more items runs hold several steps too.  4 bits: 2 x 731
+//   9.3, runs 11.4; 1 x 1000 10.4, 11.1; 16 x 1000 14.1, 15.8; 32 x 1000 18.4, 19.5; but
+//   4 x 1000 with 32 kv heads 16.9, 15.8, 32 x 1000 with heads of 32 14.3, 12.7 (11.7 and 16.4
+//   in 8 bits where the contexts differ).  8 bits, heads of 64: 2 x 1000 9.0, 10.4; 32 x 1000
+//   16.2, 16.4.  8 bits, heads of 128: 1 x 480 10.2, 10.5; 2 x 1000 17.2, 11.1; 8 x 800
+//   17.0, 14.0; 10 x 800 17.1, 18.1; 10 x 1000 18.6, 18.2; 32 x 1000 22.3, 26.5.
 //   Heads of a wave (nh): as many as fill a 128-byte line (see above).
 //   Sets of heads of a workgroup (g), each to one wave, or all four waves on one set's
 //   keys (g = 1): the first saves the waves' join, the second has more and shorter parts.
@@ -792,7 +797,7 @@ static int pow2_part(int n, int most) {
 //   and the join of twice the parts cost more than the second workgroup hides.
 static PagedShape quant_shape(int bits, bool together, int64_t max_rows, int64_t pairs, int hkv, int64_t capacity,
                               int head_dim) {
-    const int steps = (bits == 4 ? pairs <= 128 : pairs >= 64) ? 4 : 2;
+    const int steps = head_dim * bits < 1024 || pairs > 64 ? 4 : 2;
     if (max_rows <= 16 && capacity <= steps * 32 * kItemWaves && pairs <= 256) return {1, 4, 8, 1, 1, true, 1};
     if (max_rows <= 32) {
         const int qb = max_rows <= 16 ? 1 : 2, row_bytes = head_dim * bits / 8;

@@ -4,7 +4,7 @@ from __future__ import annotations
 
 import pytest
 
-from quant_forms import CALLS, kernel_of
+from quant_forms import CALLS, ITEM, kernel_of
 
 
 @pytest.mark.parametrize("call", CALLS, ids=lambda c: "-".join(map(str, c)))
@@ -26,3 +26,17 @@ def test_no_form_without_a_call(D, bits):
 
 def test_nothing_to_launch():
     assert kernel_of(64, 4, 0, 500, 1, 4, 2, True) == "" and kernel_of(64, 4, 3, 500, 0, 4, 2, True) == ""
+
+
+@pytest.mark.parametrize("D,bits", [(32, 4), (32, 8), (64, 4), (64, 8), (128, 4), (128, 8)])
+def test_a_workgroup_per_item(D, bits):
+    """Up to 4 steps of 8 waves, 1024 positions, of up to 256 (sequence, kv head) pairs; 2 steps
+    where rows of 128 bytes belong to 64 pairs or fewer."""
+    def items(B, positions, n=1):
+        return kernel_of(D, bits, B, positions, n, 4, 8, True) == ITEM
+    wide = D * bits == 1024
+    for B in (1, 2, 8):
+        assert items(B, 512) and items(B, 1024) == (not wide) and items(B, 528) == (not wide)
+    for B in (9, 16, 32):
+        assert items(B, 1024) and items(B, 1024, 4) and not items(B, 1040) and not items(B, 1024, 5)
+    assert not items(33, 512)
