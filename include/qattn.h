@@ -527,8 +527,9 @@ int qattn_quant_append(const void *k, const int64_t k_stride[3], const void *v, 
  * cu_seqlens[s] + i takes position starts[s] + i of sequence s, i < max_seqlen
  * (cu_seqlens NULL: row s takes position starts[s]).  A position that is
  * negative, has no column or whose page lies outside the cache reads as zeros;
- * rows of no sequence are left as they were.  An element past fp16's range
- * becomes an infinity there.
+ * rows of no sequence, past max_seqlen and of offsets that descend or end past
+ * total_tokens are left as they were.  An element past fp16's range becomes an
+ * infinity there.
  */
 int qattn_quant_read(const void *k_cache, const void *v_cache, const int64_t cache_stride[4],
                      const void *k_scale, const void *v_scale, const int64_t scale_stride[4],

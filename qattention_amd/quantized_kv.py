@@ -175,8 +175,10 @@ def read_quantized_kv(
     everywhere; total_tokens: rows of the result, by default cu_seqlens[-1] (read on
     the host: pass both for graph capture).  A position that is negative, has no
     column or whose page lies outside the cache reads as zeros.  Rows that belong to
-    no sequence are not written.  Values are exact in bf16, and in fp16 where they lie
-    in its range (as those written from fp16 rows do; larger ones become infinities).
+    no sequence, a sequence's rows past max_seqlen and all rows of one whose offsets
+    descend or end past total_tokens are not written: they hold whatever the memory
+    held, NaN perhaps.  Values are exact in bf16, and in fp16 where they lie in its
+    range (as those written from fp16 rows do; larger ones become infinities).
     Returns K, V [total_tokens, Hkv, D]."""
     out = _lib.calls().quant_read(cache, page_table, starts, cu_seqlens, max_seqlen, total_tokens, dtype)
     if out is not None:
