@@ -122,15 +122,29 @@ constexpr int kNarrowWaves = 4;             // waves of a STREAM workgroup
 constexpr int kItemWaves = 8;               // waves of a workgroup per item
 constexpr int kAhead = 3;                   // V operands read ahead of their product
 
-// Waves per SIMD that the registers are bounded for: what holds two steps' loads of two
-// heads, or of 128 dims, does not fit a third of them.
-constexpr int quant_waves(int d, int qb, int nh) { return d == 128 || nh > 1 ? 2 : qb > 1 ? 3 : 4; }
+// Waves per SIMD that the registers are bounded for, by what two steps' loads and the
+// accumulators take (a bound that they do not fit costs more than the wave it gains):
+//   rows of 128 bytes         2, and 1 with two tiles (at 2: 64 x 7 tokens over 5300-16000
+//                             327 us, at 1 322; 16 x 7 over 4000 42, 40)
+//   heads of 128, two heads   2
+//   heads of 64 in 8 bits     3, and 2 with two tiles (at 4, 3 spilling 6-14: 64 x 1 over
+//                             16000, 3 heads, 136, so 107; 24 x 4 tokens over 4000 42, 36;
+//                             64 x 6 tokens over 16000 407, 250; but 64 x 7 over 5300-16000
+//                             248, 255)
+//   others                    4, and 3 with two tiles
+// (Heads of 128 in 4 bits spill 19-21 registers of a lane with a tile each for two heads,
+// 1-6 with several heads in one; of 64 in 4 bits 1 with four heads.)
+constexpr int quant_waves(int d, int bits, int qb, int nh) {
+    if (d * bits == 1024) return qb > 1 ? 1 : 2;
+    if (d == 128 || nh > 1) return 2;
+    return (qb > 1 ? 3 : 4) - (d * bits == 512);
+}
 
 // NW waves for G sets of NH kv heads.  (NH > 1: QB = 1 is one tile of columns for all of
 // them, QB = NH a tile each.)
 template <typename T, int D, int BITS, int QB, int NW, int NH, int G, bool STREAM>
 __global__ __launch_bounds__(64 * NW)
-    __attribute__((amdgpu_waves_per_eu(quant_waves(D, QB, NH)))) void quant_attn_kernel(QuantParams p) {
+    __attribute__((amdgpu_waves_per_eu(quant_waves(D, BITS, QB, NH)))) void quant_attn_kernel(QuantParams p) {
     constexpr int NC = D / 32;              // k-steps of S^T over the head dim
     constexpr int ND = D / 16;              // d-tiles of O^T
     constexpr int DV = D / 8;               // 16-byte chunks per widened row
@@ -808,7 +822,7 @@ static PagedShape quant_shape(int bits, bool together, int64_t max_rows, int64_t
         int per_cu, g;
         for (;; own = false) {
             const int n = own ? 2 : nh;
-            per_cu = quant_waves(head_dim, qb, n);
+            per_cu = quant_waves(head_dim, bits, qb, n);
             g = max_rows <= 16 ? pow2_part(hkv / n, kNarrowWaves) : 1;
             const int least = own ? (head_dim == 128 ? 48 : 8) : n > 1 ? 16 : 8;
             if (pairs / (n * g) * ((capacity + 31) / 32) < least * 256 * per_cu) g = 1;
