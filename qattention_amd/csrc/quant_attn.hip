@@ -499,12 +499,16 @@ __global__ __launch_bounds__(64 * NW)
 // quarter qd lies at place 4 n + qd of its row (a quarter-row's writes side by
 // side, no bank twice), which orders the dims of S's products (Q is read alike) and
 // of O's columns (put back where they are stored).
-// 2 x 1009 tokens over 6007, 8 bits, 8 heads of 128 for 32: 202-211 us, 0.97 PFLOP/s (a
-// library product of 8192^3: 1.23), 223 over 16 bits; 4 x 60 over 10240, 4 bits: 67,
-// 15 of them the first loads and the states of the 512 workgroups' cut items.
+// 2 x 1009 tokens over 6007, 8 bits, 8 heads of 128 for 32: 212 us, 0.93 PFLOP/s of 1.23 that
+// a library product of 8192^3 reaches (229 over 16 bits); 4 x 60 over 10240, 4 bits: 66, 8 of
+// them the join and some 15 the first loads and the states of the 512 workgroups' cut
+// items.  With heads of 128, 14 to 20 registers of a lane spill.
 // ---------------------------------------------------------------------------
 constexpr int kWideKeys = 64;
-constexpr int kTable = 24;  // blocks whose keys are looked up at once: the LDS that the buffers leave two workgroups
+// Blocks whose keys are looked up at once: the LDS that the buffers leave two workgroups.  (A
+// table's end empties the loop, and the next one waits for its pages and first blocks: 0.8
+// us.  94 blocks per workgroup, 2 x 1009 tokens over 6007: 212.5 us, by tables of 12 215.8.)
+constexpr int kTable = 24;
 
 struct QuantTable {
     uint32_t row[kTable][kWideKeys];    // offsets in 16-byte units
