@@ -790,10 +790,10 @@ static int pow2_part(int n, int most) {
 // no call before left in the chip's; 32 q heads for 8 kv heads of 128 where nothing else
 // is said):
 //   A workgroup per item (8 waves, nothing joined by a second launch) or runs: up to 4
-//   steps per wave, but up to 2 where rows are 128 bytes and the items no more than 64.  A
-//   workgroup draws some 22 bytes a ns however few there are, so two more steps take 3 us
-//   in rows of up to 64 bytes, about what the second launch and the states of runs take,
-//   but 6 in rows of 128; with more items runs hold several steps too.  4 bits: 2 x 731
+//   steps per wave, but up to 2 where rows are 128 bytes and the items no more than 64.  Two
+//   more steps take 3 us in rows of up to 64 bytes, about what the second launch and the
+//   states of runs take, but 6 in rows of 128, as a workgroup draws some 22 bytes a ns however
+//   few there are; with more items runs hold several steps too.  4 bits: 2 x 731
 //   9.3, runs 11.4; 1 x 1000 10.4, 11.1; 16 x 1000 14.1, 15.8; 32 x 1000 18.4, 19.5; but
 //   4 x 1000 with 32 kv heads 16.9, 15.8, 32 x 1000 with heads of 32 14.3, 12.7 (11.7 and 16.4
 //   in 8 bits where the contexts differ).  8 bits, heads of 64: 2 x 1000 9.0, 10.4; 32 x 1000
@@ -809,7 +809,7 @@ static int pow2_part(int n, int most) {
 //   9 .. 16 rows: two heads with a tile of columns each where several sets get 8 steps per
 //   wave (48 with heads of 128, whose registers spill), else one head, 4 tokens, 4 bits: 64
 //   x 16000 with heads of 64 148, one head 183; 40 x 8000 of 64 63, 67, of 32 44, 54; 24 x
-//   8000 of 64 in 8 bits 58, 67; of 128 64 x 5300-16000 167, 182, but 24 x 16000 114, 112.
+//   8000 of 64 in 8 bits 59, 64; of 128 64 x 5300-16000 167, 182, but 24 x 16000 114, 112.
 //   Workgroups per CU with several heads per wave and g = 1: one (1 x 30000: 23.5, two
 //   25.1; 32 x 2000: 28.5, 30.2; 4 x 20000 with heads of 64: 25.6, 28.8): a wave's start
 //   and the join of twice the parts cost more than the second workgroup hides.
